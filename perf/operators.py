@@ -2,8 +2,8 @@
 
 A program that serves the language model in 8 bits holds the MLP's weights as e4m3 codes with one scale for each block of 128 x 128 and
 calls, layer by layer, the norm that joins the residual stream and leaves codes with a scale for each 128 values of a row
-(`rms_norm_fp8`), the gated pair of products that leaves codes again (`glu_fp8`) and the product that joins the stream (`linear_fp8`).
-Activations from elsewhere are cut to codes by `quantize_fp8`, weights by `quantize_weight_fp8`.  `listed()` has each of them at
+(`rms_norm_fp8`), the gated pair of products (`glu_fp8`) and the product that joins the stream (`linear_fp8`).
+Other activations, the gated pair's among them, are cut to codes by `quantize_fp8`, weights by `quantize_weight_fp8`.  `listed()` has each of them at
 the widths of the repository's configurations (256, 768, 1024 and 2048, the MLP twelve times as wide) and at ragged ones, from a
 single token to a long batch of prompts; `draw()` anywhere in between."""
 import functools
@@ -32,11 +32,11 @@ def listed():
         # a gate weight of the wide model cut to codes when the model is loaded
         dict(name="quantize_weight_24576x2048", kind="weight", rows=24576, width=2048, dtype="bf16"),
         # the gated pair of one decode step of a batch of requests: the weights' bytes
-        dict(name="glu_decode_8x768", kind="glu", rows=8, width=768, features=9216),
+        dict(name="glu_decode_8x768", kind="glu", rows=8, width=768, features=9216, dtype="bf16"),
         # the gated pair of eight prompts
-        dict(name="glu_prompt_4096x768", kind="glu", rows=4096, width=768, features=9216),
+        dict(name="glu_prompt_4096x768", kind="glu", rows=4096, width=768, features=9216, dtype="bf16"),
         # long documents on the wide model: the largest product there is
-        dict(name="glu_prompt_16384x2048", kind="glu", rows=16384, width=2048, features=24576),
+        dict(name="glu_prompt_16384x2048", kind="glu", rows=16384, width=2048, features=24576, dtype="bf16"),
         # one interactive request: the down projection of a single token
         dict(name="linear_decode_1x9216", kind="linear", rows=1, width=9216, features=768, residual=True, bias=False, dtype="bf16"),
         # a full batch on the wide model: the down projection of 32 tokens
@@ -70,7 +70,7 @@ def draw(rng):
     if kind == "weight":
         return dict(kind=kind, rows=width(64, 24576), width=width(64, 2048), dtype=dtype)
     if kind == "glu":
-        return dict(kind=kind, rows=rows, width=width(64, 2048), features=width(64, 24576))
+        return dict(kind=kind, rows=rows, width=width(64, 2048), features=width(64, 24576), dtype=dtype)
     return dict(kind=kind, rows=rows, width=width(64, 24576), features=width(64, 2048), residual=rng.choice([True, False]),
                 bias=rng.choice([True, False, False]), dtype=dtype)
 
@@ -139,7 +139,7 @@ def _plain(state):
     x = _row_values(*state["x"], torch.float32)
     if kind == "glu":
         g, u = (x @ _weight_values(*state[n], torch.float32).t() for n in ("gate", "up"))
-        return _row_codes(_gelu(g) * u)
+        return (_gelu(g) * u).to(DTYPES[case["dtype"]])
     y = x @ _weight_values(*state["weight"], torch.float32).t()
     if case["bias"]:
         y = y + state["bias"].float()
@@ -166,7 +166,7 @@ def _own(state):
     if kind == "weight":
         return flash_stu.quantize_weight_fp8(state["x"])
     if kind == "glu":
-        return flash_stu.glu_fp8(*state["x"], *state["gate"], *state["up"])
+        return flash_stu.glu_fp8(*state["x"], *state["gate"], *state["up"], dtype=DTYPES[case["dtype"]])
     return flash_stu.linear_fp8(*state["x"], *state["weight"], bias=state.get("bias"), residual=state.get("residual"),
                                 dtype=DTYPES[case["dtype"]])
 
@@ -232,7 +232,7 @@ def run(state):
         out = _own(state)
     else:
         out = _plain(state)
-    if kind == "linear":
+    if kind in ("glu", "linear"):
         return dict(y=out)
     found = dict(codes=out[0], scales=out[1])
     if "sum" in state:
@@ -296,8 +296,7 @@ def exact(case, seed):
         g = torch.mm(x, _exact_values(*state["gate"], BLOCK).t())
         u = torch.mm(x, _exact_values(*state["up"], BLOCK).t())
         t = math.sqrt(2.0 / math.pi) * (g + 0.044715 * g ** 3)
-        codes, scales = _exact_rows(g * torch.sigmoid(2.0 * t) * u)
-        return dict(codes=codes, scales=scales)
+        return dict(y=g * torch.sigmoid(2.0 * t) * u)
     y = torch.mm(x, _exact_values(*state["weight"], BLOCK).t())
     if case["bias"]:
         y = y + state["bias"].double()
@@ -316,12 +315,7 @@ def work(case):
         held = t * (3 if case.get("delta") else 1)       # with the addition: two read, the sum written
         return {"bytes": rows * width * (held + 1) + scales + (t * width if kind == "norm" else 0),
                 "flops": rows * width * (7.0 if kind == "norm" else 3.0)}
-    features, pair = case["features"], 2 if kind == "glu" else 1
-    down = -(-features // BLOCK)
-    nbytes = rows * width + pair * features * width + 4 * blocks * (rows + pair * down)
-    if kind == "glu":
-        nbytes += rows * features + 4 * rows * down
-    else:
-        t = 4 if case["dtype"] == "fp32" else 2
-        nbytes += t * rows * features * (2 if case["residual"] else 1) + (t * features if case["bias"] else 0)
+    features, pair, t = case["features"], 2 if kind == "glu" else 1, 4 if case["dtype"] == "fp32" else 2
+    nbytes = rows * width + pair * features * width + 4 * blocks * (rows + pair * -(-features // BLOCK))
+    nbytes += t * rows * features * (2 if case.get("residual") else 1) + (t * features if case.get("bias") else 0)
     return {"bytes": nbytes, "flops": 2.0 * pair * rows * features * width}
