@@ -122,6 +122,12 @@ SIGNATURES = {
     "fstu_lds_sequence_bc": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "fstu_lds_sequence": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "fstu_lds_steps": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "fstu_fp8_quantize_rows": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp],
+    "fstu_fp8_rmsnorm": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp],
+    "fstu_fp8_quantize_weight": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp],
+    "fstu_fp8_linear": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp],
+    "fstu_fp8_glu": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64,
+                     _i, _i, _i, _i, _vp],
 }
 
 
@@ -1232,3 +1238,175 @@ def lds_steps(h: torch.Tensor, x: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
     _check(load().fstu_lds_steps(_p(h), _p(x), _p(A), _p(Bm), _p(Cm), _p(out), T, Bt, d_in, S, d_out, _dt(x), _stream()),
            "fstu_lds_steps")
     return out
+
+
+# ---------------------------------------------------------------- 8-bit operators
+# Codes are float8_e4m3fn, (rows, K) with rows a multiple of 16 bytes apart; scales float32, a row's in blocks of 128 values (rows,
+# ceil(K / 128)), a weight's in blocks of 128 x 128 (ceil(N / 128), ceil(K / 128)), any strides.  A value is its code times its
+# block's scale.  What these functions leave has one block's scales of all rows beside each other.
+FP8_BLOCK = 128
+_fp8 = torch.float8_e4m3fn
+
+
+def _fp8_new(rows: int, cols: int, per: int, device):
+    """Codes and scales to be written: rows of whole 16 bytes, scales of a block beside each other (weights: row by row)."""
+    codes = torch.empty(rows, -(-cols // 16) * 16, dtype=_fp8, device=device)
+    if cols % 16:
+        codes = codes[:, :cols]
+    n, b = -(-rows // per), -(-cols // FP8_BLOCK)
+    return codes, torch.empty_strided((n, b), (1, n) if per == 1 else (b, 1), dtype=torch.float32, device=device)
+
+
+def _fp8_source(x: torch.Tensor, dev: int, what: str, like: Optional[torch.Tensor] = None) -> int:
+    """Row stride of a 2-D float32 or bfloat16 tensor with dense rows on that device (of the shape and type of `like`)."""
+    if x.get_device() != dev or dev < 0:
+        raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if x.get_device() < 0
+                               else f"{what} is on device {x.get_device()}, not on {dev}")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or not 1 <= x.shape[1] < 1 << 31 or x.shape[0] >= 1 << 31:
+        raise FlashSTUHipError(f"{what} must be 2-D with dense rows, got shape {tuple(x.shape)} stride {x.stride()}")
+    if like is not None and (x.shape != like.shape or x.dtype != like.dtype):
+        raise FlashSTUHipError(f"{what} must be {tuple(like.shape)} {like.dtype}, got {tuple(x.shape)} {x.dtype}")
+    return x.stride(0)
+
+
+def _fp8_operand(codes: torch.Tensor, scales: torch.Tensor, per: int, dev: int, what: str):
+    """(address, row stride, address and strides of the scales) of checked codes and scales."""
+    if codes.get_device() != dev or scales.get_device() != dev or dev < 0:
+        raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if min(codes.get_device(), scales.get_device()) < 0
+                               else f"codes and scales of {what} are on devices {codes.get_device()} and {scales.get_device()}, not on {dev}")
+    if codes.dtype is not _fp8 or scales.dtype is not torch.float32 or codes.dim() != 2:
+        raise FlashSTUHipError(f"{what}: codes must be 2-D float8_e4m3fn and scales float32, got {tuple(codes.shape)} {codes.dtype}, {scales.dtype}")
+    rows, K = codes.shape
+    ld, one = codes.stride()
+    if (one != 1 and K > 1) or not 1 <= K < 1 << 31 or rows >= 1 << 31:
+        raise FlashSTUHipError(f"{what}: codes must have dense rows of 1 value or more, got shape {tuple(codes.shape)} stride {codes.stride()}")
+    if scales.shape != (-(-rows // per), -(-K // FP8_BLOCK)):
+        raise FlashSTUHipError(f"{what}: scales must be {(-(-rows // per), -(-K // FP8_BLOCK))}, got {tuple(scales.shape)}")
+    sr, sb = scales.stride()
+    return codes.data_ptr(), ld if rows > 1 else -(-K // 16) * 16, scales.data_ptr(), sr, sb
+
+
+def _fp8_device(fn):
+    """The function on the device of its first argument, which need not be the current one."""
+    @functools.wraps(fn)
+    def wrapped(x, *args, **kwargs):
+        dev = x.get_device()
+        if dev >= 0 and dev != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
+                return fn(x, *args, **kwargs)
+        return fn(x, *args, **kwargs)
+    return wrapped
+
+
+@_fp8_device
+def quantize_fp8(x: torch.Tensor):
+    """Codes and scales of x (rows, d) float32 or bfloat16, one scale for each 128 values of a row: scale = max(amax, 2^-100) / 448,
+    code = x * (448 / max(amax, 2^-100)) to the nearest e4m3 value.  A block with an infinity or a NaN stands for NaN."""
+    dev = x.get_device()
+    ld = _fp8_source(x, dev, "x")
+    rows, d = x.shape
+    dt = _dt(x)
+    codes, scales = _fp8_new(rows, d, 1, x.device)
+    if rows:
+        _check(load().fstu_fp8_quantize_rows(x.data_ptr(), ld, codes.data_ptr(), -(-d // 16) * 16, scales.data_ptr(), 1, rows, rows, d, dt,
+                                             raw_stream(dev)), "fstu_fp8_quantize_rows")
+    return codes, scales
+
+
+@_fp8_device
+def quantize_weight_fp8(weight: torch.Tensor):
+    """Codes and scales of a weight (N, K) float32 or bfloat16, one scale for each 128 x 128 values (formed as in quantize_fp8)."""
+    dev = weight.get_device()
+    ld = _fp8_source(weight, dev, "weight")
+    N, K = weight.shape
+    if N < 1:
+        raise FlashSTUHipError(f"weight must have rows, got {tuple(weight.shape)}")
+    dt = _dt(weight)
+    codes, scales = _fp8_new(N, K, FP8_BLOCK, weight.device)
+    _check(load().fstu_fp8_quantize_weight(weight.data_ptr(), ld, codes.data_ptr(), -(-K // 16) * 16, scales.data_ptr(), scales.shape[1], 1,
+                                           N, K, dt, raw_stream(dev)), "fstu_fp8_quantize_weight")
+    return codes, scales
+
+
+@_fp8_device
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optional[torch.Tensor] = None,
+                 x_out: Optional[torch.Tensor] = None):
+    """Codes and scales (as quantize_fp8's) of rmsnorm(x) * weight for x (rows, d), d up to 32768; the normed values are not rounded
+    to x's type on the way.  delta (rows, d): x + delta, rounded to x's type, is what is normed and is left in x_out (x itself where that is
+    not given)."""
+    dev = x.get_device()
+    ldx = _fp8_source(x, dev, "x")
+    rows, d = x.shape
+    if weight.get_device() != dev or weight.shape != (d,) or weight.dtype != x.dtype or not weight.is_contiguous():
+        raise FlashSTUHipError(f"weight must be ({d},) {x.dtype} on device {dev}, got {tuple(weight.shape)} {weight.dtype} on {weight.get_device()}")
+    dt = _dt(x)
+    pd = po = None
+    ldd = ldo = 0
+    if delta is not None:
+        if x_out is None:
+            x_out = x
+        ldd, ldo = _fp8_source(delta, dev, "delta", x), _fp8_source(x_out, dev, "x_out", x)
+        pd, po = delta.data_ptr(), x_out.data_ptr()
+    elif x_out is not None:
+        raise FlashSTUHipError("x_out takes x + delta: it needs delta")
+    codes, scales = _fp8_new(rows, d, 1, x.device)
+    if rows:
+        _check(load().fstu_fp8_rmsnorm(x.data_ptr(), ldx, pd, ldd, po, ldo, weight.data_ptr(), eps, codes.data_ptr(), -(-d // 16) * 16,
+                                       scales.data_ptr(), 1, rows, rows, d, dt, raw_stream(dev)), "fstu_fp8_rmsnorm")
+    return codes, scales
+
+
+@_fp8_device
+def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y (M, N) = x @ w^T (+ bias (N,)) (+ residual (M, N)) for x (M, K) and w (N, K) as codes with scales, the sum in fp32 and rounded
+    once.  y is of `dtype` (float32 or bfloat16; that of out, residual or bias where not given, bfloat16 without those), and so are
+    bias, residual and out.  out may be residual.  In float32 the sums are those of fp32 products; in bfloat16 the matrix core's 8-bit
+    instruction forms them, off by some 2e-5 of the result where its rounding is 2e-3."""
+    dev = codes.get_device()
+    xa = _fp8_operand(codes, scales, 1, dev, "x")
+    wa = _fp8_operand(w_codes, w_scales, FP8_BLOCK, dev, "w")
+    (M, K), N = codes.shape, w_codes.shape[0]
+    if w_codes.shape[1] != K or N < 1:
+        raise FlashSTUHipError(f"linear_fp8: x {tuple(codes.shape)} and w {tuple(w_codes.shape)} do not go together")
+    if dtype is None:
+        dtype = next((t.dtype for t in (out, residual, bias) if t is not None), torch.bfloat16)
+    if out is None:
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
+        out = torch.empty(M, N, dtype=dtype, device=codes.device)
+    for t, what in ((out, "out"), (residual, "residual")):
+        if t is not None and (t.shape != (M, N) or t.dtype != dtype or t.get_device() != dev or (N > 1 and t.stride(1) != 1)):
+            raise FlashSTUHipError(f"linear_fp8: {what} must be {(M, N)} {dtype} with dense rows on device {dev}, got {tuple(t.shape)} {t.dtype}")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != dtype or bias.get_device() != dev or not bias.is_contiguous()):
+        raise FlashSTUHipError(f"linear_fp8: bias must be ({N},) {dtype} on device {dev}, got {tuple(bias.shape)} {bias.dtype}")
+    dt = _dt(out)
+    if M:
+        _check(load().fstu_fp8_linear(*xa, *wa, _p(bias), _p(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(),
+                                      out.stride(0), M, N, K, dt, raw_stream(dev)), "fstu_fp8_linear")
+    return out
+
+
+@_fp8_device
+def glu_fp8(codes: torch.Tensor, scales: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tensor, up_codes: torch.Tensor,
+            up_scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16, quantize: bool = False):
+    """y (M, N) = gelu_tanh(x @ gate^T) * (x @ up^T) for x (M, K), gate and up (N, K) as codes with scales, in fp32 and rounded once to
+    `dtype` (float32 or bfloat16).  quantize: the codes and scales of quantize_fp8(y) in place of y (bfloat16), in the same launch."""
+    dev = codes.get_device()
+    xa = _fp8_operand(codes, scales, 1, dev, "x")
+    ga = _fp8_operand(gate_codes, gate_scales, FP8_BLOCK, dev, "the gate")
+    ua = _fp8_operand(up_codes, up_scales, FP8_BLOCK, dev, "the up weight")
+    (M, K), N = codes.shape, gate_codes.shape[0]
+    if gate_codes.shape[1] != K or up_codes.shape != gate_codes.shape or N < 1:
+        raise FlashSTUHipError(f"glu_fp8: x {tuple(codes.shape)}, gate {tuple(gate_codes.shape)} and up {tuple(up_codes.shape)} do not go together")
+    if dtype is not torch.bfloat16 and (dtype is not torch.float32 or quantize):
+        raise FlashSTUHipError(f"glu_fp8: unsupported dtype {dtype}: bfloat16, or float32 where the result is not quantized")
+    if quantize:
+        y, s = _fp8_new(M, N, 1, codes.device)
+        where = y.data_ptr(), -(-N // 16) * 16, s.data_ptr(), 1, M
+    else:
+        y = torch.empty(M, N, dtype=dtype, device=codes.device)
+        where = y.data_ptr(), N, None, 0, 0
+    if M:
+        _check(load().fstu_fp8_glu(*xa, *ga, *ua, *where, M, N, K, _dt(y) if not quantize else FSTU_BF16, raw_stream(dev)), "fstu_fp8_glu")
+    return (y, s) if quantize else y

@@ -696,6 +696,36 @@ int fstu_prof_end(double* total_ms, int* launches);
 int fstu_prof_copy(void* dst, const void* src, size_t bytes, void* stream);
 int fstu_prof_glu_loop(const fstu_model_desc* m, int reps, double* total_ms, int* launches, void* stream);
 
+/* ---- 8-bit operators ---------------------------------------------------------
+ * Codes are e4m3 bytes (OCP: largest 448, no infinity) in rows a multiple of 16 bytes apart, from a 16-byte aligned address on
+ * (what lies between a row's end and the next multiple of 16 is read and has no effect; these entry points write it up to the next
+ * multiple of 8); scales are fp32, scale (r, b) at s[r*s_row + b*s_blk], b = k / 128.  A value is code * scale.
+ * Rows (activations) have a scale for each 128 values, weights (N,K) one for each 128 x 128, r = n / 128.
+ *   scale = max(amax, 2^-100) / 448,  code = v * (448 / max(amax, 2^-100)) to the nearest, ties to the even code.
+ * A block with a value that is not finite gets a scale that is not finite either.  dtype: that of x, w, delta, bias, res, y.
+ *
+ * fstu_fp8_quantize_rows, fstu_fp8_quantize_weight: codes and scales of x (rows,d) / w (N,K), row strides ldx / ldw in elements.
+ * fstu_fp8_rmsnorm: with delta, x_out = T(x + delta) (x_out may be x or delta) and x_out is what is normed; codes and scales of
+ *   x * rsqrt(mean(x^2) + eps) * w, not rounded to T on the way; d up to 32768.  The norm of flash_stu/layers/stu_layer.py:93-96.
+ * fstu_fp8_linear: y[m,n] = T( sum_k x[m,k] w[n,k] + bias[n] + res[m,n] ), bias and res or NULL, y may be res; sums in fp32, one
+ *   rounding.  The down projection and the add behind it (flash_stu/modules/swiglu.py:27).
+ *   With dtype FSTU_F32 the sums are those of fp32 products; with FSTU_BF16 the matrix core's 8-bit instruction forms them, off by some
+ *   2e-5 of the result (its groups of products are cut 13 bits below their largest).
+ * fstu_fp8_glu: y[m,n] = T( gelu_tanh(x . gate[n]) * (x . up[n]) ) (swiglu.py:23-26), fp32 up to the rounding; with scales not NULL
+ *   (FSTU_BF16) y is codes, rows of ldy bytes: what fstu_fp8_quantize_rows makes of that y. */
+int fstu_fp8_quantize_rows(const void* x, int64_t ldx, uint8_t* codes, int64_t ldc, float* scales, int64_t s_row, int64_t s_blk, int rows, int d,
+                           int dtype, void* stream);
+int fstu_fp8_quantize_weight(const void* w, int64_t ldw, uint8_t* codes, int64_t ldc, float* scales, int64_t s_row, int64_t s_blk, int N, int K,
+                             int dtype, void* stream);
+int fstu_fp8_rmsnorm(const void* x, int64_t ldx, const void* delta, int64_t ldd, void* x_out, int64_t ldo, const void* w, float eps, uint8_t* codes,
+                     int64_t ldc, float* scales, int64_t s_row, int64_t s_blk, int rows, int d, int dtype, void* stream);
+int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw, const float* ws,
+                    int64_t ws_row, int64_t ws_blk, const void* bias, const void* res, int64_t ldr, void* y, int64_t ldy, int M, int N, int K,
+                    int dtype, void* stream);
+int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* gate, int64_t ldg, const float* gs,
+                 int64_t gs_row, int64_t gs_blk, const uint8_t* up, int64_t ldu, const float* us, int64_t us_row, int64_t us_blk, void* y, int64_t ldy,
+                 float* scales, int64_t s_row, int64_t s_blk, int M, int N, int K, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,113 @@
+"""What the 8-bit operators refuse, without a GPU: at the C entry points before any launch, and in the Python calls."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_stu import _hip
+    return _hip.load()
+
+
+@pytest.fixture(scope="module")
+def mem():
+    buf = (ctypes.c_char * 4096)()
+    return (ctypes.addressof(buf) + 63) // 64 * 64, buf
+
+
+def why(lib):
+    return lib.fstu_last_error().decode()
+
+
+def test_quantize_entry_points_refuse(lib, mem):
+    p = mem[0]
+    q = lambda x=p, ldx=128, c=p, ldc=128, s=p, rows=2, d=128, dt=1: lib.fstu_fp8_quantize_rows(x, ldx, c, ldc, s, 1, rows, rows, d, dt, None)
+    assert q(x=None) == -1 and q(c=None) == -1 and q(s=None) == -1 and "null" in why(lib)
+    assert q(rows=0) == -3 and q(d=0) == -3 and q(ldx=127) == -3
+    assert q(c=p + 8) == -4 and q(ldc=136) == -4 and q(ldc=112) == -4 and "16" in why(lib)
+    assert q(dt=7) == -2
+    w = lambda x=p, ldx=128, c=p, ldc=128, s=p, n=2, k=128, dt=1: lib.fstu_fp8_quantize_weight(x, ldx, c, ldc, s, 1, 1, n, k, dt, None)
+    assert w(x=None) == -1 and w(n=0) == -3 and w(k=0) == -3 and w(ldx=100) == -3 and w(c=p + 1) == -4 and w(ldc=120) == -4 and w(dt=2) == -2
+    assert w(n=65535 * 128 + 1) == -3
+
+
+def test_norm_entry_point_refuses(lib, mem):
+    p = mem[0]
+    f = lambda x=p, ldx=64, de=None, ldd=64, xo=None, ldo=64, w=p, c=p, ldc=64, s=p, rows=2, d=64, dt=1: lib.fstu_fp8_rmsnorm(
+        x, ldx, de, ldd, xo, ldo, w, 1e-6, c, ldc, s, 1, rows, rows, d, dt, None)
+    assert f(x=None) == -1 and f(w=None) == -1 and f(c=None) == -1 and f(s=None) == -1
+    assert f(de=p) == -5 and f(xo=p) == -5 and "together" in why(lib)
+    assert f(rows=0) == -3 and f(d=0) == -3 and f(d=32769, ldx=40000, ldc=40000) == -3 and f(ldx=63) == -3
+    assert f(de=p, xo=p, ldd=63) == -3 and f(de=p, xo=p, ldo=63) == -3
+    assert f(c=p + 4) == -4 and f(ldc=72) == -4 and f(dt=3) == -2
+
+
+def test_product_entry_points_refuse(lib, mem):
+    p = mem[0]
+
+    def lin(x=p, ldx=128, xs=p, w=p, ldw=128, ws=p, b=None, r=None, ldr=8, y=p, ldy=8, M=2, N=8, K=128, dt=1):
+        return lib.fstu_fp8_linear(x, ldx, xs, 1, 2, w, ldw, ws, 1, 1, b, r, ldr, y, ldy, M, N, K, dt, None)
+    assert lin(x=None) == -1 and lin(xs=None) == -1 and lin(w=None) == -1 and lin(ws=None) == -1 and lin(y=None) == -1
+    assert lin(M=0) == -3 and lin(N=0) == -3 and lin(K=0) == -3 and lin(ldy=7) == -3 and lin(r=p, ldr=7) == -3
+    assert lin(x=p + 8) == -4 and lin(w=p + 4) == -4 and lin(ldx=136) == -4 and lin(ldw=112) == -4 and lin(ldx=112) == -4
+    assert "16-byte" in why(lib) and lin(dt=9) == -2
+
+    def glu(x=p, ldx=128, xs=p, g=p, ldg=128, gs=p, u=p, ldu=128, us=p, y=p, ldy=16, s=None, M=2, N=16, K=128, dt=1):
+        return lib.fstu_fp8_glu(x, ldx, xs, 1, 2, g, ldg, gs, 1, 1, u, ldu, us, 1, 1, y, ldy, s, 1, 2, M, N, K, dt, None)
+    assert glu(x=None) == -1 and glu(g=None) == -1 and glu(us=None) == -1 and glu(y=None) == -1
+    assert glu(M=0) == -3 and glu(N=0) == -3 and glu(K=0) == -3 and glu(ldy=15) == -3
+    assert glu(u=p + 1) == -4 and glu(ldg=120) == -4 and glu(s=p, y=p + 8) == -4 and glu(s=p, ldy=24) == -4
+    assert glu(s=p, dt=0) == -2 and glu(dt=5) == -2
+
+
+def test_python_calls_refuse_what_is_not_on_the_gpu():
+    import flash_stu as fs
+    from flash_stu._hip import FlashSTUHipError
+    x, w = torch.zeros(2, 128), torch.zeros(16, 128)
+    c, s = torch.zeros(2, 128).to(torch.float8_e4m3fn), torch.zeros(2, 1)
+    for call in (lambda: fs.quantize_fp8(x), lambda: fs.quantize_weight_fp8(w), lambda: fs.rms_norm_fp8(x, torch.ones(128), 1e-6),
+                 lambda: fs.linear_fp8(c, s, c, s), lambda: fs.glu_fp8(c, s, c, s, c, s)):
+        with pytest.raises(FlashSTUHipError, match="not on the GPU"):
+            call()
+
+
+@pytest.mark.gpu
+def test_python_calls_refuse_what_does_not_go_together():
+    import flash_stu as fs
+    from flash_stu._hip import FlashSTUHipError
+    g = dict(device="cuda")
+    f8 = lambda *n: torch.zeros(*n, **g).to(torch.float8_e4m3fn)
+    x, c, s, w, ws = torch.zeros(4, 256, **g), f8(4, 256), torch.ones(4, 2, **g), f8(130, 256), torch.ones(2, 2, **g)
+
+    def refused(call, what):
+        with pytest.raises(FlashSTUHipError, match=what):
+            call()
+    refused(lambda: fs.quantize_fp8(x.half()), "unsupported dtype")
+    refused(lambda: fs.quantize_fp8(x.t()), "dense rows")
+    refused(lambda: fs.quantize_fp8(x[0]), "2-D")
+    refused(lambda: fs.quantize_fp8(x[:1].expand(4, 256)), "ldx=0")
+    refused(lambda: fs.quantize_fp8(torch.zeros(4, 0, **g)), "dense rows")
+    refused(lambda: fs.quantize_weight_fp8(torch.zeros(0, 4, **g)), "must have rows")
+    refused(lambda: fs.rms_norm_fp8(x, torch.ones(255, **g), 1e-6), "weight must be")
+    refused(lambda: fs.rms_norm_fp8(x, torch.ones(256, **g).bfloat16(), 1e-6), "weight must be")
+    refused(lambda: fs.rms_norm_fp8(x, torch.ones(256, **g), 1e-6, delta=torch.zeros(4, 255, **g)), "delta must be")
+    refused(lambda: fs.rms_norm_fp8(x, torch.ones(256, **g), 1e-6, x_out=x), "needs delta")
+    refused(lambda: fs.rms_norm_fp8(x, torch.ones(256, **g), 1e-6, delta=x, x_out=x.bfloat16()), "x_out must be")
+    refused(lambda: fs.rms_norm_fp8(torch.zeros(2, 32769, **g), torch.ones(32769, **g), 1e-6), "32768")
+    refused(lambda: fs.linear_fp8(c.view(torch.uint8), s, w, ws), "float8_e4m3fn")
+    refused(lambda: fs.linear_fp8(c, s.double(), w, ws), "float32")
+    refused(lambda: fs.linear_fp8(c, s[:3], w, ws), "scales must be")
+    refused(lambda: fs.linear_fp8(c, s, w, ws[:1]), "scales must be")
+    refused(lambda: fs.linear_fp8(c, s, w[:, :128], ws[:, :1]), "do not go together")
+    refused(lambda: fs.linear_fp8(c[:, 8:136], s[:, :1], w[:, :128], ws[:, :1]), "16-byte")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, bias=torch.zeros(129, **g)), "bias must be")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, residual=torch.zeros(4, 129, **g)), "residual must be")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, residual=torch.zeros(4, 130, **g), dtype=torch.bfloat16), "residual must be")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, out=torch.zeros(130, 4, **g).t()), "out must be")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, out=torch.zeros(1, 130, **g).expand(4, 130)), "ldy=0")
+    refused(lambda: fs.linear_fp8(c, s, w, ws, dtype=torch.float16), "unsupported dtype")
+    refused(lambda: fs.glu_fp8(c, s, w, ws, w[:129], ws), "do not go together")
+    refused(lambda: fs.glu_fp8(c, s, w, ws, w, ws, dtype=torch.float32, quantize=True), "unsupported dtype")
+    refused(lambda: fs.glu_fp8(c, s, w, ws.cpu(), w, ws), "not on the GPU")

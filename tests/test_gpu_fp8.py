@@ -1,0 +1,277 @@
+"""The 8-bit operators against their definition in 64 bits: codes and scales of rows and weights, the norm that leaves codes, the product and
+the gated pair.
+
+Tolerances, all from the definition.  A code is off by at most half its step (2^-4 of the value, 2^-10 below the smallest normal code) and by
+what its argument is off: 2^-22 of it for the scale's division and the product in fp32, and what the value before it was off.  A sum over K
+products in fp32, in blocks of 128 that are scaled and added, is off by at most (128 + blocks + 4) * 2^-24 of the sum of the products'
+sizes (each addition 2^-24 of a partial sum that is no larger than that sum; the block's 128 additions, those of the blocks, the
+product of two scales, the multiplication, bias and residual), and by half a step of the type it leaves in (2^-8 of the value for bf16, 2^-24
+for fp32).  Where the result is bf16 the 8-bit instruction adds up to eight products after it has cut each of them 13 bits below the
+largest: each is off by up to 2^-13 of that, so that a sum is off by up to 8 * 2^-13 = 2^-10 of the sum of the products' sizes more.  That
+bound holds for every single value; what it lets pass is held by the 2-norm: the cuts of products go either way, so that those of K products
+add up as K^(1/2) * 2^-13 * the largest of a group (under four times the root mean square of the products, with the rows and
+weights drawn here), 2^-11 of the result, beside 2^-8 / 3^(1/2) for the rounding.
+GELU: |gelu'| <= 1.13; x / (1 + exp(-2 t)) on the hardware's exp and reciprocal is off by (8 + 3 |2 t|) * 2^-23 of its value, since
+exp's argument is off by 3 * 2^-24 of itself."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -100
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+@pytest.fixture(scope="module")
+def fs():
+    import flash_stu
+    from flash_stu import _hip
+    _hip.load()
+    return flash_stu
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def half_step(v):
+    """Half the step between e4m3 values around v (64 bits, |v| up to 448)."""
+    return torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 4.0)
+
+
+def block_amax(v, per):
+    n, k = v.shape
+    b = torch.zeros(-(-n // per) * per, -(-k // 128) * 128, dtype=torch.float64)
+    b[:n, :k] = v.abs()
+    return b.view(-1, per, b.shape[1] // 128, 128).amax((1, 3))
+
+
+def spread(s, shape, per):
+    """Scales (ceil(n / per), ceil(k / 128)) for each value of (n, k), in 64 bits."""
+    return s.double().cpu().repeat_interleave(per, 0)[:shape[0]].repeat_interleave(128, 1)[:, :shape[1]]
+
+
+def check_codes(codes, scales, ref, err=0.0, per=1):
+    """codes and scales stand for ref (64 bits), whose values were off by up to err before they were cut."""
+    codes, err = codes.cpu().double(), torch.as_tensor(err, dtype=torch.float64).expand(ref.shape)
+    assert codes.shape == ref.shape and scales.shape == (-(-ref.shape[0] // per), -(-ref.shape[1] // 128))
+    most = block_amax(ref, per).clamp_min(LEAST)
+    off = (scales.double().cpu() * 448 - most).abs()
+    assert bool((off <= block_amax(err, per) + 2.0 ** -22 * most).all()), float((off / most).max())
+    s = spread(scales, ref.shape, per)
+    want, slack = ref / s, err / s + 2.0 ** -22 * (ref / s).abs()
+    worst = (codes - want).abs() - half_step(want.abs() + slack) - slack
+    assert bool((worst <= 0).all()), float(worst.max())
+
+
+def make_codes(shape, seed, per, pad=0):
+    """Codes and scales as a program holds them (made on the CPU from the definition, not by the kernels), and what they stand for."""
+    n, k = shape
+    v = torch.randn(n, k, generator=gen(seed), dtype=torch.float64) * torch.exp(torch.randn(n, 1, generator=gen(seed + 1), dtype=torch.float64))
+    s = (block_amax(v, per).clamp_min(LEAST) / 448).float()
+    codes = (v / spread(s, shape, per)).clamp(-448, 448).float().to(torch.float8_e4m3fn)
+    held = torch.full((n, -(-k // 16) * 16 + pad), 0x7f, dtype=torch.uint8)       # NaN behind every row's end
+    held[:, :k] = codes.view(torch.uint8)
+    held = held.cuda().view(torch.float8_e4m3fn)[:, :k]
+    value = codes.double() * spread(s, shape, per)
+    return held, s.cuda(), value
+
+
+def dot_bound(x, w, k, dtype):
+    return ((128 + -(-k // 128) + 4) * 2.0 ** -24 + (2.0 ** -10 if dtype == torch.bfloat16 else 0.0)) * (x.abs() @ w.abs().t())
+
+
+def check_product(y, ref, bound, dtype):
+    """y is ref (64 bits) to within bound and its type's rounding, each value and, in bf16, all together."""
+    off = (y.double().cpu() - ref).abs()
+    worst = off - bound - torch.finfo(dtype).eps / 2 * (ref.abs() + bound)
+    assert bool((worst <= 0).all()), float(worst.max())
+    if dtype == torch.bfloat16 and ref.numel() >= 64:
+        assert float(off.norm() / ref.norm()) <= 2.0 ** -8 / 3 ** 0.5 + 2.0 ** -11
+
+
+# ---------------------------------------------------------------- codes and scales
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(1, 1), (1, 128), (3, 7), (2, 129), (17, 768), (5, 1001), (33, 2048), (2, 40000), (301, 136)])
+def test_quantize_rows(fs, rows, d, dtype):
+    x = (torch.randn(rows, d, generator=gen(d)) * torch.exp(3 * torch.randn(rows, 1, generator=gen(rows)))).to(dtype)
+    codes, scales = fs.quantize_fp8(x.cuda())
+    check_codes(codes, scales, x.double())
+    view = torch.full((rows, d + 24), 7.0, dtype=dtype, device="cuda")[:, 3:3 + d]    # rows that begin anywhere
+    view.copy_(x)
+    c2, s2 = fs.quantize_fp8(view)
+    assert torch.equal(c2.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s2, scales)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,K", [(1, 1), (128, 128), (127, 129), (300, 200), (768, 1024), (129, 1001), (16, 8)])
+def test_quantize_weight(fs, N, K, dtype):
+    w = (torch.randn(N, K, generator=gen(N + K)) * 0.03).to(dtype)
+    codes, scales = fs.quantize_weight_fp8(w.cuda())
+    check_codes(codes, scales, w.double(), per=128)
+
+
+def test_every_code_to_the_nearest(fs):
+    """All e4m3 values, the middles between neighbours (to the even one) and what lies beside those, under a scale of one."""
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()        # 0 .. 448
+    mid = (codes[1:] + codes[:-1]) / 2
+    even = torch.where(torch.arange(126) % 2 == 0, codes[:-1], codes[1:])
+    x = torch.cat([codes, mid, mid * (1 + 2.0 ** -10), mid * (1 - 2.0 ** -10)])
+    want = torch.cat([codes, even, codes[1:], codes[:-1]])
+    x, want = torch.cat([x, -x]), torch.cat([want, -want])
+    per = 127                                                   # each block: 448, whose scale is one, and 127 others
+    x, want = (torch.cat([v, v.new_zeros(-len(v) % per)]).view(-1, per) for v in (x, want))
+    x, want = (torch.cat([torch.full((len(v), 1), 448.0, dtype=torch.float64), v], 1) for v in (x, want))
+    got, scales = fs.quantize_fp8(x.float().cuda())
+    assert torch.equal(scales.cpu(), torch.ones(len(x), 1))
+    assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_zeros_small_values_and_values_that_are_not_finite(fs, dtype):
+    x = torch.zeros(6, 300, dtype=dtype)
+    x[1, :] = 2.0 ** -120
+    x[2, 140] = float("inf")
+    x[3, 299] = float("nan")
+    x[4, 5] = torch.finfo(dtype).max
+    x[5, 130] = -3.0
+    for codes, scales, per in ((*fs.quantize_fp8(x.cuda()), 1), (*fs.quantize_weight_fp8(x.cuda()), 128)):
+        value = codes.cpu().double() * spread(scales, x.shape, per)
+        if per == 1:
+            bad = torch.zeros(6, 3, dtype=torch.bool)
+            bad[2, 1] = bad[3, 2] = True
+            assert torch.equal(torch.isfinite(scales.cpu()), ~bad)
+            assert torch.equal(torch.isnan(value), spread(bad, x.shape, 1).bool())
+            assert bool((value[0] == 0).all()) and float(value[5, 130]) == pytest.approx(-3.0, rel=2.0 ** -20)
+            assert float(value[4, 5]) == pytest.approx(torch.finfo(dtype).max, rel=2.0 ** -20)
+            assert bool((value[1].abs() <= 2.0 ** -110).all())
+        else:
+            assert torch.equal(torch.isfinite(scales.cpu()), torch.tensor([[True, False, False]]))
+    w = torch.ones(300, dtype=dtype)
+    codes, scales = fs.rms_norm_fp8(x.cuda(), w.cuda(), 1e-6)
+    value = codes.cpu().double() * spread(scales, x.shape, 1)
+    assert bool(torch.isnan(value[3]).all()) and bool(torch.isnan(value[2, 128:256]).all()) and bool((value[0] == 0).all())
+    ref = x[5].double() / (x[5].double().square().mean() + 1e-6).sqrt()
+    assert bool((value[5] - ref).abs().max() <= 2.0 ** -20 * ref.abs().max())
+
+
+# ---------------------------------------------------------------- the norm
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d", [(1, 1), (8, 768), (5, 100), (3, 129), (13, 512), (7, 1000), (6, 1001), (4, 2048), (2, 4096), (3, 8200), (2, 32768)])
+@pytest.mark.parametrize("add", [False, True])
+def test_rms_norm(fs, rows, d, dtype, add):
+    x = (torch.randn(rows, d, generator=gen(d)) * torch.exp(torch.randn(rows, 1, generator=gen(1)))).to(dtype)
+    w = (1 + 0.2 * torch.randn(d, generator=gen(2))).to(dtype)
+    delta = torch.randn(rows, d, generator=gen(3)).to(dtype)
+    held = torch.full((rows, d + 16), 9.0, dtype=dtype, device="cuda")
+    out = held[:, 8:8 + d]
+    codes, scales = fs.rms_norm_fp8(x.cuda(), w.cuda(), 1e-5, **(dict(delta=delta.cuda(), x_out=out) if add else {}))
+    if add:
+        total = (x.float() + delta.float()).to(dtype)
+        assert torch.equal(out.cpu(), total) and bool((held[:, :8] == 9).all()) and bool((held[:, 8 + d:] == 9).all())
+    else:
+        total = x
+    t = total.double()
+    ref = t / (t.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    # the mean's terms all have one sign: a lane's sum, the lanes' and the waves', at most 64 additions of 2^-24; half of it through the root
+    check_codes(codes, scales, ref, err=40 * 2.0 ** -24 * ref.abs())
+
+
+def test_rms_norm_in_place(fs):
+    x = torch.randn(9, 768, generator=gen(0)).bfloat16().cuda()
+    d = torch.randn(9, 768, generator=gen(1)).bfloat16().cuda()
+    w = torch.ones(768, dtype=torch.bfloat16, device="cuda")
+    y = x.clone()
+    want = fs.rms_norm_fp8(x, w, 1e-6, delta=d, x_out=torch.empty_like(x))
+    got = fs.rms_norm_fp8(y, w, 1e-6, delta=d)
+    assert torch.equal(y, (x.float() + d.float()).bfloat16())
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+    z = d.clone()
+    fs.rms_norm_fp8(x, w, 1e-6, delta=z, x_out=z)
+    assert torch.equal(z, y)
+
+
+# ---------------------------------------------------------------- the products
+SHAPES = [(1, 1, 1), (1, 768, 9216), (2, 16, 128), (3, 100, 129), (15, 130, 256), (16, 2048, 512), (17, 129, 1000), (31, 64, 2500), (33, 300, 768),
+          (64, 256, 384), (65, 100, 640), (100, 768, 1536), (129, 257, 130), (256, 256, 1024), (257, 513, 257), (300, 1001, 300), (700, 384, 2304),
+          (2, 3, 20000), (40, 130, 8192), (520, 770, 4096)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear(fs, M, N, K, dtype):
+    xc, xs, x = make_codes((M, K), 10, 1)
+    wc, ws, w = make_codes((N, K), 20, 128, pad=16)
+    bias = torch.randn(N, generator=gen(3)).to(dtype)
+    res = torch.randn(M, N, generator=gen(4)).to(dtype)
+    ref, bound = x @ w.t(), dot_bound(x, w, K, dtype)
+    for b, r in ((None, None), (bias, None), (None, res), (bias, res)):
+        want = ref + (0 if b is None else b.double()) + (0 if r is None else r.double())
+        size = bound + 2.0 ** -23 * (ref.abs() + (0 if b is None else b.double().abs()))
+        y = fs.linear_fp8(xc, xs, wc, ws, bias=None if b is None else b.cuda(), residual=None if r is None else r.cuda(), dtype=dtype)
+        assert y.dtype == dtype and y.shape == (M, N)
+        check_product(y, want, size, dtype)
+    # rows apart, scales in the other order, the sum left in the residual itself
+    held = torch.full((M + 2, N + 9), 5.0, dtype=dtype, device="cuda")
+    inner = held[1:M + 1, 4:4 + N]
+    inner.copy_(res)
+    y = fs.linear_fp8(xc, xs.t().contiguous().t(), wc, ws.t().contiguous().t(), residual=inner, out=inner)
+    assert y is inner and bool((held[0] == 5).all()) and bool((held[M + 1] == 5).all()) and bool((held[:, :4] == 5).all()) and bool((held[:, 4 + N:] == 5).all())
+    check_product(inner, ref + res.double(), bound + 2.0 ** -23 * ref.abs(), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_glu(fs, M, N, K, dtype):
+    xc, xs, x = make_codes((M, K), 10, 1)
+    gc, gs, _ = make_codes((N, K), 20, 128, pad=32)
+    uc, us, u = make_codes((N, K), 30, 128)
+    gs = gs * (2 * K ** -0.5)                                                  # gates of a few units
+    g = gc.cpu().double() * spread(gs, (N, K), 128)
+    y = fs.glu_fp8(xc, xs, gc, gs, uc, us, dtype=dtype)
+    assert y.dtype == dtype and y.shape == (M, N)
+    a, b = x @ g.t(), x @ u.t()
+    t = math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)
+    gelu = a * torch.sigmoid(2 * t)
+    ref = gelu * b
+    ea, eb = dot_bound(x, g, K, dtype), dot_bound(x, u, K, dtype)
+    err = 1.13 * ea * (b.abs() + eb) + gelu.abs() * eb + (8 + 3 * (2 * t).abs()) * 2.0 ** -23 * ref.abs() + 2.0 ** -130
+    check_product(y, ref, err, dtype)
+    y2 = fs.glu_fp8(xc, xs.t().contiguous().t(), gc, gs, uc, us, dtype=dtype)
+    assert torch.equal(y, y2)
+    if dtype == torch.bfloat16:                                                # what the two calls give one after the other
+        codes, scales = fs.glu_fp8(xc, xs, gc, gs, uc, us, quantize=True)
+        want, want_s = fs.quantize_fp8(y)
+        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40, 300])
+def test_a_row_that_is_not_finite_stays_by_itself(fs, M):
+    N, K = 200, 512
+    xc, xs, x = make_codes((M, K), 1, 1)
+    wc, ws, w = make_codes((N, K), 2, 128)
+    want, act = fs.linear_fp8(xc, xs, wc, ws), fs.glu_fp8(xc, xs, wc, ws, wc, ws, quantize=True)
+    bad = min(M - 1, 5)
+    codes, scales = xc.clone(), xs.clone()
+    codes.view(torch.uint8)[bad, 300] = 0x7f
+    y, (c2, s2) = fs.linear_fp8(codes, scales, wc, ws), fs.glu_fp8(codes, scales, wc, ws, wc, ws, quantize=True)
+    scales[bad, 1] = float("inf")
+    z = fs.linear_fp8(xc, scales, wc, ws)
+    keep = torch.arange(M, device="cuda") != bad
+    for got in (y, z):
+        assert torch.equal(got[keep], want[keep]) and not bool(torch.isfinite(got[bad]).any())
+    assert torch.equal(c2.view(torch.uint8)[keep], act[0].view(torch.uint8)[keep]) and torch.equal(s2[keep], act[1][keep])
+    assert bool(torch.isnan(s2[bad]).all())
+
+
+def test_no_rows(fs):
+    wc, ws, _ = make_codes((64, 128), 2, 128)
+    codes, scales = fs.quantize_fp8(torch.empty(0, 128, device="cuda"))
+    assert codes.shape == (0, 128) and scales.shape == (0, 1)
+    assert fs.rms_norm_fp8(torch.empty(0, 128, device="cuda"), torch.ones(128, device="cuda"), 1e-6)[0].shape == (0, 128)
+    assert fs.linear_fp8(codes, scales, wc, ws).shape == (0, 64)
+    assert fs.glu_fp8(codes, scales, wc, ws, wc, ws).shape == (0, 64)
+    act = fs.glu_fp8(codes, scales, wc, ws, wc, ws, quantize=True)
+    assert act[0].shape == (0, 64) and act[1].shape == (0, 1)
