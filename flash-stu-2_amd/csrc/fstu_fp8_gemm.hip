@@ -14,6 +14,7 @@
 //   glu     y = T( gelu_tanh(gate) * up )                  (swiglu.py:23-26), or codes and scales of that y (bf16), as
 //           fstu_fp8_quantize_rows makes them of it
 #include <algorithm>
+#include <type_traits>
 #include "fstu_fp8.h"
 
 namespace {
@@ -77,11 +78,10 @@ __device__ __forceinline__ u32x4_t cut16(u32x4_t v, int left) {
   }
   return v;
 }
-// A chunk of 16 bytes from byte k of a row of K.  A row's last chunk is read whole: rows are 16-byte aligned, so that it lies in the
-// 16 bytes whose first the row has.
+// A chunk of 16 bytes from byte k of a row of K (behind its end zeros, and its last chunk is read in their place).  A row's last chunk is
+// read whole: rows are 16-byte aligned, so that it lies in the 16 bytes whose first the row has.
 __device__ __forceinline__ u32x4_t chunk16(const uint8_t* row, int k, int K) {
-  if (k >= K) return u32x4_t{0, 0, 0, 0};
-  return cut16(*(const u32x4_t*)(row + k), K - k);
+  return cut16(*(const u32x4_t*)(row + min(k, (K - 1) & ~15)), K - k);
 }
 // The tanh-approximated GELU, x (1 + tanh t) / 2 = x / (1 + exp(-2 t)), on the hardware exp and reciprocal.
 __device__ __forceinline__ float gelu_tanh_exp(float x) {
@@ -167,6 +167,362 @@ fp8_plain_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K) {
   }
 }
 
+
+// ---------------------------------------------------------------- 256 x 256 tiles in two alternating wave groups
+// Many rows, results in bf16.  A workgroup of 8 waves owns 256 features (glu: 128 of the gate and 128 of the up weight) x 256 rows, K in blocks
+// of 128 through two LDS stages.  Waves 0-3 and 4-7 (one of each on every SIMD) run the same program half a phase apart: while one
+// group multiplies, the other reads its next fragments and requests the blocks to come, so that a SIMD's matrix core always has one of its
+// two waves to work for.  The halves of the weight tile (W0, W1: 128 features) and of the activation tile (X0, X1: 128 rows) are parts
+// of 16 KB; a wave owns 32 features of each W half and 64 rows of each X half, and a block is two phases of 16
+// v_mfma_f32_16x16x128_f8f6f4 (512 cycles), whose results are scaled and added (64 v_fma, 256 cycles) behind the next products:
+//   phase  fragments read               multiplied      requested
+//   0      W0, W1, X0 and scales of kt  (W0, W1) X0     X1 of kt + 1
+//   1      X1 and its scales of kt      (W0, W1) X1     W0, W1, X0 and scales of kt + 2
+// A part is requested in the first phase after its last readers have left it (their reads are complete before the barrier that ends a memory
+// phase) and waited for three phases later: vmcnt(9) at the end of a memory phase leaves the two youngest requests (2 and 7
+// instructions) in flight.  Scales have three stages, since a block's are read in both of its phases.
+// LDS rows are 128 bytes with the 16-byte chunk index XOR-ed with bits of the row, so that neither fills nor fragment reads meet bank
+// conflicts.  The W rows are dealt so that a lane ends up with 8 consecutive features of a row, which leave straight from the accumulators.
+// Workgroup ids are dealt round-robin to the 8 XCDs; each XCD works through its own share of the tiles in panels of 8 feature tiles, and
+// a workgroup requests the first blocks of its next tile before it stores this one.
+#define F8_PANEL 8
+#define F8_AHEAD 3                                // products that are on their way when one is scaled and added
+#define F8_PART 16384u
+#define F8_STAGE 65536u
+#define F8_SCALES (2 * F8_STAGE)                  // three stages of 2 KB: by wave the scales of 32 rows, then the two weights' in wave 0's
+#define F8_MAXIMA (F8_SCALES + 3 * 2048u)         // codes: the largest of a wave's 32 features of each row
+#define F8_LDS(CODES) (F8_MAXIMA + ((CODES) ? 4096u : 0u))
+#define F8_MAX_LD (1 << 23)                       // 256 rows of it are what a 32-bit offset covers
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, size_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (unsigned)bytes, 0x00020000);
+}
+// 16 bytes per lane from global memory into 64 consecutive slots of LDS without a stop in registers; zeros behind the range
+__device__ __forceinline__ void fill16(rsrc_t rs, unsigned voff, unsigned soff, void* l) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)l, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void fill4(const float* p, void* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)l, 4, 0, 0);
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
+// LDS reads are written as asm: the compiler orders every one it knows of behind all outstanding fills.  Each is waited for below, before any use.
+template <int OFF>
+__device__ __forceinline__ u32x4_t lds16(unsigned addr) {
+  u32x4_t v;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ float lds4(unsigned addr) {
+  float v;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF));
+  return v;
+}
+
+// 8 consecutive bf16 of a row, any 2-byte alignment; fewer at a row's end
+typedef unsigned u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void put8(bf16_t* p, const float (&v)[8], int left) {
+  if (left >= 8) {
+    *(u32x4_any_t*)p = u32x4_any_t{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7])};
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (e < left) p[e] = f32_to_bf16(v[e]);
+}
+__device__ __forceinline__ void add8(float (&v)[8], const bf16_t* p, int left) {
+  if (left >= 8) {
+    const u32x4_any_t r = *(const u32x4_any_t*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] += __uint_as_float(r[e] << 16), v[2 * e + 1] += __uint_as_float(r[e] & 0xffff0000u);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (e < left) v[e] += bf16_to_f32(p[e]);
+}
+
+// MODE 0 linear, 1 glu, 2 glu as codes.  TAIL: K is no multiple of 128; the last block comes straight from global memory behind the loop over
+// the whole ones (cutting its chunks inside the loop cost 100 spilled registers).
+template <int MODE, bool TAIL>
+__global__ void __launch_bounds__(512)
+fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt, int nt, int share) {
+  constexpr bool GLU = MODE != 0;
+  constexpr int NF = GLU ? 128 : 256;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int per_panel = mt * F8_PANEL, xcd = (int)(blockIdx.x & 7) * share, tiles = mt * nt;
+  int idx = (int)(blockIdx.x >> 3);                    // this workgroup's next tile in its XCD's share
+  if (idx >= share || xcd + idx >= tiles) return;
+  const int K16 = (K + 15) & ~15, nkt = K >> 7;
+  int m0, n0;
+  unsigned wbytes, ubytes, xbytes;
+  const uint8_t *wb, *ub, *xb;
+  const float* sp;                                     // this lane's scale of block 0: a row's, or one of the two weights'
+  const long long sstep = lane < 32 ? X.sb : GLU && (lane & 1) ? U.sb : W.sb;
+  const auto open = [&]() __attribute__((always_inline)) {
+    const int t = xcd + idx, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
+    m0 = in_panel / pw * 256;
+    n0 = (panel * F8_PANEL + in_panel % pw) * NF;
+    wbytes = (unsigned)(min(NF, N - n0) - 1) * (unsigned)W.ld + (unsigned)K16;
+    ubytes = GLU ? (unsigned)(min(NF, N - n0) - 1) * (unsigned)U.ld + (unsigned)K16 : wbytes;
+    xbytes = (unsigned)(min(256, M - m0) - 1) * (unsigned)X.ld + (unsigned)K16;
+    wb = W.p + (size_t)n0 * W.ld;
+    ub = GLU ? U.p + (size_t)n0 * U.ld : wb;
+    xb = X.p + (size_t)m0 * X.ld;
+    const int b = n0 >> 7, last = (N - 1) >> 7;
+    sp = lane < 32 ? X.s + (long long)min(m0 + wv * 32 + lane, M - 1) * X.sr
+                   : GLU ? (lane & 1 ? U.s + b * U.sr : W.s + b * W.sr) : W.s + min(b + (lane & 1), last) * W.sr;
+  };
+  const int wn = wv & 3, wm = wv >> 2;                 // 32-feature slice and 64-row slice of every half
+  // ---- fills: a part is 128 rows x 128 bytes, a wave fills rows 16 wv .. + 15 of it with two instructions
+  unsigned wvoff[2], uvoff[2], xvoff[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = wv * 16 + j * 8 + (lane >> 3), feat = GLU ? row : (row & 31) + 2 * (row & 96);
+    const unsigned wch = (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
+    wvoff[j] = (unsigned)feat * (unsigned)W.ld + wch;
+    uvoff[j] = GLU ? (unsigned)feat * (unsigned)U.ld + wch : wvoff[j] + 32u * (unsigned)W.ld;
+    xvoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
+  }
+  const unsigned x1off = 128u * (unsigned)X.ld;
+  unsigned char* const fill0 = smem + (unsigned)wv * 2048u;
+  // beyond the last block the descriptors are empty and the scales the last block's: into stages that nobody reads
+  const auto fetch_w = [&](int kt, unsigned stage) __attribute__((always_inline)) {
+    const bool in = kt < nkt;
+    const rsrc_t rw = make_rsrc(wb, in ? wbytes : 0), ru = make_rsrc(ub, in ? ubytes : 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fill16(rw, wvoff[j], (unsigned)kt * 128u, fill0 + stage + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fill16(ru, uvoff[j], (unsigned)kt * 128u, fill0 + stage + F8_PART + j * 1024);
+  };
+  const auto fetch_x = [&](int kt, unsigned stage, int h) __attribute__((always_inline)) {
+    const rsrc_t rx = make_rsrc(xb, kt < nkt ? xbytes : 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fill16(rx, xvoff[j] + (h ? x1off : 0u), (unsigned)kt * 128u, fill0 + stage + (2 + h) * F8_PART + j * 1024);
+  };
+  const auto fetch_s = [&](int kt, unsigned third) __attribute__((always_inline)) {
+    fill4(sp + (long long)max(min(kt, nkt - 1), 0) * sstep, smem + F8_SCALES + third + (unsigned)wv * 256u);
+  };
+
+  const int l16 = lane & 15, lq = lane >> 4;
+  unsigned fw[2], fx[2];                               // fragment addresses of a block's two halves inside a part
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int rw = wn * 32 + 8 * (l16 >> 2) + (l16 & 3), rx = wm * 64 + l16, c = h * 4 + lq;
+    fw[h] = lds_addr(smem) + (unsigned)rw * 128u + (unsigned)((c ^ (((rw >> 1) & 1) | ((rw >> 2) & 6))) << 4);
+    fx[h] = lds_addr(smem) + 2 * F8_PART + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
+  }
+  const unsigned fs = lds_addr(smem) + F8_SCALES + (unsigned)wm * 512u + (unsigned)l16 * 4u;    // rows 64 wm + l16: waves 2 wm and 2 wm + 1 filled them
+  const unsigned fsw = lds_addr(smem) + F8_SCALES + 128u + (GLU ? 0u : (unsigned)(wn >> 1) * 4u);
+  Frag32 wa[4], xf[4];                                 // [W half, feature tile], [row tile]
+  float sx[4], sw, su = 0.f;
+  floatx4_t acc[4][2][4];                              // [W half, feature tile][X half][row tile]
+  bool young = false;
+  constexpr int STORES = 8;                            // a whole tile's stores, at the least
+  const auto landed = [&]() __attribute__((always_inline)) {    // all but the 9 youngest fills; the stores of the tile before are younger than what is waited for
+    if (young) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(9 + STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+  };
+  const auto read_x = [&](unsigned stage, unsigned third, auto half) __attribute__((always_inline)) {
+    constexpr int H = decltype(half)::value;
+    xf[0] = Frag32{lds16<H * 16384>(fx[0] + stage), lds16<H * 16384>(fx[1] + stage)};
+    xf[1] = Frag32{lds16<H * 16384 + 2048>(fx[0] + stage), lds16<H * 16384 + 2048>(fx[1] + stage)};
+    xf[2] = Frag32{lds16<H * 16384 + 4096>(fx[0] + stage), lds16<H * 16384 + 4096>(fx[1] + stage)};
+    xf[3] = Frag32{lds16<H * 16384 + 6144>(fx[0] + stage), lds16<H * 16384 + 6144>(fx[1] + stage)};
+    sx[0] = lds4<H * 1024>(fs + third);
+    sx[1] = lds4<H * 1024 + 64>(fs + third);
+    sx[2] = lds4<H * 1024 + 256>(fs + third);
+    sx[3] = lds4<H * 1024 + 320>(fs + third);
+  };
+  // end of a memory phase: this wave's reads are complete, its share of the parts that the next phase reads has landed
+  const auto memory_end = [&]() __attribute__((always_inline)) {
+    landed();
+    asm volatile("s_waitcnt lgkmcnt(0)"
+                 : "+v"(xf[0].lo), "+v"(xf[0].hi), "+v"(xf[1].lo), "+v"(xf[1].hi), "+v"(xf[2].lo), "+v"(xf[2].hi), "+v"(xf[3].lo), "+v"(xf[3].hi),
+                   "+v"(wa[0].lo), "+v"(wa[0].hi), "+v"(wa[1].lo), "+v"(wa[1].hi), "+v"(wa[2].lo), "+v"(wa[2].hi), "+v"(wa[3].lo), "+v"(wa[3].hi),
+                   "+v"(sx[0]), "+v"(sx[1]), "+v"(sx[2]), "+v"(sx[3]), "+v"(sw), "+v"(su)::"memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto multiply = [&](auto half) __attribute__((always_inline)) {
+    constexpr int H = decltype(half)::value;
+    __builtin_amdgcn_s_setprio(1);
+    float f[4], g[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = sx[j] * sw, g[j] = GLU ? sx[j] * su : f[j];
+    floatx4_t d[16];
+#pragma unroll
+    for (int t = 0; t < 16 + F8_AHEAD; ++t) {
+      if (t < 16) d[t] = Operand<bf16_t>::sum(Operand<bf16_t>(wa[t >> 2]), Operand<bf16_t>(xf[t & 3]));
+      if (t >= F8_AHEAD) {
+        const int p = t - F8_AHEAD, i = p >> 2, j = p & 3;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][H][j][e] = fmaf(d[p][e], GLU && i >= 2 ? g[j] : f[j], acc[i][H][j][e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);               // in this order: left to itself the compiler puts each sum right behind its product
+    }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto first = [&]() __attribute__((always_inline)) {
+    fetch_w(0, 0), fetch_x(0, 0, 0), fetch_s(0, 0), fetch_x(0, 0, 1);
+    fetch_w(1, F8_STAGE), fetch_x(1, F8_STAGE, 0), fetch_s(1, 2048);
+  };
+  open();
+  first();
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j >> 2][j & 3] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    landed();                                          // W0, W1, X0 and scales of block 0
+    __builtin_amdgcn_s_barrier();
+    if (wm) __builtin_amdgcn_s_barrier();              // the second group runs half a phase later
+    __builtin_amdgcn_sched_barrier(0);
+    unsigned stage = 0, third = 0;
+    for (int kt = 0; kt < nkt; ++kt) {
+      const unsigned two = third == 0 ? 4096u : third - 2048u;       // the stage of block kt + 2's scales
+      wa[0] = Frag32{lds16<0>(fw[0] + stage), lds16<0>(fw[1] + stage)};
+      wa[1] = Frag32{lds16<512>(fw[0] + stage), lds16<512>(fw[1] + stage)};
+      wa[2] = Frag32{lds16<16384>(fw[0] + stage), lds16<16384>(fw[1] + stage)};
+      wa[3] = Frag32{lds16<16384 + 512>(fw[0] + stage), lds16<16384 + 512>(fw[1] + stage)};
+      sw = lds4<0>(fsw + third);
+      if constexpr (GLU) su = lds4<4>(fsw + third);
+      read_x(stage, third, std::integral_constant<int, 0>{});
+      fetch_x(kt + 1, F8_STAGE - stage, 1);
+      memory_end();
+      multiply(std::integral_constant<int, 0>{});
+      young = false;
+      read_x(stage, third, std::integral_constant<int, 1>{});
+      fetch_w(kt + 2, stage), fetch_x(kt + 2, stage, 0), fetch_s(kt + 2, two);
+      memory_end();
+      multiply(std::integral_constant<int, 1>{});
+      stage = F8_STAGE - stage;
+      third = third == 4096u ? 0u : third + 2048u;
+    }
+    if (!wm) __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
+    __builtin_amdgcn_s_barrier();
+    if constexpr (TAIL) {
+      const int k = nkt * 128 + lq * 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = wn * (GLU ? 32 : 64) + 8 * (l16 >> 2) + (l16 & 3) + 4 * (i & 1) + (GLU ? 0 : 16 * (i & 2));
+        const uint8_t* const r = GLU && i >= 2 ? ub + (size_t)min(f, N - 1 - n0) * U.ld : wb + (size_t)min(f, N - 1 - n0) * W.ld;
+        wa[i] = Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)};
+      }
+      const int b = n0 >> 7;
+      sw = W.s[(GLU ? b : min(b + (wn >> 1), (N - 1) >> 7)) * W.sr + nkt * W.sb];
+      if constexpr (GLU) su = U.s[b * U.sr + nkt * U.sb];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int m = min(m0 + h * 128 + wm * 64 + j * 16 + l16, M - 1);
+          const uint8_t* const r = xb + (size_t)(m - m0) * X.ld;
+          const Operand<bf16_t> x(Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)});
+          const float s = X.s[m * X.sr + nkt * X.sb];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const floatx4_t d = Operand<bf16_t>::sum(Operand<bf16_t>(wa[i]), x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][h][j][e] = fmaf(d[e], s * (GLU && i >= 2 ? su : sw), acc[i][h][j][e]);
+          }
+        }
+    }
+    // every wave has left the stages: the next tile's first blocks are on their way while this one is stored
+    const int em0 = m0, en0 = n0;
+    idx += (int)(gridDim.x >> 3);
+    const bool more = idx < share && xcd + idx < tiles;
+    if (more) {
+      open();
+      first();
+    }
+    asm volatile("" ::: "memory");
+    // D of a 16x16 tile: lane l holds row l % 16, and of the two feature tiles of a W half features 8*(l/16) .. + 7 of its 32
+    if constexpr (MODE == 2) {
+      const unsigned fm = lds_addr(smem) + F8_MAXIMA + (unsigned)(wm * 64 + l16) * 16u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          unsigned m = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float a = DT<bf16_t>::rnd(gelu_tanh_exp(acc[e >> 2][h][j][e & 3]) * acc[2 + (e >> 2)][h][j][e & 3]);
+            acc[e >> 2][h][j][e & 3] = en0 + wn * 32 + 8 * lq + e < N ? a : 0.f;
+            m = max(m, fp8_size(acc[e >> 2][h][j][e & 3]));
+          }
+          m = max(m, (unsigned)__shfl_xor((int)m, 16));
+          m = max(m, (unsigned)__shfl_xor((int)m, 32));
+          if (lq == 0) asm volatile("ds_write_b32 %0, %1" ::"v"(fm + (unsigned)(h * 128 + j * 16) * 16u + (unsigned)wn * 4u), "v"(m) : "memory");
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          u32x4_t v = lds16<0>(fm + (unsigned)(h * 128 + j * 16) * 16u);
+          asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v)::"memory");
+          const float most = __uint_as_float(max(max(v[0], v[1]), max(v[2], v[3]))), times = fp8_times(most);
+          const int m = em0 + h * 128 + wm * 64 + j * 16 + l16, f = en0 + wn * 32 + 8 * lq;
+          const floatx4_t a = acc[0][h][j], b = acc[1][h][j];
+          if (m < M && f < N)                          // a row's codes lie in whole 16 bytes: zeros behind the last feature
+            *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + f) = make_uint2(fp8_pack4(a[0] * times, a[1] * times, a[2] * times, a[3] * times),
+                                                                          fp8_pack4(b[0] * times, b[1] * times, b[2] * times, b[3] * times));
+          if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (en0 >> 7) * o.sb] = fp8_scale(most);
+        }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int m = em0 + h * 128 + wm * 64 + j * 16 + l16;
+#pragma unroll
+          for (int i = 0; i < (GLU ? 1 : 2); ++i) {
+            const int f = en0 + wn * (GLU ? 32 : 64) + i * 32 + 8 * lq;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float a = acc[2 * i + (e >> 2)][h][j][e & 3];
+              v[e] = GLU ? gelu_tanh_exp(a) * acc[2 + (e >> 2)][h][j][e & 3] : a;
+            }
+            if (m < M && f < N) {
+              if (!GLU && o.bias) add8(v, (const bf16_t*)o.bias + f, N - f);
+              if (!GLU && o.res) add8(v, (const bf16_t*)o.res + (size_t)m * o.ldr + f, N - f);
+              put8((bf16_t*)o.y + (size_t)m * o.ldy + f, v, N - f);
+            }
+          }
+        }
+    }
+    young = em0 + 256 <= M && en0 + NF <= N;
+    if (!more) break;
+  }
+}
+
+template <int MODE, bool TAIL>
+int large_launch(const Codes& X, const Codes& W, const Codes& U, const Leave& o, int M, int N, int K, hipStream_t s, const char* name) {
+  constexpr int NF = MODE ? 128 : 256;
+  static fstu_lds_limit most;
+  if (const int rc = fstu_need_lds((const void*)fp8_large_kernel<MODE, TAIL>, most, F8_LDS(MODE == 2), name)) return rc;
+  const int mt = (M + 255) / 256, nt = (N + NF - 1) / NF, share = (int)(((long long)mt * nt + 7) / 8);
+  hipLaunchKernelGGL((fp8_large_kernel<MODE, TAIL>), dim3(8u * (unsigned)std::min(share, fstu_cus() / 8)), dim3(512), F8_LDS(MODE == 2), s, X, W, U, o,
+                     M, N, K, mt, nt, share);
+  return 0;
+}
+template <int MODE>
+int large(const Codes& X, const Codes& W, const Codes& U, const Leave& o, int M, int N, int K, hipStream_t s, const char* name) {
+  return K % 128 ? large_launch<MODE, true>(X, W, U, o, M, N, K, s, name) : large_launch<MODE, false>(X, W, U, o, M, N, K, s, name);
+}
+bool large_takes(const Codes& X, const Codes& W, const Codes& U, int M, int N) {
+  return M > 64 && std::max(X.ld, std::max(W.ld, U.ld)) < F8_MAX_LD;
+}
+
 }  // namespace
 
 #define FP8_OPERAND(name, c, rows, what)                                                                                         \
@@ -184,6 +540,11 @@ extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, i
   FP8_OPERAND("fstu_fp8_linear", W, N, "w");
   FSTU_REQUIRE(M == 1 || (ldy >= N && (!res || ldr >= N)), FSTU_ESHAPE, "fstu_fp8_linear: N=%d ldy=%lld ldr=%lld", N, (long long)ldy, (long long)ldr);
   const Leave o = {y, ldy, bias, res, ldr, nullptr, 0, 0};
+  if (dtype == FSTU_BF16 && large_takes(X, W, W, M, N)) {
+    if (const int rc = large<0>(X, W, W, o, M, N, K, (hipStream_t)stream, "fstu_fp8_linear")) return rc;
+    FSTU_CHECK_LAUNCH("fstu_fp8_linear");
+    return FSTU_OK;
+  }
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_linear", {
     hipLaunchKernelGGL((fp8_plain_kernel<false, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, (hipStream_t)stream, X, W, W, o, M, N, K);
   });
@@ -205,6 +566,12 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
   FSTU_REQUIRE(!scales || (fstu_aligned(y, 16) && ldy % 16 == 0 && ldy >= N), FSTU_EALIGN,
                "fstu_fp8_glu: rows of codes must be 16-byte aligned, a multiple of 16 bytes apart and at least %d (stride %lld)", N, (long long)ldy);
   const Leave o = {y, ldy, nullptr, nullptr, 0, scales, ss, sb};
+  if (dtype == FSTU_BF16 && large_takes(X, W, U, M, N)) {
+    if (const int rc = scales ? large<2>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")
+                              : large<1>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")) return rc;
+    FSTU_CHECK_LAUNCH("fstu_fp8_glu");
+    return FSTU_OK;
+  }
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_glu", {
     hipLaunchKernelGGL((fp8_plain_kernel<true, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, (hipStream_t)stream, X, W, U, o, M, N, K);
   });
