@@ -523,6 +523,179 @@ bool large_takes(const Codes& X, const Codes& W, const Codes& U, int M, int N) {
   return M > 64 && std::max(X.ld, std::max(W.ld, U.ld)) < F8_MAX_LD;
 }
 
+// ---------------------------------------------------------------- few rows
+// The weights' bytes bound these: a wave takes 16 features (glu: of both weights) x 16 R rows of every KH-th block of K straight from
+// global memory, U blocks in flight at once, and the KH waves of a feature tile join their sums in LDS.  A workgroup has NT feature
+// tiles, F of them to a wave; K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
+template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
+__global__ void __launch_bounds__(64 * NT * KH)
+fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partial, int M, int N, int K, int slices) {
+  constexpr bool GLU = MODE != 0;
+  constexpr int FT = GLU ? 1 : F, G = F * R;           // feature tiles side by side of a wave, its 16 x 16 sums
+  static_assert(!GLU || F == 2, "gate and up");
+  static_assert(R * FT <= KH, "one wave joins one tile's sums");
+  static_assert(MODE != 2 || NT == 8, "the block of 128 features that shares a scale");
+  extern __shared__ __align__(16) float red[];         // [KH][NT][G][64 lanes][4]
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, q = lane >> 4;
+  const int nt = wv % NT, kh = wv / NT;
+  const int n0 = ((int)blockIdx.x * NT + nt) * 16 * FT, m0 = (int)blockIdx.z * 16 * R;
+  const uint8_t *wr[F], *xr[R];
+  const float *ws[F], *xs[R];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    const Codes& c = GLU && f ? V : W;
+    const int n = min(n0 + (GLU ? 0 : f * 16), N - 1);
+    wr[f] = c.p + (size_t)min(n + l16, N - 1) * c.ld;
+    ws[f] = c.s + (n >> 7) * c.sr;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int m = min(m0 + r * 16 + l16, M - 1);
+    xr[r] = X.p + (size_t)m * X.ld;
+    xs[r] = X.s + (long long)m * X.sr;
+  }
+  const int nb = (K + 127) >> 7, s = (int)blockIdx.y;
+  const int b0 = (int)((long long)nb * s / slices), b1 = (int)((long long)nb * (s + 1) / slices);
+  floatx4_t acc[F][R];
+#pragma unroll
+  for (int i = 0; i < G; ++i) acc[i / R][i % R] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  const auto chunk = [&](const uint8_t* p, int k) __attribute__((always_inline)) { return TAIL ? chunk16(p, k, K) : *(const u32x4_t*)(p + k); };
+  for (int b = b0 + kh; b < b1; b += KH * U) {
+    Frag32 w[U][F], x[U][R];
+    float sw[U][F], sx[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int bb = b + u * KH, k = bb * 128 + q * 16;
+      if (bb < b1) {
+#pragma unroll
+        for (int f = 0; f < F; ++f) w[u][f] = Frag32{chunk(wr[f], k), chunk(wr[f], k + 64)}, sw[u][f] = ws[f][bb * (GLU && f ? V.sb : W.sb)];
+#pragma unroll
+        for (int r = 0; r < R; ++r) x[u][r] = Frag32{chunk(xr[r], k), chunk(xr[r], k + 64)}, sx[u][r] = xs[r][bb * X.sb];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (b + u * KH < b1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const Operand<T> xo(x[u][r]);
+#pragma unroll
+          for (int f = 0; f < F; ++f) {
+            const floatx4_t d = Operand<T>::sum(Operand<T>(w[u][f]), xo);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[f][r][e] = fmaf(d[e], sx[u][r] * sw[u][f], acc[f][r][e]);
+          }
+        }
+      }
+  }
+  // the sums of a tile, by the wave whose kh is its number
+  floatx4_t* const mine = (floatx4_t*)red + ((size_t)(kh * NT + nt) * G) * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < G; ++i) mine[i * 64] = acc[i / R][i % R];
+  __syncthreads();
+  const bool joins = kh < R * FT;
+  const int r = kh % R, f = kh / R;                    // this wave's row tile and, linear, feature tile
+  floatx4_t v = {0.f, 0.f, 0.f, 0.f}, w2 = v;
+  if (joins) {
+#pragma unroll
+    for (int k = 0; k < KH; ++k) {
+      const floatx4_t* const p = (const floatx4_t*)red + ((size_t)(k * NT + nt) * G) * 64 + lane;
+      v += p[(f * R + r) * 64];
+      if constexpr (GLU) w2 += p[(R + r) * 64];
+    }
+  }
+  const int fe = n0 + f * 16 + q * 4, m = m0 + r * 16 + l16;
+  if constexpr (GLU) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fe + e < N ? DT<T>::rnd(gelu_tanh_exp(v[e]) * w2[e]) : 0.f;
+  }
+  if constexpr (MODE == 2) {
+    __syncthreads();                                   // the sums have been read: the maxima take their place
+    unsigned* const most = (unsigned*)red;             // [NT][16 R]
+    if (joins) {
+      unsigned a = max(max(fp8_size(v[0]), fp8_size(v[1])), max(fp8_size(v[2]), fp8_size(v[3])));
+      a = max(a, (unsigned)__shfl_xor((int)a, 16));
+      a = max(a, (unsigned)__shfl_xor((int)a, 32));
+      if (q == 0) most[nt * 16 * R + r * 16 + l16] = a;
+    }
+    __syncthreads();
+    if (joins && m < M) {
+      unsigned a = 0;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) a = max(a, most[i * 16 * R + r * 16 + l16]);
+      const float times = fp8_times(__uint_as_float(a));
+      if (fe < N) *(unsigned*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = fp8_pack4(v[0] * times, v[1] * times, v[2] * times, v[3] * times);
+      if (nt == 0 && q == 0) o.s[m * o.sr + blockIdx.x * o.sb] = fp8_scale(__uint_as_float(a));
+    }
+    return;
+  }
+  if (!joins || m >= M) return;
+  if (!GLU && slices > 1) {
+    float* const p = partial + ((size_t)s * M + m) * N + fe;
+    if (N % 4 == 0 && fe < N) *(floatx4_t*)p = v;
+    else
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (fe + e < N) p[e] = v[e];
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (fe + e >= N) break;
+    float a = v[e];
+    if (!GLU && o.bias) a += DT<T>::ld((const T*)o.bias + fe + e);
+    if (!GLU && o.res) a += DT<T>::ld((const T*)o.res + (size_t)m * o.ldr + fe + e);
+    DT<T>::st((T*)o.y + (size_t)m * o.ldy + fe + e, a);
+  }
+}
+
+// fp32 slices (slices, M, N), added in order -> T( sum + bias + residual )
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp8_join_kernel(const float* __restrict__ partial, Leave o, int M, int N, int slices) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n = (long long)M * N;
+  if (i >= n) return;
+  const int m = (int)(i / N), f = (int)(i - (long long)m * N);
+  float v = partial[i];
+  for (int s = 1; s < slices; ++s) v += partial[s * n + i];
+  if (o.bias) v += DT<T>::ld((const T*)o.bias + f);
+  if (o.res) v += DT<T>::ld((const T*)o.res + (size_t)m * o.ldr + f);
+  DT<T>::st((T*)o.y + (size_t)m * o.ldy + f, v);
+}
+
+template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
+int skinny_launch(const Codes& X, const Codes& W, const Codes& V, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
+                  const char* name) {
+  constexpr int NF = 16 * NT * (MODE ? 1 : F);
+  constexpr unsigned lds = KH * NT * F * R * 1024;
+  static fstu_lds_limit most;
+  if (const int rc = fstu_need_lds((const void*)fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>, most, lds, name)) return rc;
+  hipLaunchKernelGGL((fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>), dim3((N + NF - 1) / NF, slices, (M + 16 * R - 1) / (16 * R)), dim3(64 * NT * KH),
+                     lds, s, X, W, V, o, partial, M, N, K, slices);
+  if (MODE == 0 && slices > 1)
+    hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
+  return 0;
+}
+template <typename T, bool TAIL>
+int skinny_linear(const Codes& X, const Codes& W, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s) {
+  const char* const name = "fstu_fp8_linear";
+  if (M <= 16) return skinny_launch<T, 0, 1, 1, 1, 16, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  return skinny_launch<T, 0, 4, 2, 1, 8, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+}
+template <typename T, bool TAIL>
+int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, int M, int N, int K, hipStream_t s) {
+  const char* const name = "fstu_fp8_glu";
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    if (o.s) {
+      if (M <= 16) return skinny_launch<T, 2, 1, 2, 8, 2, 3, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+      return skinny_launch<T, 2, 2, 2, 8, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+    }
+  }
+  if (M <= 16) return skinny_launch<T, 1, 1, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+  return skinny_launch<T, 1, 2, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+}
+
 }  // namespace
 
 #define FP8_OPERAND(name, c, rows, what)                                                                                         \
@@ -530,16 +703,34 @@ bool large_takes(const Codes& X, const Codes& W, const Codes& U, int M, int N) {
   FSTU_REQUIRE(fstu_aligned((c).p, 16) && (c).ld % 16 == 0 && (c).ld >= ((rows) > 1 ? K : 0), FSTU_EALIGN,                       \
                name ": rows of " what " must be 16-byte aligned, a multiple of 16 bytes apart and at least K=%d (stride %lld)", K, (long long)(c).ld)
 
+// Slices of K for a product of few rows (1: none).
+extern "C" int fstu_fp8_linear_slices(int M, int N, int K) {
+  if (M < 1 || M > 64 || N < 1 || K < 1) return 1;
+  const int tiles = (N + (M <= 16 ? 15 : 31)) / (M <= 16 ? 16 : 32), nb = (K + 127) / 128;
+  return std::max(1, std::min(256 / tiles, nb / 16));
+}
+
 extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw,
                                const float* ws, int64_t ws_row, int64_t ws_blk, const void* bias, const void* res, int64_t ldr, void* y, int64_t ldy,
-                               int M, int N, int K, int dtype, void* stream) {
+                               int M, int N, int K, int dtype, float* partial, int slices, void* stream) {
   const Codes X = {x, ldx, xs, xs_row, xs_blk}, W = {w, ldw, ws, ws_row, ws_blk};
   FSTU_REQUIRE(y, FSTU_ENULL, "fstu_fp8_linear: null pointer");
   FSTU_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= 65535 * 64, FSTU_ESHAPE, "fstu_fp8_linear: M=%d N=%d K=%d", M, N, K);
   FP8_OPERAND("fstu_fp8_linear", X, M, "x");
   FP8_OPERAND("fstu_fp8_linear", W, N, "w");
   FSTU_REQUIRE(M == 1 || (ldy >= N && (!res || ldr >= N)), FSTU_ESHAPE, "fstu_fp8_linear: N=%d ldy=%lld ldr=%lld", N, (long long)ldy, (long long)ldr);
+  FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && M <= 64 && slices > 1 && slices <= (K + 127) / 128), FSTU_EARG, "fstu_fp8_linear: slices=%d (M=%d K=%d)", slices, M, K);
   const Leave o = {y, ldy, bias, res, ldr, nullptr, 0, 0};
+  if (M <= 64) {
+    int rc = 0;
+    FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_linear", {
+      rc = K % 128 ? skinny_linear<T, true>(X, W, o, partial, slices, M, N, K, (hipStream_t)stream)
+                   : skinny_linear<T, false>(X, W, o, partial, slices, M, N, K, (hipStream_t)stream);
+    });
+    if (rc) return rc;
+    FSTU_CHECK_LAUNCH("fstu_fp8_linear");
+    return FSTU_OK;
+  }
   if (dtype == FSTU_BF16 && large_takes(X, W, W, M, N)) {
     if (const int rc = large<0>(X, W, W, o, M, N, K, (hipStream_t)stream, "fstu_fp8_linear")) return rc;
     FSTU_CHECK_LAUNCH("fstu_fp8_linear");
@@ -566,6 +757,15 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
   FSTU_REQUIRE(!scales || (fstu_aligned(y, 16) && ldy % 16 == 0 && ldy >= N), FSTU_EALIGN,
                "fstu_fp8_glu: rows of codes must be 16-byte aligned, a multiple of 16 bytes apart and at least %d (stride %lld)", N, (long long)ldy);
   const Leave o = {y, ldy, nullptr, nullptr, 0, scales, ss, sb};
+  if (M <= 32) {
+    int rc = 0;
+    FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_glu", {
+      rc = K % 128 ? skinny_glu<T, true>(X, W, U, o, M, N, K, (hipStream_t)stream) : skinny_glu<T, false>(X, W, U, o, M, N, K, (hipStream_t)stream);
+    });
+    if (rc) return rc;
+    FSTU_CHECK_LAUNCH("fstu_fp8_glu");
+    return FSTU_OK;
+  }
   if (dtype == FSTU_BF16 && large_takes(X, W, U, M, N)) {
     if (const int rc = scales ? large<2>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")
                               : large<1>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")) return rc;

@@ -709,6 +709,8 @@ int fstu_prof_glu_loop(const fstu_model_desc* m, int reps, double* total_ms, int
  *   x * rsqrt(mean(x^2) + eps) * w, not rounded to T on the way; d up to 32768.  The norm of flash_stu/layers/stu_layer.py:93-96.
  * fstu_fp8_linear: y[m,n] = T( sum_k x[m,k] w[n,k] + bias[n] + res[m,n] ), bias and res or NULL, y may be res; sums in fp32, one
  *   rounding.  The down projection and the add behind it (flash_stu/modules/swiglu.py:27).
+ *   slices: K in that many slices, whose sums (partial, slices * M * N fp32) a second launch adds; fstu_fp8_linear_slices says how many
+ *   pay (1: none, partial may be NULL).
  *   With dtype FSTU_F32 the sums are those of fp32 products; with FSTU_BF16 the matrix core's 8-bit instruction forms them, off by some
  *   2e-5 of the result (its groups of products are cut 13 bits below their largest).
  * fstu_fp8_glu: y[m,n] = T( gelu_tanh(x . gate[n]) * (x . up[n]) ) (swiglu.py:23-26), fp32 up to the rounding; with scales not NULL
@@ -721,7 +723,8 @@ int fstu_fp8_rmsnorm(const void* x, int64_t ldx, const void* delta, int64_t ldd,
                      int64_t ldc, float* scales, int64_t s_row, int64_t s_blk, int rows, int d, int dtype, void* stream);
 int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw, const float* ws,
                     int64_t ws_row, int64_t ws_blk, const void* bias, const void* res, int64_t ldr, void* y, int64_t ldy, int M, int N, int K,
-                    int dtype, void* stream);
+                    int dtype, float* partial, int slices, void* stream);
+int fstu_fp8_linear_slices(int M, int N, int K);
 int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* gate, int64_t ldg, const float* gs,
                  int64_t gs_row, int64_t gs_blk, const uint8_t* up, int64_t ldu, const float* us, int64_t us_row, int64_t us_blk, void* y, int64_t ldy,
                  float* scales, int64_t s_row, int64_t s_blk, int M, int N, int K, int dtype, void* stream);
