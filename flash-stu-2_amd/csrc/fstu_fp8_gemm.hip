@@ -524,9 +524,11 @@ bool large_takes(const Codes& X, const Codes& W, const Codes& U, int M, int N) {
 }
 
 // ---------------------------------------------------------------- few rows
-// The weights' bytes bound these: a wave takes 16 features (glu: of both weights) x 16 R rows of every KH-th block of K straight from
-// global memory, U blocks in flight at once, and the KH waves of a feature tile join their sums in LDS.  A workgroup has NT feature
-// tiles, F of them to a wave; K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
+// The weights' bytes bound these: a wave takes 16 features (glu: of both weights) x 16 R rows of every KH-th block of K, U blocks in
+// flight at once in registers, and the KH waves of a feature tile join their sums in LDS.  A load is 8 rows of 128 bytes, whole lines;
+// the fragments, 16 rows of 64 bytes, are taken through 2 KB of LDS that the wave has for itself (read straight as fragments, half a line to a row,
+// one compute unit gets half as much: 768 x 9216 bytes over 48 of them 5.5 us, 2.9 so).  A workgroup has NT feature tiles, F of them to
+// a wave; K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
 template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
 __global__ void __launch_bounds__(64 * NT * KH)
 fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partial, int M, int N, int K, int slices) {
@@ -535,24 +537,27 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
   static_assert(!GLU || F == 2, "gate and up");
   static_assert(R * FT <= KH, "one wave joins one tile's sums");
   static_assert(MODE != 2 || NT == 8, "the block of 128 features that shares a scale");
-  extern __shared__ __align__(16) float red[];         // [KH][NT][G][64 lanes][4]
+  extern __shared__ __align__(16) unsigned char skinny_smem[];
+  float* const red = (float*)skinny_smem;              // behind the loop: [KH][NT][G][64 lanes][4]
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, q = lane >> 4;
   const int nt = wv % NT, kh = wv / NT;
   const int n0 = ((int)blockIdx.x * NT + nt) * 16 * FT, m0 = (int)blockIdx.z * 16 * R;
-  const uint8_t *wr[F], *xr[R];
+  const int row8 = lane >> 3, ch = lane & 7;           // this lane's row (and row + 8) of a load, its chunk of a block
+  const uint8_t *wr[F][2], *xr[R][2];
   const float *ws[F], *xs[R];
 #pragma unroll
   for (int f = 0; f < F; ++f) {
     const Codes& c = GLU && f ? V : W;
     const int n = min(n0 + (GLU ? 0 : f * 16), N - 1);
-    wr[f] = c.p + (size_t)min(n + l16, N - 1) * c.ld;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) wr[f][h] = c.p + (size_t)min(n + row8 + 8 * h, N - 1) * c.ld;
     ws[f] = c.s + (n >> 7) * c.sr;
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int m = min(m0 + r * 16 + l16, M - 1);
-    xr[r] = X.p + (size_t)m * X.ld;
-    xs[r] = X.s + (long long)m * X.sr;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) xr[r][h] = X.p + (size_t)min(m0 + r * 16 + row8 + 8 * h, M - 1) * X.ld;
+    xs[r] = X.s + (long long)min(m0 + r * 16 + l16, M - 1) * X.sr;
   }
   const int nb = (K + 127) >> 7, s = (int)blockIdx.y;
   const int b0 = (int)((long long)nb * s / slices), b1 = (int)((long long)nb * (s + 1) / slices);
@@ -560,34 +565,58 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
 #pragma unroll
   for (int i = 0; i < G; ++i) acc[i / R][i % R] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   const auto chunk = [&](const uint8_t* p, int k) __attribute__((always_inline)) { return TAIL ? chunk16(p, k, K) : *(const u32x4_t*)(p + k); };
+  // the chunk index is XOR-ed with bits of the row: neither the lines' writes nor the fragments' reads meet bank conflicts
+  unsigned char* const own = skinny_smem + (size_t)wv * ((F + R) * 2048);
+  unsigned char* const to = own + row8 * 128;
+  const unsigned to0 = (unsigned)(ch ^ (row8 >> 1)) * 16u, to1 = 1024u + (unsigned)(ch ^ (4 + (row8 >> 1))) * 16u;
+  const unsigned at0 = (unsigned)l16 * 128u + (unsigned)(q ^ (l16 >> 1)) * 16u, at1 = (unsigned)l16 * 128u + (unsigned)((4 + q) ^ (l16 >> 1)) * 16u;
   for (int b = b0 + kh; b < b1; b += KH * U) {
-    Frag32 w[U][F], x[U][R];
+    u32x4_t w[U][F][2], x[U][R][2];
     float sw[U][F], sx[U][R];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int bb = b + u * KH, k = bb * 128 + q * 16;
+      const int bb = b + u * KH, k = bb * 128 + ch * 16;
       if (bb < b1) {
 #pragma unroll
-        for (int f = 0; f < F; ++f) w[u][f] = Frag32{chunk(wr[f], k), chunk(wr[f], k + 64)}, sw[u][f] = ws[f][bb * (GLU && f ? V.sb : W.sb)];
+        for (int f = 0; f < F; ++f) {
+          w[u][f][0] = chunk(wr[f][0], k), w[u][f][1] = chunk(wr[f][1], k);
+          sw[u][f] = ws[f][bb * (GLU && f ? V.sb : W.sb)];
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r) x[u][r] = Frag32{chunk(xr[r], k), chunk(xr[r], k + 64)}, sx[u][r] = xs[r][bb * X.sb];
+        for (int r = 0; r < R; ++r) {
+          x[u][r][0] = chunk(xr[r][0], k), x[u][r][1] = chunk(xr[r][1], k);
+          sx[u][r] = xs[r][bb * X.sb];
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (b + u * KH < b1) {
+        __builtin_amdgcn_wave_barrier();               // a wave's LDS operations stay in order
+#pragma unroll
+        for (int t = 0; t < F + R; ++t) {
+          *(u32x4_t*)(to + t * 2048 + to0) = t < F ? w[u][t < F ? t : 0][0] : x[u][t < F ? 0 : t - F][0];
+          *(u32x4_t*)(to + t * 2048 + to1) = t < F ? w[u][t < F ? t : 0][1] : x[u][t < F ? 0 : t - F][1];
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        const auto fragment = [&](int t) __attribute__((always_inline)) {
+          return Operand<T>(Frag32{*(const u32x4_t*)(own + t * 2048 + at0), *(const u32x4_t*)(own + t * 2048 + at1)});
+        };
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const Operand<T> xo(x[u][r]);
+          const Operand<T> xo = fragment(F + r);
 #pragma unroll
           for (int f = 0; f < F; ++f) {
-            const floatx4_t d = Operand<T>::sum(Operand<T>(w[u][f]), xo);
+            const floatx4_t d = Operand<T>::sum(fragment(f), xo);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[f][r][e] = fmaf(d[e], sx[u][r] * sw[u][f], acc[f][r][e]);
           }
         }
+        asm volatile("" ::: "memory");
       }
   }
+  __syncthreads();                                     // the sums take the place of what other waves have read
   // the sums of a tile, by the wave whose kh is its number
   floatx4_t* const mine = (floatx4_t*)red + ((size_t)(kh * NT + nt) * G) * 64 + lane;
 #pragma unroll
@@ -667,7 +696,7 @@ template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
 int skinny_launch(const Codes& X, const Codes& W, const Codes& V, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
                   const char* name) {
   constexpr int NF = 16 * NT * (MODE ? 1 : F);
-  constexpr unsigned lds = KH * NT * F * R * 1024;
+  constexpr unsigned lds = KH * NT * std::max(F * R * 1024, (F + R) * 2048);
   static fstu_lds_limit most;
   if (const int rc = fstu_need_lds((const void*)fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>, most, lds, name)) return rc;
   hipLaunchKernelGGL((fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>), dim3((N + NF - 1) / NF, slices, (M + 16 * R - 1) / (16 * R)), dim3(64 * NT * KH),
