@@ -15,6 +15,7 @@
 //           fstu_fp8_quantize_rows makes them of it
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 #include "fstu_fp8.h"
 
 namespace {
@@ -478,27 +479,33 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
           if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (en0 >> 7) * o.sb] = fp8_scale(most);
         }
     } else {
+      // whole: all of the tile's features are there (the other form's branches are many, and a launch fetches its code anew)
+      const auto leave = [&](auto whole) __attribute__((always_inline)) {
+        constexpr bool ALL = decltype(whole)::value;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = em0 + h * 128 + wm * 64 + j * 16 + l16;
+          for (int j = 0; j < 4; ++j) {
+            const int m = em0 + h * 128 + wm * 64 + j * 16 + l16;
 #pragma unroll
-          for (int i = 0; i < (GLU ? 1 : 2); ++i) {
-            const int f = en0 + wn * (GLU ? 32 : 64) + i * 32 + 8 * lq;
-            float v[8];
+            for (int i = 0; i < (GLU ? 1 : 2); ++i) {
+              const int f = en0 + wn * (GLU ? 32 : 64) + i * 32 + 8 * lq, left = ALL ? 8 : N - f;
+              float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = acc[2 * i + (e >> 2)][h][j][e & 3];
-              v[e] = GLU ? gelu_tanh_exp(a) * acc[2 + (e >> 2)][h][j][e & 3] : a;
-            }
-            if (m < M && f < N) {
-              if (!GLU && o.bias) add8(v, (const bf16_t*)o.bias + f, N - f);
-              if (!GLU && o.res) add8(v, (const bf16_t*)o.res + (size_t)m * o.ldr + f, N - f);
-              put8((bf16_t*)o.y + (size_t)m * o.ldy + f, v, N - f);
+              for (int e = 0; e < 8; ++e) {
+                const float a = acc[2 * i + (e >> 2)][h][j][e & 3];
+                v[e] = GLU ? gelu_tanh_exp(a) * acc[2 + (e >> 2)][h][j][e & 3] : a;
+              }
+              if (m < M && (ALL || left > 0)) {
+                if (!GLU && o.bias) add8(v, (const bf16_t*)o.bias + f, left);
+                if (!GLU && o.res) add8(v, (const bf16_t*)o.res + (size_t)m * o.ldr + f, left);
+                put8((bf16_t*)o.y + (size_t)m * o.ldy + f, v, left);
+              }
             }
           }
-        }
+      };
+      if (en0 + NF <= N) leave(std::true_type{});
+      else leave(std::false_type{});
     }
     young = em0 + 256 <= M && en0 + NF <= N;
     if (!more) break;
@@ -518,9 +525,6 @@ int large_launch(const Codes& X, const Codes& W, const Codes& U, const Leave& o,
 template <int MODE>
 int large(const Codes& X, const Codes& W, const Codes& U, const Leave& o, int M, int N, int K, hipStream_t s, const char* name) {
   return K % 128 ? large_launch<MODE, true>(X, W, U, o, M, N, K, s, name) : large_launch<MODE, false>(X, W, U, o, M, N, K, s, name);
-}
-bool large_takes(const Codes& X, const Codes& W, const Codes& U, int M, int N) {
-  return M > 64 && std::max(X.ld, std::max(W.ld, U.ld)) < F8_MAX_LD;
 }
 
 // ---------------------------------------------------------------- few rows
@@ -560,11 +564,12 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
     xs[r] = X.s + (long long)min(m0 + r * 16 + l16, M - 1) * X.sr;
   }
   const int nb = (K + 127) >> 7, s = (int)blockIdx.y;
-  const int b0 = (int)((long long)nb * s / slices), b1 = (int)((long long)nb * (s + 1) / slices);
+  const int b0 = (int)((unsigned)(nb * s) / (unsigned)slices), b1 = (int)((unsigned)(nb * (s + 1)) / (unsigned)slices);
   floatx4_t acc[F][R];
 #pragma unroll
   for (int i = 0; i < G; ++i) acc[i / R][i % R] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   const auto chunk = [&](const uint8_t* p, int k) __attribute__((always_inline)) { return TAIL ? chunk16(p, k, K) : *(const u32x4_t*)(p + k); };
+  const bool both = R > 1 || M - m0 > 8;               // rows 8 .. 15 of the only row tile (what lies in LDS for them reaches nobody else's sum)
   // the chunk index is XOR-ed with bits of the row: neither the lines' writes nor the fragments' reads meet bank conflicts
   unsigned char* const own = skinny_smem + (size_t)wv * ((F + R) * 2048);
   unsigned char* const to = own + row8 * 128;
@@ -584,7 +589,8 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          x[u][r][0] = chunk(xr[r][0], k), x[u][r][1] = chunk(xr[r][1], k);
+          x[u][r][0] = chunk(xr[r][0], k);
+          if (both) x[u][r][1] = chunk(xr[r][1], k);
           sx[u][r] = xs[r][bb * X.sb];
         }
       }
@@ -596,7 +602,7 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
 #pragma unroll
         for (int t = 0; t < F + R; ++t) {
           *(u32x4_t*)(to + t * 2048 + to0) = t < F ? w[u][t < F ? t : 0][0] : x[u][t < F ? 0 : t - F][0];
-          *(u32x4_t*)(to + t * 2048 + to1) = t < F ? w[u][t < F ? t : 0][1] : x[u][t < F ? 0 : t - F][1];
+          if (t < F || both) *(u32x4_t*)(to + t * 2048 + to1) = t < F ? w[u][t < F ? t : 0][1] : x[u][t < F ? 0 : t - F][1];
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
@@ -709,7 +715,7 @@ template <typename T, bool TAIL>
 int skinny_linear(const Codes& X, const Codes& W, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s) {
   const char* const name = "fstu_fp8_linear";
   if (M <= 16) return skinny_launch<T, 0, 1, 1, 1, 16, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
-  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 1, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
   return skinny_launch<T, 0, 4, 2, 1, 8, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
 }
 template <typename T, bool TAIL>
@@ -721,9 +727,310 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
       return skinny_launch<T, 2, 2, 2, 8, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
     }
   }
-  if (M <= 16) return skinny_launch<T, 1, 1, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
-  return skinny_launch<T, 1, 2, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+  // us, 8 / 32 rows: 9216 x 768 two tiles of four waves 4.2 / 5.5, one of four 4.3 / 5.0, one of eight 5.0 / 6.4; 24576 x 2048 19 / 18.6, 18.8 /
+  // 19.1, 17.6 / 19.7
+  if (M <= 16) return K > 1536 ? skinny_launch<T, 1, 1, 2, 1, 8, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name)
+                               : skinny_launch<T, 1, 1, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+  return skinny_launch<T, 1, 2, 2, 1, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
 }
+
+// ---------------------------------------------------------------- 128 x 128 tiles
+// Products of too few 256 x 256 tiles, and those whose results are fp32.  Four waves, each 64 features (glu: 32 of the gate and 32 of the
+// up weight) x 64 rows; K in blocks of 128 through four LDS stages.  One wave to a SIMD, so it does everything at once:
+//   wait for the fragments of kt (this wave has left stage kt) and for its share of block kt + 1; barrier; multiply the fragments of kt and,
+//   an instruction or two behind each product, request block kt + 4 into stage kt and read the fragments of kt + 1
+// (all requests, then all reads, then the products: 0.75 us a block, since a wave issues in order and the queues of both are short).
+// K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
+#define TL_STAGE 33792u                           // W | X | scales: by wave those of 32 rows, then the two weights'
+#define TL_STAGES 4
+#define TL_FILLS 9
+
+template <typename T> struct Put;
+template <> struct Put<bf16_t> {
+  static __device__ __forceinline__ void put(bf16_t* p, const float (&v)[8], int left) { put8(p, v, left); }
+  static __device__ __forceinline__ void add(float (&v)[8], const bf16_t* p, int left) { add8(v, p, left); }
+};
+template <> struct Put<float> {
+  typedef float floatx4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+  static __device__ __forceinline__ void put(float* p, const float (&v)[8], int left) {
+    if (left >= 8) {
+      *(floatx4_any_t*)p = floatx4_any_t{v[0], v[1], v[2], v[3]};
+      *(floatx4_any_t*)(p + 4) = floatx4_any_t{v[4], v[5], v[6], v[7]};
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < left) p[e] = v[e];
+  }
+  static __device__ __forceinline__ void add(float (&v)[8], const float* p, int left) {
+    if (left >= 8) {
+      const floatx4_any_t a = *(const floatx4_any_t*)p, b = *(const floatx4_any_t*)(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += a[e], v[4 + e] += b[e];
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < left) v[e] += p[e];
+  }
+};
+
+template <class F, int... I>
+__device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...>) {
+  (step(std::integral_constant<int, I>{}), ...);
+}
+
+template <typename T, bool GLU, bool TAIL>
+__global__ void __launch_bounds__(256, 2)
+fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial, int M, int N, int K, int mt, int nt, int share, int slices) {
+  constexpr int NF = GLU ? 64 : 128;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int t = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= share || t >= mt * nt * slices) return;
+  const int slice = t / (mt * nt);
+  t -= slice * (mt * nt);
+  const int per_panel = mt * F8_PANEL, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
+  const int m0 = in_panel / pw * 128, n0 = (panel * F8_PANEL + in_panel % pw) * NF;
+  const int nb = (K + 127) >> 7, whole = K >> 7, K16 = (K + 15) & ~15;
+  const int b0 = (int)((unsigned)(nb * slice) / (unsigned)slices), b1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices), e1 = TAIL ? min(b1, whole) : b1;
+  const uint8_t* const wb = W.p + (size_t)n0 * W.ld;
+  const uint8_t* const ub = GLU ? U.p + (size_t)n0 * U.ld : wb;
+  const uint8_t* const xb = X.p + (size_t)m0 * X.ld;
+  const unsigned wbytes = (unsigned)(min(NF, N - n0) - 1) * (unsigned)W.ld + (unsigned)K16;
+  const unsigned ubytes = GLU ? (unsigned)(min(NF, N - n0) - 1) * (unsigned)U.ld + (unsigned)K16 : 0;
+  const unsigned xbytes = (unsigned)(min(128, M - m0) - 1) * (unsigned)X.ld + (unsigned)K16;
+  const float* const sp = lane < 32 ? X.s + (long long)min(m0 + wv * 32 + lane, M - 1) * X.sr
+                                    : GLU && (lane & 1) ? U.s + (n0 >> 7) * U.sr : W.s + (n0 >> 7) * W.sr;
+  const long long sstep = lane < 32 ? X.sb : GLU && (lane & 1) ? U.sb : W.sb;
+  // ---- fills: a wave fills rows 32 wv .. + 31 of either part with four instructions (glu: waves 0 and 1 the gate's, 2 and 3 the up weight's)
+  unsigned woff[4], xoff[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = wv * 32 + j * 8 + (lane >> 3);
+    woff[j] = (unsigned)(GLU ? row & 63 : row) * (unsigned)(GLU && wv >= 2 ? U.ld : W.ld) + (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
+    xoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
+  }
+  unsigned char* const fill0 = smem + (unsigned)wv * 4096u;
+  const auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {   // beyond the last whole block nothing, into a stage that nobody reads
+    const bool in = b < e1;
+    const rsrc_t rw = make_rsrc(GLU && wv >= 2 ? ub : wb, in ? (GLU && wv >= 2 ? ubytes : wbytes) : 0), rx = make_rsrc(xb, in ? xbytes : 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fill16(rw, woff[j], (unsigned)b * 128u, fill0 + stage + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fill16(rx, xoff[j], (unsigned)b * 128u, fill0 + stage + 16384 + j * 1024);
+    fill4(sp + (long long)min(b, e1 - 1) * sstep, smem + stage + 32768 + (unsigned)wv * 256u);
+  };
+  const int l16 = lane & 15, lq = lane >> 4, wn = wv & 1, wm = wv >> 1;
+  const int rw0 = (GLU ? 32 : 64) * wn + 8 * (l16 >> 2) + (l16 & 3);       // this lane's W row of the first feature tile; + 4, + 32 (glu: 64)
+  unsigned fw[2], fx[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int rx = wm * 64 + l16, c = h * 4 + lq;
+    fw[h] = lds_addr(smem) + (unsigned)rw0 * 128u + (unsigned)((c ^ (((rw0 >> 1) & 1) | ((rw0 >> 2) & 6))) << 4);
+    fx[h] = lds_addr(smem) + 16384u + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
+  }
+  const unsigned fs = lds_addr(smem) + 32768u + (unsigned)wm * 512u + (unsigned)l16 * 4u, fsw = lds_addr(smem) + 32768u + 128u;
+  struct Set {
+    Frag32 w[4], x[4];
+    float sx[4], sw, su;
+  };
+  Set a, b;
+  // the I-th of 16 reads of a block's fragments (w first: a wave's products begin with w[0] and all of x)
+  const auto read_one = [&](Set& f, unsigned stage, auto which) __attribute__((always_inline)) {
+    constexpr int I = decltype(which)::value, H = I & 1, P = GLU ? 8192 : 4096;       // P: from the first pair of feature tiles to the second
+    if constexpr (I < 8) {
+      (H ? f.x[I >> 1].hi : f.x[I >> 1].lo) = lds16<(I >> 1) * 2048>(fx[H] + stage);
+    } else {
+      constexpr int J = (I - 8) >> 1;
+      (H ? f.w[J].hi : f.w[J].lo) = lds16<(J >> 1) * P + (J & 1) * 512>(fw[H] + stage);
+    }
+    if constexpr (I < 4) f.sx[I] = lds4<(I & 1) * 64 + (I >> 1) * 256>(fs + stage);
+    if constexpr (I == 4) f.sw = lds4<0>(fsw + stage);
+    if constexpr (I == 5) f.su = GLU ? lds4<4>(fsw + stage) : 0.f;
+  };
+  const auto each16 = [](auto&& step) __attribute__((always_inline)) { steps16(step, std::make_integer_sequence<int, 16>{}); };
+  const auto wait = [&](Set& f) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%22) lgkmcnt(0)"
+                 : "+v"(f.w[0].lo), "+v"(f.w[0].hi), "+v"(f.w[1].lo), "+v"(f.w[1].hi), "+v"(f.w[2].lo), "+v"(f.w[2].hi), "+v"(f.w[3].lo), "+v"(f.w[3].hi),
+                   "+v"(f.x[0].lo), "+v"(f.x[0].hi), "+v"(f.x[1].lo), "+v"(f.x[1].hi), "+v"(f.x[2].lo), "+v"(f.x[2].hi), "+v"(f.x[3].lo), "+v"(f.x[3].hi),
+                   "+v"(f.sx[0]), "+v"(f.sx[1]), "+v"(f.sx[2]), "+v"(f.sx[3]), "+v"(f.sw), "+v"(f.su)
+                 : "n"(TL_FILLS * (TL_STAGES - 2))
+                 : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  floatx4_t acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  // multiplies block f; behind its products block kt + TL_STAGES is requested into stage cur and block kt + 1 is read from stage nxt into g
+  const auto multiply = [&](Set& f, Set& g, int kt, unsigned cur, unsigned nxt) __attribute__((always_inline)) {
+    const bool in = kt + TL_STAGES < e1;
+    const rsrc_t rw = make_rsrc(GLU && wv >= 2 ? ub : wb, in ? (GLU && wv >= 2 ? ubytes : wbytes) : 0), rx = make_rsrc(xb, in ? xbytes : 0);
+    float s[4], u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = f.sx[j] * f.sw, u[j] = GLU ? f.sx[j] * f.su : s[j];
+    const auto request = [&](auto which) __attribute__((always_inline)) {
+      constexpr int I = decltype(which)::value;
+      if constexpr (I < 8) {
+        if constexpr (I & 1) fill16(rx, xoff[I >> 1], (unsigned)(kt + TL_STAGES) * 128u, fill0 + cur + 16384 + (I >> 1) * 1024);
+        else fill16(rw, woff[I >> 1], (unsigned)(kt + TL_STAGES) * 128u, fill0 + cur + (I >> 1) * 1024);
+      }
+      if constexpr (I == 8) fill4(sp + (long long)min(kt + TL_STAGES, e1 - 1) * sstep, smem + cur + 32768 + (unsigned)wv * 256u);
+    };
+    if constexpr (std::is_same<T, float>::value) {
+      // widened fragments: x's at once, w's one after the other, so that what comes for the next block takes the place of what has been widened
+      Operand<T> x[4] = {Operand<T>(f.x[0]), Operand<T>(f.x[1]), Operand<T>(f.x[2]), Operand<T>(f.x[3])};
+      __builtin_amdgcn_sched_barrier(0);
+      floatx4_t d[4];
+      each16([&](auto which) __attribute__((always_inline)) {
+        constexpr int I = decltype(which)::value, i = I >> 2, k = I & 3;
+        const bf16x8_t w = k < 2 ? widen8(f.w[i].lo[2 * (k & 1)], f.w[i].lo[2 * (k & 1) + 1]) : widen8(f.w[i].hi[2 * (k & 1)], f.w[i].hi[2 * (k & 1) + 1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          d[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[j].v[k], k ? d[j] : floatx4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        request(which);
+        read_one(g, nxt, which);
+        if constexpr (k == 3) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[j][e], GLU && i >= 2 ? u[j] : s[j], acc[i][j][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else {
+      floatx4_t d[16];
+      const auto add = [&](auto which) __attribute__((always_inline)) {
+        constexpr int I = decltype(which)::value, i = I >> 2, j = I & 3;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[I][e], GLU && i >= 2 ? u[j] : s[j], acc[i][j][e]);
+      };
+      each16([&](auto which) __attribute__((always_inline)) {
+        constexpr int I = decltype(which)::value;
+        d[I] = Operand<T>::sum(Operand<T>(f.w[I >> 2]), Operand<T>(f.x[I & 3]));
+        request(which);
+        read_one(g, nxt, which);
+        if constexpr (I >= F8_AHEAD) add(std::integral_constant<int, I - F8_AHEAD>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      add(std::integral_constant<int, 13>{}), add(std::integral_constant<int, 14>{}), add(std::integral_constant<int, 15>{});
+      static_assert(F8_AHEAD == 3, "the last sums");
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (b0 < e1) {
+#pragma unroll
+    for (int i = 0; i < TL_STAGES; ++i) fetch(b0 + i, i * TL_STAGE);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TL_FILLS * (TL_STAGES - 1)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    each16([&](auto which) __attribute__((always_inline)) { read_one(a, 0, which); });
+    unsigned cur = 0;                                  // the stage of block kt
+    const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (TL_STAGES - 1) * TL_STAGE ? 0u : st + TL_STAGE; };
+    // blocks in pairs; behind an odd number comes one of zeros (what a fill finds behind the range), whose scales are the last block's: where
+    // they are not finite, neither is the sum any more
+    for (int kt = b0; kt < e1; kt += 2) {
+      unsigned nxt = next(cur);
+      wait(a);
+      multiply(a, b, kt, cur, nxt);
+      cur = nxt, nxt = next(cur);
+      wait(b);
+      multiply(b, a, kt + 1, cur, nxt);
+      cur = nxt;
+    }
+    wait(a);                                           // the last reads, of a block that is not there, have to have come in
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
+  }
+  const int fe = n0 + wn * (GLU ? 32 : 64) + 8 * lq;   // this lane's features: 8 of each pair of tiles
+  if constexpr (TAIL) {
+    if (b1 == nb) {                                    // what a whole block does not hold, straight from global memory
+      const int k = whole * 128 + lq * 16;
+      Frag32 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = wn * (GLU ? 32 : 64) + 8 * (l16 >> 2) + (l16 & 3) + 4 * (i & 1) + (GLU ? 0 : 16 * (i & 2));
+        const uint8_t* const r = (GLU && i >= 2 ? ub : wb) + (size_t)min(f, N - 1 - n0) * (GLU && i >= 2 ? U.ld : W.ld);
+        w[i] = Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)};
+      }
+      const float sw = W.s[(n0 >> 7) * W.sr + whole * W.sb], su = GLU ? U.s[(n0 >> 7) * U.sr + whole * U.sb] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int m = min(m0 + wm * 64 + j * 16 + l16, M - 1);
+        const uint8_t* const r = xb + (size_t)(m - m0) * X.ld;
+        const Operand<T> x(Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)});
+        const float sx = X.s[m * X.sr + whole * X.sb];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const floatx4_t d = Operand<T>::sum(Operand<T>(w[i]), x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], sx * (GLU && i >= 2 ? su : sw), acc[i][j][e]);
+        }
+      }
+    }
+  }
+  // whole: all of the tile's features are there (the other form's branches are many, and a launch fetches its code anew)
+  const auto leave = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool ALL = decltype(whole)::value;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = m0 + wm * 64 + j * 16 + l16;
+      if (m >= M) continue;
+#pragma unroll
+      for (int p = 0; p < (GLU ? 1 : 2); ++p) {
+        const int f = fe + p * 32, left = ALL ? 8 : N - f;
+        if (!ALL && left <= 0) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float g = acc[2 * p + (e >> 2)][j][e & 3];
+          v[e] = GLU ? gelu_tanh_exp(g) * acc[2 + (e >> 2)][j][e & 3] : g;
+        }
+        if (!GLU && slices > 1) {
+          Put<float>::put(partial + ((size_t)slice * M + m) * N + f, v, left);
+          continue;
+        }
+        if (!GLU && o.bias) Put<T>::add(v, (const T*)o.bias + f, left);
+        if (!GLU && o.res) Put<T>::add(v, (const T*)o.res + (size_t)m * o.ldr + f, left);
+        Put<T>::put((T*)o.y + (size_t)m * o.ldy + f, v, left);
+      }
+    }
+  };
+  if (n0 + NF <= N) leave(std::true_type{});
+  else leave(std::false_type{});
+}
+
+template <typename T, bool GLU>
+int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s, const char* name) {
+  constexpr int NF = GLU ? 64 : 128;
+  static fstu_lds_limit most[2];
+  const bool tail = K % 128;
+  const void* const kernel = tail ? (const void*)fp8_tile_kernel<T, GLU, true> : (const void*)fp8_tile_kernel<T, GLU, false>;
+  if (const int rc = fstu_need_lds(kernel, most[tail], TL_STAGES * TL_STAGE, name)) return rc;
+  const int mt = (M + 127) / 128, nt = (N + NF - 1) / NF;
+  const long long tiles = (long long)mt * nt * slices;
+  const int share = (int)((tiles + 7) / 8);
+  if (tail)
+    hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, true>), dim3(8u * share), dim3(256), TL_STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
+  else
+    hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, false>), dim3(8u * share), dim3(256), TL_STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
+  if (!GLU && slices > 1)
+    hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
+  return 0;
+}
+
+// Which kernel a product runs on.
+enum Kind { SKINNY, TILE, LARGE };
+Kind kind_of(int M, int N, int K, int dtype, bool glu, bool codes) {
+  if (M <= (glu ? 32 : 64)) return SKINNY;
+  if (codes) return LARGE;
+  if (dtype == FSTU_F32) return TILE;
+  const long long large = (long long)((M + 255) / 256) * ((N + (glu ? 127 : 255)) / (glu ? 128 : 256));
+  return large >= fstu_cus() / 2 ? LARGE : TILE;
+}
+// Offsets inside a tile are of 32 bits.
+bool near_rows(const Codes& X, const Codes& W, const Codes& U) { return std::max(X.ld, std::max(W.ld, U.ld)) < F8_MAX_LD; }
 
 }  // namespace
 
@@ -732,11 +1039,21 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
   FSTU_REQUIRE(fstu_aligned((c).p, 16) && (c).ld % 16 == 0 && (c).ld >= ((rows) > 1 ? K : 0), FSTU_EALIGN,                       \
                name ": rows of " what " must be 16-byte aligned, a multiple of 16 bytes apart and at least K=%d (stride %lld)", K, (long long)(c).ld)
 
-// Slices of K for a product of few rows (1: none).
-extern "C" int fstu_fp8_linear_slices(int M, int N, int K) {
-  if (M < 1 || M > 64 || N < 1 || K < 1) return 1;
-  const int tiles = (N + (M <= 16 ? 15 : 31)) / (M <= 16 ? 16 : 32), nb = (K + 127) / 128;
-  return std::max(1, std::min(256 / tiles, nb / 16));
+// Slices of K (1: none).
+extern "C" int fstu_fp8_linear_slices(int M, int N, int K, int dtype) {
+  if (M < 1 || N < 1 || K < 1 || (dtype != FSTU_F32 && dtype != FSTU_BF16)) return 1;
+  const int nb = (K + 127) / 128;
+  const Kind kind = kind_of(M, N, K, dtype, false, false);
+  if (kind == LARGE) return 1;
+  const int tiles = kind == SKINNY ? (N + (M <= 16 ? 15 : 31)) / (M <= 16 ? 16 : 32) : ((M + 127) / 128) * ((N + 127) / 128);
+  const double block = kind == TILE ? 0.4 : M <= 16 ? 0.034 : M <= 32 ? 0.073 : 0.143;
+  int best = 1;
+  double least = block * nb - 1.0;
+  for (int s = 2; s <= 16 && s * tiles <= fstu_cus() && s <= nb; s *= 2) {
+    const double t = block * nb / s + 2.2 + (double)s * M * N * 8 / 1.5e6;
+    if (t < least) least = t, best = s;
+  }
+  return best;
 }
 
 extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw,
@@ -748,26 +1065,23 @@ extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, i
   FP8_OPERAND("fstu_fp8_linear", X, M, "x");
   FP8_OPERAND("fstu_fp8_linear", W, N, "w");
   FSTU_REQUIRE(M == 1 || (ldy >= N && (!res || ldr >= N)), FSTU_ESHAPE, "fstu_fp8_linear: N=%d ldy=%lld ldr=%lld", N, (long long)ldy, (long long)ldr);
-  FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && M <= 64 && slices > 1 && slices <= (K + 127) / 128), FSTU_EARG, "fstu_fp8_linear: slices=%d (M=%d K=%d)", slices, M, K);
+  FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && slices > 1 && slices <= std::min(64, (K + 127) / 128) && near_rows(X, W, W)), FSTU_EARG,
+               "fstu_fp8_linear: slices=%d (K=%d, row strides %lld and %lld)", slices, K, (long long)ldx, (long long)ldw);
   const Leave o = {y, ldy, bias, res, ldr, nullptr, 0, 0};
-  if (M <= 64) {
-    int rc = 0;
-    FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_linear", {
-      rc = K % 128 ? skinny_linear<T, true>(X, W, o, partial, slices, M, N, K, (hipStream_t)stream)
-                   : skinny_linear<T, false>(X, W, o, partial, slices, M, N, K, (hipStream_t)stream);
-    });
-    if (rc) return rc;
-    FSTU_CHECK_LAUNCH("fstu_fp8_linear");
-    return FSTU_OK;
-  }
-  if (dtype == FSTU_BF16 && large_takes(X, W, W, M, N)) {
-    if (const int rc = large<0>(X, W, W, o, M, N, K, (hipStream_t)stream, "fstu_fp8_linear")) return rc;
-    FSTU_CHECK_LAUNCH("fstu_fp8_linear");
-    return FSTU_OK;
-  }
+  const Kind kind = kind_of(M, N, K, dtype, false, false);
+  hipStream_t const s = (hipStream_t)stream;
+  int rc = 0;
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_linear", {
-    hipLaunchKernelGGL((fp8_plain_kernel<false, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, (hipStream_t)stream, X, W, W, o, M, N, K);
+    if (kind == SKINNY)
+      rc = K % 128 ? skinny_linear<T, true>(X, W, o, partial, slices, M, N, K, s) : skinny_linear<T, false>(X, W, o, partial, slices, M, N, K, s);
+    else if (!near_rows(X, W, W))
+      hipLaunchKernelGGL((fp8_plain_kernel<false, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, s, X, W, W, o, M, N, K);
+    else if (kind == LARGE && slices == 1)
+      rc = large<0>(X, W, W, o, M, N, K, s, "fstu_fp8_linear");
+    else
+      rc = tile<T, false>(X, W, W, o, partial, slices, M, N, K, s, "fstu_fp8_linear");
   });
+  if (rc) return rc;
   FSTU_CHECK_LAUNCH("fstu_fp8_linear");
   return FSTU_OK;
 }
@@ -786,24 +1100,20 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
   FSTU_REQUIRE(!scales || (fstu_aligned(y, 16) && ldy % 16 == 0 && ldy >= N), FSTU_EALIGN,
                "fstu_fp8_glu: rows of codes must be 16-byte aligned, a multiple of 16 bytes apart and at least %d (stride %lld)", N, (long long)ldy);
   const Leave o = {y, ldy, nullptr, nullptr, 0, scales, ss, sb};
-  if (M <= 32) {
-    int rc = 0;
-    FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_glu", {
-      rc = K % 128 ? skinny_glu<T, true>(X, W, U, o, M, N, K, (hipStream_t)stream) : skinny_glu<T, false>(X, W, U, o, M, N, K, (hipStream_t)stream);
-    });
-    if (rc) return rc;
-    FSTU_CHECK_LAUNCH("fstu_fp8_glu");
-    return FSTU_OK;
-  }
-  if (dtype == FSTU_BF16 && large_takes(X, W, U, M, N)) {
-    if (const int rc = scales ? large<2>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")
-                              : large<1>(X, W, U, o, M, N, K, (hipStream_t)stream, "fstu_fp8_glu")) return rc;
-    FSTU_CHECK_LAUNCH("fstu_fp8_glu");
-    return FSTU_OK;
-  }
+  const Kind kind = kind_of(M, N, K, dtype, true, scales);
+  hipStream_t const s = (hipStream_t)stream;
+  int rc = 0;
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_glu", {
-    hipLaunchKernelGGL((fp8_plain_kernel<true, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, (hipStream_t)stream, X, W, U, o, M, N, K);
+    if (kind == SKINNY)
+      rc = K % 128 ? skinny_glu<T, true>(X, W, U, o, M, N, K, s) : skinny_glu<T, false>(X, W, U, o, M, N, K, s);
+    else if (!near_rows(X, W, U))
+      hipLaunchKernelGGL((fp8_plain_kernel<true, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, s, X, W, U, o, M, N, K);
+    else if (kind == LARGE)
+      rc = scales ? large<2>(X, W, U, o, M, N, K, s, "fstu_fp8_glu") : large<1>(X, W, U, o, M, N, K, s, "fstu_fp8_glu");
+    else
+      rc = tile<T, true>(X, W, U, o, nullptr, 1, M, N, K, s, "fstu_fp8_glu");
   });
+  if (rc) return rc;
   FSTU_CHECK_LAUNCH("fstu_fp8_glu");
   return FSTU_OK;
 }

@@ -126,7 +126,7 @@ SIGNATURES = {
     "fstu_fp8_rmsnorm": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp],
     "fstu_fp8_quantize_weight": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp],
     "fstu_fp8_linear": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp, _i, _vp],
-    "fstu_fp8_linear_slices": [_i, _i, _i],
+    "fstu_fp8_linear_slices": [_i, _i, _i, _i],
     "fstu_fp8_glu": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64,
                      _i, _i, _i, _i, _vp],
 }
@@ -1358,8 +1358,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
 
 
 @functools.lru_cache(maxsize=256)
-def _fp8_slices(M: int, N: int, K: int) -> int:
-    return load().fstu_fp8_linear_slices(M, N, K)
+def _fp8_slices(M: int, N: int, K: int, dt: int) -> int:
+    return load().fstu_fp8_linear_slices(M, N, K, dt)
 
 
 @_fp8_device
@@ -1388,7 +1388,7 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
         raise FlashSTUHipError(f"linear_fp8: bias must be ({N},) {dtype} on device {dev}, got {tuple(bias.shape)} {bias.dtype}")
     dt = _dt(out)
     if M:
-        slices = _fp8_slices(M, N, K)
+        slices = _fp8_slices(M, N, K, dt)
         partial = torch.empty(slices, M, N, dtype=torch.float32, device=codes.device) if slices > 1 else None
         _check(load().fstu_fp8_linear(*xa, *wa, _p(bias), _p(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(),
                                       out.stride(0), M, N, K, dt, _p(partial), slices, raw_stream(dev)), "fstu_fp8_linear")

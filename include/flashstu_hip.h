@@ -724,7 +724,7 @@ int fstu_fp8_rmsnorm(const void* x, int64_t ldx, const void* delta, int64_t ldd,
 int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw, const float* ws,
                     int64_t ws_row, int64_t ws_blk, const void* bias, const void* res, int64_t ldr, void* y, int64_t ldy, int M, int N, int K,
                     int dtype, float* partial, int slices, void* stream);
-int fstu_fp8_linear_slices(int M, int N, int K);
+int fstu_fp8_linear_slices(int M, int N, int K, int dtype);
 int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* gate, int64_t ldg, const float* gs,
                  int64_t gs_row, int64_t gs_blk, const uint8_t* up, int64_t ldu, const float* us, int64_t us_row, int64_t us_blk, void* y, int64_t ldy,
                  float* scales, int64_t s_row, int64_t s_blk, int M, int N, int K, int dtype, void* stream);

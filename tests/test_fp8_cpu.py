@@ -53,7 +53,7 @@ def test_product_entry_points_refuse(lib, mem):
     assert lin(M=0) == -3 and lin(N=0) == -3 and lin(K=0) == -3 and lin(ldy=7) == -3 and lin(r=p, ldr=7) == -3
     assert lin(x=p + 8) == -4 and lin(w=p + 4) == -4 and lin(ldx=136) == -4 and lin(ldw=112) == -4 and lin(ldx=112) == -4
     assert "16-byte" in why(lib) and lin(dt=9) == -2
-    assert lin(slices=0) == -5 and lin(slices=2, K=256, ldx=256, ldw=256) == -5 and lin(slices=2, part=p) == -5 and "slices=2" in why(lib)
+    assert lin(slices=0) == -5 and lin(slices=2, part=p + 4, K=256, ldx=256, ldw=256) == -5 and lin(slices=2, K=256, ldx=256, ldw=256) == -5 and lin(slices=2, part=p) == -5 and "slices=2" in why(lib)
 
     def glu(x=p, ldx=128, xs=p, g=p, ldg=128, gs=p, u=p, ldu=128, us=p, y=p, ldy=16, s=None, M=2, N=16, K=128, dt=1):
         return lib.fstu_fp8_glu(x, ldx, xs, 1, 2, g, ldg, gs, 1, 1, u, ldu, us, 1, 1, y, ldy, s, 1, 2, M, N, K, dt, None)

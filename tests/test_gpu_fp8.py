@@ -196,7 +196,7 @@ def test_rms_norm_in_place(fs):
 # ---------------------------------------------------------------- the products
 SHAPES = [(1, 1, 1), (1, 768, 9216), (2, 16, 128), (3, 100, 129), (15, 130, 256), (16, 2048, 512), (17, 129, 1000), (31, 64, 2500), (33, 300, 768),
           (64, 256, 384), (65, 100, 640), (100, 768, 1536), (129, 257, 130), (256, 256, 1024), (257, 513, 257), (300, 1001, 300), (700, 384, 2304),
-          (2, 3, 20000), (40, 130, 8192), (520, 770, 4096)]
+          (2, 3, 20000), (40, 130, 8192), (520, 770, 4096), (2100, 2064, 384), (1029, 3000, 200)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
