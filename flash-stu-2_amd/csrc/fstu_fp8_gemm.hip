@@ -244,8 +244,8 @@ __device__ __forceinline__ void add8(float (&v)[8], const bf16_t* p, int left) {
     if (e < left) v[e] += bf16_to_f32(p[e]);
 }
 
-// MODE 0 linear, 1 glu, 2 glu as codes.  TAIL: K is no multiple of 128; the last block comes straight from global memory behind the loop over
-// the whole ones (cutting its chunks inside the loop cost 100 spilled registers).
+// MODE 0 linear, 1 glu, 2 glu as codes.  K a multiple of 16; TAIL: not one of 128, the last block's chunks behind K are asked for behind the
+// range, where a fill finds zeros.
 template <int MODE, bool TAIL>
 __global__ void __launch_bounds__(512)
 fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt, int nt, int share) {
@@ -256,7 +256,7 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
   const int per_panel = mt * F8_PANEL, xcd = (int)(blockIdx.x & 7) * share, tiles = mt * nt;
   int idx = (int)(blockIdx.x >> 3);                    // this workgroup's next tile in its XCD's share
   if (idx >= share || xcd + idx >= tiles) return;
-  const int K16 = (K + 15) & ~15, nkt = K >> 7;
+  const int nkt = (K + 127) >> 7;
   int m0, n0;
   unsigned wbytes, ubytes, xbytes;
   const uint8_t *wb, *ub, *xb;
@@ -266,9 +266,9 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
     const int t = xcd + idx, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
     m0 = in_panel / pw * 256;
     n0 = (panel * F8_PANEL + in_panel % pw) * NF;
-    wbytes = (unsigned)(min(NF, N - n0) - 1) * (unsigned)W.ld + (unsigned)K16;
-    ubytes = GLU ? (unsigned)(min(NF, N - n0) - 1) * (unsigned)U.ld + (unsigned)K16 : wbytes;
-    xbytes = (unsigned)(min(256, M - m0) - 1) * (unsigned)X.ld + (unsigned)K16;
+    wbytes = (unsigned)(min(NF, N - n0) - 1) * (unsigned)W.ld + (unsigned)K;
+    ubytes = GLU ? (unsigned)(min(NF, N - n0) - 1) * (unsigned)U.ld + (unsigned)K : wbytes;
+    xbytes = (unsigned)(min(256, M - m0) - 1) * (unsigned)X.ld + (unsigned)K;
     wb = W.p + (size_t)n0 * W.ld;
     ub = GLU ? U.p + (size_t)n0 * U.ld : wb;
     xb = X.p + (size_t)m0 * X.ld;
@@ -279,6 +279,7 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
   const int wn = wv & 3, wm = wv >> 2;                 // 32-feature slice and 64-row slice of every half
   // ---- fills: a part is 128 rows x 128 bytes, a wave fills rows 16 wv .. + 15 of it with two instructions
   unsigned wvoff[2], uvoff[2], xvoff[2];
+  bool wthere[2], xthere[2];                           // whether this lane's chunk of the last block is one of K's
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int row = wv * 16 + j * 8 + (lane >> 3), feat = GLU ? row : (row & 31) + 2 * (row & 96);
@@ -286,25 +287,30 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
     wvoff[j] = (unsigned)feat * (unsigned)W.ld + wch;
     uvoff[j] = GLU ? (unsigned)feat * (unsigned)U.ld + wch : wvoff[j] + 32u * (unsigned)W.ld;
     xvoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
+    wthere[j] = (nkt - 1) * 128 + (int)wch < K;
+    xthere[j] = (nkt - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < K;
   }
   const unsigned x1off = 128u * (unsigned)X.ld;
   unsigned char* const fill0 = smem + (unsigned)wv * 2048u;
   // beyond the last block the descriptors are empty and the scales the last block's: into stages that nobody reads
+  const auto there = [&](int kt, int j, bool w, unsigned off) __attribute__((always_inline)) {
+    return TAIL && kt == nkt - 1 && !(w ? wthere[j] : xthere[j]) ? 0x80000000u : off;
+  };
   const auto fetch_w = [&](int kt, unsigned stage) __attribute__((always_inline)) {
     const bool in = kt < nkt;
     const rsrc_t rw = make_rsrc(wb, in ? wbytes : 0), ru = make_rsrc(ub, in ? ubytes : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(rw, wvoff[j], (unsigned)kt * 128u, fill0 + stage + j * 1024);
+    for (int j = 0; j < 2; ++j) fill16(rw, there(kt, j, true, wvoff[j]), (unsigned)kt * 128u, fill0 + stage + j * 1024);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(ru, uvoff[j], (unsigned)kt * 128u, fill0 + stage + F8_PART + j * 1024);
+    for (int j = 0; j < 2; ++j) fill16(ru, there(kt, j, true, uvoff[j]), (unsigned)kt * 128u, fill0 + stage + F8_PART + j * 1024);
   };
   const auto fetch_x = [&](int kt, unsigned stage, int h) __attribute__((always_inline)) {
     const rsrc_t rx = make_rsrc(xb, kt < nkt ? xbytes : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(rx, xvoff[j] + (h ? x1off : 0u), (unsigned)kt * 128u, fill0 + stage + (2 + h) * F8_PART + j * 1024);
+    for (int j = 0; j < 2; ++j) fill16(rx, there(kt, j, false, xvoff[j] + (h ? x1off : 0u)), (unsigned)kt * 128u, fill0 + stage + (2 + h) * F8_PART + j * 1024);
   };
   const auto fetch_s = [&](int kt, unsigned third) __attribute__((always_inline)) {
-    fill4(sp + (long long)max(min(kt, nkt - 1), 0) * sstep, smem + F8_SCALES + third + (unsigned)wv * 256u);
+    fill4(sp + (long long)min(kt, nkt - 1) * sstep, smem + F8_SCALES + third + (unsigned)wv * 256u);
   };
 
   const int l16 = lane & 15, lq = lane >> 4;
@@ -408,33 +414,6 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
     if (!wm) __builtin_amdgcn_s_barrier();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
     __builtin_amdgcn_s_barrier();
-    if constexpr (TAIL) {
-      const int k = nkt * 128 + lq * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int f = wn * (GLU ? 32 : 64) + 8 * (l16 >> 2) + (l16 & 3) + 4 * (i & 1) + (GLU ? 0 : 16 * (i & 2));
-        const uint8_t* const r = GLU && i >= 2 ? ub + (size_t)min(f, N - 1 - n0) * U.ld : wb + (size_t)min(f, N - 1 - n0) * W.ld;
-        wa[i] = Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)};
-      }
-      const int b = n0 >> 7;
-      sw = W.s[(GLU ? b : min(b + (wn >> 1), (N - 1) >> 7)) * W.sr + nkt * W.sb];
-      if constexpr (GLU) su = U.s[b * U.sr + nkt * U.sb];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = min(m0 + h * 128 + wm * 64 + j * 16 + l16, M - 1);
-          const uint8_t* const r = xb + (size_t)(m - m0) * X.ld;
-          const Operand<bf16_t> x(Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)});
-          const float s = X.s[m * X.sr + nkt * X.sb];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const floatx4_t d = Operand<bf16_t>::sum(Operand<bf16_t>(wa[i]), x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][h][j][e] = fmaf(d[e], s * (GLU && i >= 2 ? su : sw), acc[i][h][j][e]);
-          }
-        }
-    }
     // every wave has left the stages: the next tile's first blocks are on their way while this one is stored
     const int em0 = m0, en0 = n0;
     idx += (int)(gridDim.x >> 3);
@@ -532,8 +511,10 @@ int large(const Codes& X, const Codes& W, const Codes& U, const Leave& o, int M,
 // flight at once in registers, and the KH waves of a feature tile join their sums in LDS.  A load is 8 rows of 128 bytes, whole lines;
 // the fragments, 16 rows of 64 bytes, are taken through 2 KB of LDS that the wave has for itself (read straight as fragments, half a line to a row,
 // one compute unit gets half as much: 768 x 9216 bytes over 48 of them 5.5 us, 2.9 so).  A workgroup has NT feature tiles, F of them to
-// a wave; K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
-template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
+// a wave; K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.  A wave keeps P sums, of
+// every P-th of its blocks: the pair's sums are those of every fourth block whether four waves form them or two, so that its codes are
+// those of its bf16 result to the bit.
+template <typename T, int MODE, int R, int F, int NT, int KH, int P, int U, bool TAIL>
 __global__ void __launch_bounds__(64 * NT * KH)
 fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partial, int M, int N, int K, int slices) {
   constexpr bool GLU = MODE != 0;
@@ -541,8 +522,9 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
   static_assert(!GLU || F == 2, "gate and up");
   static_assert(R * FT <= KH, "one wave joins one tile's sums");
   static_assert(MODE != 2 || NT == 8, "the block of 128 features that shares a scale");
+  static_assert(U % P == 0 && (!GLU || KH * P == 4), "sums by block");
   extern __shared__ __align__(16) unsigned char skinny_smem[];
-  float* const red = (float*)skinny_smem;              // behind the loop: [KH][NT][G][64 lanes][4]
+  float* const red = (float*)skinny_smem;              // behind the loop: [P][KH][NT][G][64 lanes][4]
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, q = lane >> 4;
   const int nt = wv % NT, kh = wv / NT;
   const int n0 = ((int)blockIdx.x * NT + nt) * 16 * FT, m0 = (int)blockIdx.z * 16 * R;
@@ -565,9 +547,9 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
   }
   const int nb = (K + 127) >> 7, s = (int)blockIdx.y;
   const int b0 = (int)((unsigned)(nb * s) / (unsigned)slices), b1 = (int)((unsigned)(nb * (s + 1)) / (unsigned)slices);
-  floatx4_t acc[F][R];
+  floatx4_t acc[P][F][R];
 #pragma unroll
-  for (int i = 0; i < G; ++i) acc[i / R][i % R] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < P * G; ++i) acc[i / G][i % G / R][i % R] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   const auto chunk = [&](const uint8_t* p, int k) __attribute__((always_inline)) { return TAIL ? chunk16(p, k, K) : *(const u32x4_t*)(p + k); };
   const bool both = R > 1 || M - m0 > 8;               // rows 8 .. 15 of the only row tile (what lies in LDS for them reaches nobody else's sum)
   // the chunk index is XOR-ed with bits of the row: neither the lines' writes nor the fragments' reads meet bank conflicts
@@ -616,7 +598,7 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
           for (int f = 0; f < F; ++f) {
             const floatx4_t d = Operand<T>::sum(fragment(f), xo);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[f][r][e] = fmaf(d[e], sx[u][r] * sw[u][f], acc[f][r][e]);
+            for (int e = 0; e < 4; ++e) acc[u % P][f][r][e] = fmaf(d[e], sx[u][r] * sw[u][f], acc[u % P][f][r][e]);
           }
         }
         asm volatile("" ::: "memory");
@@ -626,14 +608,14 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
   // the sums of a tile, by the wave whose kh is its number
   floatx4_t* const mine = (floatx4_t*)red + ((size_t)(kh * NT + nt) * G) * 64 + lane;
 #pragma unroll
-  for (int i = 0; i < G; ++i) mine[i * 64] = acc[i / R][i % R];
+  for (int i = 0; i < P * G; ++i) mine[((size_t)(i / G) * KH * NT * G + i % G) * 64] = acc[i / G][i % G / R][i % R];
   __syncthreads();
   const bool joins = kh < R * FT;
   const int r = kh % R, f = kh / R;                    // this wave's row tile and, linear, feature tile
   floatx4_t v = {0.f, 0.f, 0.f, 0.f}, w2 = v;
   if (joins) {
 #pragma unroll
-    for (int k = 0; k < KH; ++k) {
+    for (int k = 0; k < KH * P; ++k) {
       const floatx4_t* const p = (const floatx4_t*)red + ((size_t)(k * NT + nt) * G) * 64 + lane;
       v += p[(f * R + r) * 64];
       if constexpr (GLU) w2 += p[(R + r) * 64];
@@ -698,14 +680,14 @@ fp8_join_kernel(const float* __restrict__ partial, Leave o, int M, int N, int sl
   DT<T>::st((T*)o.y + (size_t)m * o.ldy + f, v);
 }
 
-template <typename T, int MODE, int R, int F, int NT, int KH, int U, bool TAIL>
+template <typename T, int MODE, int R, int F, int NT, int KH, int P, int U, bool TAIL>
 int skinny_launch(const Codes& X, const Codes& W, const Codes& V, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
                   const char* name) {
   constexpr int NF = 16 * NT * (MODE ? 1 : F);
-  constexpr unsigned lds = KH * NT * std::max(F * R * 1024, (F + R) * 2048);
+  constexpr unsigned lds = KH * NT * std::max(P * F * R * 1024, (F + R) * 2048);
   static fstu_lds_limit most;
-  if (const int rc = fstu_need_lds((const void*)fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>, most, lds, name)) return rc;
-  hipLaunchKernelGGL((fp8_skinny_kernel<T, MODE, R, F, NT, KH, U, TAIL>), dim3((N + NF - 1) / NF, slices, (M + 16 * R - 1) / (16 * R)), dim3(64 * NT * KH),
+  if (const int rc = fstu_need_lds((const void*)fp8_skinny_kernel<T, MODE, R, F, NT, KH, P, U, TAIL>, most, lds, name)) return rc;
+  hipLaunchKernelGGL((fp8_skinny_kernel<T, MODE, R, F, NT, KH, P, U, TAIL>), dim3((N + NF - 1) / NF, slices, (M + 16 * R - 1) / (16 * R)), dim3(64 * NT * KH),
                      lds, s, X, W, V, o, partial, M, N, K, slices);
   if (MODE == 0 && slices > 1)
     hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
@@ -714,35 +696,36 @@ int skinny_launch(const Codes& X, const Codes& W, const Codes& V, const Leave& o
 template <typename T, bool TAIL>
 int skinny_linear(const Codes& X, const Codes& W, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s) {
   const char* const name = "fstu_fp8_linear";
-  if (M <= 16) return skinny_launch<T, 0, 1, 1, 1, 16, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
-  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 1, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
-  return skinny_launch<T, 0, 4, 2, 1, 8, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  if (M <= 16) return skinny_launch<T, 0, 1, 1, 1, 16, 1, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 1, 1, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  return skinny_launch<T, 0, 4, 2, 1, 8, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
 }
 template <typename T, bool TAIL>
 int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, int M, int N, int K, hipStream_t s) {
   const char* const name = "fstu_fp8_glu";
   if constexpr (std::is_same<T, bf16_t>::value) {
     if (o.s) {
-      if (M <= 16) return skinny_launch<T, 2, 1, 2, 8, 2, 3, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
-      return skinny_launch<T, 2, 2, 2, 8, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+      if (M <= 16) return skinny_launch<T, 2, 1, 2, 8, 2, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+      return skinny_launch<T, 2, 2, 2, 8, 2, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
     }
   }
-  // us, 8 / 32 rows: 9216 x 768 two tiles of four waves 4.2 / 5.5, one of four 4.3 / 5.0, one of eight 5.0 / 6.4; 24576 x 2048 19 / 18.6, 18.8 /
-  // 19.1, 17.6 / 19.7
-  if (M <= 16) return K > 1536 ? skinny_launch<T, 1, 1, 2, 1, 8, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name)
-                               : skinny_launch<T, 1, 1, 2, 2, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
-  return skinny_launch<T, 1, 2, 2, 1, 4, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+  // us, 8 / 32 rows: 9216 x 768 two tiles of four waves 4.2 / 5.5, one 4.3 / 5.0
+  if (M <= 16) return skinny_launch<T, 1, 1, 2, 2, 4, 1, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
+  return skinny_launch<T, 1, 2, 2, 1, 4, 1, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
 }
 
 // ---------------------------------------------------------------- 128 x 128 tiles
 // Products of too few 256 x 256 tiles, and those whose results are fp32.  Four waves, each 64 features (glu: 32 of the gate and 32 of the
-// up weight) x 64 rows; K in blocks of 128 through four LDS stages.  One wave to a SIMD, so it does everything at once:
+// up weight) x 64 rows; K in blocks of 128 through STAGES LDS stages: two, and two workgroups to a compute unit, which cover each other's
+// waits and ends (fp32: the widening of one's codes runs beside the other's products: 8192 x 2048 x 24576 849 us with four, 707 so;
+// 4096 x 2048 x 2048 bf16 30 / 24), or four where there is no second one (4096 x 768 x 9216 51 with two, 40 so).  One wave to a SIMD
+// and workgroup, so it does everything at once:
 //   wait for the fragments of kt (this wave has left stage kt) and for its share of block kt + 1; barrier; multiply the fragments of kt and,
-//   an instruction or two behind each product, request block kt + 4 into stage kt and read the fragments of kt + 1
-// (all requests, then all reads, then the products: 0.75 us a block, since a wave issues in order and the queues of both are short).
+//   an instruction or two behind each product, request block kt + STAGES into stage kt and read the fragments of kt + 1
+// (all requests, then all reads, then the products: 0.75 us a block of the four-stage form, since a wave issues in order and the queues of
+// both are short; 0.46 to 0.5 so, of which the products are 0.25).
 // K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
 #define TL_STAGE 33792u                           // W | X | scales: by wave those of 32 rows, then the two weights'
-#define TL_STAGES 4
 #define TL_FILLS 9
 
 template <typename T> struct Put;
@@ -780,7 +763,9 @@ __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...
   (step(std::integral_constant<int, I>{}), ...);
 }
 
-template <typename T, bool GLU, bool TAIL>
+// TAIL: 1 K is no multiple of 128 (chunks behind K are asked for behind the range, where a fill finds zeros), 2 nor one of 16 (the chunk with the
+// row's end is cut in LDS by the lane that has filled it)
+template <typename T, bool GLU, int TAIL, int STAGES>
 __global__ void __launch_bounds__(256, 2)
 fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial, int M, int N, int K, int mt, int nt, int share, int slices) {
   constexpr int NF = GLU ? 64 : 128;
@@ -792,8 +777,8 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   t -= slice * (mt * nt);
   const int per_panel = mt * F8_PANEL, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
   const int m0 = in_panel / pw * 128, n0 = (panel * F8_PANEL + in_panel % pw) * NF;
-  const int nb = (K + 127) >> 7, whole = K >> 7, K16 = (K + 15) & ~15;
-  const int b0 = (int)((unsigned)(nb * slice) / (unsigned)slices), b1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices), e1 = TAIL ? min(b1, whole) : b1;
+  const int nb = (K + 127) >> 7, K16 = (K + 15) & ~15;
+  const int b0 = (int)((unsigned)(nb * slice) / (unsigned)slices), e1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices);
   const uint8_t* const wb = W.p + (size_t)n0 * W.ld;
   const uint8_t* const ub = GLU ? U.p + (size_t)n0 * U.ld : wb;
   const uint8_t* const xb = X.p + (size_t)m0 * X.ld;
@@ -805,20 +790,25 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   const long long sstep = lane < 32 ? X.sb : GLU && (lane & 1) ? U.sb : W.sb;
   // ---- fills: a wave fills rows 32 wv .. + 31 of either part with four instructions (glu: waves 0 and 1 the gate's, 2 and 3 the up weight's)
   unsigned woff[4], xoff[4];
+  bool wthere[4], xthere[4];                           // whether this lane's chunk of the last block is one of K's
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int row = wv * 32 + j * 8 + (lane >> 3);
     woff[j] = (unsigned)(GLU ? row & 63 : row) * (unsigned)(GLU && wv >= 2 ? U.ld : W.ld) + (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
     xoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
+    wthere[j] = (nb - 1) * 128 + ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16 < K;
+    xthere[j] = (nb - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < K;
   }
   unsigned char* const fill0 = smem + (unsigned)wv * 4096u;
-  const auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {   // beyond the last whole block nothing, into a stage that nobody reads
+  const auto w_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !wthere[j] ? 0x80000000u : woff[j]; };
+  const auto x_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !xthere[j] ? 0x80000000u : xoff[j]; };
+  const auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {   // beyond the last block nothing, into a stage that nobody reads
     const bool in = b < e1;
     const rsrc_t rw = make_rsrc(GLU && wv >= 2 ? ub : wb, in ? (GLU && wv >= 2 ? ubytes : wbytes) : 0), rx = make_rsrc(xb, in ? xbytes : 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fill16(rw, woff[j], (unsigned)b * 128u, fill0 + stage + j * 1024);
+    for (int j = 0; j < 4; ++j) fill16(rw, w_at(b, j), (unsigned)b * 128u, fill0 + stage + j * 1024);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fill16(rx, xoff[j], (unsigned)b * 128u, fill0 + stage + 16384 + j * 1024);
+    for (int j = 0; j < 4; ++j) fill16(rx, x_at(b, j), (unsigned)b * 128u, fill0 + stage + 16384 + j * 1024);
     fill4(sp + (long long)min(b, e1 - 1) * sstep, smem + stage + 32768 + (unsigned)wv * 256u);
   };
   const int l16 = lane & 15, lq = lane >> 4, wn = wv & 1, wm = wv >> 1;
@@ -850,13 +840,30 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     if constexpr (I == 5) f.su = GLU ? lds4<4>(fsw + stage) : 0.f;
   };
   const auto each16 = [](auto&& step) __attribute__((always_inline)) { steps16(step, std::make_integer_sequence<int, 16>{}); };
-  const auto wait = [&](Set& f) __attribute__((always_inline)) {
+  const auto cut = [&](unsigned stage) __attribute__((always_inline)) {      // block nb - 1 in that stage: what lies behind a row's end is not its own
+    int own = lane;                                    // what follows is formed here: kept over the loop it would cost registers
+    asm volatile("" : "+v"(own));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = wv * 32 + (j & 3) * 8 + (own >> 3);
+      const int ch = (own & 7) ^ (j < 4 ? ((row >> 1) & 1) | ((row >> 2) & 6) : (row >> 1) & 7);
+      const unsigned at = lds_addr(fill0) + stage + (unsigned)((j >> 2) * 16384 + (j & 3) * 1024 + own * 16);
+      u32x4_t v = lds16<0>(at);
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v)::"memory");
+      v = cut16(v, K - (nb - 1) * 128 - ch * 16);
+      asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  // the fragments f of block kt have come; this wave's share of block kt + 1 (in stage nxt) has landed
+  const auto wait = [&](Set& f, int kt, unsigned nxt) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(%22) lgkmcnt(0)"
                  : "+v"(f.w[0].lo), "+v"(f.w[0].hi), "+v"(f.w[1].lo), "+v"(f.w[1].hi), "+v"(f.w[2].lo), "+v"(f.w[2].hi), "+v"(f.w[3].lo), "+v"(f.w[3].hi),
                    "+v"(f.x[0].lo), "+v"(f.x[0].hi), "+v"(f.x[1].lo), "+v"(f.x[1].hi), "+v"(f.x[2].lo), "+v"(f.x[2].hi), "+v"(f.x[3].lo), "+v"(f.x[3].hi),
                    "+v"(f.sx[0]), "+v"(f.sx[1]), "+v"(f.sx[2]), "+v"(f.sx[3]), "+v"(f.sw), "+v"(f.su)
-                 : "n"(TL_FILLS * (TL_STAGES - 2))
+                 : "n"(TL_FILLS * (STAGES - 2))
                  : "memory");
+    if (TAIL == 2 && kt + 1 == nb - 1) cut(nxt);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -865,9 +872,9 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  // multiplies block f; behind its products block kt + TL_STAGES is requested into stage cur and block kt + 1 is read from stage nxt into g
+  // multiplies block f; behind its products block kt + STAGES is requested into stage cur and block kt + 1 is read from stage nxt into g
   const auto multiply = [&](Set& f, Set& g, int kt, unsigned cur, unsigned nxt) __attribute__((always_inline)) {
-    const bool in = kt + TL_STAGES < e1;
+    const bool in = kt + STAGES < e1;
     const rsrc_t rw = make_rsrc(GLU && wv >= 2 ? ub : wb, in ? (GLU && wv >= 2 ? ubytes : wbytes) : 0), rx = make_rsrc(xb, in ? xbytes : 0);
     float s[4], u[4];
 #pragma unroll
@@ -875,10 +882,10 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     const auto request = [&](auto which) __attribute__((always_inline)) {
       constexpr int I = decltype(which)::value;
       if constexpr (I < 8) {
-        if constexpr (I & 1) fill16(rx, xoff[I >> 1], (unsigned)(kt + TL_STAGES) * 128u, fill0 + cur + 16384 + (I >> 1) * 1024);
-        else fill16(rw, woff[I >> 1], (unsigned)(kt + TL_STAGES) * 128u, fill0 + cur + (I >> 1) * 1024);
+        if constexpr (I & 1) fill16(rx, x_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + 16384 + (I >> 1) * 1024);
+        else fill16(rw, w_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + (I >> 1) * 1024);
       }
-      if constexpr (I == 8) fill4(sp + (long long)min(kt + TL_STAGES, e1 - 1) * sstep, smem + cur + 32768 + (unsigned)wv * 256u);
+      if constexpr (I == 8) fill4(sp + (long long)min(kt + STAGES, e1 - 1) * sstep, smem + cur + 32768 + (unsigned)wv * 256u);
     };
     if constexpr (std::is_same<T, float>::value) {
       // widened fragments: x's at once, w's one after the other, so that what comes for the next block takes the place of what has been widened
@@ -921,55 +928,30 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (b0 < e1) {
+  {
 #pragma unroll
-    for (int i = 0; i < TL_STAGES; ++i) fetch(b0 + i, i * TL_STAGE);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TL_FILLS * (TL_STAGES - 1)) : "memory");
+    for (int i = 0; i < STAGES; ++i) fetch(b0 + i, i * TL_STAGE);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TL_FILLS * (STAGES - 1)) : "memory");
+    if (TAIL == 2 && b0 == nb - 1) cut(0);
     __builtin_amdgcn_s_barrier();
     each16([&](auto which) __attribute__((always_inline)) { read_one(a, 0, which); });
     unsigned cur = 0;                                  // the stage of block kt
-    const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (TL_STAGES - 1) * TL_STAGE ? 0u : st + TL_STAGE; };
+    const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (STAGES - 1) * TL_STAGE ? 0u : st + TL_STAGE; };
     // blocks in pairs; behind an odd number comes one of zeros (what a fill finds behind the range), whose scales are the last block's: where
     // they are not finite, neither is the sum any more
     for (int kt = b0; kt < e1; kt += 2) {
       unsigned nxt = next(cur);
-      wait(a);
+      wait(a, kt, nxt);
       multiply(a, b, kt, cur, nxt);
       cur = nxt, nxt = next(cur);
-      wait(b);
+      wait(b, kt + 1, nxt);
       multiply(b, a, kt + 1, cur, nxt);
       cur = nxt;
     }
-    wait(a);                                           // the last reads, of a block that is not there, have to have come in
+    wait(a, nb, 0);                                      // the last reads, of a block that is not there, have to have come in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
   }
   const int fe = n0 + wn * (GLU ? 32 : 64) + 8 * lq;   // this lane's features: 8 of each pair of tiles
-  if constexpr (TAIL) {
-    if (b1 == nb) {                                    // what a whole block does not hold, straight from global memory
-      const int k = whole * 128 + lq * 16;
-      Frag32 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int f = wn * (GLU ? 32 : 64) + 8 * (l16 >> 2) + (l16 & 3) + 4 * (i & 1) + (GLU ? 0 : 16 * (i & 2));
-        const uint8_t* const r = (GLU && i >= 2 ? ub : wb) + (size_t)min(f, N - 1 - n0) * (GLU && i >= 2 ? U.ld : W.ld);
-        w[i] = Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)};
-      }
-      const float sw = W.s[(n0 >> 7) * W.sr + whole * W.sb], su = GLU ? U.s[(n0 >> 7) * U.sr + whole * U.sb] : 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = min(m0 + wm * 64 + j * 16 + l16, M - 1);
-        const uint8_t* const r = xb + (size_t)(m - m0) * X.ld;
-        const Operand<T> x(Frag32{chunk16(r, k, K), chunk16(r, k + 64, K)});
-        const float sx = X.s[m * X.sr + whole * X.sb];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const floatx4_t d = Operand<T>::sum(Operand<T>(w[i]), x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], sx * (GLU && i >= 2 ? su : sw), acc[i][j][e]);
-        }
-      }
-    }
-  }
   // whole: all of the tile's features are there (the other form's branches are many, and a launch fetches its code anew)
   const auto leave = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool ALL = decltype(whole)::value;
@@ -1001,33 +983,86 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   else leave(std::false_type{});
 }
 
-template <typename T, bool GLU>
-int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s, const char* name) {
-  constexpr int NF = GLU ? 64 : 128;
-  static fstu_lds_limit most[2];
-  const bool tail = K % 128;
-  const void* const kernel = tail ? (const void*)fp8_tile_kernel<T, GLU, true> : (const void*)fp8_tile_kernel<T, GLU, false>;
-  if (const int rc = fstu_need_lds(kernel, most[tail], TL_STAGES * TL_STAGE, name)) return rc;
-  const int mt = (M + 127) / 128, nt = (N + NF - 1) / NF;
-  const long long tiles = (long long)mt * nt * slices;
-  const int share = (int)((tiles + 7) / 8);
-  if (tail)
-    hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, true>), dim3(8u * share), dim3(256), TL_STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
-  else
-    hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, false>), dim3(8u * share), dim3(256), TL_STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
-  if (!GLU && slices > 1)
-    hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
+template <typename T, bool GLU, int TAIL, int STAGES>
+int tile_launch(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
+                const char* name) {
+  static fstu_lds_limit most;
+  if (const int rc = fstu_need_lds((const void*)fp8_tile_kernel<T, GLU, TAIL, STAGES>, most, STAGES * TL_STAGE, name)) return rc;
+  const int mt = (M + 127) / 128, nt = (N + (GLU ? 63 : 127)) / (GLU ? 64 : 128);
+  const int share = (int)(((long long)mt * nt * slices + 7) / 8);
+  hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, TAIL, STAGES>), dim3(8u * share), dim3(256), STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
   return 0;
 }
+template <typename T, bool GLU>
+int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s, const char* name) {
+  const long long tiles = (long long)((M + 127) / 128) * ((N + (GLU ? 63 : 127)) / (GLU ? 64 : 128)) * slices;
+  const int tail = K % 16 ? 2 : K % 128 ? 1 : 0;
+  const auto run = [&](auto t) {
+    constexpr int TAIL = decltype(t)::value;
+    if constexpr (sizeof(T) == 2)
+      if (tiles <= fstu_cus()) return tile_launch<T, GLU, TAIL, 4>(X, W, U, o, partial, slices, M, N, K, s, name);
+    return tile_launch<T, GLU, TAIL, 2>(X, W, U, o, partial, slices, M, N, K, s, name);
+  };
+  const int rc = tail == 2 ? run(std::integral_constant<int, 2>{}) : tail ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 0>{});
+  if (!rc && !GLU && slices > 1)
+    hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
+  return rc;
+}
 
-// Which kernel a product runs on.
+// Which kernel a product runs on, and in how many slices of K: the least of an estimate in us, fitted to 330 products of 40 to 8192 rows, 128 to
+// 24576 features and K = 256 to 24576, which is within a tenth of the best nearly everywhere.  SKINNY and TILE are priced by rounds of
+// workgroups over the compute units, each with a start and an end of its own, a block of K the dearer the more of the chip is at work.
+// us, skinny / tile / large.  Linear, rows x features x K: 500 x 768 x 768 5.3 / 8.3 / 15.7, 3000 14 / 8.8 / 16; 200 x 2048 x 2048 6.9 / 12.8 / 26,
+// 800 23 / 13 / 26, 4096 - / 24 / 29, 8192 - / 44 / 38; 500 x 768 x 9216 16 / 39 / 87, 2000 46 / 40 / 87, 8192 - / 65 / 88; fp32 500 x 768 x
+// 768 5.7 / 12.4, 2000 15 / 13.  Gated pair: 64 x 9216 x 768 7.4 / 6.8 / 10.5, 300 26 / 9.5 / 13.4, 500 - / 15.2 / 14.4, 1200 - / 26.8 / 27, 4096 - / 79
+// / 69; 2000 x 24576 x 2048 - / 217 / 175.
 enum Kind { SKINNY, TILE, LARGE };
-Kind kind_of(int M, int N, int K, int dtype, bool glu, bool codes) {
-  if (M <= (glu ? 32 : 64)) return SKINNY;
-  if (codes) return LARGE;
-  if (dtype == FSTU_F32) return TILE;
-  const long long large = (long long)((M + 255) / 256) * ((N + (glu ? 127 : 255)) / (glu ? 128 : 256));
-  return large >= fstu_cus() / 2 ? LARGE : TILE;
+struct Plan { Kind kind; int slices; double us; };
+double estimate(Kind kind, int slices, int M, int N, int K, bool f32, bool glu) {
+  const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+  const long long nb = up(up(K, 128), slices), cus = fstu_cus();
+  double us = slices > 1 ? 2.2 + (double)slices * M * N * 8 / 3e6 : 0.0;
+  if (kind == SKINNY) {
+    const int wide = M <= 16 ? 0 : M <= 32 ? 1 : 2;
+    static const double start[3] = {2.1, 2.8, 3.5}, block[2][3] = {{0.034, 0.073, 0.15}, {0.04, 0.09, 0.2}};
+    const long long groups = up(N, wide ? 32 : 16) * up(M, 16 << wide) * slices;
+    return us + 1.0 + (double)up(groups, cus) * (start[wide] + block[f32][wide] * nb) + (double)N * K * 6e-8;
+  }
+  if (kind == TILE) {
+    const long long tiles = up(N, glu ? 64 : 128) * up(M, 128) * slices;
+    if (tiles <= cus) return us + (f32 ? 5.0 + 1.03 * nb : 4.5 + 0.45 * nb);
+    const long long rest = tiles % (2 * cus);
+    const double rounds = (double)(tiles / (2 * cus)) + (rest == 0 ? 0.0 : rest <= cus ? 0.75 : 1.0);
+    return us + 2.0 + rounds * (glu ? (f32 ? 4.0 + 1.73 * nb : 3.0 + 0.94 * nb) : f32 ? 10.0 + 1.73 * nb : 6.5 + 0.94 * nb);
+  }
+  const long long tiles = up(N, glu ? 128 : 256) * up(M, 256);
+  if (glu) return 1.0 + (double)up(tiles, cus) * (5.5 + 1.35 * nb);
+  return 5.0 + (double)up(tiles, cus) * (2.5 + (1.1 + 0.5 * std::min(1.0, (double)tiles / cus)) * nb);
+}
+// slices: 0 as many as pay, otherwise that many
+Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {
+  const bool few = M <= (glu ? 32 : 64), big = !f32 && K % 16 == 0;
+  if (codes) return {few ? SKINNY : LARGE, 1, 0.0};
+  if (glu && few) return {SKINNY, 1, 0.0};
+  // the pair of more rows adds its blocks in one order on all kernels, so that its codes are those of its bf16 result
+  Plan best = {TILE, 1, estimate(TILE, 1, M, N, K, f32, glu)};
+  if (!glu) best = {SKINNY, std::max(slices, 1), estimate(SKINNY, std::max(slices, 1), M, N, K, f32, glu)};
+  const auto take = [&](Kind kind, int s) {
+    // a slice's second launch and sums cost a caller's host what a short call takes as well: they have to gain a microsecond
+    const double us = estimate(kind, s, M, N, K, f32, glu) + (slices == 0 && s > 1 ? 1.0 : 0.0);
+    if (us < best.us) best = {kind, s, us};
+  };
+  const int nb = (K + 127) / 128;
+  static const int counts[] = {2, 3, 4, 6, 8, 12, 16};
+  if (slices <= 1 && big && !few) take(LARGE, 1);
+  if (!few) take(TILE, std::max(slices, 1));
+  if (slices == 0 && !glu)
+    for (const int s : counts) {
+      if (s > nb) break;
+      take(SKINNY, s);
+      if (!few) take(TILE, s);
+    }
+  return best;
 }
 // Offsets inside a tile are of 32 bits.
 bool near_rows(const Codes& X, const Codes& W, const Codes& U) { return std::max(X.ld, std::max(W.ld, U.ld)) < F8_MAX_LD; }
@@ -1042,18 +1077,7 @@ bool near_rows(const Codes& X, const Codes& W, const Codes& U) { return std::max
 // Slices of K (1: none).
 extern "C" int fstu_fp8_linear_slices(int M, int N, int K, int dtype) {
   if (M < 1 || N < 1 || K < 1 || (dtype != FSTU_F32 && dtype != FSTU_BF16)) return 1;
-  const int nb = (K + 127) / 128;
-  const Kind kind = kind_of(M, N, K, dtype, false, false);
-  if (kind == LARGE) return 1;
-  const int tiles = kind == SKINNY ? (N + (M <= 16 ? 15 : 31)) / (M <= 16 ? 16 : 32) : ((M + 127) / 128) * ((N + 127) / 128);
-  const double block = kind == TILE ? 0.4 : M <= 16 ? 0.034 : M <= 32 ? 0.073 : 0.143;
-  int best = 1;
-  double least = block * nb - 1.0;
-  for (int s = 2; s <= 16 && s * tiles <= fstu_cus() && s <= nb; s *= 2) {
-    const double t = block * nb / s + 2.2 + (double)s * M * N * 8 / 1.5e6;
-    if (t < least) least = t, best = s;
-  }
-  return best;
+  return plan(M, N, K, dtype == FSTU_F32, false, false, 0).slices;
 }
 
 extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_blk, const uint8_t* w, int64_t ldw,
@@ -1068,15 +1092,15 @@ extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, i
   FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && slices > 1 && slices <= std::min(64, (K + 127) / 128) && near_rows(X, W, W)), FSTU_EARG,
                "fstu_fp8_linear: slices=%d (K=%d, row strides %lld and %lld)", slices, K, (long long)ldx, (long long)ldw);
   const Leave o = {y, ldy, bias, res, ldr, nullptr, 0, 0};
-  const Kind kind = kind_of(M, N, K, dtype, false, false);
+  const Kind kind = plan(M, N, K, dtype == FSTU_F32, false, false, slices).kind;
   hipStream_t const s = (hipStream_t)stream;
   int rc = 0;
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_linear", {
     if (kind == SKINNY)
       rc = K % 128 ? skinny_linear<T, true>(X, W, o, partial, slices, M, N, K, s) : skinny_linear<T, false>(X, W, o, partial, slices, M, N, K, s);
-    else if (!near_rows(X, W, W))
+    else if (!near_rows(X, W, W) && slices == 1)
       hipLaunchKernelGGL((fp8_plain_kernel<false, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, s, X, W, W, o, M, N, K);
-    else if (kind == LARGE && slices == 1)
+    else if (kind == LARGE)
       rc = large<0>(X, W, W, o, M, N, K, s, "fstu_fp8_linear");
     else
       rc = tile<T, false>(X, W, W, o, partial, slices, M, N, K, s, "fstu_fp8_linear");
@@ -1100,13 +1124,13 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
   FSTU_REQUIRE(!scales || (fstu_aligned(y, 16) && ldy % 16 == 0 && ldy >= N), FSTU_EALIGN,
                "fstu_fp8_glu: rows of codes must be 16-byte aligned, a multiple of 16 bytes apart and at least %d (stride %lld)", N, (long long)ldy);
   const Leave o = {y, ldy, nullptr, nullptr, 0, scales, ss, sb};
-  const Kind kind = kind_of(M, N, K, dtype, true, scales);
+  const Kind kind = plan(M, N, K, dtype == FSTU_F32, true, scales, 1).kind;
   hipStream_t const s = (hipStream_t)stream;
   int rc = 0;
   FSTU_DISPATCH_DTYPE(dtype, "fstu_fp8_glu", {
     if (kind == SKINNY)
       rc = K % 128 ? skinny_glu<T, true>(X, W, U, o, M, N, K, s) : skinny_glu<T, false>(X, W, U, o, M, N, K, s);
-    else if (!near_rows(X, W, U))
+    else if (!near_rows(X, W, U) || (scales && K % 16))
       hipLaunchKernelGGL((fp8_plain_kernel<true, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, s, X, W, U, o, M, N, K);
     else if (kind == LARGE)
       rc = scales ? large<2>(X, W, U, o, M, N, K, s, "fstu_fp8_glu") : large<1>(X, W, U, o, M, N, K, s, "fstu_fp8_glu");

@@ -196,7 +196,7 @@ def test_rms_norm_in_place(fs):
 # ---------------------------------------------------------------- the products
 SHAPES = [(1, 1, 1), (1, 768, 9216), (2, 16, 128), (3, 100, 129), (15, 130, 256), (16, 2048, 512), (17, 129, 1000), (31, 64, 2500), (33, 300, 768),
           (64, 256, 384), (65, 100, 640), (100, 768, 1536), (129, 257, 130), (256, 256, 1024), (257, 513, 257), (300, 1001, 300), (700, 384, 2304),
-          (2, 3, 20000), (40, 130, 8192), (520, 770, 4096), (2100, 2064, 384), (1029, 3000, 200)]
+          (2, 3, 20000), (40, 130, 8192), (520, 770, 4096), (2100, 2064, 384), (1029, 3000, 200), (300, 640, 144), (270, 300, 2064), (1100, 4100, 401), (600, 130, 3001), (90, 260, 130), (2049, 2200, 272)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -241,10 +241,18 @@ def test_glu(fs, M, N, K, dtype):
     check_product(y, ref, err, dtype)
     y2 = fs.glu_fp8(xc, xs.t().contiguous().t(), gc, gs, uc, us, dtype=dtype)
     assert torch.equal(y, y2)
-    if dtype == torch.bfloat16:                                                # what the two calls give one after the other
-        codes, scales = fs.glu_fp8(xc, xs, gc, gs, uc, us, quantize=True)
-        want, want_s = fs.quantize_fp8(y)
-        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 9216, 768), (8, 9216, 768), (16, 4000, 2048), (17, 3000, 1000), (32, 9216, 768), (33, 2304, 1536), (100, 2304, 768), (200, 5000, 400),
+                                   (300, 2048, 272), (700, 2304, 1001), (2100, 2304, 768)])
+def test_codes_of_the_pair_are_those_of_its_result(fs, M, N, K):
+    """One launch and two, to the bit, over some millions of values."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = fs.quantize_fp8(torch.randn(M, K, generator=g, device="cuda"))
+    gate, up = (fs.quantize_weight_fp8(torch.randn(N, K, generator=g, device="cuda") * K ** -0.5) for _ in range(2))
+    codes, scales = fs.glu_fp8(*x, *gate, *up, quantize=True)
+    want, want_s = fs.quantize_fp8(fs.glu_fp8(*x, *gate, *up))
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
 
 
 @pytest.mark.parametrize("M", [1, 8, 40, 300])
