@@ -221,26 +221,40 @@ __device__ __forceinline__ float lds4(unsigned addr) {
   return v;
 }
 
-// 8 consecutive bf16 of a row, any 2-byte alignment; fewer at a row's end
+// 8 consecutive features of a row, at any element's alignment
 typedef unsigned u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ void put8(bf16_t* p, const float (&v)[8], int left) {
-  if (left >= 8) {
-    *(u32x4_any_t*)p = u32x4_any_t{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7])};
-    return;
+typedef float floatx4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct Put;
+template <> struct Put<bf16_t> {
+  typedef u32x4_any_t Eight;
+  static __device__ __forceinline__ void put(bf16_t* p, const float (&v)[8]) {
+    *(Eight*)p = Eight{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7])};
   }
-#pragma unroll
-  for (int e = 0; e < 7; ++e)
-    if (e < left) p[e] = f32_to_bf16(v[e]);
-}
-__device__ __forceinline__ void add8(float (&v)[8], const bf16_t* p, int left) {
-  if (left >= 8) {
-    const u32x4_any_t r = *(const u32x4_any_t*)p;
+  static __device__ __forceinline__ void add(float (&v)[8], Eight r) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[2 * e] += __uint_as_float(r[e] << 16), v[2 * e + 1] += __uint_as_float(r[e] & 0xffff0000u);
-    return;
   }
+};
+template <> struct Put<float> {
+  struct Eight { floatx4_any_t a, b; };
+  static __device__ __forceinline__ void put(float* p, const float (&v)[8]) {
+    *(floatx4_any_t*)p = floatx4_any_t{v[0], v[1], v[2], v[3]};
+    *(floatx4_any_t*)(p + 4) = floatx4_any_t{v[4], v[5], v[6], v[7]};
+  }
+  static __device__ __forceinline__ void add(float (&v)[8], const Eight& r) {
 #pragma unroll
-  for (int e = 0; e < 7; ++e)
+    for (int e = 0; e < 4; ++e) v[e] += r.a[e], v[4 + e] += r.b[e];
+  }
+};
+// the last features of a row, fewer than 8
+__device__ __forceinline__ void put_some(bf16_t* p, const float (&v)[8], int left) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) p[e] = f32_to_bf16(v[e]);
+}
+__device__ __forceinline__ void add_some(float (&v)[8], const bf16_t* p, int left) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
     if (e < left) v[e] += bf16_to_f32(p[e]);
 }
 
@@ -416,6 +430,17 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
     __builtin_amdgcn_s_barrier();
     // every wave has left the stages: the next tile's first blocks are on their way while this one is stored
     const int em0 = m0, en0 = n0;
+    const bool whole = en0 + NF <= N;                  // all of the tile's features are there
+    // y may be the residual, so that no load passes a store: those of an X half are asked for together, the first ahead of the fills
+    Put<bf16_t>::Eight res[GLU ? 1 : 8];
+    const auto ask = [&](int h) __attribute__((always_inline)) {
+      if (GLU || !o.res || !whole) return;
+#pragma unroll
+      for (int i = 0; i < (GLU ? 1 : 8); ++i)
+        res[i] = *(const Put<bf16_t>::Eight*)((const bf16_t*)o.res + (size_t)min(em0 + h * 128 + wm * 64 + (i >> 1) * 16 + l16, M - 1) * o.ldr + en0 + wn * 64 +
+                                              (i & 1) * 32 + 8 * lq);
+    };
+    ask(0);
     idx += (int)(gridDim.x >> 3);
     const bool more = idx < share && xcd + idx < tiles;
     if (more) {
@@ -458,35 +483,44 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
           if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (en0 >> 7) * o.sb] = fp8_scale(most);
         }
     } else {
-      // whole: all of the tile's features are there (the other form's branches are many, and a launch fetches its code anew)
-      const auto leave = [&](auto whole) __attribute__((always_inline)) {
-        constexpr bool ALL = decltype(whole)::value;
+      // whether all features are there is asked for the tile: the other form's branches are many, and a launch fetches its code anew
+      const auto leave = [&](auto every) __attribute__((always_inline)) {
+        constexpr bool ALL = decltype(every)::value;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          if (h) ask(1);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int m = em0 + h * 128 + wm * 64 + j * 16 + l16;
 #pragma unroll
             for (int i = 0; i < (GLU ? 1 : 2); ++i) {
-              const int f = en0 + wn * (GLU ? 32 : 64) + i * 32 + 8 * lq, left = ALL ? 8 : N - f;
+              const int f = en0 + wn * (GLU ? 32 : 64) + i * 32 + 8 * lq;
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float a = acc[2 * i + (e >> 2)][h][j][e & 3];
                 v[e] = GLU ? gelu_tanh_exp(a) * acc[2 + (e >> 2)][h][j][e & 3] : a;
               }
-              if (m < M && (ALL || left > 0)) {
-                if (!GLU && o.bias) add8(v, (const bf16_t*)o.bias + f, left);
-                if (!GLU && o.res) add8(v, (const bf16_t*)o.res + (size_t)m * o.ldr + f, left);
-                put8((bf16_t*)o.y + (size_t)m * o.ldy + f, v, left);
+              bf16_t* const y = (bf16_t*)o.y + (size_t)m * o.ldy + f;
+              if constexpr (ALL) {
+                if (m < M) {
+                  if (!GLU && o.bias) Put<bf16_t>::add(v, *(const Put<bf16_t>::Eight*)((const bf16_t*)o.bias + f));
+                  if (!GLU && o.res) Put<bf16_t>::add(v, res[j * 2 + i]);
+                  Put<bf16_t>::put(y, v);
+                }
+              } else if (m < M && f < N) {
+                if (!GLU && o.bias) add_some(v, (const bf16_t*)o.bias + f, N - f);
+                if (!GLU && o.res) add_some(v, (const bf16_t*)o.res + (size_t)m * o.ldr + f, N - f);
+                put_some(y, v, N - f);
               }
             }
           }
+        }
       };
-      if (en0 + NF <= N) leave(std::true_type{});
+      if (whole) leave(std::true_type{});
       else leave(std::false_type{});
     }
-    young = em0 + 256 <= M && en0 + NF <= N;
+    young = em0 + 256 <= M && whole;
     if (!more) break;
   }
 }
@@ -656,14 +690,23 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
         if (fe + e < N) p[e] = v[e];
     return;
   }
+  T* const y = (T*)o.y + (size_t)m * o.ldy + fe;
+  const T* const res = (const T*)o.res + (size_t)m * o.ldr + fe;
+  float more[4] = {0.f, 0.f, 0.f, 0.f};                // y may be the residual, so that no load passes a store
+  if constexpr (!GLU) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (fe + e >= N) break;
-    float a = v[e];
-    if (!GLU && o.bias) a += DT<T>::ld((const T*)o.bias + fe + e);
-    if (!GLU && o.res) a += DT<T>::ld((const T*)o.res + (size_t)m * o.ldr + fe + e);
-    DT<T>::st((T*)o.y + (size_t)m * o.ldy + fe + e, a);
+    for (int e = 0; e < 4; ++e) {
+      if (o.bias && fe + e < N) more[e] = DT<T>::ld((const T*)o.bias + fe + e);
+      if (o.bias) v[e] += more[e];
+      if (o.res && fe + e < N) more[e] = DT<T>::ld(res + e);
+    }
+    if (o.res)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += more[e];
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (fe + e < N) DT<T>::st(y + e, v[e]);
 }
 
 // fp32 slices (slices, M, N), added in order -> T( sum + bias + residual )
@@ -727,36 +770,6 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
 // K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
 #define TL_STAGE 33792u                           // W | X | scales: by wave those of 32 rows, then the two weights'
 #define TL_FILLS 9
-
-template <typename T> struct Put;
-template <> struct Put<bf16_t> {
-  static __device__ __forceinline__ void put(bf16_t* p, const float (&v)[8], int left) { put8(p, v, left); }
-  static __device__ __forceinline__ void add(float (&v)[8], const bf16_t* p, int left) { add8(v, p, left); }
-};
-template <> struct Put<float> {
-  typedef float floatx4_any_t __attribute__((ext_vector_type(4), aligned(4)));
-  static __device__ __forceinline__ void put(float* p, const float (&v)[8], int left) {
-    if (left >= 8) {
-      *(floatx4_any_t*)p = floatx4_any_t{v[0], v[1], v[2], v[3]};
-      *(floatx4_any_t*)(p + 4) = floatx4_any_t{v[4], v[5], v[6], v[7]};
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (e < left) p[e] = v[e];
-  }
-  static __device__ __forceinline__ void add(float (&v)[8], const float* p, int left) {
-    if (left >= 8) {
-      const floatx4_any_t a = *(const floatx4_any_t*)p, b = *(const floatx4_any_t*)(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += a[e], v[4 + e] += b[e];
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (e < left) v[e] += p[e];
-  }
-};
 
 template <class F, int... I>
 __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...>) {
@@ -952,17 +965,25 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
   }
   const int fe = n0 + wn * (GLU ? 32 : 64) + 8 * lq;   // this lane's features: 8 of each pair of tiles
-  // whole: all of the tile's features are there (the other form's branches are many, and a launch fetches its code anew)
-  const auto leave = [&](auto whole) __attribute__((always_inline)) {
-    constexpr bool ALL = decltype(whole)::value;
+  // straight from the accumulators where all of the tile's features are there, in rows of whole 16 bytes
+  const bool sliced = !GLU && slices > 1;
+  const long long apart = sliced ? 4LL * N : (o.ldy | (!GLU && o.res ? o.ldr : 0)) * (long long)sizeof(T);
+  const size_t from = sliced ? 0 : (size_t)o.y | (GLU ? 0 : (size_t)o.res | (size_t)o.bias);
+  if (n0 + NF <= N && (apart & 15) == 0 && (from & 15) == 0) {
+    // y may be the residual, so that no load passes a store: all of them are asked for first (one behind the other they took 5 us)
+    typename Put<T>::Eight res[GLU ? 1 : 8];
+    if (!GLU && o.res && slices == 1) {
+#pragma unroll
+      for (int i = 0; i < (GLU ? 1 : 8); ++i)
+        res[i] = *(const typename Put<T>::Eight*)((const T*)o.res + (size_t)min(m0 + wm * 64 + (i >> 1) * 16 + l16, M - 1) * o.ldr + fe + (i & 1) * 32);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int m = m0 + wm * 64 + j * 16 + l16;
       if (m >= M) continue;
 #pragma unroll
       for (int p = 0; p < (GLU ? 1 : 2); ++p) {
-        const int f = fe + p * 32, left = ALL ? 8 : N - f;
-        if (!ALL && left <= 0) continue;
+        const int f = fe + p * 32;
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -970,17 +991,57 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
           v[e] = GLU ? gelu_tanh_exp(g) * acc[2 + (e >> 2)][j][e & 3] : g;
         }
         if (!GLU && slices > 1) {
-          Put<float>::put(partial + ((size_t)slice * M + m) * N + f, v, left);
+          Put<float>::put(partial + ((size_t)slice * M + m) * N + f, v);
           continue;
         }
-        if (!GLU && o.bias) Put<T>::add(v, (const T*)o.bias + f, left);
-        if (!GLU && o.res) Put<T>::add(v, (const T*)o.res + (size_t)m * o.ldr + f, left);
-        Put<T>::put((T*)o.y + (size_t)m * o.ldy + f, v, left);
+        if (!GLU && o.bias) Put<T>::add(v, *(const typename Put<T>::Eight*)((const T*)o.bias + f));
+        if (!GLU && o.res) Put<T>::add(v, res[2 * j + p]);
+        Put<T>::put((T*)o.y + (size_t)m * o.ldy + f, v);
       }
     }
-  };
-  if (n0 + NF <= N) leave(std::true_type{});
-  else leave(std::false_type{});
+    return;
+  }
+  // features of any number and alignment: through LDS and one value at a time, whole lines of a row side by side
+  __syncthreads();                                     // every wave has left the stages
+  float* const rows = (float*)smem;                    // 128 rows of 132
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < (GLU ? 2 : 4); ++i) {
+      floatx4_t v = acc[i][j];
+      if constexpr (GLU)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = gelu_tanh_exp(v[e]) * acc[2 + i][j][e];
+      *(floatx4_t*)(rows + (wm * 64 + j * 16 + l16) * 132 + (fe - n0) + (i >> 1) * 32 + (i & 1) * 4) = v;
+    }
+  __syncthreads();
+  const int f = n0 + (tid & (NF - 1));
+  if (f >= N) return;
+  float bias = 0.f;
+  if (!GLU && o.bias && slices == 1) bias = DT<T>::ld((const T*)o.bias + f);
+  constexpr int STEP = 256 / NF;
+  const int end = min(128, M - m0);
+  const T* const res = GLU || sliced ? nullptr : (const T*)o.res;
+  for (int r0 = tid / NF; r0 < end; r0 += 16 * STEP) { // sixteen at a time, none behind a condition of its own: it would wait for each
+    float v[16], more[16];
+    if (res) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) more[i] = DT<T>::ld(res + (size_t)(m0 + min(r0 + i * STEP, end - 1)) * o.ldr + f);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = rows[min(r0 + i * STEP, end - 1) * 132 + f - n0] + bias;
+    if (res) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] += more[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int m = m0 + r0 + i * STEP;
+      if (r0 + i * STEP >= end) break;
+      if (sliced) partial[((size_t)slice * M + m) * N + f] = v[i];
+      else DT<T>::st((T*)o.y + (size_t)m * o.ldy + f, v[i]);
+    }
+  }
 }
 
 template <typename T, bool GLU, int TAIL, int STAGES>
