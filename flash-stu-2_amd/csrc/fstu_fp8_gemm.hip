@@ -82,7 +82,7 @@ __device__ __forceinline__ u32x4_t cut16(u32x4_t v, int left) {
 // A chunk of 16 bytes from byte k of a row of K (behind its end zeros, and its last chunk is read in their place).  A row's last chunk is
 // read whole: rows are 16-byte aligned, so that it lies in the 16 bytes whose first the row has.
 __device__ __forceinline__ u32x4_t chunk16(const uint8_t* row, int k, int K) {
-  return cut16(*(const u32x4_t*)(row + min(k, (K - 1) & ~15)), K - k);
+  return cut16(*(const u32x4_t*)(row + min(k, max(K - 1, 0) & ~15)), K - k);
 }
 // The tanh-approximated GELU, x (1 + tanh t) / 2 = x / (1 + exp(-2 t)), on the hardware exp and reciprocal.
 __device__ __forceinline__ float gelu_tanh_exp(float x) {
@@ -101,16 +101,16 @@ fp8_plain_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) acc[j] = acu[j] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   const int nb = (K + 127) / 128;
-  for (int b = 0; b < nb; ++b) {
-    const int k = b * 128 + q * 16;
-    const Operand<T> w(Frag32{chunk16(wr, k, K), chunk16(wr, k + 64, K)});
-    const Operand<T> u(GLU ? Frag32{chunk16(ur, k, K), chunk16(ur, k + 64, K)} : Frag32{});
+  for (int it = 0; it < nb + (K % 16 != 0); ++it) {      // a row's last chunk, where it is no whole one, by itself, as on the tiles
+    const int b = min(it, nb - 1), end = it < nb ? K & ~15 : K, k = it < nb ? b * 128 + q * 16 : (K & ~15) + q * 16;
+    const Operand<T> w(Frag32{chunk16(wr, k, end), chunk16(wr, k + 64, end)});
+    const Operand<T> u(GLU ? Frag32{chunk16(ur, k, end), chunk16(ur, k + 64, end)} : Frag32{});
     const float sw = W.s[blockIdx.x * W.sr + b * W.sb], su = GLU ? U.s[blockIdx.x * U.sr + b * U.sb] : 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int m = min(m0 + j * 16 + l16, M - 1);
       const uint8_t* const xr = X.p + (size_t)m * X.ld;
-      const Operand<T> x(Frag32{chunk16(xr, k, K), chunk16(xr, k + 64, K)});
+      const Operand<T> x(Frag32{chunk16(xr, k, end), chunk16(xr, k + 64, end)});
       const float sx = X.s[m * X.sr + b * X.sb];
       const floatx4_t d = Operand<T>::sum(w, x);
 #pragma unroll
@@ -776,8 +776,9 @@ __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...
   (step(std::integral_constant<int, I>{}), ...);
 }
 
-// TAIL: 1 K is no multiple of 128 (chunks behind K are asked for behind the range, where a fill finds zeros), 2 nor one of 16 (the chunk with the
-// row's end is cut in LDS by the lane that has filled it)
+// TAIL: 1 K is no multiple of 128 (chunks behind K are asked for behind the range, where a fill finds zeros), 2 nor one of 16 (the chunk with a
+// row's end is left out as well and comes straight from global memory behind the loop; cut in LDS between two blocks it cost the fp32
+// form 27 spilled registers: 4096 x 2048 x 2001 79 us)
 template <typename T, bool GLU, int TAIL, int STAGES>
 __global__ void __launch_bounds__(256, 2)
 fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial, int M, int N, int K, int mt, int nt, int share, int slices) {
@@ -809,8 +810,8 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     const int row = wv * 32 + j * 8 + (lane >> 3);
     woff[j] = (unsigned)(GLU ? row & 63 : row) * (unsigned)(GLU && wv >= 2 ? U.ld : W.ld) + (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
     xoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
-    wthere[j] = (nb - 1) * 128 + ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16 < K;
-    xthere[j] = (nb - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < K;
+    wthere[j] = (nb - 1) * 128 + ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16 < (K & ~15);
+    xthere[j] = (nb - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < (K & ~15);
   }
   unsigned char* const fill0 = smem + (unsigned)wv * 4096u;
   const auto w_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !wthere[j] ? 0x80000000u : woff[j]; };
@@ -853,30 +854,14 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     if constexpr (I == 5) f.su = GLU ? lds4<4>(fsw + stage) : 0.f;
   };
   const auto each16 = [](auto&& step) __attribute__((always_inline)) { steps16(step, std::make_integer_sequence<int, 16>{}); };
-  const auto cut = [&](unsigned stage) __attribute__((always_inline)) {      // block nb - 1 in that stage: what lies behind a row's end is not its own
-    int own = lane;                                    // what follows is formed here: kept over the loop it would cost registers
-    asm volatile("" : "+v"(own));
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int row = wv * 32 + (j & 3) * 8 + (own >> 3);
-      const int ch = (own & 7) ^ (j < 4 ? ((row >> 1) & 1) | ((row >> 2) & 6) : (row >> 1) & 7);
-      const unsigned at = lds_addr(fill0) + stage + (unsigned)((j >> 2) * 16384 + (j & 3) * 1024 + own * 16);
-      u32x4_t v = lds16<0>(at);
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v)::"memory");
-      v = cut16(v, K - (nb - 1) * 128 - ch * 16);
-      asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(v) : "memory");
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  };
-  // the fragments f of block kt have come; this wave's share of block kt + 1 (in stage nxt) has landed
-  const auto wait = [&](Set& f, int kt, unsigned nxt) __attribute__((always_inline)) {
+  // the fragments f of a block have come; this wave's share of the next one has landed
+  const auto wait = [&](Set& f) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(%22) lgkmcnt(0)"
                  : "+v"(f.w[0].lo), "+v"(f.w[0].hi), "+v"(f.w[1].lo), "+v"(f.w[1].hi), "+v"(f.w[2].lo), "+v"(f.w[2].hi), "+v"(f.w[3].lo), "+v"(f.w[3].hi),
                    "+v"(f.x[0].lo), "+v"(f.x[0].hi), "+v"(f.x[1].lo), "+v"(f.x[1].hi), "+v"(f.x[2].lo), "+v"(f.x[2].hi), "+v"(f.x[3].lo), "+v"(f.x[3].hi),
                    "+v"(f.sx[0]), "+v"(f.sx[1]), "+v"(f.sx[2]), "+v"(f.sx[3]), "+v"(f.sw), "+v"(f.su)
                  : "n"(TL_FILLS * (STAGES - 2))
                  : "memory");
-    if (TAIL == 2 && kt + 1 == nb - 1) cut(nxt);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -945,7 +930,6 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) fetch(b0 + i, i * TL_STAGE);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TL_FILLS * (STAGES - 1)) : "memory");
-    if (TAIL == 2 && b0 == nb - 1) cut(0);
     __builtin_amdgcn_s_barrier();
     each16([&](auto which) __attribute__((always_inline)) { read_one(a, 0, which); });
     unsigned cur = 0;                                  // the stage of block kt
@@ -954,17 +938,45 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     // they are not finite, neither is the sum any more
     for (int kt = b0; kt < e1; kt += 2) {
       unsigned nxt = next(cur);
-      wait(a, kt, nxt);
+      wait(a);
       multiply(a, b, kt, cur, nxt);
       cur = nxt, nxt = next(cur);
-      wait(b, kt + 1, nxt);
+      wait(b);
       multiply(b, a, kt + 1, cur, nxt);
       cur = nxt;
     }
-    wait(a, nb, 0);                                      // the last reads, of a block that is not there, have to have come in
+    wait(a);                                      // the last reads, of a block that is not there, have to have come in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the empty fills behind the last block
   }
   const int fe = n0 + wn * (GLU ? 32 : 64) + 8 * lq;   // this lane's features: 8 of each pair of tiles
+  if constexpr (TAIL == 2) {
+    if (e1 == nb) {
+      const int k = K & ~15;
+      const u32x4_t none = {0, 0, 0, 0};
+      Frag32 w[4], x[4];
+      float sx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = wn * (GLU ? 32 : 64) + 8 * (l16 >> 2) + (l16 & 3) + 4 * (i & 1) + (GLU ? 0 : 16 * (i & 2)), m = min(wm * 64 + i * 16 + l16, M - 1 - m0);
+        w[i] = Frag32{chunk16((GLU && i >= 2 ? ub : wb) + (size_t)min(f, N - 1 - n0) * (GLU && i >= 2 ? U.ld : W.ld), k, K), none};
+        x[i] = Frag32{chunk16(xb + (size_t)m * X.ld, k, K), none};
+        sx[i] = X.s[(m0 + m) * X.sr + (nb - 1) * X.sb];
+      }
+      const float sw = W.s[(n0 >> 7) * W.sr + (nb - 1) * W.sb], su = GLU ? U.s[(n0 >> 7) * U.sr + (nb - 1) * U.sb] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                    // of the four chunks that the lanes of a row hold one is meant
+        if (lq) w[i].lo = none, x[i].lo = none;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const floatx4_t d = Operand<T>::sum(Operand<T>(w[i]), Operand<T>(x[j]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], sx[j] * (GLU && i >= 2 ? su : sw), acc[i][j][e]);
+        }
+    }
+  }
   // straight from the accumulators where all of the tile's features are there, in rows of whole 16 bytes
   const bool sliced = !GLU && slices > 1;
   const long long apart = sliced ? 4LL * N : (o.ldy | (!GLU && o.res ? o.ldr : 0)) * (long long)sizeof(T);
@@ -1091,14 +1103,16 @@ double estimate(Kind kind, int slices, int M, int N, int K, bool f32, bool glu) 
   }
   if (kind == TILE) {
     const long long tiles = up(N, glu ? 64 : 128) * up(M, 128) * slices;
+    us += (N % (glu ? 64 : 128) ? 4.0 : 0.0) + (K % 16 ? 2.0 : 0.0);       // the ends by one value and one chunk at a time
     if (tiles <= cus) return us + (f32 ? 5.0 + 1.03 * nb : 4.5 + 0.45 * nb);
     const long long rest = tiles % (2 * cus);
     const double rounds = (double)(tiles / (2 * cus)) + (rest == 0 ? 0.0 : rest <= cus ? 0.75 : 1.0);
     return us + 2.0 + rounds * (glu ? (f32 ? 4.0 + 1.73 * nb : 3.0 + 0.94 * nb) : f32 ? 10.0 + 1.73 * nb : 6.5 + 0.94 * nb);
   }
   const long long tiles = up(N, glu ? 128 : 256) * up(M, 256);
-  if (glu) return 1.0 + (double)up(tiles, cus) * (5.5 + 1.35 * nb);
-  return 5.0 + (double)up(tiles, cus) * (2.5 + (1.1 + 0.5 * std::min(1.0, (double)tiles / cus)) * nb);
+  // rows of no whole 16 bytes: 16384 x 2003 x 2048 132 instead of 79 (tiles, which pass them through LDS, 105)
+  if (glu) return 1.0 + (double)up(tiles, cus) * (5.5 + 1.35 * nb) * (N % 8 ? 1.2 : 1.0);
+  return 5.0 + (N % 8 ? 1.6 : 1.0) * (double)up(tiles, cus) * (2.5 + (1.1 + 0.5 * std::min(1.0, (double)tiles / cus)) * nb);
 }
 // slices: 0 as many as pay, otherwise that many
 Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {

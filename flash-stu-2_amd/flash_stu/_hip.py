@@ -1249,13 +1249,19 @@ FP8_BLOCK = 128
 _fp8 = torch.float8_e4m3fn
 
 
+_device_now = torch._C._cuda_getDevice
+
+
 def _fp8_new(rows: int, cols: int, per: int, device):
     """Codes and scales to be written: rows of whole 16 bytes, scales of a block beside each other (weights: row by row)."""
-    codes = torch.empty(rows, -(-cols // 16) * 16, dtype=_fp8, device=device)
-    if cols % 16:
-        codes = codes[:, :cols]
-    n, b = -(-rows // per), -(-cols // FP8_BLOCK)
-    return codes, torch.empty_strided((n, b), (1, n) if per == 1 else (b, 1), dtype=torch.float32, device=device)
+    b = (cols + 127) >> 7
+    if per == 1:
+        scales = torch.empty_strided((rows, b), (1, rows), dtype=torch.float32, device=device)
+    else:
+        scales = torch.empty((rows + 127) >> 7, b, dtype=torch.float32, device=device)
+    if not cols & 15:
+        return torch.empty(rows, cols, dtype=_fp8, device=device), scales
+    return torch.empty(rows, (cols + 15) & -16, dtype=_fp8, device=device)[:, :cols], scales
 
 
 def _fp8_source(x: torch.Tensor, dev: int, what: str, like: Optional[torch.Tensor] = None) -> int:
@@ -1263,11 +1269,15 @@ def _fp8_source(x: torch.Tensor, dev: int, what: str, like: Optional[torch.Tenso
     if x.get_device() != dev or dev < 0:
         raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if x.get_device() < 0
                                else f"{what} is on device {x.get_device()}, not on {dev}")
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or not 1 <= x.shape[1] < 1 << 31 or x.shape[0] >= 1 << 31:
+    if like is not None:
+        if x.shape != like.shape or x.dtype is not like.dtype:
+            raise FlashSTUHipError(f"{what} must be {tuple(like.shape)} {like.dtype}, got {tuple(x.shape)} {x.dtype}")
+    elif x.dim() != 2 or not 1 <= x.shape[1] < 1 << 31 or x.shape[0] >= 1 << 31:
         raise FlashSTUHipError(f"{what} must be 2-D with dense rows, got shape {tuple(x.shape)} stride {x.stride()}")
-    if like is not None and (x.shape != like.shape or x.dtype != like.dtype):
-        raise FlashSTUHipError(f"{what} must be {tuple(like.shape)} {like.dtype}, got {tuple(x.shape)} {x.dtype}")
-    return x.stride(0)
+    ld, one = x.stride()
+    if one != 1 and x.shape[1] > 1:
+        raise FlashSTUHipError(f"{what} must be 2-D with dense rows, got shape {tuple(x.shape)} stride {x.stride()}")
+    return ld
 
 
 def _fp8_operand(codes: torch.Tensor, scales: torch.Tensor, per: int, dev: int, what: str):
@@ -1281,79 +1291,78 @@ def _fp8_operand(codes: torch.Tensor, scales: torch.Tensor, per: int, dev: int, 
     ld, one = codes.stride()
     if (one != 1 and K > 1) or not 1 <= K < 1 << 31 or rows >= 1 << 31:
         raise FlashSTUHipError(f"{what}: codes must have dense rows of 1 value or more, got shape {tuple(codes.shape)} stride {codes.stride()}")
-    if scales.shape != (-(-rows // per), -(-K // FP8_BLOCK)):
+    if scales.shape != ((rows + per - 1) // per, (K + 127) >> 7):
         raise FlashSTUHipError(f"{what}: scales must be {(-(-rows // per), -(-K // FP8_BLOCK))}, got {tuple(scales.shape)}")
     sr, sb = scales.stride()
-    return codes.data_ptr(), ld if rows > 1 else -(-K // 16) * 16, scales.data_ptr(), sr, sb
+    return codes.data_ptr(), ld if rows > 1 else (K + 15) & -16, scales.data_ptr(), sr, sb
 
 
-def _fp8_device(fn):
-    """The function on the device of its first argument, which need not be the current one."""
-    @functools.wraps(fn)
-    def wrapped(x, *args, **kwargs):
-        dev = x.get_device()
-        if dev >= 0 and dev != torch._C._cuda_getDevice():
-            with torch.cuda.device(dev):
-                return fn(x, *args, **kwargs)
-        return fn(x, *args, **kwargs)
-    return wrapped
-
-
-@_fp8_device
 def quantize_fp8(x: torch.Tensor):
     """Codes and scales of x (rows, d) float32 or bfloat16, one scale for each 128 values of a row: scale = max(amax, 2^-100) / 448,
     code = x * (448 / max(amax, 2^-100)) to the nearest e4m3 value.  A block with an infinity or a NaN stands for NaN."""
     dev = x.get_device()
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return quantize_fp8(x)
     ld = _fp8_source(x, dev, "x")
     rows, d = x.shape
     dt = _dt(x)
     codes, scales = _fp8_new(rows, d, 1, x.device)
     if rows:
-        _check(load().fstu_fp8_quantize_rows(x.data_ptr(), ld, codes.data_ptr(), -(-d // 16) * 16, scales.data_ptr(), 1, rows, rows, d, dt,
-                                             raw_stream(dev)), "fstu_fp8_quantize_rows")
+        rc = load().fstu_fp8_quantize_rows(x.data_ptr(), ld, codes.data_ptr(), (d + 15) & -16, scales.data_ptr(), 1, rows, rows, d, dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_fp8_quantize_rows")
     return codes, scales
 
 
-@_fp8_device
 def quantize_weight_fp8(weight: torch.Tensor):
     """Codes and scales of a weight (N, K) float32 or bfloat16, one scale for each 128 x 128 values (formed as in quantize_fp8)."""
     dev = weight.get_device()
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return quantize_weight_fp8(weight)
     ld = _fp8_source(weight, dev, "weight")
     N, K = weight.shape
     if N < 1:
         raise FlashSTUHipError(f"weight must have rows, got {tuple(weight.shape)}")
     dt = _dt(weight)
     codes, scales = _fp8_new(N, K, FP8_BLOCK, weight.device)
-    _check(load().fstu_fp8_quantize_weight(weight.data_ptr(), ld, codes.data_ptr(), -(-K // 16) * 16, scales.data_ptr(), scales.shape[1], 1,
+    _check(load().fstu_fp8_quantize_weight(weight.data_ptr(), ld, codes.data_ptr(), (K + 15) & -16, scales.data_ptr(), scales.shape[1], 1,
                                            N, K, dt, raw_stream(dev)), "fstu_fp8_quantize_weight")
     return codes, scales
 
 
-@_fp8_device
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optional[torch.Tensor] = None,
                  x_out: Optional[torch.Tensor] = None):
     """Codes and scales (as quantize_fp8's) of rmsnorm(x) * weight for x (rows, d), d up to 32768; the normed values are not rounded
     to x's type on the way.  delta (rows, d): x + delta, rounded to x's type, is what is normed and is left in x_out (x itself where that is
-    not given)."""
+    not given; a tensor that overlaps x or delta otherwise than as a whole is not a place for it)."""
     dev = x.get_device()
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return rms_norm_fp8(x, weight, eps, delta, x_out)
     ldx = _fp8_source(x, dev, "x")
     rows, d = x.shape
-    if weight.get_device() != dev or weight.shape != (d,) or weight.dtype != x.dtype or not weight.is_contiguous():
+    if weight.get_device() != dev or weight.shape != (d,) or weight.dtype is not x.dtype or not weight.is_contiguous():
         raise FlashSTUHipError(f"weight must be ({d},) {x.dtype} on device {dev}, got {tuple(weight.shape)} {weight.dtype} on {weight.get_device()}")
     dt = _dt(x)
     pd = po = None
     ldd = ldo = 0
     if delta is not None:
+        ldd = _fp8_source(delta, dev, "delta", x)
+        pd = delta.data_ptr()
         if x_out is None:
-            x_out = x
-        ldd, ldo = _fp8_source(delta, dev, "delta", x), _fp8_source(x_out, dev, "x_out", x)
-        pd, po = delta.data_ptr(), x_out.data_ptr()
+            po, ldo = x.data_ptr(), ldx
+        else:
+            po, ldo = x_out.data_ptr(), _fp8_source(x_out, dev, "x_out", x)
     elif x_out is not None:
         raise FlashSTUHipError("x_out takes x + delta: it needs delta")
     codes, scales = _fp8_new(rows, d, 1, x.device)
     if rows:
-        _check(load().fstu_fp8_rmsnorm(x.data_ptr(), ldx, pd, ldd, po, ldo, weight.data_ptr(), eps, codes.data_ptr(), -(-d // 16) * 16,
-                                       scales.data_ptr(), 1, rows, rows, d, dt, raw_stream(dev)), "fstu_fp8_rmsnorm")
+        rc = load().fstu_fp8_rmsnorm(x.data_ptr(), ldx, pd, ldd, po, ldo, weight.data_ptr(), eps, codes.data_ptr(), (d + 15) & -16,
+                                     scales.data_ptr(), 1, rows, rows, d, dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_fp8_rmsnorm")
     return codes, scales
 
 
@@ -1362,7 +1371,6 @@ def _fp8_slices(M: int, N: int, K: int, dt: int) -> int:
     return load().fstu_fp8_linear_slices(M, N, K, dt)
 
 
-@_fp8_device
 def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y (M, N) = x @ w^T (+ bias (N,)) (+ residual (M, N)) for x (M, K) and w (N, K) as codes with scales, the sum in fp32 and rounded
@@ -1370,51 +1378,81 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
     bias, residual and out.  out may be residual.  In float32 the sums are those of fp32 products; in bfloat16 the matrix core's 8-bit
     instruction forms them, off by some 2e-5 of the result where its rounding is 2e-3."""
     dev = codes.get_device()
-    xa = _fp8_operand(codes, scales, 1, dev, "x")
-    wa = _fp8_operand(w_codes, w_scales, FP8_BLOCK, dev, "w")
-    (M, K), N = codes.shape, w_codes.shape[0]
-    if w_codes.shape[1] != K or N < 1:
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return linear_fp8(codes, scales, w_codes, w_scales, bias, residual, out, dtype)
+    xp, xl, xs, xr, xb = _fp8_operand(codes, scales, 1, dev, "x")
+    wp, wl, ws, wr, wb = _fp8_operand(w_codes, w_scales, FP8_BLOCK, dev, "w")
+    M, K = codes.shape
+    N, K2 = w_codes.shape
+    if K2 != K or N < 1:
         raise FlashSTUHipError(f"linear_fp8: x {tuple(codes.shape)} and w {tuple(w_codes.shape)} do not go together")
     if dtype is None:
-        dtype = next((t.dtype for t in (out, residual, bias) if t is not None), torch.bfloat16)
+        dtype = out.dtype if out is not None else residual.dtype if residual is not None else bias.dtype if bias is not None else torch.bfloat16
+    if dtype is torch.bfloat16:
+        dt = FSTU_BF16
+    elif dtype is torch.float32:
+        dt = FSTU_F32
+    else:
+        raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
     if out is None:
-        if dtype is not torch.bfloat16 and dtype is not torch.float32:
-            raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
-        out = torch.empty(M, N, dtype=dtype, device=codes.device)
-    for t, what in ((out, "out"), (residual, "residual")):
-        if t is not None and (t.shape != (M, N) or t.dtype != dtype or t.get_device() != dev or (N > 1 and t.stride(1) != 1)):
-            raise FlashSTUHipError(f"linear_fp8: {what} must be {(M, N)} {dtype} with dense rows on device {dev}, got {tuple(t.shape)} {t.dtype}")
-    if bias is not None and (bias.shape != (N,) or bias.dtype != dtype or bias.get_device() != dev or not bias.is_contiguous()):
-        raise FlashSTUHipError(f"linear_fp8: bias must be ({N},) {dtype} on device {dev}, got {tuple(bias.shape)} {bias.dtype}")
-    dt = _dt(out)
+        out, ldy = torch.empty(M, N, dtype=dtype, device=codes.device), N
+    else:
+        ldy = _fp8_result(out, M, N, dtype, dev, "out")
+    pr, ldr = None, 0
+    if residual is not None:
+        pr, ldr = residual.data_ptr(), _fp8_result(residual, M, N, dtype, dev, "residual")
+    pb = None
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype is not dtype or bias.get_device() != dev or not bias.is_contiguous():
+            raise FlashSTUHipError(f"linear_fp8: bias must be ({N},) {dtype} on device {dev}, got {tuple(bias.shape)} {bias.dtype}")
+        pb = bias.data_ptr()
     if M:
         slices = _fp8_slices(M, N, K, dt)
-        partial = torch.empty(slices, M, N, dtype=torch.float32, device=codes.device) if slices > 1 else None
-        _check(load().fstu_fp8_linear(*xa, *wa, _p(bias), _p(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(),
-                                      out.stride(0), M, N, K, dt, _p(partial), slices, raw_stream(dev)), "fstu_fp8_linear")
+        sums = torch.empty(slices, M, N, dtype=torch.float32, device=codes.device) if slices > 1 else None
+        rc = load().fstu_fp8_linear(xp, xl, xs, xr, xb, wp, wl, ws, wr, wb, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, dt, _p(sums), slices, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_fp8_linear")
     return out
 
 
-@_fp8_device
+def _fp8_result(t: torch.Tensor, M: int, N: int, dtype: torch.dtype, dev: int, what: str) -> int:
+    """Row stride of a checked (M, N) result or residual."""
+    if t.shape != (M, N) or t.dtype is not dtype or t.get_device() != dev or (t.stride(1) != 1 and N > 1):
+        raise FlashSTUHipError(f"linear_fp8: {what} must be {(M, N)} {dtype} with dense rows on device {dev}, got {tuple(t.shape)} {t.dtype} "
+                               f"stride {t.stride()}")
+    return t.stride(0)
+
+
 def glu_fp8(codes: torch.Tensor, scales: torch.Tensor, gate_codes: torch.Tensor, gate_scales: torch.Tensor, up_codes: torch.Tensor,
             up_scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16, quantize: bool = False):
     """y (M, N) = gelu_tanh(x @ gate^T) * (x @ up^T) for x (M, K), gate and up (N, K) as codes with scales, in fp32 and rounded once to
     `dtype` (float32 or bfloat16).  quantize: the codes and scales of quantize_fp8(y) in place of y (bfloat16), in the same launch."""
     dev = codes.get_device()
-    xa = _fp8_operand(codes, scales, 1, dev, "x")
-    ga = _fp8_operand(gate_codes, gate_scales, FP8_BLOCK, dev, "the gate")
-    ua = _fp8_operand(up_codes, up_scales, FP8_BLOCK, dev, "the up weight")
-    (M, K), N = codes.shape, gate_codes.shape[0]
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return glu_fp8(codes, scales, gate_codes, gate_scales, up_codes, up_scales, dtype, quantize)
+    xp, xl, xs, xr, xb = _fp8_operand(codes, scales, 1, dev, "x")
+    gp, gl, gs, gr, gb = _fp8_operand(gate_codes, gate_scales, FP8_BLOCK, dev, "the gate")
+    up, ul, us, ur, ub = _fp8_operand(up_codes, up_scales, FP8_BLOCK, dev, "the up weight")
+    M, K = codes.shape
+    N = gate_codes.shape[0]
     if gate_codes.shape[1] != K or up_codes.shape != gate_codes.shape or N < 1:
         raise FlashSTUHipError(f"glu_fp8: x {tuple(codes.shape)}, gate {tuple(gate_codes.shape)} and up {tuple(up_codes.shape)} do not go together")
-    if dtype is not torch.bfloat16 and (dtype is not torch.float32 or quantize):
+    if dtype is torch.bfloat16:
+        dt = FSTU_BF16
+    elif dtype is torch.float32 and not quantize:
+        dt = FSTU_F32
+    else:
         raise FlashSTUHipError(f"glu_fp8: unsupported dtype {dtype}: bfloat16, or float32 where the result is not quantized")
     if quantize:
-        y, s = _fp8_new(M, N, 1, codes.device)
-        where = y.data_ptr(), -(-N // 16) * 16, s.data_ptr(), 1, M
+        y, s = out = _fp8_new(M, N, 1, codes.device)
+        ldy, ps = (N + 15) & -16, s.data_ptr()
     else:
-        y = torch.empty(M, N, dtype=dtype, device=codes.device)
-        where = y.data_ptr(), N, None, 0, 0
+        y = out = torch.empty(M, N, dtype=dtype, device=codes.device)
+        ldy, ps = N, None
     if M:
-        _check(load().fstu_fp8_glu(*xa, *ga, *ua, *where, M, N, K, _dt(y) if not quantize else FSTU_BF16, raw_stream(dev)), "fstu_fp8_glu")
-    return (y, s) if quantize else y
+        rc = load().fstu_fp8_glu(xp, xl, xs, xr, xb, gp, gl, gs, gr, gb, up, ul, us, ur, ub, y.data_ptr(), ldy, ps, 1, M, M, N, K, dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_fp8_glu")
+    return out
