@@ -9,40 +9,56 @@
 
 namespace {
 
-// 8 consecutive values from column c of a row of d (fewer behind its end: zeros there).  VEC: 16-byte loads.
+// 16 bytes at an element's alignment
+typedef unsigned u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float floatx4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// 8 consecutive values from column c of a row of d (fewer behind its end: zeros there).  VEC: rows of whole 8 values at 16-byte addresses;
+// otherwise the 8 are read at whatever address they begin (one by one 16384 x 2047 took 124 us), those of a row's end one by one.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, int c, int d, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c < d) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 a = *(const float4*)(p + c), b = *(const float4*)(p + c + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 a = *(const uint4*)(p + c);
-        const unsigned u[4] = {a.x, a.y, a.z, a.w};
+  if (VEC ? c < d : c + 8 <= d) {
+    if constexpr (sizeof(T) == 4 && VEC) {
+      const float4 a = *(const float4*)(p + c), b = *(const float4*)(p + c + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else if constexpr (sizeof(T) == 4) {
+      const floatx4_any_t a = *(const floatx4_any_t*)(p + c), b = *(const floatx4_any_t*)(p + c + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
-      }
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
     } else {
+      unsigned u[4];
+      if constexpr (VEC) {
+        const uint4 x = *(const uint4*)(p + c);
+        u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
+      } else {
+        const u32x4_any_t x = *(const u32x4_any_t*)(p + c);
+        u[0] = x[0], u[1] = x[1], u[2] = x[2], u[3] = x[3];
+      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(u[e] << 16), v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < d ? DT<T>::ld(p + c + e) : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = !VEC && c + e < d ? DT<T>::ld(p + c + e) : 0.f;
   }
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, int c, int d, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c >= d) return;
+  if (VEC ? c < d : c + 8 <= d) {
     if constexpr (sizeof(T) == 4) {
-      *(float4*)(p + c) = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4*)(p + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      if constexpr (VEC) {
+        *(float4*)(p + c) = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)(p + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        *(floatx4_any_t*)(p + c) = floatx4_any_t{v[0], v[1], v[2], v[3]};
+        *(floatx4_any_t*)(p + c + 4) = floatx4_any_t{v[4], v[5], v[6], v[7]};
+      }
     } else {
-      *(uint4*)(p + c) = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
+      const unsigned a = pack2_bf16(v[0], v[1]), b = pack2_bf16(v[2], v[3]), e = pack2_bf16(v[4], v[5]), f = pack2_bf16(v[6], v[7]);
+      if constexpr (VEC) *(uint4*)(p + c) = make_uint4(a, b, e, f);
+      else *(u32x4_any_t*)(p + c) = u32x4_any_t{a, b, e, f};
     }
-  } else {
+  } else if (!VEC) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e < d) DT<T>::st(p + c + e, v[e]);
@@ -169,7 +185,10 @@ template <typename T, bool VEC>
 void rmsnorm_pick(const void* x, int64_t ldx, const void* delta, int64_t ldd, void* xo, int64_t ldo, const void* w, float eps, uint8_t* codes,
                   int64_t ldc, float* scales, int64_t ss, int64_t sb, int rows, int d, hipStream_t s) {
   const auto go = [&](auto f) { f(x, ldx, delta, ldd, xo, ldo, w, eps, codes, ldc, scales, ss, sb, rows, d, s); };
+  // few rows: the waves that the chip has for each of them (8 x 2048 with the addition 5.1 us with one, 3.6 with four)
   if (d <= 512) go(rmsnorm_launch<T, VEC, 1, 1>);
+  else if (rows <= 512 && d <= 2048) go(rmsnorm_launch<T, VEC, 4, 1>);
+  else if (rows <= 512 && d <= 8192) go(rmsnorm_launch<T, VEC, 16, 1>);
   else if (d <= 1024) go(rmsnorm_launch<T, VEC, 1, 2>);
   else if (d <= 2048) go(rmsnorm_launch<T, VEC, 1, 4>);
   else if (d <= 8192) go(rmsnorm_launch<T, VEC, 4, 4>);
