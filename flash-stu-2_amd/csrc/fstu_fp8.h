@@ -32,3 +32,14 @@ __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d
   int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
+
+// Whether what is written to rows of b (ldb elements apart, `bytes` each) leaves unread rows of a alone: they are the same rows, or share no byte.
+inline bool fp8_same_or_apart(const void* a, int64_t lda, const void* b, int64_t ldb, int rows, int cols, int bytes) {
+  if (a == b && (lda == ldb || rows == 1)) return true;
+  const int64_t pa = (int64_t)(intptr_t)a, pb = (int64_t)(intptr_t)b, row = (int64_t)cols * bytes;
+  const int64_t ra = lda * bytes, rb = ldb * bytes;
+  if (pa + (rows - 1) * ra + row <= pb || pb + (rows - 1) * rb + row <= pa) return true;
+  if (ra != rb || rows == 1) return false;
+  const int64_t off = ((pb - pa) % ra + ra) % ra;      // columns of the same rows
+  return off >= row && off + row <= ra;
+}

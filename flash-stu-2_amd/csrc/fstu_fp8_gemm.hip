@@ -1160,12 +1160,15 @@ extern "C" int fstu_fp8_linear(const uint8_t* x, int64_t ldx, const float* xs, i
                                int M, int N, int K, int dtype, float* partial, int slices, void* stream) {
   const Codes X = {x, ldx, xs, xs_row, xs_blk}, W = {w, ldw, ws, ws_row, ws_blk};
   FSTU_REQUIRE(y, FSTU_ENULL, "fstu_fp8_linear: null pointer");
-  FSTU_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= 65535 * 64, FSTU_ESHAPE, "fstu_fp8_linear: M=%d N=%d K=%d", M, N, K);
+  FSTU_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= 65535 * 64 && N <= 1 << 26 && K <= 1 << 30 && (M / 64 + 2LL) * (N / 64 + 2) <= 1 << 25, FSTU_ESHAPE,
+               "fstu_fp8_linear: M=%d N=%d K=%d", M, N, K);
   FP8_OPERAND("fstu_fp8_linear", X, M, "x");
   FP8_OPERAND("fstu_fp8_linear", W, N, "w");
   FSTU_REQUIRE(M == 1 || (ldy >= N && (!res || ldr >= N)), FSTU_ESHAPE, "fstu_fp8_linear: N=%d ldy=%lld ldr=%lld", N, (long long)ldy, (long long)ldr);
-  FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && slices > 1 && slices <= std::min(64, (K + 127) / 128) && near_rows(X, W, W)), FSTU_EARG,
-               "fstu_fp8_linear: slices=%d (K=%d, row strides %lld and %lld)", slices, K, (long long)ldx, (long long)ldw);
+  FSTU_REQUIRE(slices == 1 || (partial && fstu_aligned(partial, 16) && slices > 1 && slices <= std::min(64, (K + 127) / 128) && near_rows(X, W, W) && (long long)M * N < 1LL << 31),
+               FSTU_EARG, "fstu_fp8_linear: slices=%d (M=%d N=%d K=%d, row strides %lld and %lld)", slices, M, N, K, (long long)ldx, (long long)ldw);
+  FSTU_REQUIRE(!res || fp8_same_or_apart(res, ldr, y, ldy, M, N, dtype == FSTU_F32 ? 4 : 2), FSTU_EARG,
+               "fstu_fp8_linear: y overlaps the residual and is not the same rows");
   const Leave o = {y, ldy, bias, res, ldr, nullptr, 0, 0};
   const Kind kind = plan(M, N, K, dtype == FSTU_F32, false, false, slices).kind;
   hipStream_t const s = (hipStream_t)stream;
@@ -1190,7 +1193,8 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
                             int64_t us_blk, void* y, int64_t ldy, float* scales, int64_t ss, int64_t sb, int M, int N, int K, int dtype, void* stream) {
   const Codes X = {x, ldx, xs, xs_row, xs_blk}, W = {gate, ldg, gs, gs_row, gs_blk}, U = {up, ldu, us, us_row, us_blk};
   FSTU_REQUIRE(y, FSTU_ENULL, "fstu_fp8_glu: null pointer");
-  FSTU_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= 65535 * 64, FSTU_ESHAPE, "fstu_fp8_glu: M=%d N=%d K=%d", M, N, K);
+  FSTU_REQUIRE(M >= 1 && N >= 1 && K >= 1 && M <= 65535 * 64 && N <= 1 << 26 && K <= 1 << 30 && (M / 64 + 2LL) * (N / 64 + 2) <= 1 << 25, FSTU_ESHAPE,
+               "fstu_fp8_glu: M=%d N=%d K=%d", M, N, K);
   FP8_OPERAND("fstu_fp8_glu", X, M, "x");
   FP8_OPERAND("fstu_fp8_glu", W, N, "the gate");
   FP8_OPERAND("fstu_fp8_glu", U, N, "the up weight");

@@ -1336,7 +1336,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
                  x_out: Optional[torch.Tensor] = None):
     """Codes and scales (as quantize_fp8's) of rmsnorm(x) * weight for x (rows, d), d up to 32768; the normed values are not rounded
     to x's type on the way.  delta (rows, d): x + delta, rounded to x's type, is what is normed and is left in x_out (x itself where that is
-    not given; a tensor that overlaps x or delta otherwise than as a whole is not a place for it)."""
+    not given; a tensor that overlaps x or delta otherwise than as a whole is refused)."""
     dev = x.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
@@ -1375,7 +1375,8 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y (M, N) = x @ w^T (+ bias (N,)) (+ residual (M, N)) for x (M, K) and w (N, K) as codes with scales, the sum in fp32 and rounded
     once.  y is of `dtype` (float32 or bfloat16; that of out, residual or bias where not given, bfloat16 without those), and so are
-    bias, residual and out.  out may be residual.  In float32 the sums are those of fp32 products; in bfloat16 the matrix core's 8-bit
+    bias, residual and out.  out may be residual; one that
+    overlaps it otherwise is refused.  In float32 the sums are those of fp32 products; in bfloat16 the matrix core's 8-bit
     instruction forms them, off by some 2e-5 of the result where its rounding is 2e-3."""
     dev = codes.get_device()
     if dev >= 0 and dev != _device_now():
@@ -1408,7 +1409,7 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
             raise FlashSTUHipError(f"linear_fp8: bias must be ({N},) {dtype} on device {dev}, got {tuple(bias.shape)} {bias.dtype}")
         pb = bias.data_ptr()
     if M:
-        slices = _fp8_slices(M, N, K, dt)
+        slices = _fp8_slices(M, N, K, dt) if xl < 1 << 23 > wl else 1       # rows further apart: one sum
         sums = torch.empty(slices, M, N, dtype=torch.float32, device=codes.device) if slices > 1 else None
         rc = load().fstu_fp8_linear(xp, xl, xs, xr, xb, wp, wl, ws, wr, wb, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, dt, _p(sums), slices, raw_stream(dev))
         if rc:

@@ -50,3 +50,43 @@ class MLP(nn.Module):
             act = _hip.gelu_mul(g, u, out=g)
             out = _hip.gemm_any(act, self.down_proj.weight)
         return out.reshape(shape)
+
+
+class FP8MLP(nn.Module):
+    """The norm and the MLP of a layer with the weights as 8-bit codes: x + delta, then x + down(gelu_tanh(gate(n)) * up(n)) with n = norm(x),
+    as the layers form them from RMSNorm and MLP, in three launches (fp32: four).  The codes are laid out here, from the weights as
+    they are now, one scale for each 128 x 128; the activations are cut to codes on their way, one scale for each 128 values of a row.  The
+    norm's weight stays the norm's own."""
+
+    def __init__(self, norm: nn.Module, mlp: MLP):
+        super().__init__()
+        if mlp.gate_proj.bias is not None:
+            raise NotImplementedError("FP8MLP covers bias-free MLPs")
+        self.norm = norm
+        self.hidden_size, self.intermediate_size = mlp.hidden_size, mlp.intermediate_size
+        for name in ("gate", "up", "down"):
+            codes, scales = _hip.quantize_weight_fp8(getattr(mlp, name + "_proj").weight.detach())
+            # whole rows of 16 bytes, so that a copy of the buffer has them too
+            self.register_buffer(name + "_codes", codes.as_strided((codes.shape[0], codes.stride(0)), codes.stride()))
+            self.register_buffer(name + "_scales", scales)
+
+    def _weight(self, name: str, width: int):
+        codes = getattr(self, name + "_codes")
+        return (codes if codes.shape[1] == width else codes[:, :width]), getattr(self, name + "_scales")
+
+    @_hip.inference
+    def forward(self, x: torch.Tensor, delta: torch.Tensor = None) -> torch.Tensor:
+        """x (..., d) contiguous, updated in place; delta (same shape) is added first where it is given.  Returns x."""
+        d = self.hidden_size
+        if x.shape[-1] != d or not x.is_contiguous():
+            raise _hip.FlashSTUHipError(f"x must be (..., {d}) and contiguous, got {tuple(x.shape)} stride {x.stride()}")
+        if delta is not None and delta.shape != x.shape:
+            raise _hip.FlashSTUHipError(f"delta must be {tuple(x.shape)}, got {tuple(delta.shape)}")
+        x2 = x.view(-1, d)
+        codes, scales = _hip.rms_norm_fp8(x2, self.norm.weight, self.norm.eps, delta=None if delta is None else delta.reshape(-1, d))
+        if x.dtype is torch.bfloat16:
+            act = _hip.glu_fp8(codes, scales, *self._weight("gate", d), *self._weight("up", d), quantize=True)
+        else:
+            act = _hip.quantize_fp8(_hip.glu_fp8(codes, scales, *self._weight("gate", d), *self._weight("up", d), dtype=x.dtype))
+        _hip.linear_fp8(*act, *self._weight("down", self.intermediate_size), residual=x2, out=x2)
+        return x

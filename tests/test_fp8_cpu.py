@@ -74,6 +74,28 @@ def test_python_calls_refuse_what_is_not_on_the_gpu():
             call()
 
 
+def test_what_overlaps_otherwise_than_as_a_whole_is_refused(lib, mem):
+    """Refusals only: a call that passes the check would be launched."""
+    p = mem[0]
+    f = lambda xo, ldo=64, de=p + 2048, rows=2, dt=1: lib.fstu_fp8_rmsnorm(p, 64, de, 64, xo, ldo, p, 1e-6, p, 64, p, 1, 2, rows, 64, dt, None)
+    assert f(p + 2) == -5 and f(p + 128) == -5 and f(p + 2050) == -5 and "overlaps" in why(lib)
+    assert f(p, ldo=65) == -5 and f(p + 2, rows=1) == -5 and f(p + 256, dt=0) == -5
+    g = lambda r, ldr, y=p, ldy=20, M=2, N=8: lib.fstu_fp8_linear(p, 128, p, 1, 2, p, 128, p, 1, 1, None, r, ldr, y, ldy, M, N, 128, 1, None, 1, None)
+    assert g(p, 21) == -5 and g(p + 2, 20) == -5 and g(p + 14, 20) == -5 and g(p + 40, 20) == -5 and g(p + 26, 20) == -5 and g(p + 14, 20, M=1) == -5
+    assert "overlaps" in why(lib)
+
+
+def test_sizes_beyond_a_launch_are_refused(lib, mem):
+    p = mem[0]
+    assert lib.fstu_fp8_quantize_rows(p, 1 << 20, p, 1 << 20, p, 1, 1, 1 << 18, 1 << 20, 1, None) == -3
+    assert lib.fstu_fp8_rmsnorm(p, 32768, None, 0, None, 0, p, 1e-6, p, 32768, p, 1, 1, 1 << 22, 32768, 1, None) == -3
+    for M, N, K in ((65535 * 64 + 1, 8, 128), (1, (1 << 26) + 1, 128), (1 << 20, 1 << 20, 128), (1, 8, (1 << 30) + 1)):
+        ld = (K + 15) & -16
+        assert lib.fstu_fp8_linear(p, ld, p, 1, 1, p, ld, p, 1, 1, None, None, 0, p, N, M, N, K, 1, None, 1, None) == -3
+        assert lib.fstu_fp8_glu(p, ld, p, 1, 1, p, ld, p, 1, 1, p, ld, p, 1, 1, p, N, None, 1, 1, M, N, K, 1, None) == -3
+    assert lib.fstu_fp8_linear(p, 256, p, 1, 1, p, 256, p, 1, 1, None, None, 0, p, 1 << 16, 1 << 15, 1 << 16, 256, 1, p, 2, None) == -5
+
+
 @pytest.mark.gpu
 def test_python_calls_refuse_what_does_not_go_together():
     import flash_stu as fs

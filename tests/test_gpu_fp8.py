@@ -283,3 +283,163 @@ def test_no_rows(fs):
     assert fs.glu_fp8(codes, scales, wc, ws, wc, ws).shape == (0, 64)
     act = fs.glu_fp8(codes, scales, wc, ws, wc, ws, quantize=True)
     assert act[0].shape == (0, 64) and act[1].shape == (0, 1)
+
+
+# ---------------------------------------------------------------- together, and where a program calls them
+def layer_parts(d, scale, dtype, seed):
+    from flash_stu.config import FlashSTUConfig
+    from flash_stu.modules import MLP, RMSNorm
+    cfg = FlashSTUConfig(n_embd=d, n_heads=1, mlp_scale=scale, torch_dtype=dtype)
+    norm, mlp = RMSNorm(d, 1e-6, dtype=dtype), MLP(cfg, dtype=dtype)
+    with torch.no_grad():
+        for i, p in enumerate((norm.weight, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight)):
+            p.copy_((1 + 0.1 * torch.randn(p.shape, generator=gen(seed))) if i == 0 else torch.randn(p.shape, generator=gen(seed + i)) * p.shape[1] ** -0.5)
+    return norm.cuda(), mlp.cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,scale,rows", [(256, 4, 1), (256, 12, 40), (200, 3, 7), (768, 12, 300), (101, 5, 33)])
+def test_the_mlp_of_a_layer(fs, d, scale, rows, dtype):
+    """FP8MLP is its calls one behind the other, and near the layer's own norm and MLP: a code is off by at most 2^-4 of its value, 2^-4 / 3^(1/2) =
+    0.036 on the average of squares; so is each weight.  gate and up are off by 0.051 of their size, their product with gelu's slope of up to
+    1.13 by 0.077, cut to codes again and multiplied with the down projection's by (0.077^2 + 2 * 0.036^2)^(1/2) = 0.092."""
+    norm, mlp = layer_parts(d, scale, dtype, rows)
+    x = torch.randn(2, rows, d, generator=gen(7)).to(dtype).cuda()
+    y = (0.5 * torch.randn(2, rows, d, generator=gen(8))).to(dtype).cuda()
+    m = fs.FP8MLP(norm, mlp)
+    got = m(x.clone(), y)
+    s = (x.float() + y.float()).to(dtype)
+    z = s.clone().view(-1, d)
+    codes = fs.rms_norm_fp8(z, norm.weight.detach(), norm.eps)
+    w = [fs.quantize_weight_fp8(getattr(mlp, n).weight.detach()) for n in ("gate_proj", "up_proj", "down_proj")]
+    act = fs.quantize_fp8(fs.glu_fp8(*codes, *w[0], *w[1], dtype=dtype))
+    want = fs.linear_fp8(*act, *w[2], residual=z)
+    assert torch.equal(got.view(-1, d), want)
+    assert torch.equal(m(s.clone()), got)
+    t = s.double().cpu()
+    n = t / (t.square().mean(-1, keepdim=True) + norm.eps).sqrt() * norm.weight.detach().double().cpu()
+    g, u, dn = (getattr(mlp, k).weight.detach().double().cpu() for k in ("gate_proj", "up_proj", "down_proj"))
+    a = n @ g.t()
+    ref = (a * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)) * (n @ u.t())) @ dn.t()
+    off = got.double().cpu() - t - ref
+    assert float(off.norm() / ref.norm()) <= 0.092 + (2.0 ** -8 * float(got.double().norm() / ref.norm()) if dtype == torch.bfloat16 else 0.0)
+    other = fs.FP8MLP(norm, mlp)
+    other.load_state_dict({k: v.clone() for k, v in m.state_dict().items()})
+    assert torch.equal(other(x.clone(), y), got)
+
+
+def test_the_mlp_refuses(fs):
+    norm, mlp = layer_parts(128, 2, torch.bfloat16, 0)
+    m = fs.FP8MLP(norm, mlp)
+    from flash_stu._hip import FlashSTUHipError
+    with pytest.raises(FlashSTUHipError, match="contiguous"):
+        m(torch.zeros(4, 256, dtype=torch.bfloat16, device="cuda")[:, ::2])
+    with pytest.raises(FlashSTUHipError, match="weight must be"):
+        m(torch.zeros(4, 128, device="cuda"))
+    mlp.gate_proj.bias = torch.nn.Parameter(torch.zeros(256, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(NotImplementedError):
+        fs.FP8MLP(norm, mlp)
+
+
+@pytest.mark.parametrize("rows", [1, 24, 100, 600])
+def test_graphs_streams_and_neighbours(fs, rows):
+    """Two graphs of the whole MLP half, replayed in turn with eager calls between and on another stream: each replay gives the eager result."""
+    norm, mlp = layer_parts(768, 12, torch.bfloat16, 3)
+    m = fs.FP8MLP(norm, mlp)
+    xs = [torch.randn(rows, 768, generator=gen(i)).bfloat16().cuda() for i in range(2)]
+    want = [m(x.clone()) for x in xs]
+    bufs = [x.clone() for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for b in bufs:
+            m(b.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for b in bufs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m(b)
+        graphs.append((g, out))
+    for turn in range(4):
+        for i in (0, 1) if turn % 2 else (1, 0):
+            bufs[i].copy_(xs[i])
+            graphs[i][0].replay()
+            assert torch.equal(m(xs[1 - i].clone()), want[1 - i])
+            torch.cuda.synchronize()
+            assert torch.equal(graphs[i][1], want[i])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [m(x.clone()) for x in xs]
+    ahead = [m(x.clone()) for x in xs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, again, ahead))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 768, 9216), (30, 2048, 24576), (60, 300, 9000), (200, 768, 9216), (1000, 768, 9216)])
+def test_slices_of_k(fs, M, N, K, dtype):
+    """Any number of slices: the same product, and each the same bits every time."""
+    from flash_stu import _hip
+    xc, xs, x = make_codes((M, K), 10, 1)
+    wc, ws, w = make_codes((N, K), 20, 128)
+    res = torch.randn(M, N, generator=gen(4)).to(dtype).cuda()
+    ref, bound = x @ w.t() + res.double().cpu(), dot_bound(x, w, K, dtype)
+    lib, dt = _hip.load(), _hip._dt(res)
+    for slices in (1, 2, 3, 7, 16):
+        outs = []
+        for _ in range(2):
+            y = torch.empty_like(res)
+            part = torch.full((slices, M, N), float("nan"), device="cuda")
+            _hip._check(lib.fstu_fp8_linear(xc.data_ptr(), xc.stride(0), xs.data_ptr(), *xs.stride(), wc.data_ptr(), wc.stride(0), ws.data_ptr(), *ws.stride(), None,
+                                            res.data_ptr(), N, y.data_ptr(), N, M, N, K, dt, part.data_ptr(), slices, _hip._stream()), "fstu_fp8_linear")
+            outs.append(y)
+        assert torch.equal(*outs)
+        check_product(outs[0], ref, bound + 2.0 ** -23 * (x @ w.t()).abs(), dtype)
+    assert 1 <= lib.fstu_fp8_linear_slices(M, N, K, dt) <= 16
+
+
+def test_more_than_32_bits_of_offsets(fs):
+    """Codes of over 4 GiB, activations of over 8: the first and last rows are those of a call on them alone.  The norm of few rows adds a row's
+    squares in another order: 38 additions and 18, each off by 2^-24 of a sum that only grows, half of that in its root, and two roundings
+    each of root, reciprocal, product and division: a scale within 36 * 2^-24 < 2^-18 of the other.  The codes come from the row and the weight alone."""
+    rows, d = (1 << 21) + 77, 2064
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = fs.quantize_weight_fp8(torch.randn(40, d, generator=g, device="cuda"))
+    value = lambda c, s, per: c.cpu().double() * spread(s, c.shape, per)
+    wv = value(*w, 128)
+    x = torch.randn(rows, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    one = torch.ones(d, device="cuda", dtype=torch.bfloat16)
+    parts = (slice(0, 130), slice(rows - 130, rows))
+    for f, off in ((lambda v: fs.quantize_fp8(v), 0.0), (lambda v: fs.rms_norm_fp8(v, one, 1e-6), 2.0 ** -18)):
+        codes, scales = f(x)
+        for part in parts:
+            c, s = f(x[part])
+            assert torch.equal(codes[part].view(torch.uint8), c.view(torch.uint8)) and bool(((scales[part] - s).abs() <= off * s).all())
+    del x
+    for dtype in DTYPES:
+        y = fs.linear_fp8(codes, scales, *w, dtype=dtype)
+        act = fs.glu_fp8(codes, scales, *w, *w, dtype=dtype)
+        for part in parts:
+            xv = value(codes[part], scales[part], 1)
+            a, ea = xv @ wv.t(), dot_bound(xv, wv, d, dtype)
+            check_product(y[part], a, ea, dtype)
+            t = math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)
+            gelu = a * torch.sigmoid(2 * t)
+            check_product(act[part], gelu * a, 1.13 * ea * (a.abs() + ea) + gelu.abs() * ea + (8 + 3 * (2 * t).abs()) * 2.0 ** -23 * (gelu * a).abs() + 2.0 ** -130, dtype)
+
+
+@pytest.mark.parametrize("M", [3, 50, 300])
+@pytest.mark.parametrize("K", [260, 9000])
+def test_rows_far_apart(fs, M, K):
+    """Row strides beyond what a tile's 32-bit offsets cover take another kernel, and no slices of K."""
+    N, far = 70, (1 << 23) + 16
+    xc, xs, x = make_codes((M, K), 5, 1)
+    wc, ws, w = make_codes((N, K), 6, 128)
+    wide = torch.zeros(M * far, dtype=torch.uint8, device="cuda").view(M, far).view(torch.float8_e4m3fn)[:, :K]
+    wide.copy_(xc)
+    ref, bound = x @ w.t(), dot_bound(x, w, K, torch.bfloat16)
+    check_product(fs.linear_fp8(wide, xs, wc, ws), ref, bound, torch.bfloat16)
+    codes, scales = fs.glu_fp8(wide, xs, wc, ws, wc, ws, quantize=True)
+    want = fs.quantize_fp8(fs.glu_fp8(wide, xs, wc, ws, wc, ws))
+    assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
