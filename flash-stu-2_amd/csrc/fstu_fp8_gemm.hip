@@ -747,10 +747,8 @@ template <typename T, bool TAIL>
 int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, int M, int N, int K, hipStream_t s) {
   const char* const name = "fstu_fp8_glu";
   if constexpr (std::is_same<T, bf16_t>::value) {
-    if (o.s) {
-      if (M <= 16) return skinny_launch<T, 2, 1, 2, 8, 2, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
-      return skinny_launch<T, 2, 2, 2, 8, 2, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
-    }
+    // 16 waves of 16 rows: those of 32 rows had to spill (32 rows, 9216 x 768 12.1 us, so 6.4; 24576 x 2048 28 and 30)
+    if (o.s) return skinny_launch<T, 2, 1, 2, 8, 2, 2, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
   }
   // us, 8 / 32 rows: 9216 x 768 two tiles of four waves 4.2 / 5.5, one 4.3 / 5.0
   if (M <= 16) return skinny_launch<T, 1, 1, 2, 2, 4, 1, 2, TAIL>(X, W, V, o, nullptr, 1, M, N, K, s, name);
