@@ -39,7 +39,14 @@ __device__ __forceinline__ void load8(const T* p, int c, int d, float (&v)[8]) {
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = !VEC && c + e < d ? DT<T>::ld(p + c + e) : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (!VEC && c < d) {                                         // all of them asked for: behind a condition each waits for the one before
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = DT<T>::ld(p + min(c + e, d - 1));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < d ? w[e] : 0.f;
+    }
   }
 }
 template <typename T, bool VEC>
@@ -185,13 +192,15 @@ template <typename T, bool VEC>
 void rmsnorm_pick(const void* x, int64_t ldx, const void* delta, int64_t ldd, void* xo, int64_t ldo, const void* w, float eps, uint8_t* codes,
                   int64_t ldc, float* scales, int64_t ss, int64_t sb, int rows, int d, hipStream_t s) {
   const auto go = [&](auto f) { f(x, ldx, delta, ldd, xo, ldo, w, eps, codes, ldc, scales, ss, sb, rows, d, s); };
-  // few rows: the waves that the chip has for each of them (8 x 2048 with the addition 5.1 us with one, 2.7 with four)
+  // A lane takes one group of 8, a row the waves that this needs: more groups to a lane left fewer waves in flight.  us, bf16 with the addition,
+  // groups to a wave / one: 8 x 2048 four 5.1 / 2.7, 1024 x 2048 5.8 / 4.1, 16384 x 2048 38.9 / 38.1, 16384 x 4096 two 89 / 83, 16384 x 8192 four
+  // 179 / 164 (5000 119 / 128).  Up to 1024 columns many rows have waves enough: 1024 x 768 two 3.6 / 3.1, 2048 4.0 / 4.3, 8192 9.5 / 11.9.
   if (d <= 512) go(rmsnorm_launch<T, VEC, 1, 1>);
-  else if (rows <= 512 && d <= 2048) go(rmsnorm_launch<T, VEC, 4, 1>);
-  else if (rows <= 512 && d <= 8192) go(rmsnorm_launch<T, VEC, 16, 1>);
+  else if (d <= 1024 && rows <= 1024) go(rmsnorm_launch<T, VEC, 2, 1>);
   else if (d <= 1024) go(rmsnorm_launch<T, VEC, 1, 2>);
-  else if (d <= 2048) go(rmsnorm_launch<T, VEC, 1, 4>);
-  else if (d <= 8192) go(rmsnorm_launch<T, VEC, 4, 4>);
+  else if (d <= 2048) go(rmsnorm_launch<T, VEC, 4, 1>);
+  else if (d <= 4096) go(rmsnorm_launch<T, VEC, 8, 1>);
+  else if (d <= 8192) go(rmsnorm_launch<T, VEC, 16, 1>);
   else go(rmsnorm_launch<T, VEC, 16, 4>);
 }
 
@@ -227,7 +236,7 @@ extern "C" int fstu_fp8_rmsnorm(const void* x, int64_t ldx, const void* delta, i
   FSTU_REQUIRE(rows >= 1 && d >= 1 && d <= 32768 && (rows == 1 || (ldx >= d && (!delta || (ldd >= d && ldo >= d)))), FSTU_ESHAPE,
                "fstu_fp8_rmsnorm: rows=%d d=%d (1..32768) ldx=%lld", rows, d, (long long)ldx);
   FP8_CODES_OK("fstu_fp8_rmsnorm", codes, ldc, d);
-  FSTU_REQUIRE((long long)rows * (d <= 2048 ? 64 : d <= 8192 ? 256 : 1024) <= 0xff000000LL, FSTU_ESHAPE, "fstu_fp8_rmsnorm: rows=%d d=%d", rows, d);
+  FSTU_REQUIRE((long long)rows * (d <= 1024 ? 64 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024) <= 0xff000000LL, FSTU_ESHAPE, "fstu_fp8_rmsnorm: rows=%d d=%d", rows, d);
   const int bytes = dtype == FSTU_F32 ? 4 : 2;
   FSTU_REQUIRE(!delta || (fp8_same_or_apart(x, ldx, x_out, ldo, rows, d, bytes) && fp8_same_or_apart(delta, ldd, x_out, ldo, rows, d, bytes)), FSTU_EARG,
                "fstu_fp8_rmsnorm: x_out overlaps x or delta and is not the same rows");
