@@ -207,7 +207,8 @@ __device__ __forceinline__ void fill4(const float* p, void* l) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)l, 4, 0, 0);
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) void*)p; }
-// LDS reads are written as asm: the compiler orders every one it knows of behind all outstanding fills.  Each is waited for below, before any use.
+// LDS reads are written as asm: the compiler orders every one it knows of behind all outstanding fills.  Each is waited for below, before any use;
+// that nothing (a spill, a copy) touches its registers before is held by a test of the built code (tests/test_fp8_registers_cpu.py).
 template <int OFF>
 __device__ __forceinline__ u32x4_t lds16(unsigned addr) {
   u32x4_t v;
