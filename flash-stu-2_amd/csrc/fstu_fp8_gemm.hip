@@ -760,10 +760,13 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
 // Products of too few 256 x 256 tiles, and those whose results are fp32.  Four waves, each 64 features (glu: 32 of the gate and 32 of the
 // up weight) x 64 rows; K in blocks of 128 through STAGES LDS stages: two, and two workgroups to a compute unit, which cover each other's
 // waits and ends (fp32: the widening of one's codes runs beside the other's products: 8192 x 2048 x 24576 849 us with four, 707 so;
-// 4096 x 2048 x 2048 bf16 30 / 24), or four where there is no second one (4096 x 768 x 9216 51 with two, 40 so).  One wave to a SIMD
-// and workgroup, so it does everything at once:
+// 4096 x 2048 x 2048 bf16 30 / 24), or four where there is no second one (4096 x 768 x 9216 51 with two, 39 so).  There fp32 takes two
+// groups of four waves with two stages each, which halve K between them and add their sums through LDS: what stands in for the second workgroup
+// (4096 x 768 x 9216 82 without, 66 so; 1000 x 2048 x 2048 24 / 21; below 7 blocks the sum costs more: 2000 x 768 x 768 13.2 / 14.3; bf16
+// 39 / 42).  One wave of a group to a SIMD, so it does everything at once:
 //   wait for the fragments of kt (this wave has left stage kt) and for its share of block kt + 1; barrier; multiply the fragments of kt and,
-//   an instruction or two behind each product, request block kt + STAGES into stage kt and read the fragments of kt + 1
+//   an instruction to three behind each product, request block kt + STAGES into stage kt and read the fragments of kt + 1 (bf16: with the first half of
+//   the products, 4096 x 768 x 9216 39.8 -> 38.5 us)
 // (all requests, then all reads, then the products: 0.75 us a block of the four-stage form, since a wave issues in order and the queues of
 // both are short; 0.46 to 0.5 so, of which the products are 0.25).
 // K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
@@ -778,12 +781,14 @@ __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...
 // TAIL: 1 K is no multiple of 128 (chunks behind K are asked for behind the range, where a fill finds zeros), 2 nor one of 16 (the chunk with a
 // row's end is left out as well and comes straight from global memory behind the loop; cut in LDS between two blocks it cost the fp32
 // form 27 spilled registers: 4096 x 2048 x 2001 79 us)
-template <typename T, bool GLU, int TAIL, int STAGES>
-__global__ void __launch_bounds__(256, 2)
+template <typename T, bool GLU, int TAIL, int STAGES, int GROUPS>
+__global__ void __launch_bounds__(256 * GROUPS, 2)
 fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial, int M, int N, int K, int mt, int nt, int share, int slices) {
   constexpr int NF = GLU ? 64 : 128;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8) : 0;
+  const int tid = threadIdx.x & 255, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned char* const own = smem + (unsigned)group * (STAGES * TL_STAGE);
   int t = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= share || t >= mt * nt * slices) return;
   const int slice = t / (mt * nt);
@@ -791,7 +796,9 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   const int per_panel = mt * F8_PANEL, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
   const int m0 = in_panel / pw * 128, n0 = (panel * F8_PANEL + in_panel % pw) * NF;
   const int nb = (K + 127) >> 7, K16 = (K + 15) & ~15;
-  const int b0 = (int)((unsigned)(nb * slice) / (unsigned)slices), e1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices);
+  // a slice's blocks; of two groups the first takes the first half of them, rounded up, and both as many steps
+  const int s0 = (int)((unsigned)(nb * slice) / (unsigned)slices), s1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices);
+  const int half = GROUPS > 1 ? (s1 - s0 + 1) >> 1 : s1 - s0, b0 = s0 + group * half, e1 = min(b0 + half, s1);
   const uint8_t* const wb = W.p + (size_t)n0 * W.ld;
   const uint8_t* const ub = GLU ? U.p + (size_t)n0 * U.ld : wb;
   const uint8_t* const xb = X.p + (size_t)m0 * X.ld;
@@ -812,7 +819,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     wthere[j] = (nb - 1) * 128 + ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16 < (K & ~15);
     xthere[j] = (nb - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < (K & ~15);
   }
-  unsigned char* const fill0 = smem + (unsigned)wv * 4096u;
+  unsigned char* const fill0 = own + (unsigned)wv * 4096u;
   const auto w_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !wthere[j] ? 0x80000000u : woff[j]; };
   const auto x_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !xthere[j] ? 0x80000000u : xoff[j]; };
   const auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {   // beyond the last block nothing, into a stage that nobody reads
@@ -822,7 +829,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     for (int j = 0; j < 4; ++j) fill16(rw, w_at(b, j), (unsigned)b * 128u, fill0 + stage + j * 1024);
 #pragma unroll
     for (int j = 0; j < 4; ++j) fill16(rx, x_at(b, j), (unsigned)b * 128u, fill0 + stage + 16384 + j * 1024);
-    fill4(sp + (long long)min(b, e1 - 1) * sstep, smem + stage + 32768 + (unsigned)wv * 256u);
+    fill4(sp + (long long)min(b, e1 - 1) * sstep, own + stage + 32768 + (unsigned)wv * 256u);
   };
   const int l16 = lane & 15, lq = lane >> 4, wn = wv & 1, wm = wv >> 1;
   const int rw0 = (GLU ? 32 : 64) * wn + 8 * (l16 >> 2) + (l16 & 3);       // this lane's W row of the first feature tile; + 4, + 32 (glu: 64)
@@ -830,10 +837,10 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rx = wm * 64 + l16, c = h * 4 + lq;
-    fw[h] = lds_addr(smem) + (unsigned)rw0 * 128u + (unsigned)((c ^ (((rw0 >> 1) & 1) | ((rw0 >> 2) & 6))) << 4);
-    fx[h] = lds_addr(smem) + 16384u + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
+    fw[h] = lds_addr(own) + (unsigned)rw0 * 128u + (unsigned)((c ^ (((rw0 >> 1) & 1) | ((rw0 >> 2) & 6))) << 4);
+    fx[h] = lds_addr(own) + 16384u + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
   }
-  const unsigned fs = lds_addr(smem) + 32768u + (unsigned)wm * 512u + (unsigned)l16 * 4u, fsw = lds_addr(smem) + 32768u + 128u;
+  const unsigned fs = lds_addr(own) + 32768u + (unsigned)wm * 512u + (unsigned)l16 * 4u, fsw = lds_addr(own) + 32768u + 128u;
   struct Set {
     Frag32 w[4], x[4];
     float sx[4], sw, su;
@@ -882,7 +889,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
         if constexpr (I & 1) fill16(rx, x_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + 16384 + (I >> 1) * 1024);
         else fill16(rw, w_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + (I >> 1) * 1024);
       }
-      if constexpr (I == 8) fill4(sp + (long long)min(kt + STAGES, e1 - 1) * sstep, smem + cur + 32768 + (unsigned)wv * 256u);
+      if constexpr (I == 8) fill4(sp + (long long)min(kt + STAGES, e1 - 1) * sstep, own + cur + 32768 + (unsigned)wv * 256u);
     };
     if constexpr (std::is_same<T, float>::value) {
       // widened fragments: x's at once, w's one after the other, so that what comes for the next block takes the place of what has been widened
@@ -915,8 +922,11 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
       each16([&](auto which) __attribute__((always_inline)) {
         constexpr int I = decltype(which)::value;
         d[I] = Operand<T>::sum(Operand<T>(f.w[I >> 2]), Operand<T>(f.x[I & 3]));
+        if constexpr (I < 8) {
+          read_one(g, nxt, std::integral_constant<int, 2 * I>{});
+          read_one(g, nxt, std::integral_constant<int, 2 * I + 1>{});
+        }
         request(which);
-        read_one(g, nxt, which);
         if constexpr (I >= F8_AHEAD) add(std::integral_constant<int, I - F8_AHEAD>{});
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -935,7 +945,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (STAGES - 1) * TL_STAGE ? 0u : st + TL_STAGE; };
     // blocks in pairs; behind an odd number comes one of zeros (what a fill finds behind the range), whose scales are the last block's: where
     // they are not finite, neither is the sum any more
-    for (int kt = b0; kt < e1; kt += 2) {
+    for (int kt = b0; kt < b0 + half; kt += 2) {
       unsigned nxt = next(cur);
       wait(a);
       multiply(a, b, kt, cur, nxt);
@@ -949,7 +959,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   }
   const int fe = n0 + wn * (GLU ? 32 : 64) + 8 * lq;   // this lane's features: 8 of each pair of tiles
   if constexpr (TAIL == 2) {
-    if (e1 == nb) {
+    if (e1 == nb && b0 < e1) {
       const int k = K & ~15;
       const u32x4_t none = {0, 0, 0, 0};
       Frag32 w[4], x[4];
@@ -976,21 +986,41 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
         }
     }
   }
+  // two groups: each hands the other half of its rows over and finishes the other half
+  constexpr int RT = 4 / GROUPS;                       // this wave's row tiles from here on, the first at row mw
+  const int mw = wm * 64 + group * 32;
+  if constexpr (GROUPS > 1) {
+    __syncthreads();                                   // every wave has left the stages
+    floatx4_t* const there = (floatx4_t*)smem + ((1 - group) * 256 + tid);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) there[(i * RT + j) * 512] = group ? acc[i][j] : acc[i][RT + j];
+    __syncthreads();
+    const floatx4_t* const here = (const floatx4_t*)smem + (group * 256 + tid);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        const floatx4_t other = here[(i * RT + j) * 512], mine = group ? acc[i][RT + j] : acc[i][j];
+        acc[i][j] = group ? other + mine : mine + other;
+      }
+  }
   // straight from the accumulators where all of the tile's features are there, in rows of whole 16 bytes
   const bool sliced = !GLU && slices > 1;
   const long long apart = sliced ? 4LL * N : (o.ldy | (!GLU && o.res ? o.ldr : 0)) * (long long)sizeof(T);
   const size_t from = sliced ? 0 : (size_t)o.y | (GLU ? 0 : (size_t)o.res | (size_t)o.bias);
   if (n0 + NF <= N && (apart & 15) == 0 && (from & 15) == 0) {
     // y may be the residual, so that no load passes a store: all of them are asked for first (one behind the other they took 5 us)
-    typename Put<T>::Eight res[GLU ? 1 : 8];
+    typename Put<T>::Eight res[GLU ? 1 : 2 * RT];
     if (!GLU && o.res && slices == 1) {
 #pragma unroll
-      for (int i = 0; i < (GLU ? 1 : 8); ++i)
-        res[i] = *(const typename Put<T>::Eight*)((const T*)o.res + (size_t)min(m0 + wm * 64 + (i >> 1) * 16 + l16, M - 1) * o.ldr + fe + (i & 1) * 32);
+      for (int i = 0; i < (GLU ? 1 : 2 * RT); ++i)
+        res[i] = *(const typename Put<T>::Eight*)((const T*)o.res + (size_t)min(m0 + mw + (i >> 1) * 16 + l16, M - 1) * o.ldr + fe + (i & 1) * 32);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + wm * 64 + j * 16 + l16;
+    for (int j = 0; j < RT; ++j) {
+      const int m = m0 + mw + j * 16 + l16;
       if (m >= M) continue;
 #pragma unroll
       for (int p = 0; p < (GLU ? 1 : 2); ++p) {
@@ -1016,24 +1046,24 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   __syncthreads();                                     // every wave has left the stages
   float* const rows = (float*)smem;                    // 128 rows of 132
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < RT; ++j)
 #pragma unroll
     for (int i = 0; i < (GLU ? 2 : 4); ++i) {
       floatx4_t v = acc[i][j];
       if constexpr (GLU)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = gelu_tanh_exp(v[e]) * acc[2 + i][j][e];
-      *(floatx4_t*)(rows + (wm * 64 + j * 16 + l16) * 132 + (fe - n0) + (i >> 1) * 32 + (i & 1) * 4) = v;
+      *(floatx4_t*)(rows + (mw + j * 16 + l16) * 132 + (fe - n0) + (i >> 1) * 32 + (i & 1) * 4) = v;
     }
   __syncthreads();
-  const int f = n0 + (tid & (NF - 1));
+  const int f = n0 + (int)(threadIdx.x & (NF - 1));
   if (f >= N) return;
   float bias = 0.f;
   if (!GLU && o.bias && slices == 1) bias = DT<T>::ld((const T*)o.bias + f);
-  constexpr int STEP = 256 / NF;
+  constexpr int STEP = 256 * GROUPS / NF;
   const int end = min(128, M - m0);
   const T* const res = GLU || sliced ? nullptr : (const T*)o.res;
-  for (int r0 = tid / NF; r0 < end; r0 += 16 * STEP) { // sixteen at a time, none behind a condition of its own: it would wait for each
+  for (int r0 = (int)threadIdx.x / NF; r0 < end; r0 += 16 * STEP) { // sixteen at a time, none behind a condition of its own: it would wait for each
     float v[16], more[16];
     if (res) {
 #pragma unroll
@@ -1055,25 +1085,30 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   }
 }
 
-template <typename T, bool GLU, int TAIL, int STAGES>
+template <typename T, bool GLU, int TAIL, int STAGES, int GROUPS>
 int tile_launch(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
                 const char* name) {
   static fstu_lds_limit most;
-  if (const int rc = fstu_need_lds((const void*)fp8_tile_kernel<T, GLU, TAIL, STAGES>, most, STAGES * TL_STAGE, name)) return rc;
+  if (const int rc = fstu_need_lds((const void*)fp8_tile_kernel<T, GLU, TAIL, STAGES, GROUPS>, most, GROUPS * STAGES * TL_STAGE, name)) return rc;
   const int mt = (M + 127) / 128, nt = (N + (GLU ? 63 : 127)) / (GLU ? 64 : 128);
   const int share = (int)(((long long)mt * nt * slices + 7) / 8);
-  hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, TAIL, STAGES>), dim3(8u * share), dim3(256), STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
+  hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, TAIL, STAGES, GROUPS>), dim3(8u * share), dim3(256 * GROUPS), GROUPS * STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
   return 0;
 }
+// fp32 in tiles that leave compute units over: two groups of waves, each with half of a slice's blocks in steps of two
+bool two_groups(int K, int slices) { return (K + 127) / 128 >= 7 * slices; }
 template <typename T, bool GLU>
 int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s, const char* name) {
   const long long tiles = (long long)((M + 127) / 128) * ((N + (GLU ? 63 : 127)) / (GLU ? 64 : 128)) * slices;
   const int tail = K % 16 ? 2 : K % 128 ? 1 : 0;
   const auto run = [&](auto t) {
     constexpr int TAIL = decltype(t)::value;
-    if constexpr (sizeof(T) == 2)
-      if (tiles <= fstu_cus()) return tile_launch<T, GLU, TAIL, 4>(X, W, U, o, partial, slices, M, N, K, s, name);
-    return tile_launch<T, GLU, TAIL, 2>(X, W, U, o, partial, slices, M, N, K, s, name);
+    if constexpr (sizeof(T) == 2) {
+      if (tiles <= fstu_cus()) return tile_launch<T, GLU, TAIL, 4, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
+    } else if constexpr (!GLU) {
+      if (tiles <= fstu_cus() && two_groups(K, slices)) return tile_launch<T, GLU, TAIL, 2, 2>(X, W, U, o, partial, slices, M, N, K, s, name);
+    }
+    return tile_launch<T, GLU, TAIL, 2, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
   };
   const int rc = tail == 2 ? run(std::integral_constant<int, 2>{}) : tail ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 0>{});
   if (!rc && !GLU && slices > 1)
@@ -1103,7 +1138,7 @@ double estimate(Kind kind, int slices, int M, int N, int K, bool f32, bool glu) 
   if (kind == TILE) {
     const long long tiles = up(N, glu ? 64 : 128) * up(M, 128) * slices;
     us += (N % (glu ? 64 : 128) ? 4.0 : 0.0) + (K % 16 ? 2.0 : 0.0);       // the ends by one value and one chunk at a time
-    if (tiles <= cus) return us + (f32 ? 5.0 + 1.03 * nb : 4.5 + 0.45 * nb);
+    if (tiles <= cus) return us + (f32 ? (!glu && two_groups(K, slices) ? 9.5 + 0.78 * (double)(up(nb, 4) * 4) : 5.0 + 1.03 * nb) : 4.5 + 0.45 * nb);
     const long long rest = tiles % (2 * cus);
     const double rounds = (double)(tiles / (2 * cus)) + (rest == 0 ? 0.0 : rest <= cus ? 0.75 : 1.0);
     return us + 2.0 + rounds * (glu ? (f32 ? 4.0 + 1.73 * nb : 3.0 + 0.94 * nb) : f32 ? 10.0 + 1.73 * nb : 6.5 + 0.94 * nb);

@@ -229,6 +229,18 @@ def test_linear(fs, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(2000, 1500, 1793), (1900, 1280, 2008), (2040, 1536, 1000), (1999, 1537, 1921)])
+def test_linear_in_tiles_of_two_groups(fs, M, N, K, dtype):
+    xc, xs, x = make_codes((M, K), 10, 1)
+    wc, ws, w = make_codes((N, K), 20, 128, pad=16)
+    bias, res = torch.randn(N, generator=gen(3)).to(dtype), torch.randn(M, N, generator=gen(4)).to(dtype)
+    ref, bound = x @ w.t(), dot_bound(x, w, K, dtype)
+    y = fs.linear_fp8(xc, xs, wc, ws, bias=bias.cuda(), residual=res.cuda())
+    check_product(y, ref + bias.double() + res.double(), bound + 2.0 ** -23 * (ref.abs() + bias.double().abs()), dtype)
+    assert torch.equal(y, fs.linear_fp8(xc, xs, wc, ws, bias=bias.cuda(), residual=res.cuda()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_glu(fs, M, N, K, dtype):
     xc, xs, x = make_codes((M, K), 10, 1)
