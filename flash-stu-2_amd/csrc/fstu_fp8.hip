@@ -144,7 +144,12 @@ fp8_rmsnorm_kernel(const T* x, long long ldx, const T* delta, long long ldd, T* 
     const int c = c0 + i * W * 512;
     const float most = __uint_as_float(fp8_max16(size8(v[i])));
     const float norm = most * rms;                               // amax of the normed values: NaN where one of them is not a number
-    const float times = norm < FP8_LEAST ? rms * (FP8_MOST / FP8_LEAST) : norm == norm ? FP8_MOST / most : norm;
+    float times = norm == norm ? FP8_MOST / most : norm;
+    if (norm < FP8_LEAST || most < FP8_LEAST) {                  // next to nothing: 448 / most would not be a number
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= rms;
+      times = fp8_times(norm);
+    }
     if (c < d) *(uint2*)(codes + (size_t)row * ldc + c) = codes8(v[i], times);
     if ((lane & 15) == 0 && c < d) scales[row * ss + (c >> 7) * sb] = fp8_scale(norm);
   }

@@ -705,6 +705,8 @@ int fstu_prof_glu_loop(const fstu_model_desc* m, int reps, double* total_ms, int
  * A block with a value that is not finite gets a scale that is not finite either.  dtype: that of x, w, delta, bias, res, y.
  *
  * fstu_fp8_quantize_rows, fstu_fp8_quantize_weight: codes and scales of x (rows,d) / w (N,K), row strides ldx / ldw in elements.
+ * Refused: an x_out or y that overlaps x, delta or res without being the same rows, and sizes beyond a launch (2^32 threads: 16 to a
+ * block of 128 values of a row, 64 to 1024 to a norm's row; M up to 4194240, N up to 2^26, K up to 2^30, (M / 64 + 2) * (N / 64 + 2) up to 2^25).
  * fstu_fp8_rmsnorm: with delta, x_out = T(x + delta) (x_out may be x or delta) and x_out is what is normed; codes and scales of
  *   x * rsqrt(mean(x^2) + eps) * w, not rounded to T on the way; d up to 32768.  The norm of flash_stu/layers/stu_layer.py:93-96.
  * fstu_fp8_linear: y[m,n] = T( sum_k x[m,k] w[n,k] + bias[n] + res[m,n] ), bias and res or NULL, y may be res; sums in fp32, one

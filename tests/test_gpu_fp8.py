@@ -185,6 +185,25 @@ def test_rms_norm_of_every_width(fs, rows, d, dtype):
     test_rms_norm(fs, rows, d, dtype, True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eps", [1e-5, 1e-12, 1e-30])
+def test_rms_norm_of_rows_of_next_to_nothing(fs, eps, dtype):
+    """Zeros (the rows of a padded batch) and values whose normed block stays below the smallest scale: codes of the values, no 0 * inf."""
+    x = torch.randn(8, 300, generator=gen(5))
+    x[0], x[1], x[3, 128:256] = 0, x[1] * 2e-37, 0
+    x[4] *= 1e-20
+    x[5, :128] *= 1e-36
+    x = x.to(dtype)
+    w = torch.ones(300, dtype=dtype)
+    codes, scales = fs.rms_norm_fp8(x.cuda(), w.cuda(), eps)
+    t = x.double()
+    mean = x.float().double().square().mean(1, keepdim=True)
+    ref = t / (mean + torch.tensor(eps, dtype=torch.float32).double()).sqrt()
+    # squares below 2^-149 leave nothing in fp32: row 1's (of 4e-74) and row 4's (of 1e-40, in steps of 2^-149, 1e-5 of them) count for less than 2^-24 of eps
+    # where eps is 1e-30 or more
+    check_codes(codes, scales, ref, err=40 * 2.0 ** -24 * ref.abs())
+
+
 def test_rms_norm_in_place(fs):
     x = torch.randn(9, 768, generator=gen(0)).bfloat16().cuda()
     d = torch.randn(9, 768, generator=gen(1)).bfloat16().cuda()
