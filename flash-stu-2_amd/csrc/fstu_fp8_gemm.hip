@@ -757,7 +757,8 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
 }
 
 // ---------------------------------------------------------------- 128 x 128 tiles
-// Products of too few 256 x 256 tiles, and those whose results are fp32.  Four waves, each 64 features (glu: 32 of the gate and 32 of the
+// Products of too few 256 x 256 tiles, and those whose results are fp32.  The pair's codes in tiles of 64 rows and the 128 features that share a scale, a
+// wave 32 of either weight's, in three stages of 41 KB.  Four waves, each 64 features (glu: 32 of the gate and 32 of the
 // up weight) x 64 rows; K in blocks of 128 through STAGES LDS stages: two, and two workgroups to a compute unit, which cover each other's
 // waits and ends (fp32: the widening of one's codes runs beside the other's products: 8192 x 2048 x 24576 849 us with four, 707 so;
 // 4096 x 2048 x 2048 bf16 30 / 24), or four where there is no second one (4096 x 768 x 9216 51 with two, 39 so).  There fp32 takes two
@@ -770,8 +771,12 @@ int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, i
 // (all requests, then all reads, then the products: 0.75 us a block of the four-stage form, since a wave issues in order and the queues of
 // both are short; 0.46 to 0.5 so, of which the products are 0.25).
 // K may be cut into slices over the grid (linear), whose fp32 sums a second launch adds in their order.
-#define TL_STAGE 33792u                           // W | X | scales: by wave those of 32 rows, then the two weights'
-#define TL_FILLS 9
+template <int MODE>
+struct Tl {                                            // MODE 0 linear, 1 glu, 2 glu codes: 64 rows x the 128 features that share a scale
+  static constexpr int NF = MODE == 1 ? 64 : 128, ROWS = MODE == 2 ? 64 : 128;
+  static constexpr int WJ = MODE == 2 ? 8 : 4, XJ = ROWS / 32, FILLS = WJ + XJ + 1;        // a wave's fills of a block, 8 rows each, and its scales
+  static constexpr unsigned X = WJ * 4096u, SCALES = X + XJ * 4096u, STAGE = SCALES + 1024u;   // W | X | scales: by wave those of 32 rows, then the two weights'
+};
 
 template <class F, int... I>
 __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...>) {
@@ -781,20 +786,22 @@ __device__ __forceinline__ void steps16(F& step, std::integer_sequence<int, I...
 // TAIL: 1 K is no multiple of 128 (chunks behind K are asked for behind the range, where a fill finds zeros), 2 nor one of 16 (the chunk with a
 // row's end is left out as well and comes straight from global memory behind the loop; cut in LDS between two blocks it cost the fp32
 // form 27 spilled registers: 4096 x 2048 x 2001 79 us)
-template <typename T, bool GLU, int TAIL, int STAGES, int GROUPS>
+template <typename T, int MODE, int TAIL, int STAGES, int GROUPS>
 __global__ void __launch_bounds__(256 * GROUPS, 2)
 fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial, int M, int N, int K, int mt, int nt, int share, int slices) {
-  constexpr int NF = GLU ? 64 : 128;
+  typedef Tl<MODE> L;
+  constexpr bool GLU = MODE != 0;
+  constexpr int NF = L::NF, WJ = L::WJ, XJ = L::XJ;
   extern __shared__ __align__(16) unsigned char smem[];
   const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8) : 0;
   const int tid = threadIdx.x & 255, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  unsigned char* const own = smem + (unsigned)group * (STAGES * TL_STAGE);
+  unsigned char* const own = smem + (unsigned)group * (STAGES * L::STAGE);
   int t = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= share || t >= mt * nt * slices) return;
   const int slice = t / (mt * nt);
   t -= slice * (mt * nt);
   const int per_panel = mt * F8_PANEL, panel = t / per_panel, in_panel = t - panel * per_panel, pw = min(F8_PANEL, nt - panel * F8_PANEL);
-  const int m0 = in_panel / pw * 128, n0 = (panel * F8_PANEL + in_panel % pw) * NF;
+  const int m0 = in_panel / pw * L::ROWS, n0 = (panel * F8_PANEL + in_panel % pw) * NF;
   const int nb = (K + 127) >> 7, K16 = (K + 15) & ~15;
   // a slice's blocks; of two groups the first takes the first half of them, rounded up, and both as many steps
   const int s0 = (int)((unsigned)(nb * slice) / (unsigned)slices), s1 = (int)((unsigned)(nb * (slice + 1)) / (unsigned)slices);
@@ -804,43 +811,47 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   const uint8_t* const xb = X.p + (size_t)m0 * X.ld;
   const unsigned wbytes = (unsigned)(min(NF, N - n0) - 1) * (unsigned)W.ld + (unsigned)K16;
   const unsigned ubytes = GLU ? (unsigned)(min(NF, N - n0) - 1) * (unsigned)U.ld + (unsigned)K16 : 0;
-  const unsigned xbytes = (unsigned)(min(128, M - m0) - 1) * (unsigned)X.ld + (unsigned)K16;
+  const unsigned xbytes = (unsigned)(min(L::ROWS, M - m0) - 1) * (unsigned)X.ld + (unsigned)K16;
   const float* const sp = lane < 32 ? X.s + (long long)min(m0 + wv * 32 + lane, M - 1) * X.sr
                                     : GLU && (lane & 1) ? U.s + (n0 >> 7) * U.sr : W.s + (n0 >> 7) * W.sr;
   const long long sstep = lane < 32 ? X.sb : GLU && (lane & 1) ? U.sb : W.sb;
-  // ---- fills: a wave fills rows 32 wv .. + 31 of either part with four instructions (glu: waves 0 and 1 the gate's, 2 and 3 the up weight's)
-  unsigned woff[4], xoff[4];
-  bool wthere[4], xthere[4];                           // whether this lane's chunk of the last block is one of K's
+  // ---- fills: a wave fills a quarter of the rows of either part, 8 to an instruction (glu: waves 0 and 1 the gate's, 2 and 3 the up weight's)
+  unsigned woff[WJ], xoff[XJ];
+  bool wthere[WJ], xthere[XJ];                         // whether this lane's chunk of the last block is one of K's
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = wv * 32 + j * 8 + (lane >> 3);
-    woff[j] = (unsigned)(GLU ? row & 63 : row) * (unsigned)(GLU && wv >= 2 ? U.ld : W.ld) + (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
-    xoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
-    wthere[j] = (nb - 1) * 128 + ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16 < (K & ~15);
-    xthere[j] = (nb - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < (K & ~15);
+  for (int j = 0; j < WJ; ++j) {
+    const int row = wv * 8 * WJ + j * 8 + (lane >> 3), ch = ((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16;
+    woff[j] = (unsigned)(GLU ? row & (NF - 1) : row) * (unsigned)(GLU && wv >= 2 ? U.ld : W.ld) + (unsigned)ch;
+    wthere[j] = (nb - 1) * 128 + ch < (K & ~15);
   }
-  unsigned char* const fill0 = own + (unsigned)wv * 4096u;
+#pragma unroll
+  for (int j = 0; j < XJ; ++j) {
+    const int row = wv * 8 * XJ + j * 8 + (lane >> 3), ch = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+    xoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)ch;
+    xthere[j] = (nb - 1) * 128 + ch < (K & ~15);
+  }
+  unsigned char* const fill0 = own + (unsigned)wv * (WJ * 1024u), * const fillx = own + L::X + (unsigned)wv * (XJ * 1024u);
   const auto w_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !wthere[j] ? 0x80000000u : woff[j]; };
   const auto x_at = [&](int b, int j) __attribute__((always_inline)) { return TAIL && b == nb - 1 && !xthere[j] ? 0x80000000u : xoff[j]; };
   const auto fetch = [&](int b, unsigned stage) __attribute__((always_inline)) {   // beyond the last block nothing, into a stage that nobody reads
     const bool in = b < e1;
     const rsrc_t rw = make_rsrc(GLU && wv >= 2 ? ub : wb, in ? (GLU && wv >= 2 ? ubytes : wbytes) : 0), rx = make_rsrc(xb, in ? xbytes : 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fill16(rw, w_at(b, j), (unsigned)b * 128u, fill0 + stage + j * 1024);
+    for (int j = 0; j < WJ; ++j) fill16(rw, w_at(b, j), (unsigned)b * 128u, fill0 + stage + j * 1024);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fill16(rx, x_at(b, j), (unsigned)b * 128u, fill0 + stage + 16384 + j * 1024);
-    fill4(sp + (long long)min(b, e1 - 1) * sstep, own + stage + 32768 + (unsigned)wv * 256u);
+    for (int j = 0; j < XJ; ++j) fill16(rx, x_at(b, j), (unsigned)b * 128u, fillx + stage + j * 1024);
+    fill4(sp + (long long)min(b, e1 - 1) * sstep, own + stage + L::SCALES + (unsigned)wv * 256u);
   };
-  const int l16 = lane & 15, lq = lane >> 4, wn = wv & 1, wm = wv >> 1;
-  const int rw0 = (GLU ? 32 : 64) * wn + 8 * (l16 >> 2) + (l16 & 3);       // this lane's W row of the first feature tile; + 4, + 32 (glu: 64)
+  const int l16 = lane & 15, lq = lane >> 4, wn = MODE == 2 ? wv : wv & 1, wm = MODE == 2 ? 0 : wv >> 1;
+  const int rw0 = (GLU ? 32 : 64) * wn + 8 * (l16 >> 2) + (l16 & 3);       // this lane's W row of the first feature tile; + 4, + 32 (glu: NF)
   unsigned fw[2], fx[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int rx = wm * 64 + l16, c = h * 4 + lq;
     fw[h] = lds_addr(own) + (unsigned)rw0 * 128u + (unsigned)((c ^ (((rw0 >> 1) & 1) | ((rw0 >> 2) & 6))) << 4);
-    fx[h] = lds_addr(own) + 16384u + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
+    fx[h] = lds_addr(own) + L::X + (unsigned)rx * 128u + (unsigned)((c ^ ((rx >> 1) & 7)) << 4);
   }
-  const unsigned fs = lds_addr(own) + 32768u + (unsigned)wm * 512u + (unsigned)l16 * 4u, fsw = lds_addr(own) + 32768u + 128u;
+  const unsigned fs = lds_addr(own) + L::SCALES + (unsigned)wm * 512u + (unsigned)l16 * 4u, fsw = lds_addr(own) + L::SCALES + 128u;
   struct Set {
     Frag32 w[4], x[4];
     float sx[4], sw, su;
@@ -848,7 +859,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   Set a, b;
   // the I-th of 16 reads of a block's fragments (w first: a wave's products begin with w[0] and all of x)
   const auto read_one = [&](Set& f, unsigned stage, auto which) __attribute__((always_inline)) {
-    constexpr int I = decltype(which)::value, H = I & 1, P = GLU ? 8192 : 4096;       // P: from the first pair of feature tiles to the second
+    constexpr int I = decltype(which)::value, H = I & 1, P = GLU ? NF * 128 : 4096;       // P: from the first pair of feature tiles to the second
     if constexpr (I < 8) {
       (H ? f.x[I >> 1].hi : f.x[I >> 1].lo) = lds16<(I >> 1) * 2048>(fx[H] + stage);
     } else {
@@ -866,7 +877,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
                  : "+v"(f.w[0].lo), "+v"(f.w[0].hi), "+v"(f.w[1].lo), "+v"(f.w[1].hi), "+v"(f.w[2].lo), "+v"(f.w[2].hi), "+v"(f.w[3].lo), "+v"(f.w[3].hi),
                    "+v"(f.x[0].lo), "+v"(f.x[0].hi), "+v"(f.x[1].lo), "+v"(f.x[1].hi), "+v"(f.x[2].lo), "+v"(f.x[2].hi), "+v"(f.x[3].lo), "+v"(f.x[3].hi),
                    "+v"(f.sx[0]), "+v"(f.sx[1]), "+v"(f.sx[2]), "+v"(f.sx[3]), "+v"(f.sw), "+v"(f.su)
-                 : "n"(TL_FILLS * (STAGES - 2))
+                 : "n"(L::FILLS * (STAGES - 2))
                  : "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
@@ -885,11 +896,13 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
     for (int j = 0; j < 4; ++j) s[j] = f.sx[j] * f.sw, u[j] = GLU ? f.sx[j] * f.su : s[j];
     const auto request = [&](auto which) __attribute__((always_inline)) {
       constexpr int I = decltype(which)::value;
-      if constexpr (I < 8) {
-        if constexpr (I & 1) fill16(rx, x_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + 16384 + (I >> 1) * 1024);
-        else fill16(rw, w_at(kt + STAGES, I >> 1), (unsigned)(kt + STAGES) * 128u, fill0 + cur + (I >> 1) * 1024);
+      if constexpr (I < L::FILLS - 1) {
+        constexpr bool TO_X = MODE == 2 ? I >= WJ : I & 1;
+        constexpr int J = MODE == 2 ? I % WJ : I >> 1;
+        if constexpr (TO_X) fill16(rx, x_at(kt + STAGES, J), (unsigned)(kt + STAGES) * 128u, fillx + cur + J * 1024);
+        else fill16(rw, w_at(kt + STAGES, J), (unsigned)(kt + STAGES) * 128u, fill0 + cur + J * 1024);
       }
-      if constexpr (I == 8) fill4(sp + (long long)min(kt + STAGES, e1 - 1) * sstep, own + cur + 32768 + (unsigned)wv * 256u);
+      if constexpr (I == L::FILLS - 1) fill4(sp + (long long)min(kt + STAGES, e1 - 1) * sstep, own + cur + L::SCALES + (unsigned)wv * 256u);
     };
     if constexpr (std::is_same<T, float>::value) {
       // widened fragments: x's at once, w's one after the other, so that what comes for the next block takes the place of what has been widened
@@ -937,12 +950,12 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   };
   {
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i) fetch(b0 + i, i * TL_STAGE);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TL_FILLS * (STAGES - 1)) : "memory");
+    for (int i = 0; i < STAGES; ++i) fetch(b0 + i, i * L::STAGE);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L::FILLS * (STAGES - 1)) : "memory");
     __builtin_amdgcn_s_barrier();
     each16([&](auto which) __attribute__((always_inline)) { read_one(a, 0, which); });
     unsigned cur = 0;                                  // the stage of block kt
-    const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (STAGES - 1) * TL_STAGE ? 0u : st + TL_STAGE; };
+    const auto next = [&](unsigned st) __attribute__((always_inline)) { return st == (STAGES - 1) * L::STAGE ? 0u : st + L::STAGE; };
     // blocks in pairs; behind an odd number comes one of zeros (what a fill finds behind the range), whose scales are the last block's: where
     // they are not finite, neither is the sum any more
     for (int kt = b0; kt < b0 + half; kt += 2) {
@@ -985,6 +998,36 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
           for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], sx[j] * (GLU && i >= 2 ? su : sw), acc[i][j][e]);
         }
     }
+  }
+  if constexpr (MODE == 2) {
+    unsigned* const most = (unsigned*)smem;            // [64 rows][4 waves]
+    __syncthreads();                                   // every wave has left the stages
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = DT<T>::rnd(gelu_tanh_exp(acc[e >> 2][j][e & 3]) * acc[2 + (e >> 2)][j][e & 3]);
+        acc[e >> 2][j][e & 3] = fe + e < N ? v : 0.f;
+        m = max(m, fp8_size(acc[e >> 2][j][e & 3]));
+      }
+      m = max(m, (unsigned)__shfl_xor((int)m, 16));
+      m = max(m, (unsigned)__shfl_xor((int)m, 32));
+      if (lq == 0) most[(j * 16 + l16) * 4 + wn] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 all = *(const uint4*)(most + (j * 16 + l16) * 4);
+      const float amax = __uint_as_float(max(max(all.x, all.y), max(all.z, all.w))), times = fp8_times(amax);
+      const int m = m0 + j * 16 + l16;
+      const floatx4_t a = acc[0][j], b = acc[1][j];
+      if (m < M && fe < N)                             // a row's codes lie in whole 16 bytes: zeros behind the last feature
+        *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = make_uint2(fp8_pack4(a[0] * times, a[1] * times, a[2] * times, a[3] * times),
+                                                                       fp8_pack4(b[0] * times, b[1] * times, b[2] * times, b[3] * times));
+      if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (n0 >> 7) * o.sb] = fp8_scale(amax);
+    }
+    return;
   }
   // two groups: each hands the other half of its rows over and finishes the other half
   constexpr int RT = 4 / GROUPS;                       // this wave's row tiles from here on, the first at row mw
@@ -1085,14 +1128,15 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   }
 }
 
-template <typename T, bool GLU, int TAIL, int STAGES, int GROUPS>
+template <typename T, int MODE, int TAIL, int STAGES, int GROUPS>
 int tile_launch(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s,
                 const char* name) {
+  typedef Tl<MODE> L;
   static fstu_lds_limit most;
-  if (const int rc = fstu_need_lds((const void*)fp8_tile_kernel<T, GLU, TAIL, STAGES, GROUPS>, most, GROUPS * STAGES * TL_STAGE, name)) return rc;
-  const int mt = (M + 127) / 128, nt = (N + (GLU ? 63 : 127)) / (GLU ? 64 : 128);
+  if (const int rc = fstu_need_lds((const void*)fp8_tile_kernel<T, MODE, TAIL, STAGES, GROUPS>, most, GROUPS * STAGES * L::STAGE, name)) return rc;
+  const int mt = (M + L::ROWS - 1) / L::ROWS, nt = (N + L::NF - 1) / L::NF;
   const int share = (int)(((long long)mt * nt * slices + 7) / 8);
-  hipLaunchKernelGGL((fp8_tile_kernel<T, GLU, TAIL, STAGES, GROUPS>), dim3(8u * share), dim3(256 * GROUPS), GROUPS * STAGES * TL_STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
+  hipLaunchKernelGGL((fp8_tile_kernel<T, MODE, TAIL, STAGES, GROUPS>), dim3(8u * share), dim3(256 * GROUPS), GROUPS * STAGES * L::STAGE, s, X, W, U, o, partial, M, N, K, mt, nt, share, slices);
   return 0;
 }
 // fp32 in tiles that leave compute units over: two groups of waves, each with half of a slice's blocks in steps of two
@@ -1104,11 +1148,11 @@ int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* 
   const auto run = [&](auto t) {
     constexpr int TAIL = decltype(t)::value;
     if constexpr (sizeof(T) == 2) {
-      if (tiles <= fstu_cus()) return tile_launch<T, GLU, TAIL, 4, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
+      if (tiles <= fstu_cus()) return tile_launch<T, GLU ? 1 : 0, TAIL, 4, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
     } else if constexpr (!GLU) {
-      if (tiles <= fstu_cus() && two_groups(K, slices)) return tile_launch<T, GLU, TAIL, 2, 2>(X, W, U, o, partial, slices, M, N, K, s, name);
+      if (tiles <= fstu_cus() && two_groups(K, slices)) return tile_launch<T, 0, TAIL, 2, 2>(X, W, U, o, partial, slices, M, N, K, s, name);
     }
-    return tile_launch<T, GLU, TAIL, 2, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
+    return tile_launch<T, GLU ? 1 : 0, TAIL, 2, 1>(X, W, U, o, partial, slices, M, N, K, s, name);
   };
   const int rc = tail == 2 ? run(std::integral_constant<int, 2>{}) : tail ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 0>{});
   if (!rc && !GLU && slices > 1)
@@ -1151,8 +1195,14 @@ double estimate(Kind kind, int slices, int M, int N, int K, bool f32, bool glu) 
 // slices: 0 as many as pay, otherwise that many
 Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {
   const bool few = M <= (glu ? 32 : 64), big = !f32 && K % 16 == 0;
-  if (codes) return {few ? SKINNY : LARGE, 1, 0.0};
   if (glu && few) return {SKINNY, 1, 0.0};
+  if (codes) {
+    // tiles of 64 rows, one to a compute unit, or of 256.  us, 64 / 256: 64 x 9216 x 768 7.9 / 14.7, 128 8.0 / 15.0, 300 15.2 / 16.1, 500 22 / 17, 1000 37 / 32;
+    // 64 x 24576 x 2048 19 / 28, 128 27 / 28, 200 37 / 29; 1000 x 1536 x 512 7.1 / 13.4
+    const long long nb = (K + 127) / 128, tiles = ((N + 127) / 128) * (long long)((M + 63) / 64);
+    const double us = 1.3 + (double)((tiles + fstu_cus() - 1) / fstu_cus()) * (2.6 + 0.6 * nb) + (double)N * K * 6e-8;
+    return {us < estimate(LARGE, 1, M, N, K, false, true) ? TILE : LARGE, 1, us};
+  }
   // the pair of more rows adds its blocks in one order on all kernels, so that its codes are those of its bf16 result
   Plan best = {TILE, 1, estimate(TILE, 1, M, N, K, f32, glu)};
   if (!glu) best = {SKINNY, std::max(slices, 1), estimate(SKINNY, std::max(slices, 1), M, N, K, f32, glu)};
@@ -1247,6 +1297,9 @@ extern "C" int fstu_fp8_glu(const uint8_t* x, int64_t ldx, const float* xs, int6
       hipLaunchKernelGGL((fp8_plain_kernel<true, T>), dim3((N + 127) / 128, (M + 63) / 64), dim3(512), 0, s, X, W, U, o, M, N, K);
     else if (kind == LARGE)
       rc = scales ? large<2>(X, W, U, o, M, N, K, s, "fstu_fp8_glu") : large<1>(X, W, U, o, M, N, K, s, "fstu_fp8_glu");
+    else if (scales)
+      rc = K % 128 ? tile_launch<bf16_t, 2, 1, 3, 1>(X, W, U, o, nullptr, 1, M, N, K, s, "fstu_fp8_glu")
+                   : tile_launch<bf16_t, 2, 0, 3, 1>(X, W, U, o, nullptr, 1, M, N, K, s, "fstu_fp8_glu");
     else
       rc = tile<T, true>(X, W, U, o, nullptr, 1, M, N, K, s, "fstu_fp8_glu");
   });

@@ -281,7 +281,8 @@ def test_glu(fs, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 9216, 768), (8, 9216, 768), (16, 4000, 2048), (17, 3000, 1000), (32, 9216, 768), (33, 2304, 1536), (100, 2304, 768), (200, 5000, 400),
-                                   (300, 2048, 272), (700, 2304, 1001), (2100, 2304, 768)])
+                                   (300, 2048, 272), (700, 2304, 1001), (2100, 2304, 768), (64, 300, 144), (65, 129, 2000), (127, 1000, 1024), (128, 9216, 768),
+                                   (513, 130, 48), (4000, 700, 640)])
 def test_codes_of_the_pair_are_those_of_its_result(fs, M, N, K):
     """One launch and two, to the bit, over some millions of values."""
     g = torch.Generator(device="cuda").manual_seed(M)
