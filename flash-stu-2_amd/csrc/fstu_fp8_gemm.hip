@@ -186,6 +186,10 @@ fp8_plain_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K) {
 // conflicts.  The W rows are dealt so that a lane ends up with 8 consecutive features of a row, which leave straight from the accumulators.
 // Workgroup ids are dealt round-robin to the 8 XCDs; each XCD works through its own share of the tiles in panels of 8 feature tiles, and
 // a workgroup requests the first blocks of its next tile before it stores this one.
+// 16384 x 2048 x 24576 620 us (2.66 PFLOP/s; a library's 8-bit product of 8192^3 2.71), the pair 16384 x 2 x 24576 x 2048 1385 us (2.38), 4096 x 2 x 9216 x
+// 768 64 to 68: the matrix cores are busy for 70 % of the cycles (pair 54 %: a tile's GELU takes 5.5 us) at the 1.8 GHz that the power leaves
+// (all zeros 482 us instead of 620).  v_mfma_f32_32x32x64_f8f6f4, twice the products for the same fragments, behind sums of 16 registers: 686 and
+// 72; a phase's last sums moved behind its barrier: 628 and 64; half of the GELU beside the last block's products: the pair 69.
 #define F8_PANEL 8
 #define F8_AHEAD 3                                // products that are on their way when one is scaled and added
 #define F8_PART 16384u
@@ -292,37 +296,41 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
                    : GLU ? (lane & 1 ? U.s + b * U.sr : W.s + b * W.sr) : W.s + min(b + (lane & 1), last) * W.sr;
   };
   const int wn = wv & 3, wm = wv >> 2;                 // 32-feature slice and 64-row slice of every half
-  // ---- fills: a part is 128 rows x 128 bytes, a wave fills rows 16 wv .. + 15 of it with two instructions
+  // ---- fills: a part is 128 rows x 128 bytes, a wave fills 16 of them with two instructions.  SPREAD: 8 rows of either half of it, so that what
+  // differs between the two is the same for all lanes and goes into the descriptors, whose ranges end where the tile's rows do (a lane keeps one
+  // offset for an operand instead of two; 16384 x 2048 x 2048 78.5 -> 77.6 us, x 2064 88.9 -> 84.8, the pair 4096 x 9216 x 784 91.5 -> 82.6).  The pair
+  // in whole blocks has registers enough and is faster on 16 rows in line: 4096 x 9216 x 768 69.4 us, 71.0 spread.
+  constexpr bool SPREAD = TAIL || !GLU;
   unsigned wvoff[2], uvoff[2], xvoff[2];
   bool wthere[2], xthere[2];                           // whether this lane's chunk of the last block is one of K's
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int row = wv * 16 + j * 8 + (lane >> 3), feat = GLU ? row : (row & 31) + 2 * (row & 96);
-    const unsigned wch = (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u;
+    const int row = SPREAD ? wv * 8 + (lane >> 3) : wv * 16 + j * 8 + (lane >> 3), feat = GLU ? row : (row & 31) + 2 * (row & 32);
+    const unsigned wch = (unsigned)((lane & 7) ^ (((row >> 1) & 1) | ((row >> 2) & 6))) * 16u, xch = (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
     wvoff[j] = (unsigned)feat * (unsigned)W.ld + wch;
-    uvoff[j] = GLU ? (unsigned)feat * (unsigned)U.ld + wch : wvoff[j] + 32u * (unsigned)W.ld;
-    xvoff[j] = (unsigned)row * (unsigned)X.ld + (unsigned)((lane & 7) ^ ((row >> 1) & 7)) * 16u;
-    wthere[j] = (nkt - 1) * 128 + (int)wch < K;
-    xthere[j] = (nkt - 1) * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16 < K;
+    uvoff[j] = GLU ? (unsigned)feat * (unsigned)U.ld + wch : wvoff[j];
+    xvoff[j] = (unsigned)row * (unsigned)X.ld + xch;
+    wthere[j] = (nkt - 1) * 128 + (int)wch < K, xthere[j] = (nkt - 1) * 128 + (int)xch < K;
   }
-  const unsigned x1off = 128u * (unsigned)X.ld;
-  unsigned char* const fill0 = smem + (unsigned)wv * 2048u;
+  unsigned char* const fill0 = smem + (unsigned)wv * (SPREAD ? 1024u : 2048u);
+  constexpr unsigned SECOND = SPREAD ? 8192 : 1024;
   // beyond the last block the descriptors are empty and the scales the last block's: into stages that nobody reads
-  const auto there = [&](int kt, int j, bool w, unsigned off) __attribute__((always_inline)) {
-    return TAIL && kt == nkt - 1 && !(w ? wthere[j] : xthere[j]) ? 0x80000000u : off;
+  const auto fetch = [&](int kt, const uint8_t* base, unsigned bytes, unsigned skip, unsigned voff, bool there, unsigned to) __attribute__((always_inline)) {
+    const rsrc_t rs = make_rsrc(base + skip, kt < nkt && bytes > skip ? bytes - skip : 0);
+    fill16(rs, TAIL && kt == nkt - 1 && !there ? 0x80000000u : voff, (unsigned)kt * 128u, fill0 + to);
   };
   const auto fetch_w = [&](int kt, unsigned stage) __attribute__((always_inline)) {
-    const bool in = kt < nkt;
-    const rsrc_t rw = make_rsrc(wb, in ? wbytes : 0), ru = make_rsrc(ub, in ? ubytes : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(rw, there(kt, j, true, wvoff[j]), (unsigned)kt * 128u, fill0 + stage + j * 1024);
+    for (int j = 0; j < 2; ++j) fetch(kt, wb, wbytes, SPREAD ? (unsigned)(j * NF / 2) * (unsigned)W.ld : 0u, wvoff[j], wthere[j], stage + j * SECOND);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(ru, there(kt, j, true, uvoff[j]), (unsigned)kt * 128u, fill0 + stage + F8_PART + j * 1024);
+    for (int j = 0; j < 2; ++j)
+      fetch(kt, ub, ubytes, !SPREAD ? 0u : GLU ? (unsigned)(j * 64) * (unsigned)U.ld : (unsigned)(j * 128 + 32) * (unsigned)W.ld, uvoff[j], wthere[j],
+            stage + F8_PART + j * SECOND);
   };
   const auto fetch_x = [&](int kt, unsigned stage, int h) __attribute__((always_inline)) {
-    const rsrc_t rx = make_rsrc(xb, kt < nkt ? xbytes : 0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fill16(rx, there(kt, j, false, xvoff[j] + (h ? x1off : 0u)), (unsigned)kt * 128u, fill0 + stage + (2 + h) * F8_PART + j * 1024);
+    for (int j = 0; j < 2; ++j)
+      fetch(kt, xb, xbytes, (unsigned)(h * 128 + (SPREAD ? j * 64 : 0)) * (unsigned)X.ld, xvoff[j], xthere[j], stage + (2 + h) * F8_PART + j * SECOND);
   };
   const auto fetch_s = [&](int kt, unsigned third) __attribute__((always_inline)) {
     fill4(sp + (long long)min(kt, nkt - 1) * sstep, smem + F8_SCALES + third + (unsigned)wv * 256u);
