@@ -437,6 +437,20 @@ def test_slices_of_k(fs, M, N, K, dtype):
     assert 1 <= lib.fstu_fp8_linear_slices(M, N, K, dt) <= 16
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 50, 200000), (300, 130, 70001), (2, 200001, 64), (5, 50257, 144), (40, 70001, 16), (70000, 1, 130), (20000, 3, 100), (1, 1, 1)])
+def test_one_long_side(fs, M, N, K, dtype):
+    xc, xs, x = make_codes((M, K), 1, 1)
+    wc, ws, w = make_codes((N, K), 2, 128)
+    bias = torch.randn(N, generator=gen(3)).to(dtype)
+    ref = x @ w.t()
+    check_product(fs.linear_fp8(xc, xs, wc, ws, bias=bias.cuda()), ref + bias.double(), dot_bound(x, w, K, dtype) + 2.0 ** -23 * ref.abs(), dtype)
+    if dtype == torch.bfloat16:
+        ws = ws * (2 * K ** -0.5)
+        got, want = fs.glu_fp8(xc, xs, wc, ws, wc, ws, quantize=True), fs.quantize_fp8(fs.glu_fp8(xc, xs, wc, ws, wc, ws))
+        assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+
+
 def test_more_than_32_bits_of_offsets(fs):
     """Codes of over 4 GiB, activations of over 8: the first and last rows are those of a call on them alone, to the bit (a norm of this width
     adds a row's squares in one order, whatever the number of rows)."""
