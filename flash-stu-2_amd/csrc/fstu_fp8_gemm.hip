@@ -14,6 +14,7 @@
 //   glu     y = T( gelu_tanh(gate) * up )                  (swiglu.py:23-26), or codes and scales of that y (bf16), as
 //           fstu_fp8_quantize_rows makes them of it
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 #include "fstu_fp8.h"
@@ -745,12 +746,35 @@ int skinny_launch(const Codes& X, const Codes& W, const Codes& V, const Leave& o
     hipLaunchKernelGGL((fp8_join_kernel<T>), dim3((unsigned)(((long long)M * N + 255) / 256)), dim3(256), 0, s, partial, o, M, N, slices);
   return 0;
 }
+#define F8_LONG 24                                // blocks of K beyond which the compute units work in rounds of one tile
+// Tiles of 16 rows and features, or of 32.
+long long skinny_groups(int M, int N, int slices) {
+  const int t = M <= 16 ? 16 : 32;
+  return ((N + t - 1) / t) * (long long)((M + t - 1) / t) * slices;
+}
+// Tiles of 64 rows where K is long and 32 rows take a second round: 500 x 768 x 9216 18.4 us, 16.4 so (300 rows, one round, 10.3 and 15.6; 1000, three and two
+// rounds, 26.4 and 30.8; short K 300 x 2304 x 768 6.4 and 9.8).
+bool skinny_64(int M, int N, int nb, int slices) {
+  return M > 32 && nb > F8_LONG && skinny_groups(M, N, slices) > fstu_cus() && ((N + 31) / 32) * (long long)((M + 63) / 64) * slices <= fstu_cus();
+}
 template <typename T, bool TAIL>
 int skinny_linear(const Codes& X, const Codes& W, const Leave& o, float* partial, int slices, int M, int N, int K, hipStream_t s) {
   const char* const name = "fstu_fp8_linear";
-  if (M <= 16) return skinny_launch<T, 0, 1, 1, 1, 16, 1, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
-  if (M <= 32) return skinny_launch<T, 0, 2, 2, 1, 16, 1, 1, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
-  return skinny_launch<T, 0, 4, 2, 1, 8, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  // eight waves to a tile, or four where the tiles are many or K is short: waves without a block of their own hold up the next workgroup.  us, 16 / 8 / 4
+  // waves: 8 rows, 50304 x 768 34 / 12.5 / 9.0, 9216 x 768 7.3 / 3.7 / 3.4, 2048 x 2048 3.6 / 3.3 / 3.5, 768 x 9216 5.3 / 5.3 / 6.9 (fp32, whose codes are widened
+  // beside the loads, 5.7 / 6.1 / 8.3, so sixteen); 32 rows, 50304 x 768 28 / 17 / 15, 2048 x 24576 in four slices 14.3 / 13.9 / 16.4, 768 x 9216 in four
+  // 6.9 / 6.7 / 7.7; 300 x 2304 x 768 - / 7.5 / 6.4, 300 x 768 x 9216 - / 10.3 / 14.9.
+  const int nb = ((K + 127) / 128 + slices - 1) / slices;
+  const long long groups = skinny_groups(M, N, slices);
+  if (M <= 16) {
+    if (nb <= 8 || groups > 2 * fstu_cus()) return skinny_launch<T, 0, 1, 1, 1, 4, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+    if constexpr (sizeof(T) == 4)
+      if (nb > F8_LONG && groups <= fstu_cus()) return skinny_launch<T, 0, 1, 1, 1, 16, 1, 4, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+    return skinny_launch<T, 0, 1, 1, 1, 8, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  }
+  if (skinny_64(M, N, nb, slices)) return skinny_launch<T, 0, 4, 2, 1, 8, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  if (nb <= F8_LONG && groups > 2 * fstu_cus()) return skinny_launch<T, 0, 2, 2, 1, 4, 1, 2, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
+  return skinny_launch<T, 0, 2, 2, 1, 8, 1, 1, TAIL>(X, W, W, o, partial, slices, M, N, K, s, name);
 }
 template <typename T, bool TAIL>
 int skinny_glu(const Codes& X, const Codes& W, const Codes& V, const Leave& o, int M, int N, int K, hipStream_t s) {
@@ -1168,24 +1192,29 @@ int tile(const Codes& X, const Codes& W, const Codes& U, const Leave& o, float* 
   return rc;
 }
 
-// Which kernel a product runs on, and in how many slices of K: the least of an estimate in us, fitted to 330 products of 40 to 8192 rows, 128 to
-// 24576 features and K = 256 to 24576, which is within a tenth of the best nearly everywhere.  SKINNY and TILE are priced by rounds of
-// workgroups over the compute units, each with a start and an end of its own, a block of K the dearer the more of the chip is at work.
-// us, skinny / tile / large.  Linear, rows x features x K: 500 x 768 x 768 5.3 / 8.3 / 15.7, 3000 14 / 8.8 / 16; 200 x 2048 x 2048 6.9 / 12.8 / 26,
-// 800 23 / 13 / 26, 4096 - / 24 / 29, 8192 - / 44 / 38; 500 x 768 x 9216 16 / 39 / 87, 2000 46 / 40 / 87, 8192 - / 65 / 88; fp32 500 x 768 x
-// 768 5.7 / 12.4, 2000 15 / 13.  Gated pair: 64 x 9216 x 768 7.4 / 6.8 / 10.5, 300 26 / 9.5 / 13.4, 500 - / 15.2 / 14.4, 1200 - / 26.8 / 27, 4096 - / 79
-// / 69; 2000 x 24576 x 2048 - / 217 / 175.
+// Which kernel a product runs on, and in how many slices of K: the least of an estimate in us, fitted to some 500 products of 1 to 8192 rows, 128 to
+// 24576 features and K = 256 to 24576, which is within a tenth of the best nearly everywhere.  TILE is priced by rounds of workgroups over the
+// compute units, each with a start and an end of its own, SKINNY by the longest of one workgroup's time, that of all of them at the chip's rate
+// and the weights' bytes.
+// us, skinny / tile / large.  Linear, rows x features x K: 500 x 768 x 768 5.2 / 8.3 / 15.7, 1000 6.5 / 8.3, 3000 - / 8.8 / 16; 200 x 2048 x 2048 6.4 / 12.8 /
+// 26, 600 14.4 / 12.5 / 26, 4096 - / 23 / 29, 8192 - / 44 / 38; 500 x 768 x 9216 16 / 39 / 87, 1000 26 / 22, 2000 - / 29 / 87, 8192 - / 65 / 88; fp32 500 x
+// 768 x 768 5.4 / 12.4, 1500 10.6 / 13.  Gated pair: 64 x 9216 x 768 7.4 / 6.8 / 10.5, 300 26 / 9.5 / 13.4, 500 - / 15.2 / 14.4, 1200 - / 26.8 / 27, 4096
+// - / 79 / 69; 2000 x 24576 x 2048 - / 217 / 175.
 enum Kind { SKINNY, TILE, LARGE };
 struct Plan { Kind kind; int slices; double us; };
 double estimate(Kind kind, int slices, int M, int N, int K, bool f32, bool glu) {
   const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
   const long long nb = up(up(K, 128), slices), cus = fstu_cus();
-  double us = slices > 1 ? 2.2 + (double)slices * M * N * 8 / 3e6 : 0.0;
+  double us = slices > 1 ? (kind == SKINNY ? 0.4 + 0.37 * slices : 2.2) + (double)slices * M * N * 8 / 3e6 : 0.0;
   if (kind == SKINNY) {
-    const int wide = M <= 16 ? 0 : M <= 32 ? 1 : 2;
-    static const double start[3] = {2.1, 2.8, 3.5}, block[2][3] = {{0.034, 0.073, 0.15}, {0.04, 0.09, 0.2}};
-    const long long groups = up(N, wide ? 32 : 16) * up(M, 16 << wide) * slices;
-    return us + 1.0 + (double)up(groups, cus) * (start[wide] + block[f32][wide] * nb) + (double)N * K * 6e-8;
+    const bool one = M <= 16;
+    const double groups = (double)skinny_groups(M, N, slices);
+    const double bytes = 1.5 + (double)N * K / (5.3e6 * std::sqrt(std::sqrt(std::min(1.0, groups / cus))));     // fewer compute units draw less
+    if (one)
+      return us + std::max(bytes, std::max(f32 ? 2.7 + 0.04 * nb : 2.6 + 0.036 * nb, 2.0 + groups * (0.0011 + (f32 ? 0.0002 : 0.00017) * nb)));
+    if (skinny_64(M, N, (int)nb, slices)) return us + std::max(bytes, 1.5 + (f32 ? 4.2 + 0.205 * nb : 4.2 + 0.15 * nb));
+    if (nb > F8_LONG) return us + std::max(bytes, 1.5 + std::ceil(groups / cus) * (f32 ? 1.5 + 0.112 * nb : 1.6 + 0.098 * nb));
+    return us + std::max(bytes, std::max(f32 ? 3.6 + 0.1 * nb : 3.4 + 0.08 * nb, 2.2 + groups * (0.0035 + (f32 ? 0.00044 : 0.00038) * nb)));
   }
   if (kind == TILE) {
     const long long tiles = up(N, glu ? 64 : 128) * up(M, 128) * slices;
@@ -1212,8 +1241,13 @@ Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {
     return {us < estimate(LARGE, 1, M, N, K, false, true) ? TILE : LARGE, 1, us};
   }
   // the pair of more rows adds its blocks in one order on all kernels, so that its codes are those of its bf16 result
-  Plan best = {TILE, 1, estimate(TILE, 1, M, N, K, f32, glu)};
-  if (!glu) best = {SKINNY, std::max(slices, 1), estimate(SKINNY, std::max(slices, 1), M, N, K, f32, glu)};
+  const int least = std::max(slices, 1);
+  const bool skinny = !glu && M <= 65535 * 32;           // rows over the grid's third side
+  Plan best = {TILE, least, estimate(TILE, least, M, N, K, f32, glu)};
+  if (skinny) {
+    const double us = estimate(SKINNY, least, M, N, K, f32, glu);
+    if (few || us < best.us) best = {SKINNY, least, us};
+  }
   const auto take = [&](Kind kind, int s) {
     // a slice's second launch and sums cost a caller's host what a short call takes as well: they have to gain a microsecond
     const double us = estimate(kind, s, M, N, K, f32, glu) + (slices == 0 && s > 1 ? 1.0 : 0.0);
@@ -1222,11 +1256,10 @@ Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {
   const int nb = (K + 127) / 128;
   static const int counts[] = {2, 3, 4, 6, 8, 12, 16};
   if (slices <= 1 && big && !few) take(LARGE, 1);
-  if (!few) take(TILE, std::max(slices, 1));
   if (slices == 0 && !glu)
     for (const int s : counts) {
       if (s > nb) break;
-      take(SKINNY, s);
+      if (skinny) take(SKINNY, s);
       if (!few) take(TILE, s);
     }
   return best;
