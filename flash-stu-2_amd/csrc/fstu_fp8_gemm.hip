@@ -1134,7 +1134,7 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
   __syncthreads();
   const int f = n0 + (int)(threadIdx.x & (NF - 1));
   if (f >= N) return;
-  float bias = 0.f;
+  float bias = -0.f;                                   // nothing: keeps the sign of a zero, which a code has too
   if (!GLU && o.bias && slices == 1) bias = DT<T>::ld((const T*)o.bias + f);
   constexpr int STEP = 256 * GROUPS / NF;
   const int end = min(128, M - m0);

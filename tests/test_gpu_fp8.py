@@ -293,6 +293,19 @@ def test_codes_of_the_pair_are_those_of_its_result(fs, M, N, K):
     assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
 
 
+@pytest.mark.parametrize("M,N,K", [(8, 300, 128), (30, 300, 100), (40, 300, 100), (40, 300, 112), (300, 300, 144), (300, 300, 1001), (200, 1500, 1001), (700, 2304, 1001), (1000, 1000, 256), (2100, 700, 384)])
+def test_codes_of_closed_gates_are_those_of_the_result(fs, M, N, K):
+    """Gates of tens: half of the activations are zeros, some of them negative ones."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = fs.quantize_fp8(torch.randn(M, K, generator=g, device="cuda"))
+    gate, up = (fs.quantize_weight_fp8(torch.randn(N, K, generator=g, device="cuda") * 3) for _ in range(2))
+    codes, scales = fs.glu_fp8(*x, *gate, *up, quantize=True)
+    y = fs.glu_fp8(*x, *gate, *up)
+    want, want_s = fs.quantize_fp8(y)
+    assert float((y == 0).float().mean()) > 0.2
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
+
+
 @pytest.mark.parametrize("M", [1, 8, 40, 300])
 def test_a_row_that_is_not_finite_stays_by_itself(fs, M):
     N, K = 200, 512
@@ -481,7 +494,7 @@ def test_more_than_32_bits_of_offsets(fs):
 
 
 @pytest.mark.parametrize("M", [3, 50, 300])
-@pytest.mark.parametrize("K", [260, 9000])
+@pytest.mark.parametrize("K", [260, 272, 9000])
 def test_rows_far_apart(fs, M, K):
     """Row strides beyond what a tile's 32-bit offsets cover take another kernel, and no slices of K."""
     N, far = 70, (1 << 23) + 16
