@@ -77,9 +77,9 @@ __device__ __forceinline__ unsigned size8(const float (&v)[8]) {
   for (int e = 1; e < 8; ++e) m = max(m, fp8_size(v[e]));
   return m;
 }
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float times) {
-  return make_uint2(fp8_pack4(v[0] * times, v[1] * times, v[2] * times, v[3] * times),
-                    fp8_pack4(v[4] * times, v[5] * times, v[6] * times, v[7] * times));
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], const fp8_cut<T>& cut) {
+  return make_uint2(fp8_pack4(cut(v[0]), cut(v[1]), cut(v[2]), cut(v[3])), fp8_pack4(cut(v[4]), cut(v[5]), cut(v[6]), cut(v[7])));
 }
 
 // One block of a row per 16 lanes.
@@ -94,7 +94,7 @@ fp8_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ co
   load8<T, VEC>(x + row * ldx, c, d, v);
   const float most = __uint_as_float(fp8_max16(size8(v)));
   if (u >= units) return;
-  if (c < d) *(uint2*)(codes + row * ldc + c) = codes8(v, fp8_times(most));
+  if (c < d) *(uint2*)(codes + row * ldc + c) = codes8(v, fp8_cut<T>(most));
   if ((threadIdx.x & 15) == 0) scales[row * ss + b * sb] = fp8_scale(most);
 }
 
@@ -144,13 +144,15 @@ fp8_rmsnorm_kernel(const T* x, long long ldx, const T* delta, long long ldd, T* 
     const int c = c0 + i * W * 512;
     const float most = __uint_as_float(fp8_max16(size8(v[i])));
     const float norm = most * rms;                               // amax of the normed values: NaN where one of them is not a number
-    float times = norm == norm ? FP8_MOST / most : norm;
+    uint2 out;
     if (norm < FP8_LEAST || most < FP8_LEAST) {                  // next to nothing: 448 / most would not be a number
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] *= rms;
-      times = fp8_times(norm);
+      out = codes8(v[i], fp8_cut<float>(norm));
+    } else {
+      out = codes8(v[i], fp8_cut<T>(norm == norm ? most : norm));
     }
-    if (c < d) *(uint2*)(codes + (size_t)row * ldc + c) = codes8(v[i], times);
+    if (c < d) *(uint2*)(codes + (size_t)row * ldc + c) = out;
     if ((lane & 15) == 0 && c < d) scales[row * ss + (c >> 7) * sb] = fp8_scale(norm);
   }
 }
@@ -176,11 +178,12 @@ fp8_weight_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ 
   m = max((unsigned)__builtin_amdgcn_readlane((int)m, 0), (unsigned)__builtin_amdgcn_readlane((int)m, 32));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
-  const float most = __uint_as_float(max(max(part[0], part[1]), max(part[2], part[3]))), times = fp8_times(most);
+  const float most = __uint_as_float(max(max(part[0], part[1]), max(part[2], part[3])));
+  const fp8_cut<T> cut(most);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    if (r < N && c < K) *(uint2*)(codes + (size_t)r * ldc + c) = codes8(v[i], times);
+    if (r < N && c < K) *(uint2*)(codes + (size_t)r * ldc + c) = codes8(v[i], cut);
   }
   if (threadIdx.x == 0) scales[blockIdx.y * ss + blockIdx.x * sb] = fp8_scale(most);
 }

@@ -144,10 +144,11 @@ fp8_plain_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K) {
         unsigned bits = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) bits = max(bits, part[i][j * 16 + l16]);
-        const float most = __uint_as_float(bits), times = fp8_times(most);
+        const float most = __uint_as_float(bits);
+        const fp8_cut<bf16_t> cut(most);
         const int m = m0 + j * 16 + l16;
         if (m < M && f0 < N)                                // a row's codes lie in whole 16 bytes: zeros behind the last feature
-          *(unsigned*)((uint8_t*)o.y + (size_t)m * o.ldy + f0) = fp8_pack4(acc[j][0] * times, acc[j][1] * times, acc[j][2] * times, acc[j][3] * times);
+          *(unsigned*)((uint8_t*)o.y + (size_t)m * o.ldy + f0) = fp8_pack4(cut(acc[j][0]), cut(acc[j][1]), cut(acc[j][2]), cut(acc[j][3]));
         if (m < M && wv == 0 && q == 0) o.s[m * o.sr + blockIdx.x * o.sb] = fp8_scale(most);
       }
       return;
@@ -484,12 +485,13 @@ fp8_large_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K, int mt
         for (int j = 0; j < 4; ++j) {
           u32x4_t v = lds16<0>(fm + (unsigned)(h * 128 + j * 16) * 16u);
           asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v)::"memory");
-          const float most = __uint_as_float(max(max(v[0], v[1]), max(v[2], v[3]))), times = fp8_times(most);
+          const float most = __uint_as_float(max(max(v[0], v[1]), max(v[2], v[3])));
+          const fp8_cut<bf16_t> cut(most);
           const int m = em0 + h * 128 + wm * 64 + j * 16 + l16, f = en0 + wn * 32 + 8 * lq;
           const floatx4_t a = acc[0][h][j], b = acc[1][h][j];
           if (m < M && f < N)                          // a row's codes lie in whole 16 bytes: zeros behind the last feature
-            *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + f) = make_uint2(fp8_pack4(a[0] * times, a[1] * times, a[2] * times, a[3] * times),
-                                                                          fp8_pack4(b[0] * times, b[1] * times, b[2] * times, b[3] * times));
+            *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + f) = make_uint2(fp8_pack4(cut(a[0]), cut(a[1]), cut(a[2]), cut(a[3])),
+                                                                          fp8_pack4(cut(b[0]), cut(b[1]), cut(b[2]), cut(b[3])));
           if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (en0 >> 7) * o.sb] = fp8_scale(most);
         }
     } else {
@@ -685,8 +687,8 @@ fp8_skinny_kernel(Codes X, Codes W, Codes V, Leave o, float* __restrict__ partia
       unsigned a = 0;
 #pragma unroll
       for (int i = 0; i < NT; ++i) a = max(a, most[i * 16 * R + r * 16 + l16]);
-      const float times = fp8_times(__uint_as_float(a));
-      if (fe < N) *(unsigned*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = fp8_pack4(v[0] * times, v[1] * times, v[2] * times, v[3] * times);
+      const fp8_cut<bf16_t> cut(__uint_as_float(a));
+      if (fe < N) *(unsigned*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = fp8_pack4(cut(v[0]), cut(v[1]), cut(v[2]), cut(v[3]));
       if (nt == 0 && q == 0) o.s[m * o.sr + blockIdx.x * o.sb] = fp8_scale(__uint_as_float(a));
     }
     return;
@@ -1052,12 +1054,13 @@ fp8_tile_kernel(Codes X, Codes W, Codes U, Leave o, float* __restrict__ partial,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint4 all = *(const uint4*)(most + (j * 16 + l16) * 4);
-      const float amax = __uint_as_float(max(max(all.x, all.y), max(all.z, all.w))), times = fp8_times(amax);
+      const float amax = __uint_as_float(max(max(all.x, all.y), max(all.z, all.w)));
+      const fp8_cut<bf16_t> cut(amax);
       const int m = m0 + j * 16 + l16;
       const floatx4_t a = acc[0][j], b = acc[1][j];
       if (m < M && fe < N)                             // a row's codes lie in whole 16 bytes: zeros behind the last feature
-        *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = make_uint2(fp8_pack4(a[0] * times, a[1] * times, a[2] * times, a[3] * times),
-                                                                       fp8_pack4(b[0] * times, b[1] * times, b[2] * times, b[3] * times));
+        *(uint2*)((uint8_t*)o.y + (size_t)m * o.ldy + fe) = make_uint2(fp8_pack4(cut(a[0]), cut(a[1]), cut(a[2]), cut(a[3])),
+                                                                       fp8_pack4(cut(b[0]), cut(b[1]), cut(b[2]), cut(b[3])));
       if (m < M && wn == 0 && lq == 0) o.s[m * o.sr + (n0 >> 7) * o.sb] = fp8_scale(amax);
     }
     return;

@@ -1299,7 +1299,8 @@ def _fp8_operand(codes: torch.Tensor, scales: torch.Tensor, per: int, dev: int, 
 
 def quantize_fp8(x: torch.Tensor):
     """Codes and scales of x (rows, d) float32 or bfloat16, one scale for each 128 values of a row: scale = max(amax, 2^-100) / 448,
-    code = x * (448 / max(amax, 2^-100)) to the nearest e4m3 value.  A block with an infinity or a NaN stands for NaN."""
+    code = the e4m3 value nearest to x * 448 / max(amax, 2^-100), ties to the even one (exactly that in bfloat16; the quotient of a float32 x is
+    off by up to 2^-23 of itself).  A block with an infinity or a NaN stands for NaN."""
     dev = x.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):

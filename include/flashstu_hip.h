@@ -701,7 +701,8 @@ int fstu_prof_glu_loop(const fstu_model_desc* m, int reps, double* total_ms, int
  * (what lies between a row's end and the next multiple of 16 is read and has no effect; these entry points write it up to the next
  * multiple of 8); scales are fp32, scale (r, b) at s[r*s_row + b*s_blk], b = k / 128.  A value is code * scale.
  * Rows (activations) have a scale for each 128 values, weights (N,K) one for each 128 x 128, r = n / 128.
- *   scale = max(amax, 2^-100) / 448,  code = v * (448 / max(amax, 2^-100)) to the nearest, ties to the even code.
+ *   scale = max(amax, 2^-100) / 448,  code = the nearest to v * 448 / max(amax, 2^-100), ties to the even code (bf16: exactly; fp32: of a quotient that is
+ *   off by up to 2^-23 of itself).
  * A block with a value that is not finite gets a scale that is not finite either.  dtype: that of x, w, delta, bias, res, y.
  *
  * fstu_fp8_quantize_rows, fstu_fp8_quantize_weight: codes and scales of x (rows,d) / w (N,K), row strides ldx / ldw in elements.

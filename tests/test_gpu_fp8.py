@@ -507,3 +507,51 @@ def test_rows_far_apart(fs, M, K):
     codes, scales = fs.glu_fp8(wide, xs, wc, ws, wc, ws, quantize=True)
     want = fs.quantize_fp8(fs.glu_fp8(wide, xs, wc, ws, wc, ws))
     assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+
+
+# ---------------------------------------------------------------- ties, by whole-number arithmetic
+def nearest(num, den):
+    """The e4m3 value nearest to num / den (|num| <= 448 den), ties to the even one.  num and den in 64 bits, num of at most 27 and den of at most 16
+    bits, so that den times the middle between two codes (5 bits) is exact and nothing is divided."""
+    values = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    middles = (values[1:] + values[:-1]) / 2
+    size = num.abs()
+    at = (torch.bucketize(size / den, middles) - 1).clamp(0, 125)         # at most one too low or one too high
+    for _ in range(3):
+        m = den * middles[at.clamp(max=125)]
+        at = torch.where((at < 126) & ((size > m) | ((size == m) & (at % 2 == 1))), at + 1, at)
+    return torch.copysign(values[at], num)
+
+
+def blocks_of(v, per=1):
+    """Each value's block's amax, laid out as v."""
+    return spread(block_amax(v, per), v.shape, per)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bf16_values_to_the_nearest_code(fs, dtype):
+    """Every 200th quotient of bf16 values is a tie; the same values in fp32 have the same codes."""
+    x = (torch.randn(700, 1000, generator=gen(1)) * torch.exp(0.7 * torch.randn(1, 1000, generator=gen(2)))).bfloat16()
+    v, cuda = x.double(), x.to(dtype).cuda()
+    assert torch.equal(fs.quantize_fp8(cuda)[0].cpu().double(), nearest(v * 448, blocks_of(v)))
+    assert torch.equal(fs.quantize_weight_fp8(cuda)[0].cpu().double(), nearest(v * 448, blocks_of(v, 128)))
+
+
+@pytest.mark.parametrize("d", [512, 768, 1001, 2048, 4096, 8200])
+def test_bf16_norms_to_the_nearest_code(fs, d):
+    """The root mean square is a factor of a block's values and of its amax: the codes are those of the products x * w, of 16 bits."""
+    x, w = torch.randn(200, d, generator=gen(d)).bfloat16(), (1 + 0.2 * torch.randn(d, generator=gen(2))).bfloat16()
+    codes, _ = fs.rms_norm_fp8(x.cuda(), w.cuda(), 1e-6)
+    n = x.double() * w.double()
+    assert torch.equal(codes.cpu().double(), nearest(n * 448, blocks_of(n)))
+
+
+@pytest.mark.parametrize("M,N,K", [(8, 1000, 256), (40, 1000, 250), (60, 1000, 256), (700, 1000, 384), (2100, 1000, 256)])
+def test_the_pair_to_the_nearest_code(fs, M, N, K):
+    """Each kernel that leaves codes, against the bf16 values that the same products leave."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = fs.quantize_fp8(torch.randn(M, K, generator=g, device="cuda"))
+    gate, up = (fs.quantize_weight_fp8(torch.randn(N, K, generator=g, device="cuda") * K ** -0.5) for _ in range(2))
+    codes, _ = fs.glu_fp8(*x, *gate, *up, quantize=True)
+    y = fs.glu_fp8(*x, *gate, *up).cpu().double()
+    assert torch.equal(codes.cpu().double(), nearest(y * 448, blocks_of(y).clamp_min(LEAST)))
