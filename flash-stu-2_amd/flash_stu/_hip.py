@@ -1248,8 +1248,7 @@ def lds_steps(h: torch.Tensor, x: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
 FP8_BLOCK = 128
 _fp8 = torch.float8_e4m3fn
 
-
-_device_now = torch._C._cuda_getDevice
+_device_now = getattr(torch._C, "_cuda_getDevice", None)             # asked where a tensor is on the GPU
 
 
 def _fp8_new(rows: int, cols: int, per: int, device):

@@ -1,5 +1,8 @@
 """What the 8-bit operators refuse, without a GPU: at the C entry points before any launch, and in the Python calls."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -134,3 +137,26 @@ def test_python_calls_refuse_what_does_not_go_together():
     refused(lambda: fs.glu_fp8(c, s, w, ws, w[:129], ws), "do not go together")
     refused(lambda: fs.glu_fp8(c, s, w, ws, w, ws, dtype=torch.float32, quantize=True), "unsupported dtype")
     refused(lambda: fs.glu_fp8(c, s, w, ws.cpu(), w, ws), "not on the GPU")
+
+
+def test_a_torch_without_gpu_bindings_imports_the_package():
+    """And is told by each call that its tensors are not on the GPU."""
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import flash_stu as fs
+x = torch.zeros(2, 128)
+c, s = x.to(torch.float8_e4m3fn), torch.zeros(2, 1)
+for call in (lambda: fs.quantize_fp8(x), lambda: fs.quantize_weight_fp8(x), lambda: fs.rms_norm_fp8(x, torch.ones(128), 1e-6),
+             lambda: fs.linear_fp8(c, s, c, s[:1]), lambda: fs.glu_fp8(c, s, c, s[:1], c, s[:1])):
+    try:
+        call()
+        raise SystemExit("not refused")
+    except RuntimeError as e:
+        assert "not on the GPU" in str(e), e
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    found = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=os.path.join(root, "flash-stu-2_amd")), capture_output=True, text=True)
+    assert found.returncode == 0, found.stderr + found.stdout
