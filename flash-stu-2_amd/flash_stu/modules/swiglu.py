@@ -70,6 +70,17 @@ class FP8MLP(nn.Module):
             self.register_buffer(name + "_codes", codes.as_strided((codes.shape[0], codes.stride(0)), codes.stride()))
             self.register_buffer(name + "_scales", scales)
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves codes and scales as the bits they are: both count as floating point, and .to(dtype) or .float() of a model would round them.  The
+        norm's weight takes the type, as the layers' own do."""
+        def move(t):
+            if not any(t is b for b in self._buffers.values()):
+                return fn(t)
+            bits = t.view(torch.uint8 if t.dtype is torch.float8_e4m3fn else torch.int32)
+            moved = fn(bits)
+            return (moved if moved.dtype is bits.dtype else bits.to(moved.device)).view(t.dtype)
+        return super()._apply(move, recurse)
+
     def _weight(self, name: str, width: int):
         codes = getattr(self, name + "_codes")
         return (codes if codes.shape[1] == width else codes[:, :width]), getattr(self, name + "_scales")

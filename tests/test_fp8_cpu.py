@@ -160,3 +160,46 @@ for call in (lambda: fs.quantize_fp8(x), lambda: fs.quantize_weight_fp8(x), lamb
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     found = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=os.path.join(root, "flash-stu-2_amd")), capture_output=True, text=True)
     assert found.returncode == 0, found.stderr + found.stdout
+
+
+def parts_without_a_gpu(monkeypatch, d=72, scale=3):
+    """An FP8MLP on the CPU: codes and scales from the definition, where the module asks the kernels for them."""
+    import flash_stu as fs
+    from flash_stu import _hip
+    from flash_stu.config import FlashSTUConfig
+    from flash_stu.modules import MLP, RMSNorm
+
+    def codes(w):
+        n, k = w.shape
+        held = torch.zeros(n, (k + 15) & -16, dtype=torch.uint8).view(torch.float8_e4m3fn)[:, :k]
+        held.copy_((w.float() * 50).to(torch.float8_e4m3fn))
+        return held, torch.rand((n + 127) // 128, (k + 127) // 128) / 3
+    monkeypatch.setattr(_hip, "quantize_weight_fp8", codes)
+    cfg = FlashSTUConfig(n_embd=d, n_heads=1, mlp_scale=scale, torch_dtype=torch.bfloat16)
+    return fs.FP8MLP(RMSNorm(d, 1e-6, dtype=torch.bfloat16), MLP(cfg, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("change", [lambda m: m.to(torch.bfloat16), lambda m: m.float(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float32),
+                                    lambda m: m.type(torch.float32), lambda m: m.cpu()])
+@pytest.mark.parametrize("inside", [False, True])
+def test_the_8_bit_mlp_keeps_its_weights_through_a_change_of_type(monkeypatch, change, inside):
+    m = parts_without_a_gpu(monkeypatch)
+    before = {k: v.clone() for k, v in m.state_dict().items()}
+    change(torch.nn.Sequential(m) if inside else m)
+    after = m.state_dict()
+    assert list(after) == list(before)
+    for k, v in before.items():
+        if not k.startswith("norm."):
+            assert after[k].dtype is v.dtype and after[k].stride() == v.stride()
+            assert torch.equal(after[k].view(torch.uint8), v.view(torch.uint8))
+    want = change(torch.nn.Linear(2, 2, dtype=torch.bfloat16)).weight.dtype
+    assert after["norm.weight"].dtype is want
+
+
+def test_the_8_bit_mlp_moves_to_another_device(monkeypatch):
+    m = parts_without_a_gpu(monkeypatch)
+    kinds = {k: v.dtype for k, v in m.state_dict().items()}
+    m.to("meta")
+    assert all(v.device.type == "meta" and v.dtype is kinds[k] for k, v in m.state_dict().items())
+    m.to_empty(device="cpu")
+    assert all(v.device.type == "cpu" and v.dtype is kinds[k] for k, v in m.state_dict().items())

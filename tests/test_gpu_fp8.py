@@ -555,3 +555,13 @@ def test_the_pair_to_the_nearest_code(fs, M, N, K):
     codes, _ = fs.glu_fp8(*x, *gate, *up, quantize=True)
     y = fs.glu_fp8(*x, *gate, *up).cpu().double()
     assert torch.equal(codes.cpu().double(), nearest(y * 448, blocks_of(y).clamp_min(LEAST)))
+
+
+def test_the_mlp_keeps_its_weights_through_a_change_of_type(fs):
+    norm, mlp = layer_parts(200, 3, torch.bfloat16, 4)
+    m = fs.FP8MLP(norm, mlp)
+    x = torch.randn(5, 200, generator=gen(1)).bfloat16().cuda()
+    want = m(x.clone())
+    for change in (lambda: m.to(torch.bfloat16), lambda: m.float().bfloat16(), lambda: m.cpu().cuda(), lambda: torch.nn.Sequential(m).half().to(torch.bfloat16)):
+        change()
+        assert torch.equal(m(x.clone()), want)
