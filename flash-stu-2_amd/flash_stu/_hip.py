@@ -1244,7 +1244,8 @@ def lds_steps(h: torch.Tensor, x: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
 # ---------------------------------------------------------------- 8-bit operators
 # Codes are float8_e4m3fn, (rows, K) with rows a multiple of 16 bytes apart; scales float32, a row's in blocks of 128 values (rows,
 # ceil(K / 128)), a weight's in blocks of 128 x 128 (ceil(N / 128), ceil(K / 128)), any strides.  A value is its code times its
-# block's scale.  What these functions leave has one block's scales of all rows beside each other.
+# block's scale.  What these functions leave has one block's scales of all rows beside each other.  They are forward only: where gradients are on, a
+# tensor that requires one is refused (but for a weight whose codes are made, once, when a model is loaded).
 FP8_BLOCK = 128
 _fp8 = torch.float8_e4m3fn
 
@@ -1296,10 +1297,25 @@ def _fp8_operand(codes: torch.Tensor, scales: torch.Tensor, per: int, dev: int, 
     return codes.data_ptr(), ld if rows > 1 else (K + 15) & -16, scales.data_ptr(), sr, sb
 
 
+def _fp8_cut_off(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether a gradient would be lost without a word: gradients are on and one of the tensors requires one."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _fp8_forward_only(what: str):
+    return NotImplementedError(f"{what} is forward only: call it under torch.no_grad(), or with detached tensors")
+
+
 def quantize_fp8(x: torch.Tensor):
     """Codes and scales of x (rows, d) float32 or bfloat16, one scale for each 128 values of a row: scale = max(amax, 2^-100) / 448,
     code = the e4m3 value nearest to x * 448 / max(amax, 2^-100), ties to the even one (exactly that in bfloat16; the quotient of a float32 x is
     off by up to 2^-23 of itself).  A block with an infinity or a NaN stands for NaN."""
+    if _fp8_cut_off(x):
+        raise _fp8_forward_only("quantize_fp8")
     dev = x.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
@@ -1316,7 +1332,8 @@ def quantize_fp8(x: torch.Tensor):
 
 
 def quantize_weight_fp8(weight: torch.Tensor):
-    """Codes and scales of a weight (N, K) float32 or bfloat16, one scale for each 128 x 128 values (formed as in quantize_fp8)."""
+    """Codes and scales of a weight (N, K) float32 or bfloat16, one scale for each 128 x 128 values (formed as in quantize_fp8).
+    They are constants made of the weight as it is now, whether or not it requires a gradient."""
     dev = weight.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
@@ -1337,6 +1354,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
     """Codes and scales (as quantize_fp8's) of rmsnorm(x) * weight for x (rows, d), d up to 32768; the normed values are not rounded
     to x's type on the way.  delta (rows, d): x + delta, rounded to x's type, is what is normed and is left in x_out (x itself where that is
     not given; a tensor that overlaps x or delta otherwise than as a whole is refused)."""
+    if _fp8_cut_off(x, weight, delta, x_out):
+        raise _fp8_forward_only("rms_norm_fp8")
     dev = x.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
@@ -1378,6 +1397,8 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
     bias, residual and out.  out may be residual; one that
     overlaps it otherwise is refused.  In float32 the sums are those of fp32 products; in bfloat16 the matrix core's 8-bit
     instruction forms them, off by some 2e-5 of the result where its rounding is 2e-3."""
+    if _fp8_cut_off(codes, scales, w_codes, w_scales, bias, residual, out):
+        raise _fp8_forward_only("linear_fp8")
     dev = codes.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
@@ -1430,6 +1451,8 @@ def glu_fp8(codes: torch.Tensor, scales: torch.Tensor, gate_codes: torch.Tensor,
     """y (M, N) = gelu_tanh(x @ gate^T) * (x @ up^T) for x (M, K), gate and up (N, K) as codes with scales, in fp32 and rounded once to
     `dtype` (float32 or bfloat16).  quantize: the codes and scales of quantize_fp8(y) in place of y (bfloat16), in the same launch (in a
     second one for large products of more than 32 rows whose K is no multiple of 16)."""
+    if _fp8_cut_off(codes, scales, gate_codes, gate_scales, up_codes, up_scales):
+        raise _fp8_forward_only("glu_fp8")
     dev = codes.get_device()
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):

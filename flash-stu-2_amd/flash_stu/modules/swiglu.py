@@ -56,7 +56,7 @@ class FP8MLP(nn.Module):
     """The norm and the MLP of a layer with the weights as 8-bit codes: x + delta, then x + down(gelu_tanh(gate(n)) * up(n)) with n = norm(x),
     as the layers form them from RMSNorm and MLP, in three launches (fp32: four).  The codes are laid out here, from the weights as
     they are now, one scale for each 128 x 128; the activations are cut to codes on their way, one scale for each 128 values of a row.  The
-    norm's weight stays the norm's own."""
+    norm's weight stays the norm's own.  Inference only, as RMSNorm and MLP are: nothing here has a gradient."""
 
     def __init__(self, norm: nn.Module, mlp: MLP):
         super().__init__()

@@ -203,3 +203,30 @@ def test_the_8_bit_mlp_moves_to_another_device(monkeypatch):
     assert all(v.device.type == "meta" and v.dtype is kinds[k] for k, v in m.state_dict().items())
     m.to_empty(device="cpu")
     assert all(v.device.type == "cpu" and v.dtype is kinds[k] for k, v in m.state_dict().items())
+
+
+def calls_with(grad_of):
+    """Each operator with one of its tensors asking for a gradient: (name, call)."""
+    import flash_stu as fs
+    g = lambda name, t: t.requires_grad_() if name == grad_of else t
+    x, d, w = g("x", torch.zeros(2, 128)), g("delta", torch.zeros(2, 128)), g("weight", torch.ones(128))
+    c, s = torch.zeros(2, 128).to(torch.float8_e4m3fn), g("scales", torch.zeros(2, 1))
+    wc, ws = torch.zeros(16, 128).to(torch.float8_e4m3fn), g("w_scales", torch.zeros(1, 1))
+    bias, res, out = g("bias", torch.zeros(16)), g("residual", torch.zeros(2, 16)), g("out", torch.zeros(2, 16))
+    return {"quantize_fp8": (("x",), lambda: fs.quantize_fp8(x)), "quantize_weight_fp8": ((), lambda: fs.quantize_weight_fp8(x)),
+            "rms_norm_fp8": (("x", "delta", "weight", "out"), lambda: fs.rms_norm_fp8(x, w, 1e-6, delta=d, x_out=out)),
+            "linear_fp8": (("scales", "w_scales", "bias", "residual", "out"), lambda: fs.linear_fp8(c, s, wc, ws, bias=bias, residual=res, out=out)),
+            "glu_fp8": (("scales", "w_scales"), lambda: fs.glu_fp8(c, s, wc, ws, wc, ws))}
+
+
+@pytest.mark.parametrize("grad_of", ["x", "delta", "weight", "scales", "w_scales", "bias", "residual", "out"])
+def test_a_gradient_that_would_be_lost_is_refused(grad_of):
+    """Results have no graph: a tensor that requires a gradient is refused where gradients are on, and taken where they are off.  A weight
+    is taken as it is: its codes are made when a model is loaded, from its parameters."""
+    from flash_stu._hip import FlashSTUHipError
+    for name, (takes, call) in calls_with(grad_of).items():
+        if grad_of in takes:
+            with pytest.raises(NotImplementedError, match=name + " is forward only"):
+                call()
+        with torch.no_grad(), pytest.raises(FlashSTUHipError, match="not on the GPU"):
+            call()

@@ -565,3 +565,18 @@ def test_the_mlp_keeps_its_weights_through_a_change_of_type(fs):
     for change in (lambda: m.to(torch.bfloat16), lambda: m.float().bfloat16(), lambda: m.cpu().cuda(), lambda: torch.nn.Sequential(m).half().to(torch.bfloat16)):
         change()
         assert torch.equal(m(x.clone()), want)
+
+
+def test_gradients_are_refused_and_their_absence_is_not(fs):
+    x, w = torch.randn(4, 256, device="cuda"), torch.nn.Parameter(torch.ones(256, device="cuda"))
+    with pytest.raises(NotImplementedError, match="rms_norm_fp8 is forward only"):
+        fs.rms_norm_fp8(x, w, 1e-6)
+    with torch.no_grad():
+        codes = fs.rms_norm_fp8(x, w, 1e-6)
+    weight = fs.quantize_weight_fp8(torch.nn.Parameter(torch.randn(32, 256, device="cuda")))
+    res = torch.zeros(4, 32, device="cuda", requires_grad=True) * 2
+    with pytest.raises(NotImplementedError, match="linear_fp8 is forward only"):
+        fs.linear_fp8(*codes, *weight, residual=res)
+    with torch.inference_mode():
+        want = fs.linear_fp8(*codes, *weight, residual=res)
+    assert torch.equal(fs.linear_fp8(*codes, *weight, residual=res.detach()), want) and not want.requires_grad
