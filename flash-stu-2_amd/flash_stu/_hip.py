@@ -1306,6 +1306,9 @@ def _fp8_cut_off(*ts: Optional[torch.Tensor]) -> bool:
     return False
 
 
+_written = torch.autograd.graph.increment_version        # a caller's tensor was written: a graph that has saved its old values must not use these
+
+
 def _fp8_forward_only(what: str):
     return NotImplementedError(f"{what} is forward only: call it under torch.no_grad(), or with detached tensors")
 
@@ -1382,6 +1385,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: Optio
                                      scales.data_ptr(), 1, rows, rows, d, dt, raw_stream(dev))
         if rc:
             _check(rc, "fstu_fp8_rmsnorm")
+        if delta is not None:
+            _written(x if x_out is None else x_out)
     return codes, scales
 
 
@@ -1417,7 +1422,8 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
         dt = FSTU_F32
     else:
         raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldy = torch.empty(M, N, dtype=dtype, device=codes.device), N
     else:
         ldy = _fp8_result(out, M, N, dtype, dev, "out")
@@ -1435,6 +1441,8 @@ def linear_fp8(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Tensor,
         rc = load().fstu_fp8_linear(xp, xl, xs, xr, xb, wp, wl, ws, wr, wb, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, dt, _p(sums), slices, raw_stream(dev))
         if rc:
             _check(rc, "fstu_fp8_linear")
+        if given:
+            _written(out)
     return out
 
 

@@ -580,3 +580,28 @@ def test_gradients_are_refused_and_their_absence_is_not(fs):
     with torch.inference_mode():
         want = fs.linear_fp8(*codes, *weight, residual=res)
     assert torch.equal(fs.linear_fp8(*codes, *weight, residual=res.detach()), want) and not want.requires_grad
+
+
+def test_what_is_written_in_place_is_known_to_autograd(fs):
+    """A graph that has saved a tensor's values refuses its backward pass once they have been written over, as behind torch's own in-place operations."""
+    def stale(write):
+        x, w = torch.randn(4, 256, device="cuda"), torch.randn(4, 256, device="cuda", requires_grad=True)
+        y = (x.view(2, 512) * w.view(2, 512)).sum()                       # saves a view of x
+        write(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    one, d = torch.ones(256, device="cuda"), torch.randn(4, 256, device="cuda")
+    codes, weight = fs.quantize_fp8(d), fs.quantize_weight_fp8(torch.randn(256, 256, device="cuda"))
+    stale(lambda x: fs.rms_norm_fp8(x, one, 1e-6, delta=d))
+    stale(lambda x: fs.rms_norm_fp8(d, one, 1e-6, delta=d.clone(), x_out=x))
+    stale(lambda x: fs.linear_fp8(*codes, *weight, residual=x, out=x))
+    stale(lambda x: fs.linear_fp8(*codes, *weight, out=x, dtype=torch.float32))
+    norm, mlp = layer_parts(256, 2, torch.float32, 1)
+    stale(fs.FP8MLP(norm, mlp))
+    version = d._version                                                  # what is only read stays valid
+    fs.quantize_fp8(d), fs.rms_norm_fp8(d, one, 1e-6), fs.linear_fp8(*codes, *weight, residual=d)
+    assert d._version == version
+    with torch.inference_mode():                                          # tensors without a version
+        x = torch.randn(4, 256, device="cuda")
+        fs.rms_norm_fp8(x, one, 1e-6, delta=d)
+        fs.linear_fp8(*codes, *weight, residual=x, out=x)
