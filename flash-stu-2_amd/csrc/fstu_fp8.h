@@ -34,16 +34,18 @@ template <typename T> struct fp8_cut;
 // units too large, and without its last two bits on the tie or on its own side of it: one instruction a value.
 template <> struct fp8_cut<bf16_t> {
   float times;
-  __device__ __forceinline__ explicit fp8_cut(float most)
-      : times(most < __builtin_inff() ? __uint_as_float(__float_as_uint(FP8_MOST / (most < FP8_LEAST ? FP8_LEAST : most)) + 1u) : __builtin_nanf("")) {}
+  __device__ __forceinline__ explicit fp8_cut(float most, bool ordinary = false) {      // ordinary: finite and at least 2^-100
+    if (!ordinary && most < FP8_LEAST) most = FP8_LEAST;
+    times = ordinary || most < __builtin_inff() ? __uint_as_float(__float_as_uint(FP8_MOST / most) + 1u) : __builtin_nanf("");
+  }
   __device__ __forceinline__ float operator()(float v) const { return __uint_as_float(__float_as_uint(v * times) & ~3u); }
 };
 // fp32: the quotient, corrected by its remainder v * 448/512 - q * most/512, which is exact for values of up to 21 bits.
 template <> struct fp8_cut<float> {
   float times, most, inv;
-  __device__ __forceinline__ explicit fp8_cut(float m) {
-    m = m < FP8_LEAST ? FP8_LEAST : m;
-    times = m < __builtin_inff() ? FP8_MOST / m : __builtin_nanf(""), most = m * (1.f / 512.f), inv = times * (512.f / FP8_MOST);
+  __device__ __forceinline__ explicit fp8_cut(float m, bool ordinary = false) {
+    if (!ordinary && m < FP8_LEAST) m = FP8_LEAST;
+    times = ordinary || m < __builtin_inff() ? FP8_MOST / m : __builtin_nanf(""), most = m * (1.f / 512.f), inv = times * (512.f / FP8_MOST);
   }
   __device__ __forceinline__ float operator()(float v) const {
     const float q = v * times;

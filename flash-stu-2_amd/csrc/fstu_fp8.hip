@@ -49,6 +49,16 @@ __device__ __forceinline__ void load8(const T* p, int c, int d, float (&v)[8]) {
     }
   }
 }
+// The same where few rows ever come: one by one in place of unaligned vectors, whose registers and code all other rows would pay for.
+template <typename T, bool VEC>
+__device__ __forceinline__ void again8(const T* p, int c, int d, float (&v)[8]) {
+  if constexpr (VEC) {
+    load8<T, true>(p, c, d, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < d ? DT<T>::ld(p + c + e) : 0.f;
+  }
+}
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, int c, int d, const float (&v)[8]) {
   if (VEC ? c < d : c + 8 <= d) {
@@ -129,28 +139,48 @@ fp8_rmsnorm_kernel(const T* x, long long ldx, const T* delta, long long ldd, T* 
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e], v[i][e], sum), v[i][e] *= g[i][e];
-  sum = wave_sum(sum);
-  if constexpr (W > 1) {
-    __shared__ float part[W];
-    if (lane == 0) part[wv] = sum;
-    __syncthreads();
-    sum = 0.f;
+  __shared__ float part[2][W];
+  const auto join = [&](float s, int turn) __attribute__((always_inline)) {     // over the lanes and waves of the row
+    s = wave_sum(s);
+    if constexpr (W > 1) {
+      if (lane == 0) part[turn][wv] = s;
+      __syncthreads();
+      s = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) sum += part[i];
+      for (int i = 0; i < W; ++i) s += part[turn][i];
+    }
+    return s;
+  };
+  const T* const src = delta ? xo + (size_t)row * ldo : x + (size_t)row * ldx;     // what is normed: a lane has read, or written, all that it reads here again
+  float up = 1.f;
+  sum = join(sum, 0);
+  if (__builtin_expect(sum == __builtin_inff(), 0)) {                                 // squares beyond fp32 (values of 1e17 and more): those of 2^-80 of the values
+    up = 0x1p-80f, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      again8<T, VEC>(src, c0 + i * W * 512, d, g[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[i][e] *= up, sum = fmaf(g[i][e], g[i][e], sum);
+    }
+    sum = join(sum, 1);
   }
-  const float rms = 1.0f / sqrtf(sum / (float)d + eps);
+  const float rms = 1.0f / sqrtf(sum / (float)d + eps * up * up);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + i * W * 512;
     const float most = __uint_as_float(fp8_max16(size8(v[i])));
-    const float norm = most * rms;                               // amax of the normed values: NaN where one of them is not a number
+    float norm = most * up * rms;                                // amax of the normed values: NaN where one of them is not a number
     uint2 out;
-    if (norm < FP8_LEAST || most < FP8_LEAST) {                  // next to nothing: 448 / most would not be a number
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] *= rms;
-      out = codes8(v[i], fp8_cut<float>(norm));
+    if (__builtin_expect(norm >= FP8_LEAST && most >= FP8_LEAST && most < __builtin_inff(), 1)) {
+      out = codes8(v[i], fp8_cut<T>(most, true));
     } else {
-      out = codes8(v[i], fp8_cut<T>(norm == norm ? most : norm));
+      // next to nothing, not a number, or products x * w beyond fp32's range whose normed values are not: these themselves, from the row as it was read
+      again8<T, VEC>(src, c, d, v[i]);
+      again8<T, VEC>(w, c, d, g[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * up * rms * g[i][e];
+      norm = __uint_as_float(fp8_max16(size8(v[i])));            // all of the 16 lanes are here
+      out = codes8(v[i], fp8_cut<float>(norm));
     }
     if (c < d) *(uint2*)(codes + (size_t)row * ldc + c) = out;
     if ((lane & 15) == 0 && c < d) scales[row * ss + (c >> 7) * sb] = fp8_scale(norm);

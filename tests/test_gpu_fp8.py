@@ -605,3 +605,20 @@ def test_what_is_written_in_place_is_known_to_autograd(fs):
         x = torch.randn(4, 256, device="cuda")
         fs.rms_norm_fp8(x, one, 1e-6, delta=d)
         fs.linear_fp8(*codes, *weight, residual=x, out=x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("size,weight,eps", [(1e-12, 1e-28, 1e-26), (1e-15, 1e-26, 1e-32), (1e14, 1e26, 1e-6), (1e18, 1e30, 1e-6)])
+def test_rms_norm_of_products_beyond_fp32(fs, size, weight, eps, add, dtype):
+    """x * w leaves fp32's range, above or below, where rmsnorm(x) * w is well inside it; the first half of each row is ordinary."""
+    x = (torch.randn(6, 600, generator=gen(1)) * size).to(dtype)
+    w = torch.cat([torch.ones(300), torch.full((300,), weight)]).mul(1 + 0.2 * torch.randn(600, generator=gen(2))).to(dtype)
+    delta = (torch.randn(6, 600, generator=gen(3)) * size).to(dtype)
+    total = (x.float() + delta.float()).to(dtype) if add else x
+    codes, scales = fs.rms_norm_fp8(x.cuda(), w.cuda(), eps, **(dict(delta=delta.cuda(), x_out=torch.empty_like(x, device="cuda")) if add else {}))
+    t = total.double()
+    ref = t / (t.square().mean(1, keepdim=True) + torch.tensor(eps, dtype=torch.float32).double()).sqrt() * w.double()
+    assert LEAST < float(ref[:, 384:].abs().amax()) and float(ref.abs().amax()) < 3e38
+    # squares of 1e-30 lie in steps of 2^-149, 1e-15 of them
+    check_codes(codes, scales, ref, err=40 * 2.0 ** -24 * ref.abs())
