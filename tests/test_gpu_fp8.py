@@ -622,3 +622,64 @@ def test_rms_norm_of_products_beyond_fp32(fs, size, weight, eps, add, dtype):
     assert LEAST < float(ref[:, 384:].abs().amax()) and float(ref.abs().amax()) < 3e38
     # squares of 1e-30 lie in steps of 2^-149, 1e-15 of them
     check_codes(codes, scales, ref, err=40 * 2.0 ** -24 * ref.abs())
+
+
+# ---------------------------------------------------------------- more 256 x 256 tiles than compute units: a workgroup's second and third
+# (rows, features, K) on the kernel of large tiles (tests/test_fp8_plan_cpu.py holds that they are), tiles whole and ragged, so that a tile's stores, whose number
+# the next one's waits go by, are all there, some or none
+SECOND_LINEAR = [(4352, 4352, 256), (4100, 4400, 272), (4353, 4104, 256), (4600, 8000, 144)]
+SECOND_PAIR = [(4096, 2304, 768), (4100, 2320, 272), (4097, 4504, 512), (8000, 4500, 512)]
+SECOND_CODES = [(4096, 2304, 256), (4100, 2320, 272), (4097, 4500, 400), (8448, 2176, 128)]
+
+
+@pytest.mark.parametrize("M,N,K", SECOND_LINEAR)
+def test_linear_over_several_rounds_of_tiles(fs, M, N, K):
+    xc, xs, x = make_codes((M, K), 10, 1)
+    wc, ws, w = make_codes((N, K), 20, 128, pad=16)
+    bias, res = torch.randn(N, generator=gen(3)).bfloat16(), torch.randn(M, N, generator=gen(4)).bfloat16()
+    ref, bound = x @ w.t(), dot_bound(x, w, K, torch.bfloat16)
+    y = fs.linear_fp8(xc, xs, wc, ws)
+    check_product(y, ref, bound, torch.bfloat16)
+    z = res.cuda()
+    fs.linear_fp8(xc, xs, wc, ws, bias=bias.cuda(), residual=z, out=z)
+    check_product(z, ref + bias.double() + res.double(), bound + 2.0 ** -23 * (ref.abs() + bias.double().abs()), torch.bfloat16)
+    for _ in range(3):
+        assert torch.equal(fs.linear_fp8(xc, xs, wc, ws), y)
+        assert torch.equal(fs.linear_fp8(xc, xs, wc, ws, bias=bias.cuda(), residual=res.cuda()), z)
+
+
+@pytest.mark.parametrize("M,N,K", SECOND_PAIR)
+def test_the_pair_over_several_rounds_of_tiles(fs, M, N, K):
+    xc, xs, x = make_codes((M, K), 10, 1)
+    gc, gs, _ = make_codes((N, K), 20, 128, pad=32)
+    uc, us, u = make_codes((N, K), 30, 128)
+    gs = gs * (2 * K ** -0.5)
+    g = gc.cpu().double() * spread(gs, (N, K), 128)
+    a, b = x @ g.t(), x @ u.t()
+    t = math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)
+    gelu = a * torch.sigmoid(2 * t)
+    ea, eb = dot_bound(x, g, K, torch.bfloat16), dot_bound(x, u, K, torch.bfloat16)
+    err = 1.13 * ea * (b.abs() + eb) + gelu.abs() * eb + (8 + 3 * (2 * t).abs()) * 2.0 ** -23 * (gelu * b).abs() + 2.0 ** -130
+    y = fs.glu_fp8(xc, xs, gc, gs, uc, us)
+    check_product(y, gelu * b, err, torch.bfloat16)
+    for _ in range(3):
+        assert torch.equal(fs.glu_fp8(xc, xs, gc, gs, uc, us), y)
+
+
+@pytest.mark.parametrize("M,N,K", SECOND_CODES)
+def test_codes_of_the_pair_over_several_rounds_of_tiles(fs, M, N, K):
+    """Those of a few rows at a time, which are one round of smaller tiles and the same sums, and those of the bf16 result."""
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, xs = fs.quantize_fp8(torch.randn(M, K, generator=g, device="cuda"))
+    gate, up = (fs.quantize_weight_fp8(torch.randn(N, K, generator=g, device="cuda") * K ** -0.5) for _ in range(2))
+    codes, scales = fs.glu_fp8(x, xs, *gate, *up, quantize=True)
+    want, want_s = fs.quantize_fp8(fs.glu_fp8(x, xs, *gate, *up))
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
+    for r in range(0, M, 500):
+        part = slice(r, min(r + 500, M))
+        if part.stop - part.start > 32:                                    # fewer rows add their blocks in another order
+            c, s = fs.glu_fp8(x[part], xs[part], *gate, *up, quantize=True)
+            assert torch.equal(codes[part].view(torch.uint8), c.view(torch.uint8)) and torch.equal(scales[part], s)
+    for _ in range(3):
+        c, s = fs.glu_fp8(x, xs, *gate, *up, quantize=True)
+        assert torch.equal(codes.view(torch.uint8), c.view(torch.uint8)) and torch.equal(scales, s)
