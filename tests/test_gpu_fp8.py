@@ -628,7 +628,7 @@ def test_rms_norm_of_products_beyond_fp32(fs, size, weight, eps, add, dtype):
 # (rows, features, K) on the kernel of large tiles (tests/test_fp8_plan_cpu.py holds that they are), tiles whole and ragged, so that a tile's stores, whose number
 # the next one's waits go by, are all there, some or none
 SECOND_LINEAR = [(4352, 4352, 256), (4100, 4400, 272), (4353, 4104, 256), (4600, 8000, 144)]
-SECOND_PAIR = [(4096, 2304, 768), (4100, 2320, 272), (4097, 4504, 512), (8000, 4500, 512)]
+SECOND_PAIR = [(4096, 4608, 512), (4100, 2320, 272), (4097, 4504, 512), (8000, 4500, 512)]
 SECOND_CODES = [(4096, 2304, 256), (4100, 2320, 272), (4097, 4500, 400), (8448, 2176, 128)]
 
 
