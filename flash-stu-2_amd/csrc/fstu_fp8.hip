@@ -171,7 +171,8 @@ fp8_rmsnorm_kernel(const T* x, long long ldx, const T* delta, long long ldd, T* 
     const float most = __uint_as_float(fp8_max16(size8(v[i])));
     float norm = most * up * rms;                                // amax of the normed values: NaN where one of them is not a number
     uint2 out;
-    if (__builtin_expect(norm >= FP8_LEAST && most >= FP8_LEAST && most < __builtin_inff(), 1)) {
+    const bool none = (c & ~(FP8_BLOCK - 1)) >= d;                // a block behind the row's end: nothing of it is stored
+    if (__builtin_expect(none || (norm >= FP8_LEAST && most >= FP8_LEAST && most < __builtin_inff()), 1)) {
       out = codes8(v[i], fp8_cut<T>(most, true));
     } else {
       // next to nothing, not a number, or products x * w beyond fp32's range whose normed values are not: these themselves, from the row as it was read
