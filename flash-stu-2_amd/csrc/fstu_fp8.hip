@@ -232,8 +232,8 @@ void rmsnorm_pick(const void* x, int64_t ldx, const void* delta, int64_t ldd, vo
                   int64_t ldc, float* scales, int64_t ss, int64_t sb, int rows, int d, hipStream_t s) {
   const auto go = [&](auto f) { f(x, ldx, delta, ldd, xo, ldo, w, eps, codes, ldc, scales, ss, sb, rows, d, s); };
   // A lane takes one group of 8, a row the waves that this needs: more groups to a lane left fewer waves in flight.  us, bf16 with the addition,
-  // groups to a wave / one: 8 x 2048 four 5.1 / 2.7, 1024 x 2048 5.8 / 4.1, 16384 x 2048 38.9 / 38.1, 16384 x 4096 two 89 / 83, 16384 x 8192 four
-  // 179 / 164 (5000 119 / 128).  Up to 1024 columns many rows have waves enough: 1024 x 768 two 3.6 / 3.1, 2048 4.0 / 4.3, 8192 9.5 / 11.9.
+  // groups to a wave / one: 8 x 2048 four 5.7 / 3.3, 1024 x 2048 6.7 / 4.9, 16384 x 2048 42.3 / 38.0, 16384 x 4096 two 90 / 86, 16384 x 8192 four
+  // 200 / 167 (5000 61 / 52).  Up to 1024 columns many rows have waves enough: 1024 x 768 two 4.2 / 3.6, 2048 4.7 / 4.6, 8192 10.9 / 10.7, x 1024 12.8 / 13.2.
   if (d <= 512) go(rmsnorm_launch<T, VEC, 1, 1>);
   else if (d <= 1024 && rows <= 1024) go(rmsnorm_launch<T, VEC, 2, 1>);
   else if (d <= 1024) go(rmsnorm_launch<T, VEC, 1, 2>);

@@ -189,7 +189,7 @@ fp8_plain_kernel(Codes X, Codes W, Codes U, Leave o, int M, int N, int K) {
 // Workgroup ids are dealt round-robin to the 8 XCDs; each XCD works through its own share of the tiles in panels of 8 feature tiles, and
 // a workgroup requests the first blocks of its next tile before it stores this one.
 // 16384 x 2048 x 24576 620 us (2.66 PFLOP/s; a library's 8-bit product of 8192^3 2.71), the pair 16384 x 2 x 24576 x 2048 1385 us (2.38), 4096 x 2 x 9216 x
-// 768 64 to 68: the matrix cores are busy for 70 % of the cycles (pair 54 %: a tile's GELU takes 5.5 us) at the 1.8 GHz that the power leaves
+// 768 64 to 70: the matrix cores are busy for 70 % of the cycles (pair 54 %: a tile's GELU takes 5.5 us) at the 1.8 GHz that the power leaves
 // (all zeros 482 us instead of 620).  v_mfma_f32_32x32x64_f8f6f4, twice the products for the same fragments, behind sums of 16 registers: 686 and
 // 72; a phase's last sums moved behind its barrier: 628 and 64; half of the GELU beside the last block's products: the pair 69.
 #define F8_PANEL 8
@@ -553,7 +553,8 @@ int large(const Codes& X, const Codes& W, const Codes& U, const Leave& o, int M,
 }
 
 // ---------------------------------------------------------------- few rows
-// The weights' bytes bound these (8 rows, 2 x 24576 x 2048 17.3 us, 5.8 TB/s; 2048 x 24576 12.6, 4.0; 50304 x 768 9.0, 4.3): a wave takes 16 features
+// The weights' bytes bound these (8 rows, weights that come from memory: 2 x 24576 x 2048 20.3 us, 5.0 TB/s; 2048 x 24576 20.1, 2.5; 50304 x 768 12.3, 3.1; the
+// same weight again and again, which the caches hold, 17.8, 13.4 and 9.8, as the figures below are): a wave takes 16 features
 // (glu: of both weights; linear 16 F) x 16 R rows of every KH-th block of K, U blocks in
 // flight at once in registers, and the KH waves of a feature tile join their sums in LDS.  A load is 8 rows of 128 bytes, whole lines;
 // the fragments, 16 rows of 64 bytes, are taken through 2 KB of LDS that the wave has for itself (read straight as fragments, half a line to a row,

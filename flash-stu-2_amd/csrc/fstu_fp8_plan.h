@@ -19,8 +19,9 @@ bool skinny_64(int M, int N, int nb, int slices) {
 // fp32 in tiles that leave compute units over: two groups of waves, each with half of a slice's blocks in steps of two
 bool two_groups(int K, int slices) { return (K + 127) / 128 >= 7 * slices; }
 
-// Which kernel a product runs on, and in how many slices of K: the least of an estimate in us, fitted to some 500 products of 1 to 8192 rows, 128 to
-// 24576 features and K = 256 to 24576, which is within a tenth of the best nearly everywhere.  TILE is priced by rounds of workgroups over the
+// Which kernel a product runs on, and in how many slices of K: the least of an estimate in us, fitted to products of 1 to 8192 rows, 128 to
+// 24576 features and K = 256 to 24576.  Of 226 products timed on each kernel (profiles/fp8_plan.txt) the one chosen is within a tenth of the best for 211; the
+// farthest, 1.2 to 1.6 times it, are pairs of K = 256 whose features are no multiple of 64, and 64 x 24576 x 2048 (23 us, tiles 15).  TILE is priced by rounds of workgroups over the
 // compute units, each with a start and an end of its own, SKINNY by the longest of one workgroup's time, that of all of them at the chip's rate
 // and the weights' bytes.
 // us, skinny / tile / large.  Linear, rows x features x K: 500 x 768 x 768 5.2 / 8.3 / 15.7, 1000 6.5 / 8.3, 3000 - / 8.8 / 16; 200 x 2048 x 2048 6.4 / 12.8 /
@@ -61,8 +62,8 @@ Plan plan(int M, int N, int K, bool f32, bool glu, bool codes, int slices) {
   const bool few = M <= (glu ? 32 : 64), big = !f32 && K % 16 == 0;
   if (glu && few) return {SKINNY, 1, 0.0};
   if (codes) {
-    // tiles of 64 rows, one to a compute unit, or of 256.  us, 64 / 256: 64 x 9216 x 768 7.9 / 14.7, 128 8.0 / 15.0, 300 15.2 / 16.1, 500 22 / 17, 1000 37 / 32;
-    // 64 x 24576 x 2048 19 / 28, 128 27 / 28, 200 37 / 29; 1000 x 1536 x 512 7.1 / 13.4
+    // tiles of 64 rows, one to a compute unit, or of 256.  us, 64 / 256: 64 x 9216 x 768 9.2 / 16.2, 100 9.5 / 16.6, 300 17.3 / 18.0, 500 26 / 19, 1000 42 / 35;
+    // 64 x 24576 x 2048 20 / 31, 100 29 / 32, 200 43 / 33; 700 x 2304 x 768 9.9 / 17.3
     const long long nb = (K + 127) / 128, tiles = ((N + 127) / 128) * (long long)((M + 63) / 64);
     const double us = 1.3 + (double)((tiles + fstu_cus() - 1) / fstu_cus()) * (2.6 + 0.6 * nb) + (double)N * K * 6e-8;
     return {us < estimate(LARGE, 1, M, N, K, false, true) ? TILE : LARGE, 1, us};

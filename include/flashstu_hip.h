@@ -703,7 +703,8 @@ int fstu_prof_glu_loop(const fstu_model_desc* m, int reps, double* total_ms, int
  * Rows (activations) have a scale for each 128 values, weights (N,K) one for each 128 x 128, r = n / 128.
  *   scale = max(amax, 2^-100) / 448,  code = the nearest to v * 448 / max(amax, 2^-100), ties to the even code (bf16: exactly; fp32: of a quotient that is
  *   off by up to 2^-23 of itself).
- * A block with a value that is not finite gets a scale that is not finite either.  dtype: that of x, w, delta, bias, res, y.
+ * A block with a value that is not finite gets a scale that is not finite either.  Products form the scale of an activation's
+ * block times that of a weight's first, in fp32, whose range it should not leave.  dtype: that of x, w, delta, bias, res, y.
  *
  * fstu_fp8_quantize_rows, fstu_fp8_quantize_weight: codes and scales of x (rows,d) / w (N,K), row strides ldx / ldw in elements.
  * Refused: an x_out or y that overlaps x, delta or res without being the same rows, and sizes beyond a launch (2^32 threads: 16 to a
