@@ -49,7 +49,7 @@ template <> struct fp8_cut<float> {
   }
   __device__ __forceinline__ float operator()(float v) const {
     const float q = v * times;
-    return fmaf(fmaf(-q, most, v * (FP8_MOST / 512.f)), inv, q);
+    return fmaf(-fmaf(q, most, v * (-FP8_MOST / 512.f)), inv, q);      // of this sign, so that a zero keeps its own
   }
 };
 // Four codes in a word, the first in its low byte.

@@ -683,3 +683,12 @@ def test_codes_of_the_pair_over_several_rounds_of_tiles(fs, M, N, K):
     for _ in range(3):
         c, s = fs.glu_fp8(x, xs, *gate, *up, quantize=True)
         assert torch.equal(codes.view(torch.uint8), c.view(torch.uint8)) and torch.equal(scales, s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_zeros_keep_their_sign(fs, dtype):
+    x = torch.randn(20, 200, generator=gen(1)).to(dtype)
+    x[::2, ::3], x[::2, 1::3], x[3], x[5] = 0.0, -0.0, -0.0, 0.0
+    w = torch.ones(200, dtype=dtype)
+    for codes in (fs.quantize_fp8(x.cuda())[0], fs.quantize_weight_fp8(x.cuda())[0], fs.rms_norm_fp8(x.cuda(), w.cuda(), 1e-6)[0]):
+        assert torch.equal(codes.cpu().view(torch.uint8) >= 128, torch.signbit(x))
