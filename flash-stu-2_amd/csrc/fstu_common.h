@@ -92,6 +92,15 @@ int fstu_stu_res_inproj_step_dyn(const void* x_in, const float* slices, int nsli
                                  const float* fir, int fir_taps, void* y, int ldy, int B, int S, int d, int K, int t,
                                  const int* dyn, const int* pos_dyn, void* stream);
 static inline bool fstu_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+// rows of heads by strides in elements: whether they begin at multiples of 16 bytes, and whether n bytes from out on touch what lies between the
+// first one's begin and the last one's end
+static inline bool fstu_heads_aligned(const void* p, int64_t row, int64_t head, int size) {
+  return fstu_aligned(p, 16) && row >= 0 && head >= 0 && row % (16 / size) == 0 && head % (16 / size) == 0;
+}
+static inline bool fstu_heads_touch(const void* p, int64_t row, int64_t head, int rows, int heads, int hd, int size, const void* out, int64_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), o = reinterpret_cast<uintptr_t>(out);
+  return rows > 0 && n > 0 && o < a + ((rows - 1) * row + (heads - 1) * head + hd) * size && a < o + n;
+}
 // the optional exact head of the distilled filter: ring, taps and their count go together; count a power of two in 8..1024
 static inline bool fstu_fir_ok(const void* ring, const float* fir, int taps) {
   if (!ring && !fir && taps == 0) return true;

@@ -77,6 +77,11 @@ SIGNATURES = {
     "fstu_swa_prefill": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp],
     "fstu_swa_prefill_ws_elems": [_i, _i, _i, _i],
     "fstu_swa_prefill_mfma": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp],
+    "fstu_swa_packed": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "fstu_kv4_bytes": [_i, _i, _i, _i],
+    "fstu_kv4_write": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "fstu_kv4_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "fstu_sample": [_vp, _vp, _i64, _i, _i, _f, _i, _f, _i, _u64, _i, _i, _vp],
     "fstu_sample_ws_bytes": [],
     "fstu_head_maxima": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp],
@@ -156,6 +161,7 @@ def load(path: Optional[str] = None):
     lib.fstu_packed_elems.restype = ctypes.c_int64
     lib.fstu_sample_ws_bytes.restype = ctypes.c_int64
     lib.fstu_swa_prefill_ws_elems.restype = ctypes.c_int64
+    lib.fstu_kv4_bytes.restype = ctypes.c_int64
     lib.fstu_lds_sequence_ws_floats.restype = ctypes.c_size_t
     lib.fstu_stu_conv_fft_grad_ws.restype = ctypes.c_int64
     lib.fstu_stu_conv_mfma_grad_ws.restype = ctypes.c_int64
@@ -1488,4 +1494,159 @@ def glu_fp8(codes: torch.Tensor, scales: torch.Tensor, gate_codes: torch.Tensor,
         rc = load().fstu_fp8_glu(xp, xl, xs, xr, xb, gp, gl, gs, gr, gb, up, ul, us, ur, ub, y.data_ptr(), ldy, ps, 1, M, M, N, K, dt, raw_stream(dev))
         if rc:
             _check(rc, "fstu_fp8_glu")
+    return out
+
+
+# ---------------------------------------------------------------- packed prompts and the 4-bit cache
+# Rows of all sequences lie behind one another; cu_seqlens (sequences + 1,) int32 on the GPU holds where each begins and, last, where the last ends.
+# Positions are int32 on the GPU, one a sequence.  Heads are (rows, heads, head_dim) with dense head_dim and rows and heads that begin at multiples of 16
+# bytes, so that the parts of a fused projection are taken as they lie.  Forward only, as the attention of the layers is: where gradients are on, a
+# tensor that requires one is refused.
+def _heads(x: torch.Tensor, dev: int, what: str):
+    """(address, row stride, head stride) of a checked (rows, heads, head_dim) tensor."""
+    if x.get_device() != dev or dev < 0:
+        raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if x.get_device() < 0
+                               else f"{what} is on device {x.get_device()}, not on {dev}")
+    if x.dim() != 3 or x.shape[0] >= 1 << 30:
+        raise FlashSTUHipError(f"{what} must be (rows, heads, head_dim), got {tuple(x.shape)}")
+    row, head, one = x.stride()
+    if one != 1:
+        raise FlashSTUHipError(f"{what} must have a dense head_dim, got stride {x.stride()}")
+    return x.data_ptr(), row if x.shape[0] > 1 else 0, head if x.shape[1] > 1 else 0
+
+
+def _int32s(x: torch.Tensor, n: int, dev: int, what: str) -> int:
+    if x.dtype is not torch.int32 or x.dim() != 1 or x.shape[0] != n or x.get_device() != dev or not x.is_contiguous():
+        raise FlashSTUHipError(f"{what} must be ({n},) int32, contiguous, on device {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    return x.data_ptr()
+
+
+def _slopes_of(slopes: Optional[torch.Tensor], heads: int, dev: int):
+    if slopes is None:
+        return None
+    if slopes.dtype is not torch.float32 or slopes.shape != (heads,) or slopes.get_device() != dev or not slopes.is_contiguous():
+        raise FlashSTUHipError(f"slopes must be ({heads},) float32, contiguous, on device {dev}, got {tuple(slopes.shape)} {slopes.dtype} on {slopes.device}")
+    return slopes.data_ptr()
+
+
+def swa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, slopes: Optional[torch.Tensor] = None,
+               window: Optional[int] = None, softcap: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention over whole prompts packed behind one another: q (rows, heads, head_dim), k and v (rows, key_heads, head_dim) float32 or
+    bfloat16, key_heads a divisor of heads (query head h reads key head h // (heads / key_heads)), head_dim 32, 64, 128 or 256.  Row i of a sequence
+    sees its rows max(0, i - window) .. i (window None: all of them); scores are softcap * tanh(q . k * head_dim^-1/2 / softcap) - slopes[h] *
+    distance (softcap 0 or None: uncapped; slopes (heads,) float32, None: zero).  Returns out (rows, heads, head_dim); rows in front of the first
+    sequence and behind the last are left as they were (without out: they are not set)."""
+    if (q.requires_grad or k.requires_grad or v.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
+        raise _fp8_forward_only("swa_packed")
+    dev = q.get_device()
+    if dev >= 0 and dev != _device_now():
+        with torch.cuda.device(dev):
+            return swa_packed(q, k, v, cu_seqlens, slopes, window, softcap, out)
+    qp, qr, qh = _heads(q, dev, "q")
+    kp, kr, kh = _heads(k, dev, "k")
+    vp, vr, vh = _heads(v, dev, "v")
+    rows, heads, hd = q.shape
+    kvh = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != rows or k.shape[2] != hd or not q.dtype is k.dtype is v.dtype:
+        raise FlashSTUHipError(f"swa_packed: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} do not go together")
+    dt = _dt(q)
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise FlashSTUHipError(f"cu_seqlens must be (sequences + 1,) int32, got {tuple(cu_seqlens.shape)} {cu_seqlens.dtype}")
+    seqs = cu_seqlens.shape[0] - 1
+    cu, sp = _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens"), _slopes_of(slopes, heads, dev)
+    window = 0x7fffffff if window is None else min(int(window), 0x7fffffff)
+    if out is None:
+        out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
+            raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
+        _written(out)
+    rc = load().fstu_swa_packed(qp, qr, qh, kp, kr, kh, vp, vr, vh, out.data_ptr(), cu, sp, rows, seqs, heads, kvh, hd, window, float(softcap or 0.0), dt,
+                                raw_stream(dev)) if rows else 0
+    if rc:
+        _check(rc, "fstu_swa_packed")
+    return out
+
+
+def kv4_bytes(seqs: int, kv_heads: int, head_dim: int, capacity: int) -> int:
+    """Bytes of a 4-bit ring cache (17/16 of a byte for a key and its value)."""
+    return load().fstu_kv4_bytes(seqs, kv_heads, head_dim, capacity)
+
+
+def kv4_write(cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    if (k.requires_grad or v.requires_grad) and _grad_on():
+        raise _fp8_forward_only("KV4Cache.write")
+    dev = cache.data.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
+            return kv4_write(cache, k, v, pos, cu_seqlens)
+    kp, kr, kh = _heads(k, dev, "k")
+    vp, vr, vh = _heads(v, dev, "v")
+    seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
+    rows = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != kvh or k.shape[2] != hd or k.dtype is not v.dtype:
+        raise FlashSTUHipError(f"KV4Cache.write: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are not rows of {kvh} heads of {hd}")
+    if cu_seqlens is None and rows != seqs:
+        raise FlashSTUHipError(f"KV4Cache.write: without cu_seqlens there is a row to each of the {seqs} sequences, got {rows}")
+    dt = _dt(k)
+    rc = load().fstu_kv4_write(kp, kr, kh, vp, vr, vh, cache.data.data_ptr(), _int32s(pos, seqs, dev, "pos"),
+                               None if cu_seqlens is None else _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens"), rows, seqs, kvh, hd, cache.capacity, dt,
+                               raw_stream(dev)) if rows else 0
+    if rc:
+        _check(rc, "fstu_kv4_write")
+
+
+def kv4_read(cache, pos: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, rows: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
+    dev = cache.data.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
+            return kv4_read(cache, pos, cu_seqlens, rows, dtype)
+    seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
+    if cu_seqlens is None:
+        if rows is not None and rows != seqs:
+            raise FlashSTUHipError(f"KV4Cache.read: without cu_seqlens there is a row to each of the {seqs} sequences, not {rows}")
+        rows = seqs
+    elif rows is None or not 0 <= rows < 1 << 30:
+        raise FlashSTUHipError(f"KV4Cache.read: with cu_seqlens it needs the number of rows, got {rows}")
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
+    pp, cp = _int32s(pos, seqs, dev, "pos"), None if cu_seqlens is None else _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens")
+    k = torch.empty(rows, kvh, hd, dtype=dtype, device=cache.data.device)
+    v = torch.empty_like(k)
+    rc = load().fstu_kv4_read(cache.data.data_ptr(), k.data_ptr(), v.data_ptr(), pp, cp, rows, seqs, kvh, hd, cache.capacity,
+                              FSTU_BF16 if dtype is torch.bfloat16 else FSTU_F32, raw_stream(dev)) if rows else 0
+    if rc:
+        _check(rc, "fstu_kv4_read")
+    return k, v
+
+
+def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, softcap: float = 0.0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if (q.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
+        raise _fp8_forward_only("KV4Cache.attend")
+    dev = cache.data.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
+            return kv4_attend(cache, q, pos, slopes, window, softcap, out)
+    qp, qr, qh = _heads(q, dev, "q")
+    seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
+    heads = q.shape[1]
+    if q.shape[0] != seqs or q.shape[2] != hd or heads < 1 or heads % kvh:
+        raise FlashSTUHipError(f"KV4Cache.attend: q {tuple(q.shape)} is not one row of heads of {hd} to each of {seqs} sequences, heads a multiple of {kvh}")
+    dt = _dt(q)
+    pp, sp = _int32s(pos, seqs, dev, "pos"), _slopes_of(slopes, heads, dev)
+    if window is None:
+        window = cache.capacity - 1
+    elif not 0 <= window < cache.capacity:
+        raise FlashSTUHipError(f"KV4Cache.attend: window {window} does not fit a ring of {cache.capacity} (0 to {cache.capacity - 1})")
+    if out is None:
+        out = torch.empty(seqs, heads, hd, dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
+            raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
+        _written(out)
+    rc = load().fstu_kv4_attend(qp, qr, qh, cache.data.data_ptr(), out.data_ptr(), pp, sp, seqs, heads, kvh, hd, cache.capacity, window, float(softcap or 0.0), dt,
+                                raw_stream(dev))
+    if rc:
+        _check(rc, "fstu_kv4_attend")
     return out

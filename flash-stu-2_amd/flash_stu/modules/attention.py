@@ -85,3 +85,45 @@ class Attention(nn.Module):
         o = _hip.swa_decode(qkv, kr, vr, slopes, pos, W, self.softcap, append=True)
         y = _hip.linear(o, self.c_proj.weight, self.c_proj.bias).reshape(B, 1, d)
         return (y, (kr, vr, pos_t + 1)) if use_cache else y
+
+
+class KV4Cache:
+    """A ring cache of keys and values in 4 bits for a batch of sequences, each at a position of its own.
+
+    Position j of a sequence lives in slot j % capacity.  Values are e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives); 32 values of a head's
+    row share a power of two 2^e, e the smallest whole number from -120 to 125 with amax <= 7 * 2^e; a value's code is the nearest, ties to the even
+    one.  32 values with an infinity or a NaN among them stand for NaN.  A key and its value take 17/16 of a byte for each dim, bf16 ones 4.
+
+    `pos` is (batch,) int32 on the GPU and counted by the caller, so that a captured step runs for every position; a sequence at a negative position
+    is not in use.  capacity beyond the window leaves room for nothing but is allowed; head_dim is 32, 64, 128 or 256.  Forward only."""
+
+    def __init__(self, batch: int, kv_heads: int, head_dim: int, capacity: int, device=None):
+        if batch < 1 or kv_heads < 1 or not 1 <= capacity <= 1 << 30 or head_dim not in (32, 64, 128, 256):
+            raise _hip.FlashSTUHipError(f"KV4Cache: batch {batch}, {kv_heads} key heads, capacity {capacity} (up to 2^30) and head_dim {head_dim} "
+                                        "(32, 64, 128 or 256) are no cache")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise _hip.FlashSTUHipError("KV4Cache lives on the GPU: the HIP path has no CPU fallback")
+        self.batch, self.kv_heads, self.head_dim, self.capacity = batch, kv_heads, head_dim, capacity
+        self.data = torch.zeros(_hip.kv4_bytes(batch, kv_heads, head_dim, capacity), dtype=torch.uint8, device=device)
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, cu_seqlens: torch.Tensor = None) -> None:
+        """Rows of k and v (rows, kv_heads, head_dim) float32 or bfloat16 become positions pos[s], pos[s] + 1, ... of sequence s: rows cu_seqlens[s] ..
+        cu_seqlens[s + 1] - 1 (of more than `capacity` the last ones), or row s alone without cu_seqlens."""
+        _hip.kv4_write(self, k, v, pos, cu_seqlens)
+
+    def read(self, pos: torch.Tensor, cu_seqlens: torch.Tensor = None, rows: int = None, dtype: torch.dtype = torch.bfloat16):
+        """What write's rows are held as: (k, v), each (rows, kv_heads, head_dim) of dtype (exact in both); zero for rows of no sequence.  A position that
+        the ring no longer holds reads as the one that took its slot."""
+        return _hip.kv4_read(self, pos, cu_seqlens, rows, dtype)
+
+    def attend(self, q: torch.Tensor, pos: torch.Tensor, k: torch.Tensor = None, v: torch.Tensor = None, slopes: torch.Tensor = None, window: int = None,
+               softcap: float = 0.0, out: torch.Tensor = None) -> torch.Tensor:
+        """One query a sequence, q (batch, heads, head_dim), at position pos[s], over the positions max(0, pos[s] - window) .. pos[s] as the cache holds
+        them (window None: capacity - 1); heads a multiple of kv_heads, scores as swa_packed's.  k, v (batch, kv_heads, head_dim): those of position
+        pos[s], written first.  Returns out (batch, heads, head_dim), zero for a sequence not in use."""
+        if (k is None) != (v is None):
+            raise _hip.FlashSTUHipError("KV4Cache.attend: k and v go together")
+        if k is not None:
+            _hip.kv4_write(self, k, v, pos)
+        return _hip.kv4_attend(self, q, pos, slopes, window, softcap, out)

@@ -1,0 +1,106 @@
+"""What the packed attention and the 4-bit cache refuse, without a GPU: at the C entry points before any launch, and in the Python calls."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_stu import _hip
+    return _hip.load()
+
+
+@pytest.fixture(scope="module")
+def mem():
+    buf = (ctypes.c_char * (1 << 16))()
+    return (ctypes.addressof(buf) + 63) // 64 * 64, buf
+
+
+def why(lib):
+    return lib.fstu_last_error().decode()
+
+
+def test_bytes(lib):
+    assert lib.fstu_kv4_bytes(1, 1, 32, 1) == 32 * 34 and lib.fstu_kv4_bytes(3, 2, 128, 33) == 3 * 2 * 64 * (128 + 8)
+    assert lib.fstu_kv4_bytes(64, 16, 256, 1 << 20) == 64 * 16 * 272 << 20
+
+
+def test_cache_entry_points_refuse(lib, mem):
+    p = mem[0]
+
+    def write(k=p, kr=128, kh=64, v=p, c=p, pos=p, cu=p, rows=2, seqs=2, kvh=2, hd=64, cap=8, dt=1):
+        return lib.fstu_kv4_write(k, kr, kh, v, 128, 64, c, pos, cu, rows, seqs, kvh, hd, cap, dt, None)
+
+    def read(c=p, k=p, v=p, pos=p, cu=p, rows=2, seqs=2, kvh=2, hd=64, cap=8, dt=1):
+        return lib.fstu_kv4_read(c, k, v, pos, cu, rows, seqs, kvh, hd, cap, dt, None)
+
+    for f in (write, read):
+        assert f(k=None) == -1 and f(v=None) == -1 and f(c=None) == -1 and f(pos=None) == -1 and "null" in why(lib)
+        assert f(hd=48) == -3 and f(hd=0) == -3 and f(seqs=0) == -3 and f(kvh=0) == -3 and f(cap=0) == -3 and f(cap=(1 << 30) + 1) == -3
+        assert f(rows=1 << 29, kvh=64, hd=256) == -3 and "launch" in why(lib)
+        assert f(rows=-1) == -5 and f(cu=None, rows=3) == -5 and "rows" in why(lib)
+        assert f(c=p + 8) == -4 and f(k=p + 2) == -4 and f(v=p + 8) == -4
+        assert f(dt=7) == -2
+        assert f(rows=0) == 0
+    assert write(kr=100) == -4 and write(kh=33) == -4 and write(kr=-128) == -4
+
+    def attend(q=p, qr=256, qh=64, c=p + 8192, out=p + 4096, pos=p, slopes=None, seqs=2, heads=4, kvh=2, hd=64, cap=8, window=7, softcap=0.0, dt=1):
+        return lib.fstu_kv4_attend(q, qr, qh, c, out, pos, slopes, seqs, heads, kvh, hd, cap, window, softcap, dt, None)
+
+    assert attend(q=None) == -1 and attend(c=None) == -1 and attend(out=None) == -1 and attend(pos=None) == -1
+    assert attend(hd=96) == -3 and attend(heads=3) == -3 and attend(heads=0) == -3 and attend(seqs=65536) == -3 and attend(cap=0) == -3
+    assert attend(window=8) == -5 and attend(window=-1) == -5 and "window" in why(lib)
+    assert attend(softcap=-1.0) == -5 and attend(softcap=math.nan) == -5 and attend(softcap=math.inf) == -5
+    assert attend(q=p + 8) == -4 and attend(qr=100) == -4 and attend(qh=-64) == -4 and attend(out=p + 4096 + 4) == -4 and attend(c=p + 8200) == -4
+    assert attend(out=p) == -5 and "overlaps" in why(lib)
+    assert attend(out=p + 8192) == -5 and attend(out=p + 8192 + 2 * 2 * 32 * 68 - 16) == -5
+    assert attend(dt=2) == -2
+
+
+def test_packed_entry_point_refuses(lib, mem):
+    p = mem[0]
+
+    def f(q=p, qr=256, qh=64, k=p, kr=128, kh=64, v=p, out=p + 8192, cu=p, rows=8, seqs=2, heads=4, kvh=2, hd=64, window=7, softcap=0.0, dt=1):
+        return lib.fstu_swa_packed(q, qr, qh, k, kr, kh, v, 128, 64, out, cu, None, rows, seqs, heads, kvh, hd, window, softcap, dt, None)
+
+    assert f(q=None) == -1 and f(k=None) == -1 and f(v=None) == -1 and f(out=None) == -1 and f(cu=None) == -1
+    assert f(hd=80) == -3 and f(heads=5) == -3 and f(kvh=0) == -3 and f(rows=-1) == -3 and f(seqs=-1) == -3 and f(heads=0) == -3
+    assert f(rows=(1 << 30) + 1) == -3
+    assert f(window=-1) == -5 and f(softcap=-0.5) == -5 and f(softcap=math.nan) == -5 and f(softcap=math.inf) == -5
+    assert f(q=p + 4) == -4 and f(k=p + 2) == -4 and f(v=p + 8) == -4 and f(out=p + 8196) == -4 and f(qr=257) == -4 and f(kh=60) == -4 and f(kr=-8) == -4
+    assert f(out=p) == -5 and f(out=p + 256 * 7 * 2) == -5 and "overlaps" in why(lib)
+    assert f(dt=3) == -2
+    assert f(rows=0) == 0 and f(seqs=0) == 0
+
+
+def test_the_calls_refuse_tensors_of_the_cpu():
+    from flash_stu import KV4Cache, _hip, swa_packed
+    q, k, cu = torch.zeros(4, 2, 64), torch.zeros(4, 1, 64), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(_hip.FlashSTUHipError, match="no CPU fallback"):
+        swa_packed(q, k, k, cu)
+    with pytest.raises(_hip.FlashSTUHipError, match="no CPU fallback"):
+        KV4Cache(1, 1, 64, 8, device="cpu")
+    with pytest.raises(NotImplementedError, match="forward only"):
+        swa_packed(q.requires_grad_(), k, k, cu)
+    for bad in ((0, 1, 64, 8), (1, 1, 65, 8), (1, 1, 64, 0)):
+        with pytest.raises(_hip.FlashSTUHipError, match="no cache"):
+            KV4Cache(*bad)
+
+
+def test_the_reference_of_the_tests():
+    """The cache's definition by hand, and the attention's against torch's softmax."""
+    from attention_reference import attention, held
+    x = torch.zeros(4, 32)
+    x[0, :4] = torch.tensor([7.0, 5.0, 0.25, -0.75])
+    x[1, :4] = torch.tensor([7.1, 5.0, 0.5, -2.6])
+    x[2, 0] = 2.0 ** -126
+    x[3, 5] = math.inf
+    y = held(x)
+    assert y[0, :4].tolist() == [6.0, 4.0, 0.0, -1.0] and y[1, :4].tolist() == [8.0, 4.0, 0.0, -3.0] and not y[2].any() and bool(torch.isnan(y[3]).all())
+    q, k, v = (torch.randn(5, 8, dtype=torch.float64) for _ in range(3))
+    far = (torch.arange(5)[:, None] - torch.arange(5)).double().clamp_min(-1)
+    o, bound = attention(q, k, v, far, 0.0, 0.0, 0.0)
+    want = torch.nn.functional.scaled_dot_product_attention(q[None], k[None], v[None], is_causal=True)[0]
+    assert torch.allclose(o, want) and bool((bound < 1e-4).all())
