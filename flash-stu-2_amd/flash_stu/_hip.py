@@ -81,7 +81,8 @@ SIGNATURES = {
     "fstu_kv4_bytes": [_i, _i, _i, _i],
     "fstu_kv4_write": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "fstu_kv4_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "fstu_kv4_attend_splits": [_i, _i, _i, _i, _i, _i],
     "fstu_sample": [_vp, _vp, _i64, _i, _i, _f, _i, _f, _i, _u64, _i, _i, _vp],
     "fstu_sample_ws_bytes": [],
     "fstu_head_maxima": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp],
@@ -1620,6 +1621,11 @@ def kv4_read(cache, pos: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None
     return k, v
 
 
+@functools.lru_cache(maxsize=256)
+def _kv4_splits(seqs: int, heads: int, kvh: int, hd: int, cap: int, window: int) -> int:
+    return load().fstu_kv4_attend_splits(seqs, heads, kvh, hd, cap, window)
+
+
 def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, softcap: float = 0.0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     if (q.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
@@ -1645,7 +1651,9 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch
         if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
             raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
         _written(out)
-    rc = load().fstu_kv4_attend(qp, qr, qh, cache.data.data_ptr(), out.data_ptr(), pp, sp, seqs, heads, kvh, hd, cache.capacity, window, float(softcap or 0.0), dt,
+    splits = _kv4_splits(seqs, heads, kvh, hd, cache.capacity, window)
+    ws = torch.empty(seqs * heads * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    rc = load().fstu_kv4_attend(qp, qr, qh, cache.data.data_ptr(), out.data_ptr(), _p(ws), splits, pp, sp, seqs, heads, kvh, hd, cache.capacity, window, float(softcap or 0.0), dt,
                                 raw_stream(dev))
     if rc:
         _check(rc, "fstu_kv4_attend")

@@ -46,8 +46,9 @@ def test_cache_entry_points_refuse(lib, mem):
         assert f(rows=0) == 0
     assert write(kr=100) == -4 and write(kh=33) == -4 and write(kr=-128) == -4
 
-    def attend(q=p, qr=256, qh=64, c=p + 8192, out=p + 4096, pos=p, slopes=None, seqs=2, heads=4, kvh=2, hd=64, cap=8, window=7, softcap=0.0, dt=1):
-        return lib.fstu_kv4_attend(q, qr, qh, c, out, pos, slopes, seqs, heads, kvh, hd, cap, window, softcap, dt, None)
+    def attend(q=p, qr=256, qh=64, c=p + 8192, out=p + 4096, pos=p, slopes=None, seqs=2, heads=4, kvh=2, hd=64, cap=8, window=7, softcap=0.0, dt=1, splits=1,
+               ws=None):
+        return lib.fstu_kv4_attend(q, qr, qh, c, out, ws, splits, pos, slopes, seqs, heads, kvh, hd, cap, window, softcap, dt, None)
 
     assert attend(q=None) == -1 and attend(c=None) == -1 and attend(out=None) == -1 and attend(pos=None) == -1
     assert attend(hd=96) == -3 and attend(heads=3) == -3 and attend(heads=0) == -3 and attend(seqs=65536) == -3 and attend(cap=0) == -3
@@ -57,6 +58,8 @@ def test_cache_entry_points_refuse(lib, mem):
     assert attend(out=p) == -5 and "overlaps" in why(lib)
     assert attend(out=p + 8192) == -5 and attend(out=p + 8192 + 2 * 2 * 32 * 68 - 16) == -5
     assert attend(dt=2) == -2
+    assert attend(splits=0) == -5 and attend(splits=2) == -5 and attend(splits=70000, ws=p) == -5 and attend(splits=2, ws=p + 2) == -4
+    assert lib.fstu_kv4_attend_splits(64, 8, 8, 64, 100, 99) == 1 and 1 < lib.fstu_kv4_attend_splits(1, 8, 8, 64, 1 << 20, (1 << 20) - 1) <= 64
 
 
 def test_packed_entry_point_refuses(lib, mem):
