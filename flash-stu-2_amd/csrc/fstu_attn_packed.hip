@@ -18,11 +18,7 @@ struct Heads {                 // rows of heads: strides in elements
 // The sequence that row tile t (of `per` rows) belongs to, and its number there: sequence i has the tiles from cu[i] / per + i on, which are as many as it
 // needs or one more (a sequence's rows begin anywhere), so that no count has to be added up on the way.
 __device__ __forceinline__ int packed_tile(const int* cu, int seqs, int rows, int per, int t, int* at, int* len, int* first) {
-  int lo = 0, hi = seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (max(cu[mid], 0) / per + mid <= t) lo = mid; else hi = mid;
-  }
+  const int lo = fstu_last_where(seqs, [&](int i) { return max(cu[i], 0) / per + i <= t; });
   const int a = min(max(cu[lo], 0), rows), b = min(max(cu[lo + 1], a), rows);
   *at = a;
   *len = b - a;

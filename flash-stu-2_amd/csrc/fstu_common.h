@@ -163,6 +163,22 @@ __device__ __forceinline__ float wave_max(float v) {
                __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32)));
 }
 
+// The last i of 0..n-1 for which below(i) holds (which holds up to some i and for none behind it; 0 where it holds for none): a wave looks at 64 of them at
+// once, every lane active.
+template <class F>
+__device__ __forceinline__ int fstu_last_where(int n, F below) {
+  const int lane = (int)threadIdx.x & 63;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const unsigned long long yes = __ballot(lane * (int64_t)step < n && below(min(i, lo + n - 1)));
+    const int last = yes ? 63 - __builtin_clzll(yes) : 0;
+    lo += last * step;
+    n = min(step, n - last * step);
+  }
+  return lo;
+}
+
 // tanh-approximated GELU as torch evaluates it in fp32
 __device__ __forceinline__ float gelu_tanh_f32(float x) {
   const float kBeta = 0.7978845608028654f;  // sqrt(2/pi)

@@ -16,19 +16,6 @@ __device__ __forceinline__ unsigned kv4_scale(unsigned amax) {
 }
 __device__ __forceinline__ float kv4_scale_value(unsigned byte) { return __uint_as_float(byte << 23); }
 
-// The sequence that row belongs to (the last one that begins at or in front of it), -1 where none does; *at: its first row, *len: its rows.
-__device__ __forceinline__ int kv4_sequence(const int* cu, int seqs, int row, int* at, int* len) {
-  int lo = 0, hi = seqs;              // cu[lo] <= row < cu[hi], as far as cu rises
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= row) lo = mid; else hi = mid;
-  }
-  const int a = cu[lo], b = cu[lo + 1];
-  *at = a;
-  *len = b - a;
-  return row >= a && row < b ? lo : -1;
-}
-
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float* o) {
   if constexpr (sizeof(T) == 2) {
@@ -52,36 +39,83 @@ __device__ __forceinline__ void store8(T* p, const float* o) {
   }
 }
 
-// Eight values of a key's or value's row, dims 8u..8u+7, in the cache: codes in a word, low nibble first.
+// Codes of dims 8u .. 8u + 7 of a value at one slot (a word, low nibble first), in the pieces of hd/16 dims that the cache deals them to.
 template <int HD>
-__device__ __forceinline__ void kv4_put_value(unsigned char* vc, int64_t head, int slots, int slot, int u, unsigned code) {
-  constexpr int PB = HD / 32;                                  // bytes of a piece: hd/16 dims
-  unsigned char* tile = vc + (head * slots + (slot & ~7)) * (HD / 2) + (slot & 7) * PB;
+__device__ __forceinline__ void put_value(unsigned char* tile, int i, int u, unsigned code) {       // slot i of the eight at `tile`
+  constexpr int PB = HD / 32;                                  // bytes of a piece
+  tile += i * PB;
   if constexpr (PB >= 4) *(unsigned*)(tile + (u * 4 / PB) * 8 * PB + (u * 4) % PB) = code;
   else if constexpr (PB == 2) {
     *(unsigned short*)(tile + (2 * u) * 16) = (unsigned short)code;
     *(unsigned short*)(tile + (2 * u + 1) * 16) = (unsigned short)(code >> 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tile[(4 * u + i) * 8] = (unsigned char)(code >> (8 * i));
+    for (int e = 0; e < 4; ++e) tile[(4 * u + e) * 8] = (unsigned char)(code >> (8 * e));
   }
 }
 template <int HD>
-__device__ __forceinline__ unsigned kv4_get_value(const unsigned char* vc, int64_t head, int slots, int slot, int u) {
+__device__ __forceinline__ unsigned get_value(const unsigned char* tile, int i, int u) {
   constexpr int PB = HD / 32;
-  const unsigned char* tile = vc + (head * slots + (slot & ~7)) * (HD / 2) + (slot & 7) * PB;
+  tile += i * PB;
   if constexpr (PB >= 4) return *(const unsigned*)(tile + (u * 4 / PB) * 8 * PB + (u * 4) % PB);
   else if constexpr (PB == 2) return *(const unsigned short*)(tile + (2 * u) * 16) | (unsigned)*(const unsigned short*)(tile + (2 * u + 1) * 16) << 16;
   else {
     unsigned code = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) code |= (unsigned)tile[(4 * u + i) * 8] << (8 * i);
+    for (int e = 0; e < 4; ++e) code |= (unsigned)tile[(4 * u + e) * 8] << (8 * e);
     return code;
   }
 }
+// The same at all eight slots, as the 32 bytes beside each other that they are (hd up to 128): pieces of four, two or one byte a slot.
 template <int HD>
-__device__ __forceinline__ unsigned char* kv4_scale_at(unsigned char* s, int64_t head, int slots, int slot, int blk) {
-  return s + (head * slots + (slot & ~7)) * (HD / 32) + blk * 8 + (slot & 7);
+__device__ __forceinline__ void eight_to_pieces(const unsigned* code, unsigned* w) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = code[i];
+  } else if constexpr (HD == 64) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __builtin_amdgcn_perm(code[2 * i + 1], code[2 * i], 0x05040100);
+      w[4 + i] = __builtin_amdgcn_perm(code[2 * i + 1], code[2 * i], 0x07060302);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                              // a 4 x 4 transposition of bytes
+      const unsigned ab = __builtin_amdgcn_perm(code[4 * i + 1], code[4 * i], 0x05010400), cd = __builtin_amdgcn_perm(code[4 * i + 3], code[4 * i + 2], 0x05010400);
+      const unsigned AB = __builtin_amdgcn_perm(code[4 * i + 1], code[4 * i], 0x07030602), CD = __builtin_amdgcn_perm(code[4 * i + 3], code[4 * i + 2], 0x07030602);
+      w[0 + i] = __builtin_amdgcn_perm(cd, ab, 0x05040100);
+      w[2 + i] = __builtin_amdgcn_perm(cd, ab, 0x07060302);
+      w[4 + i] = __builtin_amdgcn_perm(CD, AB, 0x05040100);
+      w[6 + i] = __builtin_amdgcn_perm(CD, AB, 0x07060302);
+    }
+  }
+}
+template <int HD>
+__device__ __forceinline__ void pieces_to_eight(const unsigned* w, unsigned* code) {
+  if constexpr (HD == 128) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = w[i];
+  } else if constexpr (HD == 64) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      code[2 * i] = __builtin_amdgcn_perm(w[4 + i], w[i], 0x05040100);
+      code[2 * i + 1] = __builtin_amdgcn_perm(w[4 + i], w[i], 0x07060302);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned ab = __builtin_amdgcn_perm(w[2 + i], w[i], 0x05010400), cd = __builtin_amdgcn_perm(w[6 + i], w[4 + i], 0x05010400);
+      const unsigned AB = __builtin_amdgcn_perm(w[2 + i], w[i], 0x07030602), CD = __builtin_amdgcn_perm(w[6 + i], w[4 + i], 0x07030602);
+      code[4 * i] = __builtin_amdgcn_perm(cd, ab, 0x05040100);
+      code[4 * i + 1] = __builtin_amdgcn_perm(cd, ab, 0x07060302);
+      code[4 * i + 2] = __builtin_amdgcn_perm(CD, AB, 0x05040100);
+      code[4 * i + 3] = __builtin_amdgcn_perm(CD, AB, 0x07060302);
+    }
+  }
+}
+template <int HD>
+__device__ __forceinline__ unsigned char* kv4_scale_at(unsigned char* s, int64_t at, int slot, int blk) {      // at: the head's first slot
+  return s + (at + (slot & ~7)) * (HD / 32) + blk * 8 + (slot & 7);
 }
 
 __device__ __forceinline__ unsigned quad_max(unsigned v) {     // over each four lanes
@@ -109,58 +143,171 @@ __device__ __forceinline__ void kv4_values(unsigned code, unsigned byte, float* 
   o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y; o[4] = c.x; o[5] = c.y; o[6] = d.x; o[7] = d.y;
 }
 
-// Eight values a thread; threads of y = 1 take the values, of y = 0 the keys.
-template <typename T, int HD>
+// Eight slots' worth of a sequence's new rows: the rows that go to slots sl .. sl + 7 of it, as far as there are such.
+struct Eight {
+  int s, at, len, t, slot, p;      // sequence, its first row and rows, the group's first row in it (or up to 7 in front of it), that one's slot, position
+  bool whole;                      // eight rows and eight slots beside each other, from a multiple of 8 on
+};
+// Group number n: a sequence's groups begin at cu[s] / 8 + 2 s, which leaves room for a partial one at each end.
+__device__ __forceinline__ Eight eight_of(const int* cu, const int* pos, int seqs, int rows, int cap, int n) {
+  Eight g;
+  g.s = fstu_last_where(seqs, [&](int i) { return max(cu[i], 0) / 8 + 2 * i <= n; });
+  g.at = min(max(cu[g.s], 0), rows);
+  g.len = min(max(cu[g.s + 1], g.at), rows) - g.at;
+  g.p = pos[g.s];
+  const int first = g.p < 0 ? 0 : g.p % cap;
+  g.t = (n - (g.at / 8 + 2 * g.s)) * 8 - (first & 7);
+  g.slot = (int)((unsigned)(first + g.t) % (unsigned)cap);
+  g.whole = g.t >= 0 && g.t + 8 <= g.len && g.slot % 8 == 0 && g.slot + 8 <= cap;
+  return g;
+}
+
+// A workgroup takes a group of eight slots (ONE: one row of a sequence), keys where y = 0 and values where y = 1; a thread eight dims of a head.  Each thread's
+// eight rows are asked for together, and what it leaves is 32 bytes beside each other (keys: 4 in each of eight rows).  16384 rows of 16 x 128 in bf16, written and
+// read back: 134 us with a row's eight dims to a thread, WRITE_US now.
+template <typename T, int HD, bool ONE>
 __global__ void __launch_bounds__(256)
-kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* cache, const int* pos, const int* cu,
-                 int rows, int seqs, int kvh, int cap) {
+kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* cache, const int* pos, const int* cu, int rows,
+                 int seqs, int kvh, int cap) {
   constexpr int P = HD / 8;
   const Kv4 c = kv4_at(cache, (int64_t)seqs * kvh, HD, cap);
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int u = (int)(idx % P), h = (int)(idx / P % kvh);
-  const int64_t row = idx / P / kvh;
-  if (row >= rows) return;
-  int at = (int)row, len = 1, s = (int)row;
-  if (cu) s = kv4_sequence(cu, seqs, (int)row, &at, &len);
-  const int p = s < 0 ? -1 : pos[s], t = (int)row - at;
-  if (p < 0 || t < len - cap) return;                         // four lanes of a block go together
-  const int slot = (int)(((unsigned)p + (unsigned)t) % (unsigned)cap);
-  const int64_t head = (int64_t)s * kvh + h;
-  float x[8];
-  unsigned byte;
-  if (blockIdx.y == 0) {
-    load8(k + row * k_row + h * k_head + u * 8, x);
-    const unsigned code = kv4_quantise(x, &byte);
-    *(unsigned*)(c.kc + (head * c.slots + slot) * (HD / 2) + u * 4) = code;
-    if ((u & 3) == 0) *kv4_scale_at<HD>(c.ks, head, c.slots, slot, u / 4) = (unsigned char)byte;
-  } else {
-    load8(v + row * v_row + h * v_head + u * 8, x);
-    const unsigned code = kv4_quantise(x, &byte);
-    kv4_put_value<HD>(c.vc, head, c.slots, slot, u, code);
-    if ((u & 3) == 0) *kv4_scale_at<HD>(c.vs, head, c.slots, slot, u / 4) = (unsigned char)byte;
+  const bool keys = blockIdx.y == 0;
+  const T* const x = keys ? k : v;
+  const int64_t x_row = keys ? k_row : v_row, x_head = keys ? k_head : v_head;
+  if constexpr (ONE) {
+    const int s = blockIdx.x, p = pos[s];
+    if (p < 0) return;
+    const int slot = p % cap;
+    for (int e = threadIdx.x; e < kvh * P; e += blockDim.x) {
+      const int h = e / P, u = e % P;
+      const int64_t at = ((int64_t)s * kvh + h) * c.slots;
+      float f[8];
+      unsigned byte;
+      load8(x + s * x_row + h * x_head + u * 8, f);
+      const unsigned code = kv4_quantise(f, &byte);
+      if (keys) *(unsigned*)(c.kc + (at + slot) * (HD / 2) + u * 4) = code;
+      else put_value<HD>(c.vc + (at + (slot & ~7)) * (HD / 2), slot & 7, u, code);
+      if ((u & 3) == 0) *kv4_scale_at<HD>(keys ? c.ks : c.vs, at, slot, u / 4) = (unsigned char)byte;
+    }
+    return;
+  }
+  const Eight g = eight_of(cu, pos, seqs, rows, cap, blockIdx.x);
+  if (g.p < 0 || g.len == 0 || g.t >= g.len || g.t <= -8) return;
+  const int from = max(0, g.len - cap);
+  for (int e = threadIdx.x; e < kvh * P; e += blockDim.x) {
+    const int h = e / P, u = e % P;
+    const int64_t at = ((int64_t)g.s * kvh + h) * c.slots;
+    const T* src = x + h * x_head + u * 8;
+    float f[8][8];
+    unsigned code[8], byte[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load8(src + (g.at + min(max(g.t + i, 0), g.len - 1)) * x_row, f[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = kv4_quantise(f[i], &byte[i]);
+    if (g.whole && g.t >= from) {
+      if (keys) {
+        unsigned char* dst = c.kc + (at + g.slot) * (HD / 2) + u * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *(unsigned*)(dst + i * (HD / 2)) = code[i];
+      } else {
+        unsigned char* tile = c.vc + (at + g.slot) * (HD / 2);
+        if constexpr (HD <= 128) {
+          unsigned w[8];
+          eight_to_pieces<HD>(code, w);
+          *(uint4*)(tile + u * 32) = make_uint4(w[0], w[1], w[2], w[3]);
+          *(uint4*)(tile + u * 32 + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) put_value<HD>(tile, i, u, code[i]);
+        }
+      }
+      if ((u & 3) == 0)
+        *(uint2*)kv4_scale_at<HD>(keys ? c.ks : c.vs, at, g.slot, u / 4) = make_uint2(byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24,
+                                                                                    byte[4] | byte[5] << 8 | byte[6] << 16 | byte[7] << 24);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (g.t + i < from || g.t + i >= g.len) continue;
+      const int slot = (int)((unsigned)(g.slot + i) % (unsigned)cap);
+      if (keys) *(unsigned*)(c.kc + (at + slot) * (HD / 2) + u * 4) = code[i];
+      else put_value<HD>(c.vc + (at + (slot & ~7)) * (HD / 2), slot & 7, u, code[i]);
+      if ((u & 3) == 0) *kv4_scale_at<HD>(keys ? c.ks : c.vs, at, slot, u / 4) = (unsigned char)byte[i];
+    }
   }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool ONE>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const void* cache, T* k, T* v, const int* pos, const int* cu, int rows, int seqs, int kvh, int cap) {
   constexpr int P = HD / 8;
   const Kv4 c = kv4_at((void*)cache, (int64_t)seqs * kvh, HD, cap);
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int u = (int)(idx % P), h = (int)(idx / P % kvh);
-  const int64_t row = idx / P / kvh;
-  if (row >= rows) return;
-  int at = (int)row, len = 1, s = (int)row;
-  if (cu) s = kv4_sequence(cu, seqs, (int)row, &at, &len);
-  const int p = s < 0 ? -1 : pos[s];
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (p >= 0) {
-    const int slot = (int)(((unsigned)p + (unsigned)((int)row - at)) % (unsigned)cap);
-    const int64_t head = (int64_t)s * kvh + h;
-    if (blockIdx.y == 0) kv4_values(*(const unsigned*)(c.kc + (head * c.slots + slot) * (HD / 2) + u * 4), *kv4_scale_at<HD>(c.ks, head, c.slots, slot, u / 4), x);
-    else kv4_values(kv4_get_value<HD>(c.vc, head, c.slots, slot, u), *kv4_scale_at<HD>(c.vs, head, c.slots, slot, u / 4), x);
+  const bool keys = blockIdx.y == 0;
+  T* const y = keys ? k : v;
+  const int64_t row = (int64_t)kvh * HD;
+  if constexpr (ONE) {
+    const int s = blockIdx.x, p = pos[s];
+    const int slot = p < 0 ? 0 : p % cap;
+    for (int e = threadIdx.x; e < kvh * P; e += blockDim.x) {
+      const int h = e / P, u = e % P;
+      const int64_t at = ((int64_t)s * kvh + h) * c.slots;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (p >= 0)
+        kv4_values(keys ? *(const unsigned*)(c.kc + (at + slot) * (HD / 2) + u * 4) : get_value<HD>(c.vc + (at + (slot & ~7)) * (HD / 2), slot & 7, u),
+                   *kv4_scale_at<HD>(keys ? c.ks : c.vs, at, slot, u / 4), f);
+      store8(y + s * row + e * 8, f);
+    }
+    return;
   }
-  store8((blockIdx.y == 0 ? k : v) + idx * 8, x);
+  const int begin = min(max(cu[0], 0), rows), end = min(max(cu[seqs], begin), rows);
+  for (int r = blockIdx.x; r < begin + rows - end; r += gridDim.x)               // rows of no sequence
+    for (int e = threadIdx.x; e < kvh * P; e += blockDim.x) {
+      const float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      store8(y + (r < begin ? r : end + r - begin) * row + e * 8, f);
+    }
+  const Eight g = eight_of(cu, pos, seqs, rows, cap, blockIdx.x);
+  if (g.t >= g.len || g.t <= -8) return;
+  for (int e = threadIdx.x; e < kvh * P; e += blockDim.x) {
+    const int h = e / P, u = e % P;
+    const int64_t at = ((int64_t)g.s * kvh + h) * c.slots;
+    T* dst = y + (int64_t)(g.at + g.t) * row + e * 8;
+    if (g.whole && g.p >= 0) {
+      unsigned code[8];
+      if (keys) {
+        const unsigned char* src = c.kc + (at + g.slot) * (HD / 2) + u * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = *(const unsigned*)(src + i * (HD / 2));
+      } else {
+        const unsigned char* tile = c.vc + (at + g.slot) * (HD / 2);
+        if constexpr (HD <= 128) {
+          const uint4 a = *(const uint4*)(tile + u * 32), b = *(const uint4*)(tile + u * 32 + 16);
+          const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          pieces_to_eight<HD>(w, code);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) code[i] = get_value<HD>(tile, i, u);
+        }
+      }
+      const uint2 b = *(const uint2*)kv4_scale_at<HD>(keys ? c.ks : c.vs, at, g.slot, u / 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+        kv4_values(code[i], ((i < 4 ? b.x : b.y) >> (8 * (i & 3))) & 255, f);
+        store8(dst + i * row, f);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (g.t + i < 0 || g.t + i >= g.len) continue;
+      const int slot = (int)((unsigned)(g.slot + i) % (unsigned)cap);
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (g.p >= 0)
+        kv4_values(keys ? *(const unsigned*)(c.kc + (at + slot) * (HD / 2) + u * 4) : get_value<HD>(c.vc + (at + (slot & ~7)) * (HD / 2), slot & 7, u),
+                   *kv4_scale_at<HD>(keys ? c.ks : c.vs, at, slot, u / 4), f);
+      store8(dst + i * row, f);
+    }
+  }
 }
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -455,6 +602,12 @@ int kv4_check(const char* name, const void* cache, int seqs, int kvh, int hd, in
     if (dtype == FSTU_F32) by_width(float{}); else by_width(bf16_t{});                                                          \
   } while (0)
 
+// Whole waves over the dims of a row's heads, up to 256 threads.
+int kv4_threads(int kvh, int hd) {
+  const int64_t n = (int64_t)kvh * (hd / 8);
+  return n > 192 ? 256 : (int)((n + 63) / 64 * 64);
+}
+
 }  // namespace
 
 extern "C" int64_t fstu_kv4_bytes(int seqs, int kvh, int hd, int cap) {
@@ -470,12 +623,17 @@ extern "C" int fstu_kv4_write(const void* k, int64_t k_row, int64_t k_head, cons
   const int size = dtype == FSTU_BF16 ? 2 : 4;
   FSTU_REQUIRE(fstu_heads_aligned(k, k_row, k_head, size) && fstu_heads_aligned(v, v_row, v_head, size), FSTU_EALIGN,
                "fstu_kv4_write: rows and heads of k and v must begin at multiples of 16 bytes");
-  const int64_t blocks = ((int64_t)rows * kvh * (hd / 8) + 255) / 256;
-  FSTU_REQUIRE(blocks <= 0x7fffff, FSTU_ESHAPE, "fstu_kv4_write: %d rows of %d heads of %d are more than a launch takes", rows, kvh, hd);
+  const int64_t groups = cu ? (int64_t)rows / 8 + 2 * (int64_t)seqs : rows;
+  FSTU_REQUIRE(groups < 1 << 23, FSTU_ESHAPE, "fstu_kv4_write: %d rows of %d sequences are more than a launch takes", rows, seqs);
   if (rows == 0) return FSTU_OK;
-  KV4_DISPATCH(dtype, hd, "fstu_kv4_write",
-               hipLaunchKernelGGL((kv4_write_kernel<T, HD>), dim3((unsigned)blocks, 2), dim3(256), 0, (hipStream_t)stream, (const T*)k, (const T*)v, k_row, k_head,
-                                  v_row, v_head, cache, pos, cu, rows, seqs, kvh, cap));
+  const int threads = kv4_threads(kvh, hd);
+  KV4_DISPATCH(dtype, hd, "fstu_kv4_write", {
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups, 2), dim3(threads), 0, (hipStream_t)stream, (const T*)k, (const T*)v, k_row, k_head, v_row, v_head, cache,
+                         pos, cu, rows, seqs, kvh, cap);
+    };
+    cu ? run(kv4_write_kernel<T, HD, false>) : run(kv4_write_kernel<T, HD, true>);
+  });
   FSTU_CHECK_LAUNCH("fstu_kv4_write");
   return FSTU_OK;
 }
@@ -487,12 +645,16 @@ extern "C" int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos
   FSTU_REQUIRE(k && v && pos, FSTU_ENULL, "fstu_kv4_read: null pointer");
   FSTU_REQUIRE(rows >= 0 && (cu || rows == seqs), FSTU_EARG, "fstu_kv4_read: %d rows for %d sequences", rows, seqs);
   FSTU_REQUIRE(fstu_aligned(k, 16) && fstu_aligned(v, 16), FSTU_EALIGN, "fstu_kv4_read: k and v must be 16-byte aligned");
-  const int64_t blocks = ((int64_t)rows * kvh * (hd / 8) + 255) / 256;
-  FSTU_REQUIRE(blocks <= 0x7fffff, FSTU_ESHAPE, "fstu_kv4_read: %d rows of %d heads of %d are more than a launch takes", rows, kvh, hd);
+  const int64_t groups = cu ? (int64_t)rows / 8 + 2 * (int64_t)seqs : rows;
+  FSTU_REQUIRE(groups < 1 << 23, FSTU_ESHAPE, "fstu_kv4_read: %d rows of %d sequences are more than a launch takes", rows, seqs);
   if (rows == 0) return FSTU_OK;
-  KV4_DISPATCH(dtype, hd, "fstu_kv4_read",
-               hipLaunchKernelGGL((kv4_read_kernel<T, HD>), dim3((unsigned)blocks, 2), dim3(256), 0, (hipStream_t)stream, cache, (T*)k, (T*)v, pos, cu, rows, seqs,
-                                  kvh, cap));
+  const int threads = kv4_threads(kvh, hd);
+  KV4_DISPATCH(dtype, hd, "fstu_kv4_read", {
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups, 2), dim3(threads), 0, (hipStream_t)stream, cache, (T*)k, (T*)v, pos, cu, rows, seqs, kvh, cap);
+    };
+    cu ? run(kv4_read_kernel<T, HD, false>) : run(kv4_read_kernel<T, HD, true>);
+  });
   FSTU_CHECK_LAUNCH("fstu_kv4_read");
   return FSTU_OK;
 }
