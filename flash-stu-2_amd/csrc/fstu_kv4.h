@@ -4,7 +4,8 @@
 // two as their scale, held as its biased exponent (a byte; 255: the block stands for NaN).  A value is code * 2^(byte - 127), which is
 // exact in bf16.  Slots are padded to a multiple of 32; head = sequence * kv_heads + key head.
 //   key codes     (head, slot, hd/2)                         a row as it is
-//   value codes   (head, slot/8, 16, slot%8, hd/32)          a lane of the second product takes hd/16 dims of eight slots: one piece
+//   value codes   (head, slot/8, plane, 16, ...)             a lane of the second product takes hd/16 dims (hd/32 bytes) of eight slots, slot by slot; what
+//                                                            is more than 16 bytes of that is cut into planes of 16, so that 16 lanes read 256 beside each other
 //   key scales    (head, slot/8, hd/32, slot%8)              eight slots' scales of a block beside each other
 //   value scales  the same
 #pragma once

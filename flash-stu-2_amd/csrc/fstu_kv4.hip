@@ -39,34 +39,37 @@ __device__ __forceinline__ void store8(T* p, const float* o) {
   }
 }
 
-// Codes of dims 8u .. 8u + 7 of a value at one slot (a word, low nibble first), in the pieces of hd/16 dims that the cache deals them to.
+// Where byte b of chunk c's (hd/16 dims) piece at slot i of eight lies: pieces of hd/4 bytes in planes of 16.
+template <int HD>
+__device__ __forceinline__ int value_at(int c, int i, int b) {
+  const int at = i * (HD / 32) + b;
+  return HD <= 64 ? c * (HD / 4) + at : (at & ~15) * 16 + c * 16 + (at & 15);
+}
+// Codes of dims 8u .. 8u + 7 of a value at one slot (a word, low nibble first).
 template <int HD>
 __device__ __forceinline__ void put_value(unsigned char* tile, int i, int u, unsigned code) {       // slot i of the eight at `tile`
-  constexpr int PB = HD / 32;                                  // bytes of a piece
-  tile += i * PB;
-  if constexpr (PB >= 4) *(unsigned*)(tile + (u * 4 / PB) * 8 * PB + (u * 4) % PB) = code;
-  else if constexpr (PB == 2) {
-    *(unsigned short*)(tile + (2 * u) * 16) = (unsigned short)code;
-    *(unsigned short*)(tile + (2 * u + 1) * 16) = (unsigned short)(code >> 16);
+  if constexpr (HD >= 128) *(unsigned*)(tile + value_at<HD>(u * 128 / HD, i, u * 4 % (HD / 32))) = code;
+  else if constexpr (HD == 64) {
+    *(unsigned short*)(tile + value_at<HD>(2 * u, i, 0)) = (unsigned short)code;
+    *(unsigned short*)(tile + value_at<HD>(2 * u + 1, i, 0)) = (unsigned short)(code >> 16);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tile[(4 * u + e) * 8] = (unsigned char)(code >> (8 * e));
+    for (int e = 0; e < 4; ++e) tile[value_at<HD>(4 * u + e, i, 0)] = (unsigned char)(code >> (8 * e));
   }
 }
 template <int HD>
 __device__ __forceinline__ unsigned get_value(const unsigned char* tile, int i, int u) {
-  constexpr int PB = HD / 32;
-  tile += i * PB;
-  if constexpr (PB >= 4) return *(const unsigned*)(tile + (u * 4 / PB) * 8 * PB + (u * 4) % PB);
-  else if constexpr (PB == 2) return *(const unsigned short*)(tile + (2 * u) * 16) | (unsigned)*(const unsigned short*)(tile + (2 * u + 1) * 16) << 16;
+  if constexpr (HD >= 128) return *(const unsigned*)(tile + value_at<HD>(u * 128 / HD, i, u * 4 % (HD / 32)));
+  else if constexpr (HD == 64)
+    return *(const unsigned short*)(tile + value_at<HD>(2 * u, i, 0)) | (unsigned)*(const unsigned short*)(tile + value_at<HD>(2 * u + 1, i, 0)) << 16;
   else {
     unsigned code = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) code |= (unsigned)tile[(4 * u + e) * 8] << (8 * e);
+    for (int e = 0; e < 4; ++e) code |= (unsigned)tile[value_at<HD>(4 * u + e, i, 0)] << (8 * e);
     return code;
   }
 }
-// The same at all eight slots, as the 32 bytes beside each other that they are (hd up to 128): pieces of four, two or one byte a slot.
+// The same at all eight slots (hd up to 128), pieces of four, two or one byte a slot: 32 bytes beside each other, at hd 128 two halves of a plane each.
 template <int HD>
 __device__ __forceinline__ void eight_to_pieces(const unsigned* code, unsigned* w) {
   if constexpr (HD == 128) {
@@ -164,12 +167,12 @@ __device__ __forceinline__ Eight eight_of(const int* cu, const int* pos, int seq
 
 // A workgroup takes a group of eight slots (ONE: one row of a sequence), keys where y = 0 and values where y = 1; a thread eight dims of a head.  Each thread's
 // eight rows are asked for together, and what it leaves is 32 bytes beside each other (keys: 4 in each of eight rows).  16384 rows of 16 x 128 in bf16, written and
-// read back: 134 us with a row's eight dims to a thread, WRITE_US now.
+// read back: 132 us with a row's eight dims to a thread, 76 so.
 template <typename T, int HD, bool ONE>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* cache, const int* pos, const int* cu, int rows,
                  int seqs, int kvh, int cap) {
-  constexpr int P = HD / 8;
+  constexpr int P = HD / 8, kPiece = HD == 128 ? 16 : 32, kPlane = HD == 128 ? 256 : 16;
   const Kv4 c = kv4_at(cache, (int64_t)seqs * kvh, HD, cap);
   const bool keys = blockIdx.y == 0;
   const T* const x = keys ? k : v;
@@ -214,8 +217,8 @@ kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t 
         if constexpr (HD <= 128) {
           unsigned w[8];
           eight_to_pieces<HD>(code, w);
-          *(uint4*)(tile + u * 32) = make_uint4(w[0], w[1], w[2], w[3]);
-          *(uint4*)(tile + u * 32 + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+          *(uint4*)(tile + u * kPiece) = make_uint4(w[0], w[1], w[2], w[3]);
+          *(uint4*)(tile + u * kPiece + kPlane) = make_uint4(w[4], w[5], w[6], w[7]);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) put_value<HD>(tile, i, u, code[i]);
@@ -240,7 +243,7 @@ kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t 
 template <typename T, int HD, bool ONE>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const void* cache, T* k, T* v, const int* pos, const int* cu, int rows, int seqs, int kvh, int cap) {
-  constexpr int P = HD / 8;
+  constexpr int P = HD / 8, kPiece = HD == 128 ? 16 : 32, kPlane = HD == 128 ? 256 : 16;
   const Kv4 c = kv4_at((void*)cache, (int64_t)seqs * kvh, HD, cap);
   const bool keys = blockIdx.y == 0;
   T* const y = keys ? k : v;
@@ -280,7 +283,7 @@ kv4_read_kernel(const void* cache, T* k, T* v, const int* pos, const int* cu, in
       } else {
         const unsigned char* tile = c.vc + (at + g.slot) * (HD / 2);
         if constexpr (HD <= 128) {
-          const uint4 a = *(const uint4*)(tile + u * 32), b = *(const uint4*)(tile + u * 32 + 16);
+          const uint4 a = *(const uint4*)(tile + u * kPiece), b = *(const uint4*)(tile + u * kPiece + kPlane);
           const unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
           pieces_to_eight<HD>(w, code);
         } else {
@@ -327,14 +330,19 @@ __device__ __forceinline__ float capped(float s, float scale, float capA) {
 
 #define KV4_COLS 8        // query heads of a key head that a workgroup takes
 
-template <int N>
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_from(const void* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const V*)p);
+  return *(const V*)p;
+}
+template <int N, bool STREAM>
 __device__ __forceinline__ void load_words(unsigned* w, const unsigned char* p) {
-  if constexpr (N == 1) w[0] = *(const unsigned*)p;
-  else if constexpr (N == 2) { const u32x2_t v = *(const u32x2_t*)p; w[0] = v[0]; w[1] = v[1]; }
+  if constexpr (N == 1) w[0] = load_from<STREAM, unsigned>(p);
+  else if constexpr (N == 2) { const u32x2_t v = load_from<STREAM, u32x2_t>(p); w[0] = v[0]; w[1] = v[1]; }
   else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const u32x4_t v = ((const u32x4_t*)p)[i];
+      const u32x4_t v = load_from<STREAM, u32x4_t>(p + 16 * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
     }
@@ -347,8 +355,12 @@ __device__ __forceinline__ unsigned two_values(unsigned word, float scale) {
 __device__ __forceinline__ bf16x8_t eight_values(unsigned word, float scale) {
   return __builtin_bit_cast(bf16x8_t, u32x4_t{two_values<0>(word, scale), two_values<1>(word, scale), two_values<2>(word, scale), two_values<3>(word, scale)});
 }
-template <int SEL>
-__device__ __forceinline__ float scale_of(u32x2_t bytes) { return kv4_scale_value((SEL < 4 ? bytes[0] >> (8 * SEL) : bytes[1] >> (8 * (SEL - 4))) & 255); }
+// A scale for the conversions above, byte J of eight: they look at the exponent's bits of it and at nothing beside them, so that one shift does.
+template <int J>
+__device__ __forceinline__ float scale_of(u32x2_t bytes) {
+  const unsigned w = bytes[J / 4];
+  return __uint_as_float((J & 3) < 3 ? w << (23 - 8 * (J & 3)) : w >> 1);
+}
 template <int HD>      // dims 2b, 2b + 1 of a piece of hd/16 at slot j
 __device__ __forceinline__ unsigned piece_pair(const unsigned* w, float scale, int j, int b) {
   const int byte = j * (HD / 32) + b;
@@ -367,217 +379,361 @@ struct Kv4Tile {
   static constexpr int KW = HD / 32, VW = HD / 16, KN = HD == 256 ? 2 : 1;
   unsigned k[2][KW], v[VW];
   u32x2_t ks[KN], vs;
+  // STREAM: codes past the caches, which a ring of more than they hold would only push other data out of
+  template <bool STREAM>
   __device__ __forceinline__ void load(const Kv4& c, int64_t slot0, int g, int col) {
     const unsigned char* kt = c.kc + slot0 * (HD / 2);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const unsigned at = (8 * (col >> 2) + 4 * t + (col & 3)) * (HD / 2) + g * (HD / 8 / KN);
 #pragma unroll
-      for (int n = 0; n < KN; ++n) load_words<KW / KN>(k[t] + n * (KW / KN), kt + at + n * (HD / 4));
+      for (int n = 0; n < KN; ++n) load_words<KW / KN, STREAM>(k[t] + n * (KW / KN), kt + at + n * (HD / 4));
     }
-    load_words<VW>(v, c.vc + slot0 * (HD / 2) + (g * 16 + col) * (HD / 4));
     const unsigned char *kst = c.ks + slot0 * (HD / 32), *vst = c.vs + slot0 * (HD / 32);
 #pragma unroll
     for (int n = 0; n < KN; ++n) ks[n] = *(const u32x2_t*)(kst + (col >> 2) * (HD / 4) + (g * (HD / KN) / 128 + 4 * n) * 8);
+    const unsigned char* vt = c.vc + slot0 * (HD / 2) + g * (4 * HD);
+    if constexpr (HD <= 64) load_words<VW, STREAM>(v, vt + col * (HD / 4));
+    else {
+#pragma unroll
+      for (int n = 0; n < VW / 4; ++n) load_words<4, STREAM>(v + 4 * n, vt + n * 256 + col * 16);
+    }
     vs = *(const u32x2_t*)(vst + g * (HD / 4) + (col * HD / 512) * 8);
   }
 };
 
-template <typename T, int HD, int NW, bool CAP>
-__global__ void __launch_bounds__(NW * 64)
+// The tiles of 32 slots that the query of a sequence at position p looks at: `count` of them from `start` on, around the ring's end.
+struct Tiles {
+  int slot, lim, start, count;       // the query's own slot, how far behind it the last key is
+};
+__device__ __forceinline__ Tiles tiles_of(int p, int cap, int window, int tiles) {
+  Tiles t;
+  t.slot = p < 0 ? 0 : p % cap;
+  t.lim = p < 0 ? -1 : min(window, p);
+  const int lo = t.slot - t.lim;
+  t.start = (lo < 0 ? lo + cap : lo) / KV4_TILE;
+  t.count = p < 0 ? 0 : lo < 0 ? min(tiles, tiles - t.start + t.slot / KV4_TILE + 1) : t.slot / KV4_TILE - t.start + 1;
+  return t;
+}
+
+// All sequences' tiles behind one another, `per_seq` groups (key heads, chunks of query heads) each: workgroup w of W takes per or per + 1 of them.
+struct Plan {
+  int total, per, more;
+  __device__ __forceinline__ int begin(int w) const { return w * per + min(w, more); }
+  __device__ __forceinline__ int owner(int x) const { return x < more * (per + 1) ? x / (per + 1) : more + (x - more * (per + 1)) / per; }
+};
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }      // zero where there is no such lane
+__device__ __forceinline__ int wave_prefix(int v) {          // inclusive: inside rows of 16 lanes, then their last lanes onto the rows behind
+  v += dpp_int<0x111, 0xf>(v);
+  v += dpp_int<0x112, 0xf>(v);
+  v += dpp_int<0x114, 0xf>(v);
+  v += dpp_int<0x118, 0xf>(v);
+  v += dpp_int<0x142, 0xa>(v);
+  return v + dpp_int<0x143, 0xc>(v);
+}
+__device__ __forceinline__ int tiles_behind(const int* pos, int seqs, int at, int cap, int window, int tiles) {      // of the lane's sequence
+  const int b = at + ((int)threadIdx.x & 63);
+  return b < seqs ? tiles_of(pos[b], cap, window, tiles).count : 0;
+}
+__device__ __forceinline__ Plan plan_of(const int* pos, int seqs, int cap, int window, int tiles, int per_seq, int W) {
+  int n = 0;
+  for (int at = 0; at < seqs; at += 64) n += __builtin_amdgcn_readlane(wave_prefix(tiles_behind(pos, seqs, at, cap, window, tiles)), 63);
+  Plan p;
+  p.total = n * per_seq;
+  p.per = p.total / W;
+  p.more = p.total - p.per * W;
+  return p;
+}
+// The sequence whose tiles hold tile x (x < total), and where they begin.
+__device__ __forceinline__ int sequence_of(const int* pos, int seqs, int cap, int window, int tiles, int per_seq, int x, int* begin, int* count) {
+  int sum = 0, at = 0;
+  for (;;) {
+    const int n = tiles_behind(pos, seqs, at, cap, window, tiles), end = wave_prefix(n), all = __builtin_amdgcn_readlane(end, 63);
+    if (x < (sum + all) * per_seq || at + 64 >= seqs) {
+      const unsigned long long yes = __ballot((sum + end - n) * per_seq <= x && at + ((int)threadIdx.x & 63) < seqs);
+      const int i = 63 - __builtin_clzll(yes | 1);
+      *count = __builtin_amdgcn_readlane(n, i);
+      *begin = (sum + __builtin_amdgcn_readlane(end - n, i)) * per_seq;
+      return at + i;
+    }
+    sum += all;
+    at += 64;
+  }
+}
+
+// One query a sequence.  S^T = K Q^T over 32 slots at a time as two tiles of 16 keys, rows dealt so that lane (g, col) ends up with query col's scores of slots
+// 8 g .. 8 g + 7, which is what it holds of the second product O^T = V^T P^T: no score crosses a lane, only the maxima do.  Codes become bf16 in registers (exact),
+// probabilities go in as a bf16 head and, in the columns 8 further on, what its rounding left (fp32: two such parts).
+// PLAN: the tiles of all sequences are dealt evenly to the workgroups, whose parts kv4_join_kernel adds up; without, a workgroup takes a key head of a sequence.
+template <typename T, int HD, int NW, bool CAP, bool PLAN>
+__global__ void __launch_bounds__(NW * 64, HD == 256 || NW == 8 ? 1 : HD == 128 ? 2 : 3)
 kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, T* out, float* ws, const int* pos, const float* slopes, int seqs, int heads,
                   int kvh, int cap, int window, float softcap, int chunks) {
   constexpr int KS = HD / 32, NV = HD / 16, QP = sizeof(T) == 2 ? 1 : 3;     // steps of a score's product, tiles of dims, bf16 parts of a query
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int splits = gridDim.x, split = blockIdx.x, hk = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
-  const int group = heads / kvh, cols = min(KV4_COLS, group - chunk * KV4_COLS);
-  const int h0 = hk * group + chunk * KV4_COLS;
+  const int group = heads / kvh, per_seq = kvh * chunks;
   const Kv4 c = kv4_at((void*)cache, (int64_t)seqs * kvh, HD, cap);
-  const int64_t head0 = ((int64_t)b * kvh + hk) * c.slots;
-  const int p = pos[b], tiles = c.slots / KV4_TILE;
-  const int ps = p < 0 ? 0 : p % cap, lim = p < 0 ? -1 : min(window, p);
-  const int lo = ps - lim < 0 ? ps - lim + cap : ps - lim, start = lo / KV4_TILE;
-  const int n = p < 0 ? 0 : ps - lim < 0 ? min(tiles, tiles - start + ps / KV4_TILE + 1) : ps / KV4_TILE - start + 1;
-  const int first = (int)((int64_t)n * split / splits), last = (int)((int64_t)n * (split + 1) / splits);
-
-  // queries: column col and col + 8 are the same head
-  const int h = h0 + min(col & 7, cols - 1);
-  bf16x8_t qf[KS][QP];
-  {
-    const T* qr = q + b * q_row + h * q_head;
-#pragma unroll
-    for (int x = 0; x < KS; ++x) {
-      float f[8];
-      load8(qr + (HD == 256 ? (x >> 2) * 128 + g * 32 + (x & 3) * 8 : g * (HD / 4) + x * 8), f);
-#pragma unroll
-      for (int e = 0; e < QP; ++e) {
-        u32x4_t part;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          part[i] = pack2_bf16(f[2 * i], f[2 * i + 1]);
-          f[2 * i] -= __uint_as_float(part[i] << 16);
-          f[2 * i + 1] -= __uint_as_float(part[i] & 0xffff0000u);
-        }
-        qf[x][e] = __builtin_bit_cast(bf16x8_t, part);
-      }
-    }
-  }
-  const float kLog2e = 1.4426950408889634f, slope = slopes ? slopes[h] * kLog2e : 0.f, capA = softcap * kLog2e;
+  const int tiles = c.slots / KV4_TILE;
+  const float kLog2e = 1.4426950408889634f, capA = softcap * kLog2e;
   const float scale = rsqrtf((float)HD) * (CAP ? cap_scale<T>(softcap) : kLog2e);
   const unsigned low_part = col < 8 ? 0u : 0xffffffffu;
-  float m = -INFINITY, l = 0.f;
-  floatx4_t o[NV];
-#pragma unroll
-  for (int t = 0; t < NV; ++t) o[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-
-  auto tile_at = [&](int i) { const int t = start + i; return t >= tiles ? t - tiles : t; };
-  Kv4Tile<HD> now, next;
-  int i = first + w;
-  if (i < last) next.load(c, head0 + (int64_t)tile_at(i) * KV4_TILE, g, col);
-  for (; i < last; i += NW) {
-    now = next;
-    const int t0 = tile_at(i) * KV4_TILE;
-    if (i + NW < last) next.load(c, head0 + (int64_t)tile_at(i + NW) * KV4_TILE, g, col);
-    float s[8];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      floatx4_t d = {0.f, 0.f, 0.f, 0.f};
-      float f[Kv4Tile<HD>::KN];
-#pragma unroll
-      for (int e = 0; e < Kv4Tile<HD>::KN; ++e) f[e] = kv4_scale_value((now.ks[e][t] >> (8 * (col & 3))) & 255);
-#pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        const bf16x8_t kf = eight_values(now.k[t][x], f[HD == 256 ? x >> 2 : 0]);
-#pragma unroll
-        for (int e = 0; e < QP; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][e], d, 0, 0, 0);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[4 * t + r] = d[r];
-    }
-    // slot t0 + 8 g + j is score j of this lane
-    const int far0 = t0 <= ps ? ps - t0 : ps + cap - t0;
-    const bool whole = t0 + KV4_TILE <= cap && far0 <= lim && (t0 + KV4_TILE - 1 <= ps || t0 > ps);      // wave-uniform
-    const float tb = whole ? -slope * (float)(far0 - 8 * g) : 0.f;
-    float vs[8] = {scale_of<0>(now.vs), scale_of<1>(now.vs), scale_of<2>(now.vs), scale_of<3>(now.vs),
-                   scale_of<4>(now.vs), scale_of<5>(now.vs), scale_of<6>(now.vs), scale_of<7>(now.vs)};
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (CAP) s[j] = capped<T>(s[j], scale, capA);
-      if (whole) s[j] = fmaf(s[j], CAP ? 1.f : scale, slope * (float)j);
-    }
-    if (!whole) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int slot = t0 + 8 * g + j, far = slot <= ps ? ps - slot : ps + cap - slot;
-        const bool seen = slot < cap && far <= lim;
-        s[j] = seen ? fmaf(s[j], CAP ? 1.f : scale, -slope * (float)far) : -INFINITY;
-        vs[j] = seen ? vs[j] : 1.f;                              // a scale of NaN times a weight of zero
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j]);
-    top += tb;
-    if (__any(top > m)) {
-      top = fmaxf(top, fstu_swz16(top));
-      top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
-      const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= corr;
-#pragma unroll
-      for (int t = 0; t < NV; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[t][r] *= corr;
-      m = mn;
-    }
-    const float off = tb - (m == -INFINITY ? 0.f : m);
-    // probabilities in bf16 parts: the columns of the upper half hold what the lower half's rounding left
-    u32x4_t pf, pf2;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float a = __builtin_amdgcn_exp2f(s[2 * e] + off), z = __builtin_amdgcn_exp2f(s[2 * e + 1] + off);
-      l += a + z;
-      const unsigned head = pack2_bf16(a, z) & low_part;
-      a -= __uint_as_float(head << 16);
-      z -= __uint_as_float(head & 0xffff0000u);
-      pf[e] = pack2_bf16(a, z);
-      if (QP == 3) {                                             // and, for fp32, a third part beside the second
-        a -= __uint_as_float(pf[e] << 16);
-        z -= __uint_as_float(pf[e] & 0xffff0000u);
-        pf2[e] = pack2_bf16(a, z) & low_part;
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NV / 2; ++t) {
-      u32x4_t even, odd;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned a = piece_pair<HD>(now.v, vs[2 * e], 2 * e, t), z = piece_pair<HD>(now.v, vs[2 * e + 1], 2 * e + 1, t);
-        even[e] = __builtin_amdgcn_perm(z, a, 0x05040100);
-        odd[e] = __builtin_amdgcn_perm(z, a, 0x07060302);
-      }
-      o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), __builtin_bit_cast(bf16x8_t, pf), o[2 * t], 0, 0, 0);
-      o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd), __builtin_bit_cast(bf16x8_t, pf), o[2 * t + 1], 0, 0, 0);
-      if (QP == 3) {
-        o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), __builtin_bit_cast(bf16x8_t, pf2), o[2 * t], 0, 0, 0);
-        o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd), __builtin_bit_cast(bf16x8_t, pf2), o[2 * t + 1], 0, 0, 0);
-      }
-    }
-  }
-  l += fstu_swz16(l);
-  l += __shfl_xor(l, 32, FSTU_WAVE);
+  const unsigned turn = (8 * (col & 3) + 9) & 31;                // turns byte col & 3 to where a float has its exponent
   extern __shared__ float sm[];                                  // (NW, cols) maxima, sums, then (NW, cols, HD)
   float* const sl = sm + NW * KV4_COLS;
   float* const so = sl + NW * KV4_COLS;
-#pragma unroll
-  for (int t = 0; t < NV; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[t][r] += fstu_dpp<0x128>(o[t][r]);         // row_ror:8: the other part's column
-  if (col < cols) {
-    if (g == 0) { sm[w * KV4_COLS + col] = m; sl[w * KV4_COLS + col] = l; }
-    float* dst = so + (w * cols + col) * HD + 4 * g * NV;        // dim (4 g + r) * NV + t
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int t = 0; t < NV; ++t) dst[r * NV + t] = o[t][r];
+
+  Plan plan;
+  int x = 0, x_end = 1;
+  if (PLAN) {
+    plan = plan_of(pos, seqs, cap, window, tiles, per_seq, gridDim.x);
+    x = plan.begin(blockIdx.x);
+    x_end = plan.begin(blockIdx.x + 1);
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < cols * HD; e += NW * 64) {
-    const int cc = e / HD, d = e % HD;
-    float M = -INFINITY, L = 0.f, y = 0.f;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) M = fmaxf(M, sm[x * KV4_COLS + cc]);
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      const float f = sm[x * KV4_COLS + cc] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[x * KV4_COLS + cc] - M);
-      const float lx = sl[x * KV4_COLS + cc], yx = so[(x * cols + cc) * HD + d];
-      L = fmaf(lx, f, L);
-      y = fmaf(yx, f, y);
+  while (x < x_end) {                                            // a stretch of one key head's tiles
+    int b, y, first = 0, last, all;
+    if (PLAN) {
+      int begin;
+      b = sequence_of(pos, seqs, cap, window, tiles, per_seq, x, &begin, &all);
+      all = max(all, 1);                                         // (whatever becomes of pos meanwhile: an end, and no head that is not there)
+      y = min(max((x - begin) / all, 0), per_seq - 1);
+      first = max(x - begin - y * all, 0);
+      last = min(all, first + x_end - x);
+      x += max(last - first, 1);
+    } else {
+      b = blockIdx.y;
+      y = blockIdx.x;
+      x = x_end;
     }
-    const int64_t row = (int64_t)b * heads + h0 + cc;
-    if (splits == 1) DT<T>::st(out + row * HD + d, n ? y / L : 0.f);
-    else {
-      float* part = ws + (row * splits + split) * (HD + 2);
-      part[2 + d] = y;
-      if (d == 0) { part[0] = M; part[1] = L; }
+    const Tiles tl = tiles_of(pos[b], cap, window, tiles);
+    const int ps = tl.slot, lim = tl.lim, start = tl.start;
+    if (!PLAN) last = all = tl.count;
+    const int hk = y / chunks, h0 = hk * group + y % chunks * KV4_COLS, cols = min(KV4_COLS, hk * group + group - h0);
+    const int64_t head0 = ((int64_t)b * kvh + hk) * c.slots;
+
+    // queries: column col and col + 8 are the same head
+    const int h = h0 + min(col & 7, cols - 1);
+    bf16x8_t qf[KS][QP];
+    {
+      const T* qr = q + b * q_row + h * q_head;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        float f[8];
+        load8(qr + (HD == 256 ? (k >> 2) * 128 + g * 32 + (k & 3) * 8 : g * (HD / 4) + k * 8), f);
+#pragma unroll
+        for (int e = 0; e < QP; ++e) {
+          u32x4_t part;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            part[i] = pack2_bf16(f[2 * i], f[2 * i + 1]);
+            f[2 * i] -= __uint_as_float(part[i] << 16);
+            f[2 * i + 1] -= __uint_as_float(part[i] & 0xffff0000u);
+          }
+          qf[k][e] = __builtin_bit_cast(bf16x8_t, part);
+        }
+      }
     }
+    const float slope = slopes ? slopes[h] * kLog2e : 0.f;
+    float m = -INFINITY, l = 0.f;
+    floatx4_t o[NV];
+#pragma unroll
+    for (int t = 0; t < NV; ++t) o[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    auto tile_at = [&](int i) { const int t = start + i; return t >= tiles ? t - tiles : t; };
+    auto take = [&](const Kv4Tile<HD>& now, int i) {
+      const int t0 = tile_at(i) * KV4_TILE;
+      float s[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        floatx4_t d = {0.f, 0.f, 0.f, 0.f};
+        float f[Kv4Tile<HD>::KN];
+#pragma unroll
+        for (int e = 0; e < Kv4Tile<HD>::KN; ++e) f[e] = __uint_as_float(__builtin_amdgcn_alignbit(now.ks[e][t], now.ks[e][t], turn));
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+          const bf16x8_t kf = eight_values(now.k[t][x], f[HD == 256 ? x >> 2 : 0]);
+#pragma unroll
+          for (int e = 0; e < QP; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[x][e], d, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * t + r] = d[r];
+      }
+      // slot t0 + 8 g + j is score j of this lane
+      const int far0 = t0 <= ps ? ps - t0 : ps + cap - t0;
+      const bool whole = __builtin_amdgcn_readfirstlane(t0 + KV4_TILE <= cap && far0 <= lim && (t0 + KV4_TILE - 1 <= ps || t0 > ps)) != 0;      // wave-uniform
+      const float tb = whole ? -slope * (float)(far0 - 8 * g) : 0.f;
+      float vs[8] = {scale_of<0>(now.vs), scale_of<1>(now.vs), scale_of<2>(now.vs), scale_of<3>(now.vs),
+                     scale_of<4>(now.vs), scale_of<5>(now.vs), scale_of<6>(now.vs), scale_of<7>(now.vs)};
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (CAP) s[j] = capped<T>(s[j], scale, capA);
+      }
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = fmaf(s[j], CAP ? 1.f : scale, slope * (float)j);
+      } else {
+        asm volatile("");                                          // a branch: most tiles need none of this
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int slot = t0 + 8 * g + j, far = slot <= ps ? ps - slot : ps + cap - slot;
+          const bool seen = slot < cap && far <= lim;
+          s[j] = seen ? fmaf(s[j], CAP ? 1.f : scale, -slope * (float)far) : -INFINITY;
+          vs[j] = seen ? vs[j] : 1.f;                              // a scale of NaN times a weight of zero
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j]);
+      top += tb;
+      if (__any(top > m)) {
+        top = fmaxf(top, fstu_swz16(top));
+        top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
+        const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= corr;
+#pragma unroll
+        for (int t = 0; t < NV; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t][r] *= corr;
+        m = mn;
+      }
+      const float off = tb - (m == -INFINITY ? 0.f : m);
+      // probabilities in bf16 parts: the columns of the upper half hold what the lower half's rounding left
+      u32x4_t pf, pf2;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float a = __builtin_amdgcn_exp2f(s[2 * e] + off), z = __builtin_amdgcn_exp2f(s[2 * e + 1] + off);
+        l += a + z;
+        const unsigned head = pack2_bf16(a, z) & low_part;
+        a -= __uint_as_float(head << 16);
+        z -= __uint_as_float(head & 0xffff0000u);
+        pf[e] = pack2_bf16(a, z);
+        if (QP == 3) {                                             // and, for fp32, a third part beside the second
+          a -= __uint_as_float(pf[e] << 16);
+          z -= __uint_as_float(pf[e] & 0xffff0000u);
+          pf2[e] = pack2_bf16(a, z) & low_part;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NV / 2; ++t) {
+        u32x4_t low, high;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned a = piece_pair<HD>(now.v, vs[2 * e], 2 * e, t), z = piece_pair<HD>(now.v, vs[2 * e + 1], 2 * e + 1, t);
+          low[e] = __builtin_amdgcn_perm(z, a, 0x05040100);
+          high[e] = __builtin_amdgcn_perm(z, a, 0x07060302);
+        }
+        o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, low), __builtin_bit_cast(bf16x8_t, pf), o[2 * t], 0, 0, 0);
+        o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, high), __builtin_bit_cast(bf16x8_t, pf), o[2 * t + 1], 0, 0, 0);
+        if (QP == 3) {
+          o[2 * t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, low), __builtin_bit_cast(bf16x8_t, pf2), o[2 * t], 0, 0, 0);
+          o[2 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, high), __builtin_bit_cast(bf16x8_t, pf2), o[2 * t + 1], 0, 0, 0);
+        }
+      }
+    };
+    // AHEAD tiles on their way at any time, each asked for without a branch (behind the last one the last again), so that a wait is for one tile and not for all
+    constexpr int AHEAD = 2;
+    Kv4Tile<HD> ring[AHEAD];
+    int i = first + w;
+    if (i < last) {
+      const int end = i + (last - 1 - i) / NW * NW;
+      auto ask = [&](Kv4Tile<HD>& t, int n) {
+        t.template load<PLAN>(c, head0 + (int64_t)tile_at(min(n, end)) * KV4_TILE, g, col);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) ask(ring[a], i + a * NW);
+      for (bool more = true; more;) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          take(ring[a], i);
+          i += NW;
+          if (i > end) { more = false; break; }
+          ask(ring[a], i + (AHEAD - 1) * NW);
+        }
+      }
+    }
+    l += fstu_swz16(l);
+    l += __shfl_xor(l, 32, FSTU_WAVE);
+#pragma unroll
+    for (int t = 0; t < NV; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[t][r] += fstu_dpp<0x128>(o[t][r]);       // row_ror:8: the other part's column
+    if (col < cols) {
+      if (g == 0) { sm[w * KV4_COLS + col] = m; sl[w * KV4_COLS + col] = l; }
+      float* dst = so + (w * cols + col) * HD + 4 * g * NV;      // dim (4 g + r) * NV + t
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int t = 0; t < NV; ++t) dst[r * NV + t] = o[t][r];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < cols * HD; e += NW * 64) {
+      const int cc = e / HD, d = e % HD;
+      float M = -INFINITY, L = 0.f, v = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) M = fmaxf(M, sm[k * KV4_COLS + cc]);
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float f = sm[k * KV4_COLS + cc] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[k * KV4_COLS + cc] - M);
+        L = fmaf(sl[k * KV4_COLS + cc], f, L);
+        v = fmaf(so[(k * cols + cc) * HD + d], f, v);
+      }
+      if (!PLAN || last - first == all) DT<T>::st(out + ((int64_t)b * heads + h0 + cc) * HD + d, all ? v / L : 0.f);
+      else {
+        // one place to each pair of workgroup and key head that meet: both rise from one to the next
+        float* part = ws + ((int64_t)(blockIdx.x + b * per_seq + y) * KV4_COLS + cc) * (HD + 2);
+        part[2 + d] = v;
+        if (d == 0) { part[0] = M; part[1] = L; }
+      }
+    }
+    if (PLAN) __syncthreads();
   }
 }
 
-// Splits of a query's keys, in their order.
+// The parts of a query head, in the order of its keys: several to a thread row, joined through LDS.
 template <typename T, int HD>
-__global__ void __launch_bounds__(HD)
-kv4_join_kernel(const float* ws, T* out, int splits) {
-  const int64_t row = blockIdx.x;
-  const float* part = ws + row * splits * (HD + 2);
-  float M = -INFINITY, L = 0.f, y = 0.f;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, part[s * (HD + 2)]);
-  for (int s = 0; s < splits; ++s) {
-    const float* ps = part + s * (HD + 2);
-    const float f = ps[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ps[0] - M);
-    L = fmaf(ps[1], f, L);
-    y = fmaf(ps[2 + threadIdx.x], f, y);
+__global__ void __launch_bounds__(512)
+kv4_join_kernel(const float* ws, T* out, const int* pos, int seqs, int heads, int kvh, int cap, int window, int chunks, int W) {
+  constexpr int R = 512 / HD;
+  const int b = blockIdx.x / heads, h = blockIdx.x % heads, group = heads / kvh, hk = h / group, per_seq = kvh * chunks;
+  const int y = hk * chunks + (h - hk * group) / KV4_COLS, cc = (h - hk * group) % KV4_COLS, d = threadIdx.x % HD, r = threadIdx.x / HD;
+  const int tiles = kv4_slots(cap) / KV4_TILE, count = tiles_of(pos[b], cap, window, tiles).count;
+  T* const dst = out + (int64_t)blockIdx.x * HD + d;
+  if (count == 0) {
+    if (r == 0) DT<T>::st(dst, 0.f);
+    return;
   }
-  DT<T>::st(out + row * HD + threadIdx.x, L == 0.f ? 0.f : y / L);
+  const Plan plan = plan_of(pos, seqs, cap, window, tiles, per_seq, W);
+  int before = 0;
+  for (int at = 0; at < b; at += 64) before += __builtin_amdgcn_readlane(wave_prefix(tiles_behind(pos, b, at, cap, window, tiles)), 63);
+  const int begin = min(before * per_seq + y * count, plan.total - 1), w0 = plan.owner(begin), w1 = min(plan.owner(begin + count - 1), W - 1);
+  if (w0 == w1) return;                                          // whole, and there already
+  const float* part = ws + ((int64_t)(w0 + b * per_seq + y) * KV4_COLS + cc) * (HD + 2);
+  constexpr int STEP = KV4_COLS * (HD + 2);
+  const int n = w1 - w0 + 1;
+  float M = -INFINITY, L = 0.f, v = 0.f;
+#pragma unroll 4
+  for (int s = r; s < n; s += R) {
+    const float m = part[(int64_t)s * STEP], l = part[(int64_t)s * STEP + 1], o = part[(int64_t)s * STEP + 2 + d];
+    const float top = fmaxf(M, m), f = M == top ? 1.f : __builtin_amdgcn_exp2f(M - top), e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    L = fmaf(L, f, l * e);
+    v = fmaf(v, f, o * e);
+    M = top;
+  }
+  __shared__ float sm[R], sl[R], so[R][HD];
+  if (d == 0) { sm[r] = M; sl[r] = L; }
+  so[r][d] = v;
+  __syncthreads();
+  if (r) return;
+  M = -INFINITY;
+  for (int s = 0; s < R; ++s) M = fmaxf(M, sm[s]);
+  L = v = 0.f;
+  for (int s = 0; s < R; ++s) {
+    const float e = sm[s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[s] - M);
+    const float ls = sl[s], os = so[s][d];
+    L = fmaf(ls, e, L);
+    v = fmaf(os, e, v);
+  }
+  DT<T>::st(dst, v / L);
 }
 
 int kv4_check(const char* name, const void* cache, int seqs, int kvh, int hd, int cap) {
@@ -659,16 +815,21 @@ extern "C" int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos
   return FSTU_OK;
 }
 
-#define KV4_WAVES 4
-
+// Workgroups of a call whose keys are dealt evenly; 1: a workgroup to each key head of a sequence.  Dealing costs a second launch and two looks at all positions,
+// some 8 us, and pays where few heads leave compute units idle through a long ring or where long rings end unevenly.  us, a workgroup to a head / dealt: 32 heads of
+// 128 over 2100 positions 13.9 / 15.7, 4200 22.3 / 17.4; 12 heads of 64 over 2048 9.9 / 10.5, 4000 15.4 / 12.2; 4 heads of 128 over 32768 135 / 14.9; 256 heads of 128
+// over up to 4096 24 / 32, 512 over 4096 49 / 52, 640 over 8192 125 / 112, 384 over 16384 166 / 136, 128 over 32768 155 / 89 (512 workgroups 96, 128 128).
 extern "C" int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window) {
   if (seqs < 1 || kvh < 1 || heads < kvh || cap < 1 || window < 0) return 1;
   const int chunks = (heads / kvh + KV4_COLS - 1) / KV4_COLS;
+  const int64_t tiles = ((int64_t)(window < cap ? window : cap - 1) + 2 * KV4_TILE - 1) / KV4_TILE;
   const int64_t groups = (int64_t)seqs * kvh * chunks;
-  const int tiles = (int)(((int64_t)(window < cap ? window : cap - 1) + 2 * KV4_TILE - 1) / KV4_TILE);
-  int64_t splits = 1024 / groups;
-  if (splits > tiles / (4 * KV4_WAVES)) splits = tiles / (4 * KV4_WAVES);
-  return splits < 2 ? 1 : (int)(splits > 64 ? 64 : splits);
+  if (tiles <= 96 || (groups > 192 && tiles <= 192)) return 1;
+  const int64_t most = groups * tiles / 16;
+  return (int)(most < 256 ? most : 256);
+}
+extern "C" int64_t fstu_kv4_attend_ws(int seqs, int heads, int kvh, int hd, int splits) {
+  return splits <= 1 ? 0 : ((int64_t)seqs * kvh * ((heads / kvh + KV4_COLS - 1) / KV4_COLS) + splits) * KV4_COLS * (hd + 2);
 }
 
 extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, const void* cache, void* out, float* ws, int splits, const int* pos,
@@ -676,7 +837,7 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
   const int rc = kv4_check("fstu_kv4_attend", cache, seqs, kvh, hd, cap);
   if (rc) return rc;
   FSTU_REQUIRE(q && out && pos, FSTU_ENULL, "fstu_kv4_attend: null pointer");
-  FSTU_REQUIRE(heads >= 1 && heads % kvh == 0 && heads <= 65535 && seqs <= 65535, FSTU_ESHAPE, "fstu_kv4_attend: %d heads over %d key heads, %d sequences", heads,
+  FSTU_REQUIRE(heads >= 1 && heads % kvh == 0 && heads <= 65535 && seqs <= 65535 && (int64_t)seqs * heads <= 0x7fffffff, FSTU_ESHAPE, "fstu_kv4_attend: %d heads over %d key heads, %d sequences", heads,
                kvh, seqs);
   FSTU_REQUIRE(window >= 0 && window < cap, FSTU_EARG, "fstu_kv4_attend: window %d with a capacity of %d", window, cap);
   FSTU_REQUIRE(softcap >= 0.f && softcap < INFINITY, FSTU_EARG, "fstu_kv4_attend: softcap must be zero (none) or a positive number");
@@ -690,13 +851,23 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
                FSTU_EARG, "fstu_kv4_attend: out overlaps q or the cache");
   const int group = heads / kvh, chunks = (group + KV4_COLS - 1) / KV4_COLS;
   KV4_DISPATCH(dtype, hd, "fstu_kv4_attend", {
-    const unsigned lds = KV4_WAVES * (2 * KV4_COLS + (group < KV4_COLS ? group : KV4_COLS) * HD) * sizeof(float);
-    auto run = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(splits, kvh * chunks, seqs), dim3(KV4_WAVES * 64), lds, (hipStream_t)stream, (const T*)q, q_row, q_head, cache, (T*)out, ws,
-                         pos, slopes, seqs, heads, kvh, cap, window, softcap, chunks);
+    auto run = [&](auto kernel, dim3 grid, int waves) {
+      const unsigned lds = waves * (2 * KV4_COLS + (group < KV4_COLS ? group : KV4_COLS) * HD) * sizeof(float);
+      hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), lds, (hipStream_t)stream, (const T*)q, q_row, q_head, cache, (T*)out, ws, pos, slopes, seqs, heads, kvh,
+                         cap, window, softcap, chunks);
     };
-    softcap > 0.f ? run(kv4_attend_kernel<T, HD, KV4_WAVES, true>) : run(kv4_attend_kernel<T, HD, KV4_WAVES, false>);
-    if (splits > 1) hipLaunchKernelGGL((kv4_join_kernel<T, HD>), dim3(seqs * heads), dim3(HD), 0, (hipStream_t)stream, ws, (T*)out, splits);
+    constexpr int WIDE = HD == 256 ? 4 : 8;
+    if (splits > 1) {
+      softcap > 0.f ? run(kv4_attend_kernel<T, HD, WIDE, true, true>, dim3(splits), WIDE) : run(kv4_attend_kernel<T, HD, WIDE, false, true>, dim3(splits), WIDE);
+      hipLaunchKernelGGL((kv4_join_kernel<T, HD>), dim3(seqs * heads), dim3(512), 0, (hipStream_t)stream, ws, (T*)out, pos, seqs, heads, kvh, cap, window, chunks,
+                         splits);
+    } else if ((int64_t)seqs * kvh * chunks <= 256) {            // one to a compute unit: eight waves (12 heads of 64 over 513 positions 5.7 us, 6.6 with four)
+      const dim3 grid(kvh * chunks, seqs);
+      softcap > 0.f ? run(kv4_attend_kernel<T, HD, WIDE, true, false>, grid, WIDE) : run(kv4_attend_kernel<T, HD, WIDE, false, false>, grid, WIDE);
+    } else {
+      const dim3 grid(kvh * chunks, seqs);
+      softcap > 0.f ? run(kv4_attend_kernel<T, HD, 4, true, false>, grid, 4) : run(kv4_attend_kernel<T, HD, 4, false, false>, grid, 4);
+    }
   });
   FSTU_CHECK_LAUNCH("fstu_kv4_attend");
   return FSTU_OK;

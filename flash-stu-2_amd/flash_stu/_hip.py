@@ -83,6 +83,7 @@ SIGNATURES = {
     "fstu_kv4_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "fstu_kv4_attend_splits": [_i, _i, _i, _i, _i, _i],
+    "fstu_kv4_attend_ws": [_i, _i, _i, _i, _i],
     "fstu_sample": [_vp, _vp, _i64, _i, _i, _f, _i, _f, _i, _u64, _i, _i, _vp],
     "fstu_sample_ws_bytes": [],
     "fstu_head_maxima": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp],
@@ -163,6 +164,7 @@ def load(path: Optional[str] = None):
     lib.fstu_sample_ws_bytes.restype = ctypes.c_int64
     lib.fstu_swa_prefill_ws_elems.restype = ctypes.c_int64
     lib.fstu_kv4_bytes.restype = ctypes.c_int64
+    lib.fstu_kv4_attend_ws.restype = ctypes.c_int64
     lib.fstu_lds_sequence_ws_floats.restype = ctypes.c_size_t
     lib.fstu_stu_conv_fft_grad_ws.restype = ctypes.c_int64
     lib.fstu_stu_conv_mfma_grad_ws.restype = ctypes.c_int64
@@ -1652,7 +1654,7 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch
             raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
         _written(out)
     splits = _kv4_splits(seqs, heads, kvh, hd, cache.capacity, window)
-    ws = torch.empty(seqs * heads * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    ws = torch.empty(load().fstu_kv4_attend_ws(seqs, heads, kvh, hd, splits), dtype=torch.float32, device=q.device) if splits > 1 else None
     rc = load().fstu_kv4_attend(qp, qr, qh, cache.data.data_ptr(), out.data_ptr(), _p(ws), splits, pp, sp, seqs, heads, kvh, hd, cache.capacity, window, float(softcap or 0.0), dt,
                                 raw_stream(dev))
     if rc:

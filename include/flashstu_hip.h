@@ -372,8 +372,8 @@ int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k,
  * fstu_kv4_write: rows cu[s].. become positions pos[s].. (of more than cap rows the last cap).
  * fstu_kv4_read: the same positions back, k and v (rows,kvh,hd) dense, exact in either dtype; rows of no sequence zero.
  * fstu_kv4_attend: one query a sequence, q (seqs,heads,hd) by strides, over positions max(0,pos-window)..pos, window < cap; out (seqs,heads,hd) dense.
- *   The keys go to `splits` groups of workgroups, whose parts a second launch joins (ws: seqs * heads * splits * (hd + 2) floats, not shared with a
- *   call that may run at the same time); fstu_kv4_attend_splits says how many pay (1: none, ws may be NULL). */
+ *   splits > 1: the keys of all sequences are dealt evenly to that many workgroups, whose parts a second launch joins (ws: fstu_kv4_attend_ws floats, not
+ *   shared with a call that may run at the same time); fstu_kv4_attend_splits says how many pay (1: a workgroup to each key head, ws may be NULL). */
 int64_t fstu_kv4_bytes(int seqs, int kvh, int hd, int cap);
 int fstu_kv4_write(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* cache, const int* pos,
                    const int* cu, int rows, int seqs, int kvh, int hd, int cap, int dtype, void* stream);
@@ -382,6 +382,7 @@ int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos, const int
 int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, const void* cache, void* out, float* ws, int splits, const int* pos,
                     const float* slopes, int seqs, int heads, int kvh, int hd, int cap, int window, float softcap, int dtype, void* stream);
 int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window);
+int64_t fstu_kv4_attend_ws(int seqs, int heads, int kvh, int hd, int splits);
 
 /* ---- sampling --------------------------------------------------------------
  * Per row of logits (B,V): l = clamp(T(logit/temperature), -1e4, 1e4); optional
