@@ -2,11 +2,15 @@
 //   s_ij = softcap * tanh(q_i . k_j * hd^-1/2 / softcap) - slope * (i - j),  0 <= i - j <= window,  o_i = sum_j softmax_j(s_ij) v_j
 #include "fstu_common.h"
 
+#ifndef PK_NW
+#define PK_NW 4
+#define PK_NQ 2
+#endif
+
 namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float floatx16_t __attribute__((ext_vector_type(16)));
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -85,179 +89,209 @@ swa_packed_kernel(Heads q, Heads k, Heads v, T* out, const int* cu, const float*
                     out + ((int64_t)(at + i) * heads + h) * HD, k.row, v.row, i, window, slopes ? slopes[h] : 0.f, softcap);
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, FSTU_WAVE); }
+template <int HD>
+__device__ __forceinline__ int key_turn(int row) {
+  return HD >= 128 ? (row & 3) | (row >> 3 & 3) << 2 : HD == 64 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : row >> 3 & 3;
+}
+template <int HD>
+__device__ __forceinline__ int value_turn(int row) {
+  return HD >= 128 ? (row & 3) | (row >> 3 & 1) << 2 : HD == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : row >> 3 & 1;
+}
 
-template <int HD, int NW, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : 2)
+// bf16 on the matrix cores: a wave owns NQ tiles of 16 queries of one head and walks their keys 32 at a time,
+//   S^T (keys x queries) = K Q^T      rows dealt so that lane (g, c) ends up with query c's scores of keys 8 g .. 8 g + 7 of the 32, which is
+//   O^T (dims x queries) = V^T P^T    what it holds of the second product: no score crosses a lane, only the maxima do.
+// Tiles of KB keys and values go through LDS by way of registers, one barrier a tile; values are read back transposed.
+template <int HD, int NW, int NQ, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NW * 64, HD == 256 || NW == 8 ? 1 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
                        float softcap) {
-  constexpr int KB = HD == 256 ? 32 : 64, NS = KB / 32, CH = HD / 8, KS = HD / 16, ND = HD / 32, NT = NW * 64;
+  constexpr int KB = HD == 256 ? 32 : 64, NS = KB / 32, CH = HD / 8, KS = HD / 32, ND = HD / 16, NT = NW * 64, WQ = NQ * 16;
   constexpr int PT = (KB * CH + NT - 1) / NT;                    // 16-byte pieces of a tile to a thread
   __shared__ u32x4_t k_two[2][KB * CH], v_two[2][KB * CH];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 31, hi = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % heads, hk = h / (heads / kvh);
   int at, len, first;
-  packed_tile(cu, seqs, rows, NW * 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  packed_tile(cu, seqs, rows, NW * WQ, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int qs = first + w * 32, qi = qs + c;                    // the wave's first query, this lane's
+  const int qs = first + w * WQ;                                 // the wave's first query
   const bool on = qs < len;
-  const bf16_t* kb = (const bf16_t*)k.p + at * k.row + hk * k.head;
-  const bf16_t* vb = (const bf16_t*)v.p + at * v.row + hk * v.head;
   const int64_t k_row = k.row, v_row = v.row;
+  const bf16_t* kb = (const bf16_t*)k.p + at * k_row + hk * k.head;
+  const bf16_t* vb = (const bf16_t*)v.p + at * v_row + hk * v.head;
   const float kLog2e = 1.4426950408889634f, raw_slope = BIAS ? slopes[h] : 0.f, slope = raw_slope * kLog2e;
   const float scale = rsqrtf((float)HD) * (CAP ? 2.0f * kLog2e / softcap : kLog2e), capA = softcap * kLog2e;
 
-  u32x4_t qf[KS];
-  {
-    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + hi * 8;
+  u32x4_t qf[NQ][KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *(const u32x4_t*)(qr + s * 16);
+  for (int n = 0; n < NQ; ++n) {
+    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qs + n * 16 + c, len - 1)) * q.row + h * q.head + g * 8;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[n][s] = *(const u32x4_t*)(qr + s * 32);
   }
-  floatx16_t o[ND];
+  floatx4_t o[NQ][ND];
+  float m[NQ], l[NQ];
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-  float bias[16];                                                // of row (r & 3) + 8 (r >> 2) + 4 hi of a tile of 32 keys
+    for (int d = 0; d < ND; ++d) o[n][d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // ALiBi of key 8 g + 4 t + r of 32: without a soft-cap what the scores' sums begin with, in units of theirs
+  floatx4_t bias[2];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) bias[r] = BIAS ? slope * (float)((r & 3) + 8 * (r >> 2) + 4 * hi) * (CAP ? 1.f : 1.f / scale) : 0.f;
-  float m = -INFINITY, l = 0.f;
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bias[t][r] = BIAS ? slope * (float)(8 * g + 4 * t + r) / (CAP ? 1.f : scale) : 0.f;
 
-  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NW * 32 - 1);
+  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NW * WQ - 1);
   u32x4_t kr[PT], vr[PT];
   auto fetch = [&](int b) {
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
-      const int e = min(tid + i * NT, KB * CH - 1);
+      const int e = min(tid + i * NT, KB * CH - 1);              // threads beyond the tile's pieces hold the last one too
       const int64_t row = min(b + e / CH, len - 1);              // rows behind the sequence: its last one, which no query of these sees
       kr[i] = *(const u32x4_t*)(kb + row * k_row + e % CH * 8);
       vr[i] = *(const u32x4_t*)(vb + row * v_row + e % CH * 8);
     }
   };
+  // The 16-byte pieces of a row are XOR-ed with bits of it, so that what 16 lanes read together lies in different banks: 16 keys' rows one piece each (rows
+  // differ in bits 0, 1, 3 and 4), four values' rows 32 bytes each (bits 0, 1 and 3: two blocks of lanes).
   auto store = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int e = min(tid + i * NT, KB * CH - 1), row = e / CH, ch = e % CH;
-      const int ks = HD >= 128 ? row & 15 : HD == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
-      const int vs = HD >= 128 ? (row & 3) << 2 : HD == 64 ? (row >> 1 & 1) << 2 : 0;
-      k_two[buf][row * CH + (ch ^ ks)] = kr[i];
-      v_two[buf][row * CH + (ch ^ vs)] = vr[i];
+      k_two[buf][row * CH + (ch ^ key_turn<HD>(row))] = kr[i];
+      v_two[buf][row * CH + (ch ^ value_turn<HD>(row) << 1)] = vr[i];
     }
   };
+  int k_at[KS], v_at[ND];                                        // in pieces, and in elements
+  {
+    const int row = 8 * (c >> 2) + (c & 3), vrow = 8 * g + (c >> 2);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k_at[s] = row * CH + ((4 * s + g) ^ key_turn<HD>(row));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) v_at[d] = vrow * HD + (d ^ value_turn<HD>(vrow)) * 16 + 4 * (c & 3);
+  }
   fetch(k_first);
   store(0);
   if (k_first + KB <= k_last) fetch(k_first + KB);
   __syncthreads();
-  const int ksw = HD >= 128 ? c & 15 : HD == 64 ? (c >> 1) & 7 : (c >> 2) & 3;
-  const int li = lane & 15, vx = HD >= 128 ? (li >> 2) & 3 : HD == 64 ? (li >> 3) & 1 : 0;
-  const int v_at = (4 * hi + (li >> 2)) * HD + 16 * (lane >> 4 & 1) + 4 * (li & 3);      // in elements, without the tile of 32 dims
   int buf = 0;
   for (int b = k_first; b <= k_last; b += KB, buf ^= 1) {
     if (b > k_first) __syncthreads();                            // this tile is there, and the one before it has been read
     if (b + KB <= k_last) store(buf ^ 1);
     if (b + 2 * KB <= k_last) fetch(b + 2 * KB);
-    if (!on || b > qs + 31 || b + KB - 1 < qs - window) continue;     // wave-uniform: the wave sees none of it
-    const u32x4_t* kl = k_two[buf];
-    const bf16_t* vl = (const bf16_t*)v_two[buf];
-    floatx16_t s[NS];
+    if (!on) continue;
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = CAP ? 0.f : bias[r];
-#pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        const u32x4_t f = kl[(u * 32 + c) * CH + ((2 * x + hi) ^ ksw)];
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, f), __builtin_bit_cast(bf16x8_t, qf[x]), s[u], 0, 0, 0);
-      }
-    }
-    const float base = slope * (float)(b - qi);
-    if (CAP) {
-#pragma unroll
-      for (int u = 0; u < NS; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[u][r] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][r] * scale) + 1.0f), capA + bias[r]);
-    }
-    if (b + KB - 1 > qs || b < qs + 31 - window) {               // wave-uniform: some key is not visible to some query
-#pragma unroll
-      for (int u = 0; u < NS; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int far = qi - b - u * 32 - ((r & 3) + 8 * (r >> 2) + 4 * hi);
-          s[u][r] = far >= 0 && far <= window ? s[u][r] : -INFINITY;
-        }
-    }
-    const float kk = CAP ? 1.f : scale;
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      float t = s[u][0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) t = fmaxf(t, s[u][r]);
-      top = fmaxf(top, fmaf(t, kk, base + slope * (float)(32 * u)));
-    }
-    if (__any(top > m + 8.f)) {
-      top = fmaxf(top, other_half(top));
-      const float mn = fmaxf(m, top);
-      const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= corr;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= corr;
-      m = mn;
-    }
-    const float off = base - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      const float ou = off + slope * (float)(32 * u);
-      unsigned pk[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = CAP ? s[u][2 * e] + ou : fmaf(s[u][2 * e], scale, ou), bb = CAP ? s[u][2 * e + 1] + ou : fmaf(s[u][2 * e + 1], scale, ou);
-        pk[e] = pack2_bf16(__builtin_amdgcn_exp2f(a), __builtin_amdgcn_exp2f(bb));
-        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pk[e]), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
-      }
+      const int b0 = b + 32 * u;
+      if (b0 > qs + WQ - 1 || b0 + 31 < qs - window) continue;   // wave-uniform: the wave sees none of it
+      const u32x4_t* kl = k_two[buf] + u * 32 * CH;
+      const bf16_t* vl = (const bf16_t*)v_two[buf] + u * 32 * HD;
+      floatx4_t s[NQ][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4_t pf = u32x4_t{pk[4 * t], pk[4 * t + 1], pk[4 * t + 2], pk[4 * t + 3]};
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const bf16_t* va = vl + v_at + (u * 32 + t * 16) * HD + (d ^ vx) * 32;
-          struct { s16x4_t a, b; } f;
-          f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)va);
-          f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(va + 8 * HD));
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, f), __builtin_bit_cast(bf16x8_t, pf), o[d], 0, 0, 0);
+        for (int n = 0; n < NQ; ++n) s[n][t] = CAP || !BIAS ? floatx4_t{0.f, 0.f, 0.f, 0.f} : bias[t];
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+          const bf16x8_t f = __builtin_bit_cast(bf16x8_t, kl[k_at[x] + t * 4 * CH]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8_t, qf[n][x]), s[n][t], 0, 0, 0);
         }
+      }
+      const bool edge = b0 + 31 > qs || b0 < qs + WQ - 1 - window;     // wave-uniform: some key is not visible to some query
+      u32x4_t pf[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int far0 = qs + n * 16 + c - b0;                   // how far behind the lane's query key 0 of the 32 is
+        const float base = -slope * (float)far0;
+        if (CAP) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][e >> 2][e & 3] * scale) + 1.0f);
+            s[n][e >> 2][e & 3] = fmaf(-2.0f * capA, r, BIAS ? capA + bias[e >> 2][e & 3] : capA);
+          }
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int far = far0 - 8 * g - e;
+            s[n][e >> 2][e & 3] = far >= 0 && far <= window ? s[n][e >> 2][e & 3] : -INFINITY;
+          }
+        }
+        const float kk = CAP ? 1.f : scale;
+        float top = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), s[n][0][2]);
+        top = fmaxf(fmaxf(top, s[n][0][3]), s[n][1][0]);
+        top = fmaxf(fmaxf(top, s[n][1][1]), s[n][1][2]);
+        top = fmaf(fmaxf(top, s[n][1][3]), kk, base);
+        // Lanes exchange their maxima, and what was summed so far is rescaled, only where a score exceeds the running maximum by 2^8: a probability is up to 2^8
+        // then, which costs neither the sums (fp32) nor its rounding to bf16 (relative) anything.
+        if (__any(top > m[n] + 8.f)) {
+          top = fmaxf(top, fstu_swz16(top));
+          top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
+          const float mn = fmaxf(m[n], top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+          l[n] *= corr;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[n][d][r] *= corr;
+          m[n] = mn;
+        }
+        const float off = base - (m[n] == -INFINITY ? 0.f : m[n]);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = s[n][e >> 2][e & 3];
+          p[e] = __builtin_amdgcn_exp2f(CAP ? x + off : fmaf(x, scale, off));
+          l[n] += p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[n][e] = pack2_bf16(p[2 * e], p[2 * e + 1]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        struct { s16x4_t a, b; } f;
+        f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + v_at[d]));
+        f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + v_at[d] + 4 * HD));
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+          o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f), __builtin_bit_cast(bf16x8_t, pf[n]), o[n][d], 0, 0, 0);
       }
     }
   }
   if (!on) return;
-  l += other_half(l);
-  const float inv = 1.0f / l;
-  bool fine = true;
+  unsigned long long bad = 0;
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      o[d][r] *= inv;
-      fine = fine && o[d][r] == o[d][r];
-    }
-  if (qi < len) {
-    bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + 4 * hi;
+  for (int n = 0; n < NQ; ++n) {
+    l[n] += fstu_swz16(l[n]);
+    l[n] += __shfl_xor(l[n], 32, FSTU_WAVE);
+    const float inv = 1.0f / l[n];
+    const int qi = qs + n * 16 + c;
+    bool fine = true;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *(uint2*)(orow + d * 32 + e * 8) = make_uint2(pack2_bf16(o[d][4 * e], o[d][4 * e + 1]), pack2_bf16(o[d][4 * e + 2], o[d][4 * e + 3]));
+      for (int r = 0; r < 4; ++r) {
+        o[n][d][r] *= inv;
+        fine = fine && o[n][d][r] == o[n][d][r];
+      }
+    if (qi < len) {
+      bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + 4 * g;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *(uint2*)(orow + d * 16) = make_uint2(pack2_bf16(o[n][d][0], o[n][d][1]), pack2_bf16(o[n][d][2], o[n][d][3]));
+    }
+    unsigned long long here = __ballot(!fine && qi < len);
+    here |= here >> 32;
+    bad |= ((here | here >> 16) & 0xffffull) << (16 * n);
   }
   // A NaN comes from a row's own scores and values, or from a value that it does not see (0 * infinity): the wave forms such rows once more, key by key.
-  unsigned long long bad = __ballot(!fine && qi < len);
-  bad = (bad | bad >> 32) & 0xffffffffull;
   while (bad) {
     const int i = qs + __builtin_ctzll(bad);
     bad &= bad - 1;
-    packed_one<bf16_t, HD>((const bf16_t*)q.p + (at + i) * q.row + h * q.head, kb, vb, out + ((int64_t)(at + i) * heads + h) * HD, k.row, v.row, i, window,
+    packed_one<bf16_t, HD>((const bf16_t*)q.p + (at + i) * q.row + h * q.head, kb, vb, out + ((int64_t)(at + i) * heads + h) * HD, k_row, v_row, i, window,
                            raw_slope, softcap);
   }
 }
@@ -291,13 +325,16 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
                          seqs, heads, kvh, window, softcap);
       return;
     }
-    constexpr int NW = 4;
-    auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * 32) + seqs) * heads), dim3(NW * 64), 0, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes,
-                         rows, seqs, heads, kvh, window, softcap);
+    auto bf16 = [&](auto nw, auto nq) {
+      constexpr int NW = decltype(nw)::value, NQ = decltype(nq)::value;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * NQ * 16) + seqs) * heads), dim3(NW * 64), 0, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu,
+                           slopes, rows, seqs, heads, kvh, window, softcap);
+      };
+      if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, NQ, true, true>) : go(swa_packed_mfma_kernel<HD, NW, NQ, true, false>);
+      else slopes ? go(swa_packed_mfma_kernel<HD, NW, NQ, false, true>) : go(swa_packed_mfma_kernel<HD, NW, NQ, false, false>);
     };
-    if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, true, true>) : go(swa_packed_mfma_kernel<HD, NW, true, false>);
-    else slopes ? go(swa_packed_mfma_kernel<HD, NW, false, true>) : go(swa_packed_mfma_kernel<HD, NW, false, false>);
+    bf16(std::integral_constant<int, PK_NW>{}, std::integral_constant<int, HD == 256 ? 2 : PK_NQ>{});
   };
   if (hd == 32) run(std::integral_constant<int, 32>{});
   else if (hd == 64) run(std::integral_constant<int, 64>{});

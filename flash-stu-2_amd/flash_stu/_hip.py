@@ -1504,32 +1504,37 @@ def glu_fp8(codes: torch.Tensor, scales: torch.Tensor, gate_codes: torch.Tensor,
 # Rows of all sequences lie behind one another; cu_seqlens (sequences + 1,) int32 on the GPU holds where each begins and, last, where the last ends.
 # Positions are int32 on the GPU, one a sequence.  Heads are (rows, heads, head_dim) with dense head_dim and rows and heads that begin at multiples of 16
 # bytes, so that the parts of a fused projection are taken as they lie.  Forward only, as the attention of the layers is: where gradients are on, a
-# tensor that requires one is refused.
-def _heads(x: torch.Tensor, dev: int, what: str):
-    """(address, row stride, head stride) of a checked (rows, heads, head_dim) tensor."""
-    if x.get_device() != dev or dev < 0:
-        raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if x.get_device() < 0
-                               else f"{what} is on device {x.get_device()}, not on {dev}")
-    if x.dim() != 3 or x.shape[0] >= 1 << 30:
-        raise FlashSTUHipError(f"{what} must be (rows, heads, head_dim), got {tuple(x.shape)}")
-    row, head, one = x.stride()
-    if one != 1:
-        raise FlashSTUHipError(f"{what} must have a dense head_dim, got stride {x.stride()}")
-    return x.data_ptr(), row if x.shape[0] > 1 else 0, head if x.shape[1] > 1 else 0
+# tensor that requires one is refused.  What is right is seen in one expression in line; the functions here say what was wrong (a function for each tensor
+# took 1.5 us of a call's 8).
+_bf16, _f32, _i32 = torch.bfloat16, torch.float32, torch.int32
+_empty = torch.empty
+_kv4_types = {torch.bfloat16: FSTU_BF16, torch.float32: FSTU_F32}
 
 
-def _int32s(x: torch.Tensor, n: int, dev: int, what: str) -> int:
-    if x.dtype is not torch.int32 or x.dim() != 1 or x.shape[0] != n or x.get_device() != dev or not x.is_contiguous():
-        raise FlashSTUHipError(f"{what} must be ({n},) int32, contiguous, on device {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-    return x.data_ptr()
-
-
-def _slopes_of(slopes: Optional[torch.Tensor], heads: int, dev: int):
-    if slopes is None:
-        return None
-    if slopes.dtype is not torch.float32 or slopes.shape != (heads,) or slopes.get_device() != dev or not slopes.is_contiguous():
-        raise FlashSTUHipError(f"slopes must be ({heads},) float32, contiguous, on device {dev}, got {tuple(slopes.shape)} {slopes.dtype} on {slopes.device}")
-    return slopes.data_ptr()
+def _refuse_heads(what: str, dev: int, heads=(), ints=(), slopes=None, out=None):
+    """Raises for the first of these that is not as it has to be: heads (name, tensor, shape or None, type), ints (name, tensor, length), slopes (tensor,
+    heads), out (tensor, like)."""
+    for name, x, shape, dtype in heads:
+        if x.get_device() != dev or dev < 0:
+            raise FlashSTUHipError("tensor is not on the GPU: the HIP path has no CPU fallback" if x.get_device() < 0
+                                   else f"{what}: {name} is on device {x.get_device()}, not on {dev}")
+        if x.dtype not in _kv4_types:
+            raise FlashSTUHipError(f"unsupported dtype {x.dtype}: the HIP kernels take float32 or bfloat16")
+        if x.dim() != 3 or shape is not None and tuple(x.shape) != tuple(shape) or x.dtype is not dtype:
+            raise FlashSTUHipError(f"{what}: {name} must be {'(rows, heads, head_dim)' if shape is None else tuple(shape)} {dtype}, got {tuple(x.shape)} {x.dtype}")
+        if x.stride(2) != 1 or x.shape[0] >= 1 << 30:
+            raise FlashSTUHipError(f"{what}: {name} must have a dense head_dim and less than 2^30 rows, got {tuple(x.shape)} stride {x.stride()}")
+    for name, x, n in ints:
+        if x.dtype is not _i32 or tuple(x.shape) != (n,) or x.get_device() != dev or not x.is_contiguous():
+            raise FlashSTUHipError(f"{what}: {name} must be ({n},) int32, contiguous, on device {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    if slopes is not None and slopes[0] is not None:
+        x, n = slopes
+        if x.dtype is not _f32 or tuple(x.shape) != (n,) or x.get_device() != dev or not x.is_contiguous():
+            raise FlashSTUHipError(f"{what}: slopes must be ({n},) float32, contiguous, on device {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    if out is not None and out[0] is not None:
+        x, like = out
+        if x.shape != like.shape or x.dtype is not like.dtype or x.get_device() != dev or not x.is_contiguous():
+            raise FlashSTUHipError(f"{what}: out must be {tuple(like.shape)} {like.dtype}, contiguous, on device {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
 
 
 def swa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, slopes: Optional[torch.Tensor] = None,
@@ -1545,34 +1550,36 @@ def swa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     if dev >= 0 and dev != _device_now():
         with torch.cuda.device(dev):
             return swa_packed(q, k, v, cu_seqlens, slopes, window, softcap, out)
-    qp, qr, qh = _heads(q, dev, "q")
-    kp, kr, kh = _heads(k, dev, "k")
-    vp, vr, vh = _heads(v, dev, "v")
+    dt, ks, dtype = _kv4_types.get(q.dtype), k.shape, q.dtype
+    if not (dev >= 0 and dt is not None and k.get_device() == v.get_device() == cu_seqlens.get_device() == dev and k.dtype is dtype and v.dtype is dtype and len(ks) == 3
+            and v.shape == ks and q.dim() == 3):
+        _refuse_heads("swa_packed", dev, [("q", q, None, dtype), ("k", k, None, dtype), ("v", v, tuple(ks), dtype)])
+        raise FlashSTUHipError(f"swa_packed: cu_seqlens is on {cu_seqlens.device}")
     rows, heads, hd = q.shape
-    kvh = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != rows or k.shape[2] != hd or not q.dtype is k.dtype is v.dtype:
-        raise FlashSTUHipError(f"swa_packed: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} do not go together")
-    dt = _dt(q)
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise FlashSTUHipError(f"cu_seqlens must be (sequences + 1,) int32, got {tuple(cu_seqlens.shape)} {cu_seqlens.dtype}")
-    seqs = cu_seqlens.shape[0] - 1
-    cu, sp = _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens"), _slopes_of(slopes, heads, dev)
-    window = 0x7fffffff if window is None else min(int(window), 0x7fffffff)
+    (qr, qh, q1), (kr, kh, k1), (vr, vh, v1) = q.stride(), k.stride(), v.stride()
+    kvh = ks[1]
+    seqs = cu_seqlens.numel() - 1
+    if not (ks[0] == rows and ks[2] == hd and q1 == k1 == v1 == 1 and rows < 1 << 30 and seqs >= 0 and cu_seqlens.dtype is _i32 and cu_seqlens.dim() == 1
+            and cu_seqlens.is_contiguous()
+            and (slopes is None or slopes.dtype is _f32 and slopes.shape == (heads,) and slopes.get_device() == dev and slopes.is_contiguous())
+            and (out is None or out.dtype is dtype and out.shape == q.shape and out.get_device() == dev and out.is_contiguous())):
+        _refuse_heads("swa_packed", dev, [("q", q, None, dtype), ("k", k, (rows, kvh, hd), dtype), ("v", v, (rows, kvh, hd), dtype)],
+                      [("cu_seqlens", cu_seqlens, max(seqs, 0) + 1)], (slopes, heads), (out, q))
     if out is None:
-        out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
+        out = _empty((rows, heads, hd), dtype=dtype, device=q.device)
     else:
-        if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
-            raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
         _written(out)
-    rc = load().fstu_swa_packed(qp, qr, qh, kp, kr, kh, vp, vr, vh, out.data_ptr(), cu, sp, rows, seqs, heads, kvh, hd, window, float(softcap or 0.0), dt,
-                                raw_stream(dev)) if rows else 0
-    if rc:
-        _check(rc, "fstu_swa_packed")
+    if rows:
+        rc = load().fstu_swa_packed(q.data_ptr(), qr if rows > 1 else 0, qh, k.data_ptr(), kr if rows > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(),
+                                    vr if rows > 1 else 0, vh if kvh > 1 else 0, out.data_ptr(), cu_seqlens.data_ptr(), None if slopes is None else slopes.data_ptr(),
+                                    rows, seqs, heads, kvh, hd, 0x7fffffff if window is None or window > 0x7fffffff else window, softcap or 0.0, dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_swa_packed")
     return out
 
 
 def kv4_bytes(seqs: int, kv_heads: int, head_dim: int, capacity: int) -> int:
-    """Bytes of a 4-bit ring cache (17/16 of a byte for a key and its value)."""
+    """Bytes of a 4-bit ring cache (17/16 of a byte for a key's and a value's dim together)."""
     return load().fstu_kv4_bytes(seqs, kv_heads, head_dim, capacity)
 
 
@@ -1583,20 +1590,23 @@ def kv4_write(cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, cu_seq
     if dev != _device_now():
         with torch.cuda.device(dev):
             return kv4_write(cache, k, v, pos, cu_seqlens)
-    kp, kr, kh = _heads(k, dev, "k")
-    vp, vr, vh = _heads(v, dev, "v")
     seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
-    rows = k.shape[0]
-    if k.shape != v.shape or k.shape[1] != kvh or k.shape[2] != hd or k.dtype is not v.dtype:
-        raise FlashSTUHipError(f"KV4Cache.write: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} are not rows of {kvh} heads of {hd}")
-    if cu_seqlens is None and rows != seqs:
+    rows, dtype = k.shape[0] if k.dim() else 0, k.dtype
+    dt = _kv4_types.get(dtype)
+    if not (dt is not None and v.dtype is dtype and k.shape == v.shape == (rows, kvh, hd) and k.get_device() == v.get_device() == pos.get_device() == dev
+            and k.stride(2) == v.stride(2) == 1 and rows < 1 << 30 and pos.dtype is _i32 and pos.shape == (seqs,) and pos.is_contiguous()
+            and (rows == seqs if cu_seqlens is None else cu_seqlens.dtype is _i32 and cu_seqlens.shape == (seqs + 1,) and cu_seqlens.get_device() == dev
+                 and cu_seqlens.is_contiguous())):
+        _refuse_heads("KV4Cache.write", dev, [("k", k, (rows, kvh, hd), dtype), ("v", v, (rows, kvh, hd), dtype)],
+                      [("pos", pos, seqs)] + ([] if cu_seqlens is None else [("cu_seqlens", cu_seqlens, seqs + 1)]))
         raise FlashSTUHipError(f"KV4Cache.write: without cu_seqlens there is a row to each of the {seqs} sequences, got {rows}")
-    dt = _dt(k)
-    rc = load().fstu_kv4_write(kp, kr, kh, vp, vr, vh, cache.data.data_ptr(), _int32s(pos, seqs, dev, "pos"),
-                               None if cu_seqlens is None else _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens"), rows, seqs, kvh, hd, cache.capacity, dt,
-                               raw_stream(dev)) if rows else 0
-    if rc:
-        _check(rc, "fstu_kv4_write")
+    if rows:
+        (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
+        rc = load().fstu_kv4_write(k.data_ptr(), kr if rows > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(), vr if rows > 1 else 0, vh if kvh > 1 else 0,
+                                   cache.data.data_ptr(), pos.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), rows, seqs, kvh, hd, cache.capacity,
+                                   dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_kv4_write")
 
 
 def kv4_read(cache, pos: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, rows: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
@@ -1605,58 +1615,64 @@ def kv4_read(cache, pos: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None
         with torch.cuda.device(dev):
             return kv4_read(cache, pos, cu_seqlens, rows, dtype)
     seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
-    if cu_seqlens is None:
-        if rows is not None and rows != seqs:
-            raise FlashSTUHipError(f"KV4Cache.read: without cu_seqlens there is a row to each of the {seqs} sequences, not {rows}")
+    dt = _kv4_types.get(dtype)
+    if cu_seqlens is None and rows is None:
         rows = seqs
-    elif rows is None or not 0 <= rows < 1 << 30:
-        raise FlashSTUHipError(f"KV4Cache.read: with cu_seqlens it needs the number of rows, got {rows}")
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
-        raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
-    pp, cp = _int32s(pos, seqs, dev, "pos"), None if cu_seqlens is None else _int32s(cu_seqlens, seqs + 1, dev, "cu_seqlens")
-    k = torch.empty(rows, kvh, hd, dtype=dtype, device=cache.data.device)
+    if not (dt is not None and pos.dtype is _i32 and pos.shape == (seqs,) and pos.get_device() == dev and pos.is_contiguous() and rows is not None and 0 <= rows < 1 << 30
+            and (rows == seqs if cu_seqlens is None else cu_seqlens.dtype is _i32 and cu_seqlens.shape == (seqs + 1,) and cu_seqlens.get_device() == dev
+                 and cu_seqlens.is_contiguous())):
+        _refuse_heads("KV4Cache.read", dev, (), [("pos", pos, seqs)] + ([] if cu_seqlens is None else [("cu_seqlens", cu_seqlens, seqs + 1)]))
+        if dt is None:
+            raise FlashSTUHipError(f"unsupported dtype {dtype}: the HIP kernels take float32 or bfloat16")
+        raise FlashSTUHipError(f"KV4Cache.read: it takes the number of rows with cu_seqlens, and without has one to each of the {seqs} sequences, got {rows}")
+    k = _empty((rows, kvh, hd), dtype=dtype, device=cache.data.device)
     v = torch.empty_like(k)
-    rc = load().fstu_kv4_read(cache.data.data_ptr(), k.data_ptr(), v.data_ptr(), pp, cp, rows, seqs, kvh, hd, cache.capacity,
-                              FSTU_BF16 if dtype is torch.bfloat16 else FSTU_F32, raw_stream(dev)) if rows else 0
-    if rc:
-        _check(rc, "fstu_kv4_read")
+    if rows:
+        rc = load().fstu_kv4_read(cache.data.data_ptr(), k.data_ptr(), v.data_ptr(), pos.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), rows, seqs,
+                                  kvh, hd, cache.capacity, dt, raw_stream(dev))
+        if rc:
+            _check(rc, "fstu_kv4_read")
     return k, v
 
 
 @functools.lru_cache(maxsize=256)
-def _kv4_splits(seqs: int, heads: int, kvh: int, hd: int, cap: int, window: int) -> int:
-    return load().fstu_kv4_attend_splits(seqs, heads, kvh, hd, cap, window)
+def _kv4_splits(seqs: int, heads: int, kvh: int, hd: int, cap: int, window: int):
+    """Workgroups that share a call's keys, and the floats of their parts."""
+    splits = load().fstu_kv4_attend_splits(seqs, heads, kvh, hd, cap, window)
+    return splits, load().fstu_kv4_attend_ws(seqs, heads, kvh, hd, splits)
 
 
 def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, softcap: float = 0.0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     if (q.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
         raise _fp8_forward_only("KV4Cache.attend")
-    dev = cache.data.get_device()
+    data = cache.data
+    dev = data.get_device()
     if dev != _device_now():
         with torch.cuda.device(dev):
             return kv4_attend(cache, q, pos, slopes, window, softcap, out)
-    qp, qr, qh = _heads(q, dev, "q")
-    seqs, kvh, hd = cache.batch, cache.kv_heads, cache.head_dim
-    heads = q.shape[1]
-    if q.shape[0] != seqs or q.shape[2] != hd or heads < 1 or heads % kvh:
-        raise FlashSTUHipError(f"KV4Cache.attend: q {tuple(q.shape)} is not one row of heads of {hd} to each of {seqs} sequences, heads a multiple of {kvh}")
-    dt = _dt(q)
-    pp, sp = _int32s(pos, seqs, dev, "pos"), _slopes_of(slopes, heads, dev)
+    seqs, kvh, hd, cap = cache.batch, cache.kv_heads, cache.head_dim, cache.capacity
+    shape, dtype = q.shape, q.dtype
+    dt, heads = _kv4_types.get(dtype), shape[1] if len(shape) == 3 else 0
+    if not (dt is not None and heads > 0 and shape[0] == seqs and shape[2] == hd and heads % kvh == 0 and q.get_device() == pos.get_device() == dev and q.stride(2) == 1
+            and pos.dtype is _i32 and pos.shape == (seqs,) and pos.is_contiguous()
+            and (slopes is None or slopes.dtype is _f32 and slopes.shape == (heads,) and slopes.get_device() == dev and slopes.is_contiguous())
+            and (out is None or out.dtype is dtype and out.shape == shape and out.get_device() == dev and out.is_contiguous())):
+        _refuse_heads("KV4Cache.attend", dev, [("q", q, None, dtype)], [("pos", pos, seqs)], (slopes, heads), (out, q))
+        raise FlashSTUHipError(f"KV4Cache.attend: q {tuple(shape)} is not one row of heads of {hd} to each of {seqs} sequences, heads a multiple of {kvh}")
     if window is None:
-        window = cache.capacity - 1
-    elif not 0 <= window < cache.capacity:
-        raise FlashSTUHipError(f"KV4Cache.attend: window {window} does not fit a ring of {cache.capacity} (0 to {cache.capacity - 1})")
+        window = cap - 1
+    elif not 0 <= window < cap:
+        raise FlashSTUHipError(f"KV4Cache.attend: window {window} does not fit a ring of {cap} (0 to {cap - 1})")
     if out is None:
-        out = torch.empty(seqs, heads, hd, dtype=q.dtype, device=q.device)
+        out = _empty(shape, dtype=dtype, device=data.device)
     else:
-        if out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or not out.is_contiguous():
-            raise FlashSTUHipError(f"out must be {tuple(q.shape)} {q.dtype}, contiguous, on device {dev}, got {tuple(out.shape)} {out.dtype} on {out.device}")
         _written(out)
-    splits = _kv4_splits(seqs, heads, kvh, hd, cache.capacity, window)
-    ws = torch.empty(load().fstu_kv4_attend_ws(seqs, heads, kvh, hd, splits), dtype=torch.float32, device=q.device) if splits > 1 else None
-    rc = load().fstu_kv4_attend(qp, qr, qh, cache.data.data_ptr(), out.data_ptr(), _p(ws), splits, pp, sp, seqs, heads, kvh, hd, cache.capacity, window, float(softcap or 0.0), dt,
-                                raw_stream(dev))
+    splits, floats = _kv4_splits(seqs, heads, kvh, hd, cap, window)
+    ws = _empty(floats, dtype=_f32, device=data.device).data_ptr() if floats else None      # its memory is this stream's until what runs on it next
+    qr, qh, _ = q.stride()
+    rc = load().fstu_kv4_attend(q.data_ptr(), qr if seqs > 1 else 0, qh if heads > 1 else 0, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(),
+                                None if slopes is None else slopes.data_ptr(), seqs, heads, kvh, hd, cap, window, softcap or 0.0, dt, raw_stream(dev))
     if rc:
         _check(rc, "fstu_kv4_attend")
     return out
