@@ -328,6 +328,7 @@ __device__ __forceinline__ float capped(float s, float scale, float capA) {
   return capA * tanhf(s * scale);
 }
 
+#define KV4_MOST_PARTS 64  // more: workgroups that all keys are dealt to
 #define KV4_COLS 8        // query heads of a key head that a workgroup takes
 
 template <bool STREAM, typename V>
@@ -465,7 +466,8 @@ __device__ __forceinline__ int sequence_of(const int* pos, int seqs, int cap, in
 // One query a sequence.  S^T = K Q^T over 32 slots at a time as two tiles of 16 keys, rows dealt so that lane (g, col) ends up with query col's scores of slots
 // 8 g .. 8 g + 7, which is what it holds of the second product O^T = V^T P^T: no score crosses a lane, only the maxima do.  Codes become bf16 in registers (exact),
 // probabilities go in as a bf16 head and, in the columns 8 further on, what its rounding left (fp32: two such parts).
-// PLAN: the tiles of all sequences are dealt evenly to the workgroups, whose parts kv4_join_kernel adds up; without, a workgroup takes a key head of a sequence.
+// PLAN: the tiles of all sequences are dealt evenly to the workgroups; without, a workgroup takes a key head of a sequence or one of gridDim.z parts of its tiles.
+// kv4_join_kernel adds up what is in parts.
 template <typename T, int HD, int NW, bool CAP, bool PLAN>
 __global__ void __launch_bounds__(NW * 64, HD == 256 || NW == 8 ? 1 : HD == 128 ? 2 : 3)
 kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, T* out, float* ws, const int* pos, const float* slopes, int seqs, int heads,
@@ -507,7 +509,13 @@ kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, 
     }
     const Tiles tl = tiles_of(pos[b], cap, window, tiles);
     const int ps = tl.slot, lim = tl.lim, start = tl.start;
-    if (!PLAN) last = all = tl.count;
+    const int parts = PLAN ? 1 : gridDim.z, part_no = PLAN ? 0 : blockIdx.z;
+    if (!PLAN) {
+      all = tl.count;
+      const int per = all / parts, more = all - per * parts;     // the first `more` parts take one tile more
+      first = per * part_no + min(part_no, more);
+      last = first + per + (part_no < more ? 1 : 0);
+    }
     const int hk = y / chunks, h0 = hk * group + y % chunks * KV4_COLS, cols = min(KV4_COLS, hk * group + group - h0);
     const int64_t head0 = ((int64_t)b * kvh + hk) * c.slots;
 
@@ -677,10 +685,11 @@ kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, 
         L = fmaf(sl[k * KV4_COLS + cc], f, L);
         v = fmaf(so[(k * cols + cc) * HD + d], f, v);
       }
-      if (!PLAN || last - first == all) DT<T>::st(out + ((int64_t)b * heads + h0 + cc) * HD + d, all ? v / L : 0.f);
+      if (PLAN ? last - first == all : parts == 1) DT<T>::st(out + ((int64_t)b * heads + h0 + cc) * HD + d, all ? v / L : 0.f);
       else {
-        // one place to each pair of workgroup and key head that meet: both rise from one to the next
-        float* part = ws + ((int64_t)(blockIdx.x + b * per_seq + y) * KV4_COLS + cc) * (HD + 2);
+        // PLAN: one place to each pair of workgroup and key head that meet: both rise from one to the next
+        const int64_t place = PLAN ? (int64_t)blockIdx.x + b * per_seq + y : ((int64_t)b * per_seq + y) * parts + part_no;
+        float* part = ws + (place * KV4_COLS + cc) * (HD + 2);
         part[2 + d] = v;
         if (d == 0) { part[0] = M; part[1] = L; }
       }
@@ -692,7 +701,7 @@ kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, 
 // The parts of a query head, in the order of its keys: several to a thread row, joined through LDS.
 template <typename T, int HD>
 __global__ void __launch_bounds__(512)
-kv4_join_kernel(const float* ws, T* out, const int* pos, int seqs, int heads, int kvh, int cap, int window, int chunks, int W) {
+kv4_join_kernel(const float* ws, T* out, const int* pos, int seqs, int heads, int kvh, int cap, int window, int chunks, int splits) {
   constexpr int R = 512 / HD;
   const int b = blockIdx.x / heads, h = blockIdx.x % heads, group = heads / kvh, hk = h / group, per_seq = kvh * chunks;
   const int y = hk * chunks + (h - hk * group) / KV4_COLS, cc = (h - hk * group) % KV4_COLS, d = threadIdx.x % HD, r = threadIdx.x / HD;
@@ -702,14 +711,19 @@ kv4_join_kernel(const float* ws, T* out, const int* pos, int seqs, int heads, in
     if (r == 0) DT<T>::st(dst, 0.f);
     return;
   }
-  const Plan plan = plan_of(pos, seqs, cap, window, tiles, per_seq, W);
-  int before = 0;
-  for (int at = 0; at < b; at += 64) before += __builtin_amdgcn_readlane(wave_prefix(tiles_behind(pos, b, at, cap, window, tiles)), 63);
-  const int begin = min(before * per_seq + y * count, plan.total - 1), w0 = plan.owner(begin), w1 = min(plan.owner(begin + count - 1), W - 1);
-  if (w0 == w1) return;                                          // whole, and there already
-  const float* part = ws + ((int64_t)(w0 + b * per_seq + y) * KV4_COLS + cc) * (HD + 2);
+  int n = splits;
+  int64_t place = ((int64_t)b * per_seq + y) * splits;
+  if (splits > KV4_MOST_PARTS) {
+    const Plan plan = plan_of(pos, seqs, cap, window, tiles, per_seq, splits);
+    int before = 0;
+    for (int at = 0; at < b; at += 64) before += __builtin_amdgcn_readlane(wave_prefix(tiles_behind(pos, b, at, cap, window, tiles)), 63);
+    const int begin = min(before * per_seq + y * count, plan.total - 1), w0 = plan.owner(begin), w1 = min(plan.owner(begin + count - 1), splits - 1);
+    if (w0 == w1) return;                                        // whole, and there already
+    n = w1 - w0 + 1;
+    place = (int64_t)w0 + b * per_seq + y;
+  }
+  const float* part = ws + (place * KV4_COLS + cc) * (HD + 2);
   constexpr int STEP = KV4_COLS * (HD + 2);
-  const int n = w1 - w0 + 1;
   float M = -INFINITY, L = 0.f, v = 0.f;
 #pragma unroll 4
   for (int s = r; s < n; s += R) {
@@ -815,21 +829,25 @@ extern "C" int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos
   return FSTU_OK;
 }
 
-// Workgroups of a call whose keys are dealt evenly; 1: a workgroup to each key head of a sequence.  Dealing costs a second launch and two looks at all positions,
-// some 8 us, and pays where few heads leave compute units idle through a long ring or where long rings end unevenly.  us, a workgroup to a head / dealt: 32 heads of
-// 128 over 2100 positions 13.9 / 15.7, 4200 22.3 / 17.4; 12 heads of 64 over 2048 9.9 / 10.5, 4000 15.4 / 12.2; 4 heads of 128 over 32768 135 / 14.9; 256 heads of 128
-// over up to 4096 24 / 32, 512 over 4096 49 / 52, 640 over 8192 125 / 112, 384 over 16384 166 / 136, 128 over 32768 155 / 89 (512 workgroups 96, 128 128).
+// How a call's keys are cut: 1: a workgroup to each key head of a sequence; up to 64: that many parts of each; more: that many workgroups, to which all keys are
+// dealt evenly.  Parts cost a second launch and its boundary, some 3 us, and pay where few heads leave compute units idle through more than a thousand positions;
+// dealing evenly costs two looks at all positions besides, and pays where there is so much to do that an uneven end is more.  us, a workgroup to a head / parts (how
+// many) / dealt to 256: 16 heads of 128 over 1025 positions 9.1 / 7.5 (16) / -, 700 7.9 / 7.4 (16), 2048 12.5 / 7.8 (16) / 9.9; 12 heads of 64 over 2048 9.9 / 7.6 (16) /
+// 11.0; 4 of 128 over 32768 138 / 12.9 (64) / 14.9; 32 of 128 over 4200 23.8 / 11.8 (8) / 17.8; 8 of 256 over 700 12.7 / 8.8 (16); sequences of uneven length, 128
+// heads of 128: 8192 39 / 27 (2) / 31, 32768 155 / 106 (2) / 88; 512 of 128 over 4096 49 / - / 52.
 extern "C" int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window) {
   if (seqs < 1 || kvh < 1 || heads < kvh || cap < 1 || window < 0) return 1;
   const int chunks = (heads / kvh + KV4_COLS - 1) / KV4_COLS;
-  const int64_t tiles = ((int64_t)(window < cap ? window : cap - 1) + 2 * KV4_TILE - 1) / KV4_TILE;
-  const int64_t groups = (int64_t)seqs * kvh * chunks;
-  if (tiles <= 96 || (groups > 192 && tiles <= 192)) return 1;
-  const int64_t most = groups * tiles / 16;
-  return (int)(most < 256 ? most : 256);
+  const int64_t tiles = ((int64_t)(window < cap ? window : cap - 1) + 2 * KV4_TILE - 1) / KV4_TILE, groups = (int64_t)seqs * kvh * chunks;
+  if (groups * tiles >= 98304 && tiles >= 192) return 256;
+  int64_t parts = 256 / groups;
+  if (parts > tiles / 3) parts = tiles / 3;
+  return tiles < (hd == 256 ? 20 : 40) || parts < 2 ? 1 : (int)(parts < KV4_MOST_PARTS ? parts : KV4_MOST_PARTS);
 }
 extern "C" int64_t fstu_kv4_attend_ws(int seqs, int heads, int kvh, int hd, int splits) {
-  return splits <= 1 ? 0 : ((int64_t)seqs * kvh * ((heads / kvh + KV4_COLS - 1) / KV4_COLS) + splits) * KV4_COLS * (hd + 2);
+  if (seqs < 1 || kvh < 1 || heads < kvh || splits <= 1) return 0;
+  const int64_t groups = (int64_t)seqs * kvh * ((heads / kvh + KV4_COLS - 1) / KV4_COLS);
+  return (splits > KV4_MOST_PARTS ? groups + splits : groups * splits) * KV4_COLS * (hd + 2);
 }
 
 extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, const void* cache, void* out, float* ws, int splits, const int* pos,
@@ -857,17 +875,16 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
                          cap, window, softcap, chunks);
     };
     constexpr int WIDE = HD == 256 ? 4 : 8;
-    if (splits > 1) {
+    const dim3 grid(kvh * chunks, seqs, splits);
+    if (splits > KV4_MOST_PARTS)
       softcap > 0.f ? run(kv4_attend_kernel<T, HD, WIDE, true, true>, dim3(splits), WIDE) : run(kv4_attend_kernel<T, HD, WIDE, false, true>, dim3(splits), WIDE);
+    else if ((int64_t)seqs * kvh * chunks * splits <= 256)      // one to a compute unit: eight waves (12 heads of 64 over 513 positions 5.7 us, 6.6 with four)
+      softcap > 0.f ? run(kv4_attend_kernel<T, HD, WIDE, true, false>, grid, WIDE) : run(kv4_attend_kernel<T, HD, WIDE, false, false>, grid, WIDE);
+    else
+      softcap > 0.f ? run(kv4_attend_kernel<T, HD, 4, true, false>, grid, 4) : run(kv4_attend_kernel<T, HD, 4, false, false>, grid, 4);
+    if (splits > 1)
       hipLaunchKernelGGL((kv4_join_kernel<T, HD>), dim3(seqs * heads), dim3(512), 0, (hipStream_t)stream, ws, (T*)out, pos, seqs, heads, kvh, cap, window, chunks,
                          splits);
-    } else if ((int64_t)seqs * kvh * chunks <= 256) {            // one to a compute unit: eight waves (12 heads of 64 over 513 positions 5.7 us, 6.6 with four)
-      const dim3 grid(kvh * chunks, seqs);
-      softcap > 0.f ? run(kv4_attend_kernel<T, HD, WIDE, true, false>, grid, WIDE) : run(kv4_attend_kernel<T, HD, WIDE, false, false>, grid, WIDE);
-    } else {
-      const dim3 grid(kvh * chunks, seqs);
-      softcap > 0.f ? run(kv4_attend_kernel<T, HD, 4, true, false>, grid, 4) : run(kv4_attend_kernel<T, HD, 4, false, false>, grid, 4);
-    }
   });
   FSTU_CHECK_LAUNCH("fstu_kv4_attend");
   return FSTU_OK;

@@ -372,8 +372,9 @@ int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k,
  * fstu_kv4_write: rows cu[s].. become positions pos[s].. (of more than cap rows the last cap).
  * fstu_kv4_read: the same positions back, k and v (rows,kvh,hd) dense, exact in either dtype; rows of no sequence zero.
  * fstu_kv4_attend: one query a sequence, q (seqs,heads,hd) by strides, over positions max(0,pos-window)..pos, window < cap; out (seqs,heads,hd) dense.
- *   splits > 1: the keys of all sequences are dealt evenly to that many workgroups, whose parts a second launch joins (ws: fstu_kv4_attend_ws floats, not
- *   shared with a call that may run at the same time); fstu_kv4_attend_splits says how many pay (1: a workgroup to each key head, ws may be NULL). */
+ *   splits: 1: a workgroup to each key head of a sequence; up to 64: that many parts of its keys each; more: that many workgroups, to which the keys of all
+ *   sequences are dealt evenly.  Parts are joined by a second launch (ws: fstu_kv4_attend_ws floats, not shared with a call that may run at the same
+ *   time; NULL with 1); fstu_kv4_attend_splits says what pays. */
 int64_t fstu_kv4_bytes(int seqs, int kvh, int hd, int cap);
 int fstu_kv4_write(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* cache, const int* pos,
                    const int* cu, int rows, int seqs, int kvh, int hd, int cap, int dtype, void* stream);

@@ -187,6 +187,33 @@ def test_attend(fs, heads, kvh, hd, cap, window, pos, softcap, alibi, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("splits", [1, 2, 7, 64, 65, 100, 300])
+@pytest.mark.parametrize("heads,kvh,hd,cap,window,pos", [(4, 2, 64, 700, None, [699, 20, -1, 1500]), (9, 1, 128, 300, 250, [299, 0, 310]), (2, 2, 256, 90, 63, [-1, 500]),
+                                                        (3, 3, 32, 64, None, [-1, -1])])
+def test_attend_in_any_number_of_parts(fs, monkeypatch, heads, kvh, hd, cap, window, pos, splits, dtype):
+    """Every way to cut the keys, more parts than tiles among them."""
+    from flash_stu import _hip
+    monkeypatch.setattr(_hip, "_kv4_splits", lambda *a: (splits, _hip.load().fstu_kv4_attend_ws(*a[:4], splits)))
+    cache, ring = filled(fs, len(pos), kvh, hd, cap, 40)
+    q, slopes = rand(5, len(pos), heads, hd, dtype=dtype), slopes_of(heads)
+    y = cache.attend(q.cuda(), ints(pos), slopes=slopes.cuda(), window=window, softcap=50.0)
+    check(y, *ring.attend(q, pos, slopes, window, 50.0, P_STEP), dtype)
+
+
+def test_attend_dealt_evenly_over_many_sequences(fs, monkeypatch):
+    """More sequences than a wave has lanes, many of them not in use."""
+    from flash_stu import _hip
+    batch, cap = 150, 200
+    pos = [-1 if i % 3 == 1 or 60 <= i < 130 else (i * 37) % 450 for i in range(batch)]
+    cache, ring = filled(fs, batch, 1, 32, cap, 50)
+    q = rand(6, batch, 2, 32, dtype=torch.bfloat16)
+    o, bound = ring.attend(q, pos, None, None, 0.0, P_STEP)
+    for splits in (65, 256, 1):
+        monkeypatch.setattr(_hip, "_kv4_splits", lambda *a: (splits, _hip.load().fstu_kv4_attend_ws(*a[:4], splits)))
+        check(cache.attend(q.cuda(), ints(pos)), o, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
 def test_what_the_window_leaves_out_may_be_anything(fs, hd, dtype):
     """NaN in every slot that the query does not see, at every offset of the window's ends in a tile."""
