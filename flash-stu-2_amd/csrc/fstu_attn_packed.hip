@@ -2,15 +2,10 @@
 //   s_ij = softcap * tanh(q_i . k_j * hd^-1/2 / softcap) - slope * (i - j),  0 <= i - j <= window,  o_i = sum_j softmax_j(s_ij) v_j
 #include "fstu_common.h"
 
-#ifndef PK_NW
-#define PK_NW 4
-#define PK_NQ 2
-#endif
-
 namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float floatx4_t __attribute__((ext_vector_type(4)));
+typedef float floatx16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -77,44 +72,140 @@ __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb,
   }
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(256)
-swa_packed_kernel(Heads q, Heads k, Heads v, T* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
-  const int h = blockIdx.y, hk = h / (heads / kvh);
-  int at, len, first;
-  packed_tile(cu, seqs, rows, 4, blockIdx.x, &at, &len, &first);
-  const int i = first + (threadIdx.x >> 6);
-  if (i < 0 || i >= len) return;
-  packed_one<T, HD>((const T*)q.p + (at + i) * q.row + h * q.head, (const T*)k.p + at * k.row + hk * k.head, (const T*)v.p + at * v.row + hk * v.head,
-                    out + ((int64_t)(at + i) * heads + h) * HD, k.row, v.row, i, window, slopes ? slopes[h] : 0.f, softcap);
-}
-
-template <int HD>
-__device__ __forceinline__ int key_turn(int row) {
-  return HD >= 128 ? (row & 3) | (row >> 3 & 3) << 2 : HD == 64 ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : row >> 3 & 3;
-}
-template <int HD>
-__device__ __forceinline__ int value_turn(int row) {
-  return HD >= 128 ? (row & 3) | (row >> 3 & 1) << 2 : HD == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : row >> 3 & 1;
-}
-
-// bf16 on the matrix cores: a wave owns NQ tiles of 16 queries of one head and walks their keys 32 at a time,
-//   S^T (keys x queries) = K Q^T      rows dealt so that lane (g, c) ends up with query c's scores of keys 8 g .. 8 g + 7 of the 32, which is
-//   O^T (dims x queries) = V^T P^T    what it holds of the second product: no score crosses a lane, only the maxima do.
-// Tiles of KB keys and values go through LDS by way of registers, one barrier a tile; values are read back transposed.
-template <int HD, int NW, int NQ, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64, HD == 256 || NW == 8 ? 1 : 2)
-swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
-                       float softcap) {
-  constexpr int KB = HD == 256 ? 32 : 64, NS = KB / 32, CH = HD / 8, KS = HD / 32, ND = HD / 16, NT = NW * 64, WQ = NQ * 16;
-  constexpr int PT = (KB * CH + NT - 1) / NT;                    // 16-byte pieces of a tile to a thread
-  __shared__ u32x4_t k_two[2][KB * CH], v_two[2][KB * CH];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+// fp32: v_mfma_f32_32x32x2_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
+// A workgroup takes 32 queries of one head; its waves take 32 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
+// first product and of keys in the second is what lanes hold: step s of the first is dims s and hd/2 + s, step r of the second the keys of score r.
+// FP32_FIGURES
+template <int HD, int NW, bool CAP>
+__global__ void __launch_bounds__(NW * 64, HD >= 128 ? 1 : 2)
+swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
+  constexpr int ND = HD / 32, HALF = HD / 2;
+  __shared__ float sm[NW][32], sl[NW][32], so[32][HD + 1];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hi = lane >> 5;
   const int h = blockIdx.x % heads, hk = h / (heads / kvh);
   int at, len, first;
-  packed_tile(cu, seqs, rows, NW * WQ, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  packed_tile(cu, seqs, rows, 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int qs = first + w * WQ;                                 // the wave's first query
+  const int qi = first + c, last = min(len - 1, first + 31);
+  const int64_t k_row = k.row, v_row = v.row;
+  const float* kb = (const float*)k.p + at * k_row + hk * k.head;
+  const float* vb = (const float*)v.p + at * v_row + hk * v.head;
+  const float kLog2e = 1.4426950408889634f, raw_slope = slopes ? slopes[h] : 0.f, slope = raw_slope * kLog2e;
+  const float scale = rsqrtf((float)HD) * (CAP ? 1.0f / softcap : kLog2e), capA = softcap * kLog2e;
+  float4 qf[HALF / 4];
+  {
+    const float* qr = (const float*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + hi * HALF;
+#pragma unroll
+    for (int s = 0; s < HALF / 4; ++s) qf[s] = *(const float4*)(qr + 4 * s);
+  }
+  floatx16_t o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int b = max(0, first - window) / 32 * 32 + 32 * w; b <= last; b += 32 * NW) {
+    floatx16_t s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    const float* kr = kb + min(b + c, len - 1) * k_row + hi * HALF;            // rows behind the sequence: its last one, which no query of these sees
+#pragma unroll
+    for (int x = 0; x < HALF / 4; ++x) {
+      const float4 f = *(const float4*)(kr + 4 * x);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.x, qf[x].x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.y, qf[x].y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.z, qf[x].z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.w, qf[x].w, s, 0, 0, 0);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int far = qi - b - ((r & 3) + 8 * (r >> 2) + 4 * hi);
+      const float x = (CAP ? capA * tanhf(s[r] * scale) : s[r] * scale) - slope * (float)far;
+      s[r] = far >= 0 && far <= window ? x : -INFINITY;
+      top = fmaxf(top, s[r]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
+    if (__any(top > m)) {
+      const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+      m = mn;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = __builtin_amdgcn_exp2f(s[r] - off);
+      l += p;
+      const float* vr = vb + min(b + (r & 3) + 8 * (r >> 2) + 4 * hi, len - 1) * v_row + c;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[32 * d], p, o[d], 0, 0, 0);
+    }
+  }
+  l += __shfl_xor(l, 32, FSTU_WAVE);
+  if (hi == 0) { sm[w][c] = m; sl[w][c] = l; }
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NW; ++n) M = fmaxf(M, sm[n][c]);
+  const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+#pragma unroll
+  for (int n = 0; n < NW; ++n) {
+    if (w == n) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float& sum = so[c][d * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi];
+          sum = fmaf(o[d][r], mine, n ? sum : 0.f);
+        }
+    }
+    __syncthreads();
+  }
+  for (int row = w; row < 32 && first + row < len; row += NW) {
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < NW; ++n) top = fmaxf(top, sm[n][row]);
+#pragma unroll
+    for (int n = 0; n < NW; ++n) sum = fmaf(sl[n][row], sm[n][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[n][row] - top), sum);
+    bool fine = true;
+#pragma unroll
+    for (int d = lane; d < HD; d += 64) fine = fine && so[row][d] / sum == so[row][d] / sum;
+    float* const dst = out + ((int64_t)(at + first + row) * heads + h) * HD;
+    if (__all(fine)) {
+#pragma unroll
+      for (int d = lane; d < HD; d += 64) dst[d] = so[row][d] / sum;
+    } else   // a NaN comes from the row's own scores and values, or from a value that it does not see (0 * infinity): once more, key by key
+      packed_one<float, HD>((const float*)q.p + (at + first + row) * q.row + h * q.head, kb, vb, dst, k_row, v_row, first + row, window, raw_slope, softcap);
+  }
+}
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+struct Frag8 { u32x2_t lo, hi; };
+
+// bf16 on the matrix cores: a wave owns 32 queries of one head and walks their keys 64 at a time in two halves,
+//   S^T (keys x queries) = K Q^T      lane (c, hi) ends up with query c's scores of keys (r & 3) + 8 (r >> 2) + 4 hi of 32, which is
+//   O^T (dims x queries) = V^T P^T    what it holds of the second product: no score crosses a lane, only the maxima do, between two lanes.
+// Keys and values go straight to LDS, one barrier a tile; values are read back transposed.  The second half's first product runs beside the
+// first half's softmax, the first half's second product beside the second half's: the maximum that a probability is taken from is the one
+// before these keys, and where a score exceeds it by more than 2^16 (the first keys, and hardly any after) that half is formed once more.
+template <int HD, int NW, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : HD <= 64 && NW == 4 ? 3 : 2)
+swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
+                       float softcap) {
+  constexpr int KB = HD == 256 ? 32 : 64, CH = HD / 8, KS = HD / 16, ND = HD / 32;
+  constexpr int TILE = KB * CH;                              // 16-byte pieces
+  extern __shared__ u32x4_t lds[];                               // two tiles of keys, two of values
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
+  const int h = blockIdx.x % heads, hk = h / (heads / kvh);
+  int at, len, first;
+  packed_tile(cu, seqs, rows, NW * 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  if (first < 0 || first >= len) return;
+  const int qs = first + w * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
   const int64_t k_row = k.row, v_row = v.row;
   const bf16_t* kb = (const bf16_t*)k.p + at * k_row + hk * k.head;
@@ -122,172 +213,206 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   const float kLog2e = 1.4426950408889634f, raw_slope = BIAS ? slopes[h] : 0.f, slope = raw_slope * kLog2e;
   const float scale = rsqrtf((float)HD) * (CAP ? 2.0f * kLog2e / softcap : kLog2e), capA = softcap * kLog2e;
 
-  u32x4_t qf[NQ][KS];
+  u32x4_t qf[KS];
+  {
+    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + hi * 8;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qs + n * 16 + c, len - 1)) * q.row + h * q.head + g * 8;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = *(const u32x4_t*)(qr + s * 32);
+    for (int s = 0; s < KS; ++s) qf[s] = *(const u32x4_t*)(qr + s * 16);
   }
-  floatx4_t o[NQ][ND];
-  float m[NQ], l[NQ];
+  floatx16_t o[ND];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
+  for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[n][d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  // ALiBi of key 8 g + 4 t + r of 32: without a soft-cap what the scores' sums begin with, in units of theirs
-  floatx4_t bias[2];
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  // ALiBi of a half's key: without a soft-cap what the scores' sums begin with, in units of theirs
+  floatx16_t bias;
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) bias[t][r] = BIAS ? slope * (float)(8 * g + 4 * t + r) / (CAP ? 1.f : scale) : 0.f;
+  for (int r = 0; r < 16; ++r) bias[r] = BIAS ? slope * (float)((r & 3) + 8 * (r >> 2) + 4 * hi) / (CAP ? 1.f : scale) : 0.f;
+  float m = -INFINITY, l = 0.f;
 
-  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NW * WQ - 1);
-  u32x4_t kr[PT], vr[PT];
+  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NW * 32 - 1);
+  // A tile's rows through a buffer descriptor: what lies behind the sequence's last row reads as zeros
+  constexpr int NT = NW * 64, PR = (TILE + NT - 1) / NT, STEP = NT / CH;      // 16-byte pieces of a tile to a thread, rows between them
+  u32x4_t kr[PR], vr[PR];
+  const int row0 = tid / CH, ch0 = tid % CH;
+  const int k_off = (row0 * (int)k_row + ch0 * 8) * 2, v_off = (row0 * (int)v_row + ch0 * 8) * 2;
   auto fetch = [&](int b) {
+    const int last = min(KB, len - b) - 1;
+    const rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + b * k_row), 0, (unsigned)(last * (int)k_row + HD) * 2, 0x00020000);
+    const rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + b * v_row), 0, (unsigned)(last * (int)v_row + HD) * 2, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int e = min(tid + i * NT, KB * CH - 1);              // threads beyond the tile's pieces hold the last one too
-      const int64_t row = min(b + e / CH, len - 1);              // rows behind the sequence: its last one, which no query of these sees
-      kr[i] = *(const u32x4_t*)(kb + row * k_row + e % CH * 8);
-      vr[i] = *(const u32x4_t*)(vb + row * v_row + e % CH * 8);
+    for (int i = 0; i < PR; ++i) {
+      kr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, i * STEP * (int)k_row * 2, 0));
+      vr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, i * STEP * (int)v_row * 2, 0));
     }
   };
-  // The 16-byte pieces of a row are XOR-ed with bits of it, so that what 16 lanes read together lies in different banks: 16 keys' rows one piece each (rows
-  // differ in bits 0, 1, 3 and 4), four values' rows 32 bytes each (bits 0, 1 and 3: two blocks of lanes).
+  // The 16-byte pieces of a row are XOR-ed with bits of it, so that what 16 lanes read together lies in different banks
   auto store = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int e = min(tid + i * NT, KB * CH - 1), row = e / CH, ch = e % CH;
-      k_two[buf][row * CH + (ch ^ key_turn<HD>(row))] = kr[i];
-      v_two[buf][row * CH + (ch ^ value_turn<HD>(row) << 1)] = vr[i];
+    for (int i = 0; i < PR; ++i) {
+      const int row = row0 + i * STEP;
+      const int ks = HD >= 128 ? row & 15 : HD == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+      const int vs = HD >= 128 ? (row & 3) << 2 : HD == 64 ? (row >> 1 & 1) << 2 : 0;
+      if (TILE % NT == 0 || row < KB) {
+        lds[buf * TILE + row * CH + (ch0 ^ ks)] = kr[i];
+        lds[(2 + buf) * TILE + row * CH + (ch0 ^ vs)] = vr[i];
+      }
     }
   };
   int k_at[KS], v_at[ND];                                        // in pieces, and in elements
   {
-    const int row = 8 * (c >> 2) + (c & 3), vrow = 8 * g + (c >> 2);
+    const int ksw = HD >= 128 ? c & 15 : HD == 64 ? (c >> 1) & 7 : (c >> 2) & 3;
+    const int li = lane & 15, vx = HD >= 128 ? (li >> 2) & 3 : HD == 64 ? (li >> 3) & 1 : 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_at[s] = row * CH + ((4 * s + g) ^ key_turn<HD>(row));
+    for (int s = 0; s < KS; ++s) k_at[s] = c * CH + ((2 * s + hi) ^ ksw);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) v_at[d] = vrow * HD + (d ^ value_turn<HD>(vrow)) * 16 + 4 * (c & 3);
+    for (int d = 0; d < ND; ++d) v_at[d] = (4 * hi + (li >> 2)) * HD + 16 * (lane >> 4 & 1) + 4 * (li & 3) + (d ^ vx) * 32;
   }
+  const float kk = CAP ? 1.f : scale;
+  unsigned pk[8];
+  float add, top;
+  struct Keys { u32x4_t f[KS]; };
+  struct Values { Frag8 f[2][ND]; };
+  auto get_keys = [&](int buf, int half) {
+    Keys k;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) k.f[x] = lds[buf * TILE + half * 32 * CH + k_at[x]];
+    return k;
+  };
+  auto get_values = [&](int buf, int half) {
+    const bf16_t* vl = (const bf16_t*)(lds + (2 + buf) * TILE) + half * 32 * HD;
+    Values v;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        v.f[t][d].lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + t * 16 * HD + v_at[d])));
+        v.f[t][d].hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + t * 16 * HD + v_at[d] + 8 * HD)));
+      }
+    return v;
+  };
+  auto scores = [&](const Keys& k) {                             // first product of a half
+    floatx16_t s = bias;
+    if (CAP || !BIAS)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k.f[x]), __builtin_bit_cast(bf16x8_t, qf[x]), s, 0, 0, 0);
+    return s;
+  };
+  auto shape = [&](floatx16_t& s, int b0) {                      // soft-cap, and what the lane's query does not see
+    if (CAP) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * scale) + 1.0f), BIAS ? capA + bias[r] : capA);
+    }
+    if (b0 + 31 > qs || b0 < qs + 31 - window) {                 // wave-uniform: some key is not visible to some query
+      asm volatile("");
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int far = qi - b0 - ((r & 3) + 8 * (r >> 2) + 4 * hi);
+        s[r] = far >= 0 && far <= window ? s[r] : -INFINITY;
+      }
+    }
+  };
+  auto weigh = [&](const floatx16_t& s, float base) {            // probabilities and their sum, by the maximum as it stands
+    const float off = base - (m == -INFINITY ? 0.f : m);
+    add = 0.f;
+    float t = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = __builtin_amdgcn_exp2f(CAP ? s[2 * e] + off : fmaf(s[2 * e], scale, off));
+      const float z = __builtin_amdgcn_exp2f(CAP ? s[2 * e + 1] + off : fmaf(s[2 * e + 1], scale, off));
+      add += a;
+      add += z;
+      pk[e] = pack2_bf16(a, z);
+      if (e) t = fmaxf(fmaxf(t, s[2 * e]), s[2 * e + 1]);
+    }
+    top = fmaf(t, kk, base);
+  };
+  auto settle = [&](const floatx16_t& s, float base) {
+    if (__any(top > m + 16.f)) {
+      top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
+      const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+      m = mn;
+      weigh(s, base);
+    }
+    l += add;
+  };
+  auto add_values = [&](const Values& v) {                       // second product of a half
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const u32x4_t pf = u32x4_t{pk[4 * t], pk[4 * t + 1], pk[4 * t + 2], pk[4 * t + 3]};
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v.f[t][d]), __builtin_bit_cast(bf16x8_t, pf), o[d], 0, 0, 0);
+    }
+  };
   fetch(k_first);
   store(0);
   if (k_first + KB <= k_last) fetch(k_first + KB);
-  __syncthreads();
-  int buf = 0;
-  for (int b = k_first; b <= k_last; b += KB, buf ^= 1) {
-    if (b > k_first) __syncthreads();                            // this tile is there, and the one before it has been read
+  auto tile = [&](int b, auto bufs) {
+    constexpr int buf = decltype(bufs)::value;
+    __syncthreads();                                             // this tile is there, and the one before it has been read
     if (b + KB <= k_last) store(buf ^ 1);
     if (b + 2 * KB <= k_last) fetch(b + 2 * KB);
-    if (!on) continue;
-#pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      const int b0 = b + 32 * u;
-      if (b0 > qs + WQ - 1 || b0 + 31 < qs - window) continue;   // wave-uniform: the wave sees none of it
-      const u32x4_t* kl = k_two[buf] + u * 32 * CH;
-      const bf16_t* vl = (const bf16_t*)v_two[buf] + u * 32 * HD;
-      floatx4_t s[NQ][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) s[n][t] = CAP || !BIAS ? floatx4_t{0.f, 0.f, 0.f, 0.f} : bias[t];
-#pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          const bf16x8_t f = __builtin_bit_cast(bf16x8_t, kl[k_at[x] + t * 4 * CH]);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8_t, qf[n][x]), s[n][t], 0, 0, 0);
-        }
-      }
-      const bool edge = b0 + 31 > qs || b0 < qs + WQ - 1 - window;     // wave-uniform: some key is not visible to some query
-      u32x4_t pf[NQ];
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        const int far0 = qs + n * 16 + c - b0;                   // how far behind the lane's query key 0 of the 32 is
-        const float base = -slope * (float)far0;
-        if (CAP) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][e >> 2][e & 3] * scale) + 1.0f);
-            s[n][e >> 2][e & 3] = fmaf(-2.0f * capA, r, BIAS ? capA + bias[e >> 2][e & 3] : capA);
-          }
-        }
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int far = far0 - 8 * g - e;
-            s[n][e >> 2][e & 3] = far >= 0 && far <= window ? s[n][e >> 2][e & 3] : -INFINITY;
-          }
-        }
-        const float kk = CAP ? 1.f : scale;
-        float top = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), s[n][0][2]);
-        top = fmaxf(fmaxf(top, s[n][0][3]), s[n][1][0]);
-        top = fmaxf(fmaxf(top, s[n][1][1]), s[n][1][2]);
-        top = fmaf(fmaxf(top, s[n][1][3]), kk, base);
-        // Lanes exchange their maxima, and what was summed so far is rescaled, only where a score exceeds the running maximum by 2^8: a probability is up to 2^8
-        // then, which costs neither the sums (fp32) nor its rounding to bf16 (relative) anything.
-        if (__any(top > m[n] + 8.f)) {
-          top = fmaxf(top, fstu_swz16(top));
-          top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
-          const float mn = fmaxf(m[n], top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
-          l[n] *= corr;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[n][d][r] *= corr;
-          m[n] = mn;
-        }
-        const float off = base - (m[n] == -INFINITY ? 0.f : m[n]);
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = s[n][e >> 2][e & 3];
-          p[e] = __builtin_amdgcn_exp2f(CAP ? x + off : fmaf(x, scale, off));
-          l[n] += p[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pf[n][e] = pack2_bf16(p[2 * e], p[2 * e + 1]);
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        struct { s16x4_t a, b; } f;
-        f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + v_at[d]));
-        f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(vl + v_at[d] + 4 * HD));
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-          o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f), __builtin_bit_cast(bf16x8_t, pf[n]), o[n][d], 0, 0, 0);
-      }
+    if (!on || b > qs + 31 || b + KB - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
+    const float base = slope * (float)(b - qi), base1 = base + slope * 32.f;
+    const Keys k0 = get_keys(buf, 0);
+    if constexpr (KB == 32) {
+      floatx16_t s0 = scores(k0);
+      shape(s0, b);
+      weigh(s0, base);
+      settle(s0, base);
+      add_values(get_values(buf, 0));
+      return;
     }
+    const Keys k1 = get_keys(buf, KB / 32 - 1);
+    floatx16_t s0 = scores(k0);
+    shape(s0, b);
+    const Values v0 = get_values(buf, 0);
+    floatx16_t s1 = scores(k1);
+    weigh(s0, base);
+    settle(s0, base);
+    shape(s1, b + 32);
+    const Values v1 = get_values(buf, KB / 32 - 1);
+    add_values(v0);
+    weigh(s1, base1);
+    settle(s1, base1);
+    add_values(v1);
+  };
+  for (int b = k_first; b <= k_last; b += 2 * KB) {
+    tile(b, std::integral_constant<int, 0>{});
+    if (b + KB <= k_last) tile(b + KB, std::integral_constant<int, 1>{});
   }
   if (!on) return;
-  unsigned long long bad = 0;
+  l += __shfl_xor(l, 32, FSTU_WAVE);
+  const float inv = 1.0f / l;
+  bool fine = true;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] += fstu_swz16(l[n]);
-    l[n] += __shfl_xor(l[n], 32, FSTU_WAVE);
-    const float inv = 1.0f / l[n];
-    const int qi = qs + n * 16 + c;
-    bool fine = true;
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      o[d][r] *= inv;
+      fine = fine && o[d][r] == o[d][r];
+    }
+  if (qi < len) {
+    bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + 4 * hi;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        o[n][d][r] *= inv;
-        fine = fine && o[n][d][r] == o[n][d][r];
-      }
-    if (qi < len) {
-      bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + 4 * g;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) *(uint2*)(orow + d * 16) = make_uint2(pack2_bf16(o[n][d][0], o[n][d][1]), pack2_bf16(o[n][d][2], o[n][d][3]));
-    }
-    unsigned long long here = __ballot(!fine && qi < len);
-    here |= here >> 32;
-    bad |= ((here | here >> 16) & 0xffffull) << (16 * n);
+      for (int e = 0; e < 4; ++e)
+        *(uint2*)(orow + d * 32 + e * 8) = make_uint2(pack2_bf16(o[d][4 * e], o[d][4 * e + 1]), pack2_bf16(o[d][4 * e + 2], o[d][4 * e + 3]));
   }
   // A NaN comes from a row's own scores and values, or from a value that it does not see (0 * infinity): the wave forms such rows once more, key by key.
+  unsigned long long bad = __ballot(!fine && qi < len);
+  bad = (bad | bad >> 32) & 0xffffffffull;
   while (bad) {
     const int i = qs + __builtin_ctzll(bad);
     bad &= bad - 1;
@@ -312,6 +437,7 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   FSTU_REQUIRE(fstu_heads_aligned(q, q_row, q_head, size) && fstu_heads_aligned(k, k_row, k_head, size) && fstu_heads_aligned(v, v_row, v_head, size) &&
                    fstu_aligned(out, 16),
                FSTU_EALIGN, "fstu_swa_packed: rows and heads of q, k and v and out must begin at multiples of 16 bytes");
+  FSTU_REQUIRE(rows == 0 || (k_row < (1 << 23) && v_row < (1 << 23)), FSTU_ESHAPE, "fstu_swa_packed: rows of k and v 2^23 elements apart and more");
   const int64_t n = (int64_t)rows * heads * hd * size;
   FSTU_REQUIRE(!fstu_heads_touch(q, q_row, q_head, rows, heads, hd, size, out, n) && !fstu_heads_touch(k, k_row, k_head, rows, kvh, hd, size, out, n) &&
                    !fstu_heads_touch(v, v_row, v_head, rows, kvh, hd, size, out, n),
@@ -321,20 +447,29 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   auto run = [&](auto w) {
     constexpr int HD = decltype(w)::value;
     if (dtype == FSTU_F32) {
-      hipLaunchKernelGGL((swa_packed_kernel<float, HD>), dim3(rows / 4 + seqs, heads), dim3(256), 0, (hipStream_t)stream, hq, hk, hv, (float*)out, cu, slopes, rows,
-                         seqs, heads, kvh, window, softcap);
+      const dim3 grid((unsigned)(rows / 32 + seqs) * heads);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, hq, hk, hv, (float*)out, cu, slopes, rows, seqs, heads, kvh, window, softcap);
+      };
+      softcap > 0.f ? go(swa_packed_f32_kernel<HD, 4, true>) : go(swa_packed_f32_kernel<HD, 4, false>);
       return;
     }
-    auto bf16 = [&](auto nw, auto nq) {
-      constexpr int NW = decltype(nw)::value, NQ = decltype(nq)::value;
+    auto bf16 = [&](auto nw) {
+      constexpr int NW = decltype(nw)::value;
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * NQ * 16) + seqs) * heads), dim3(NW * 64), 0, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu,
-                           slopes, rows, seqs, heads, kvh, window, softcap);
+        constexpr unsigned lds = 4 * (HD == 256 ? 32 : 64) * HD * 2;       // two tiles of keys, two of values
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * 32) + seqs) * heads), dim3(NW * 64), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes,
+                           rows, seqs, heads, kvh, window, softcap);
       };
-      if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, NQ, true, true>) : go(swa_packed_mfma_kernel<HD, NW, NQ, true, false>);
-      else slopes ? go(swa_packed_mfma_kernel<HD, NW, NQ, false, true>) : go(swa_packed_mfma_kernel<HD, NW, NQ, false, false>);
+      if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, true, true>) : go(swa_packed_mfma_kernel<HD, NW, true, false>);
+      else slopes ? go(swa_packed_mfma_kernel<HD, NW, false, true>) : go(swa_packed_mfma_kernel<HD, NW, false, false>);
     };
-    bf16(std::integral_constant<int, PK_NW>{}, std::integral_constant<int, HD == 256 ? 2 : PK_NQ>{});
+    // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 720 us,
+    // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238), two where there are few (4096 rows of 12 heads of 64, window 512, 25 and 30; heads of
+    // 128 do not fit their tiles' share into registers then).
+    if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(std::integral_constant<int, HD == 128 ? 8 : 4>{});
+    else if (HD <= 64 && (int64_t)(rows / 128) * heads < 768) bf16(std::integral_constant<int, HD <= 64 ? 2 : 4>{});
+    else bf16(std::integral_constant<int, 4>{});
   };
   if (hd == 32) run(std::integral_constant<int, 32>{});
   else if (hd == 64) run(std::integral_constant<int, 64>{});
