@@ -72,81 +72,84 @@ __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb,
   }
 }
 
-// fp32: v_mfma_f32_32x32x2_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
-// A workgroup takes 32 queries of one head; its waves take 32 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
-// first product and of keys in the second is what lanes hold: step s of the first is dims s and hd/2 + s, step r of the second the keys of score r.
-// FP32_FIGURES
+typedef float floatx4_t __attribute__((ext_vector_type(4)));
+
+// fp32: v_mfma_f32_16x16x4_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
+// A workgroup takes 16 queries of one head; its waves take 32 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
+// first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 16 t + 4 g + r.
+// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / so: 777 rows of 4 x 64 under a window of 129 12.7 / 13.1 / 9.8, 4096 of 8 x 64 under 512 267 / 76 / 74.
 template <int HD, int NW, bool CAP>
-__global__ void __launch_bounds__(NW * 64, HD >= 128 ? 1 : 2)
+__global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : 2)
 swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
-  constexpr int ND = HD / 32, HALF = HD / 2;
-  __shared__ float sm[NW][32], sl[NW][32], so[32][HD + 1];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, hi = lane >> 5;
+  constexpr int ND = HD / 16, PART = HD / 4;
+  __shared__ float sm[NW][16], sl[NW][16], so[16][HD + 1];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % heads, hk = h / (heads / kvh);
   int at, len, first;
-  packed_tile(cu, seqs, rows, 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  packed_tile(cu, seqs, rows, 16, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int qi = first + c, last = min(len - 1, first + 31);
+  const int qi = first + c, last = min(len - 1, first + 15);
   const int64_t k_row = k.row, v_row = v.row;
   const float* kb = (const float*)k.p + at * k_row + hk * k.head;
   const float* vb = (const float*)v.p + at * v_row + hk * v.head;
   const float kLog2e = 1.4426950408889634f, raw_slope = slopes ? slopes[h] : 0.f, slope = raw_slope * kLog2e;
   const float scale = rsqrtf((float)HD) * (CAP ? 1.0f / softcap : kLog2e), capA = softcap * kLog2e;
-  float4 qf[HALF / 4];
+  floatx4_t qf[PART / 4];
   {
-    const float* qr = (const float*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + hi * HALF;
+    const float* qr = (const float*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + g * PART;
 #pragma unroll
-    for (int s = 0; s < HALF / 4; ++s) qf[s] = *(const float4*)(qr + 4 * s);
+    for (int s = 0; s < PART / 4; ++s) qf[s] = *(const floatx4_t*)(qr + 4 * s);
   }
-  floatx16_t o[ND];
+  floatx4_t o[ND];
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  for (int d = 0; d < ND; ++d) o[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   for (int b = max(0, first - window) / 32 * 32 + 32 * w; b <= last; b += 32 * NW) {
-    floatx16_t s;
+    floatx4_t s[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-    const float* kr = kb + min(b + c, len - 1) * k_row + hi * HALF;            // rows behind the sequence: its last one, which no query of these sees
+    for (int t = 0; t < 2; ++t) {
+      s[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+      const float* kr = kb + min(b + 16 * t + c, len - 1) * k_row + g * PART;            // rows behind the sequence: its last one, which no query of these sees
 #pragma unroll
-    for (int x = 0; x < HALF / 4; ++x) {
-      const float4 f = *(const float4*)(kr + 4 * x);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.x, qf[x].x, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.y, qf[x].y, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.z, qf[x].z, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(f.w, qf[x].w, s, 0, 0, 0);
+      for (int x = 0; x < PART / 4; ++x) {
+        const floatx4_t f = *(const floatx4_t*)(kr + 4 * x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[e], qf[x][e], s[t], 0, 0, 0);
+      }
     }
-    float top = -INFINITY;
+    float top = -INFINITY, y[8];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int far = qi - b - ((r & 3) + 8 * (r >> 2) + 4 * hi);
-      const float x = (CAP ? capA * tanhf(s[r] * scale) : s[r] * scale) - slope * (float)far;
-      s[r] = far >= 0 && far <= window ? x : -INFINITY;
-      top = fmaxf(top, s[r]);
+    for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3] * scale;
+    if (CAP) fstu_tanh(y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int far = qi - b - (16 * (e >> 2) + 4 * g + (e & 3));
+      const float x = (CAP ? capA * y[e] : y[e]) - slope * (float)far;
+      s[e >> 2][e & 3] = far >= 0 && far <= window ? x : -INFINITY;
+      top = fmaxf(top, s[e >> 2][e & 3]);
     }
+    top = fmaxf(top, fstu_swz16(top));
     top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
     if (__any(top > m)) {
       const float mn = fmaxf(m, top), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= corr;
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+      for (int d = 0; d < ND; ++d) o[d] *= corr;
       m = mn;
     }
     const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float p = __builtin_amdgcn_exp2f(s[r] - off);
+    for (int e = 0; e < 8; ++e) {
+      const float p = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - off);
       l += p;
-      const float* vr = vb + min(b + (r & 3) + 8 * (r >> 2) + 4 * hi, len - 1) * v_row + c;
+      const float* vr = vb + min(b + 16 * (e >> 2) + 4 * g + (e & 3), len - 1) * v_row + c;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[32 * d], p, o[d], 0, 0, 0);
+      for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[16 * d], p, o[d], 0, 0, 0);
     }
   }
+  l += fstu_swz16(l);
   l += __shfl_xor(l, 32, FSTU_WAVE);
-  if (hi == 0) { sm[w][c] = m; sl[w][c] = l; }
+  if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
   __syncthreads();
   float M = -INFINITY;
 #pragma unroll
@@ -158,14 +161,14 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float& sum = so[c][d * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi];
+        for (int r = 0; r < 4; ++r) {
+          float& sum = so[c][d * 16 + 4 * g + r];
           sum = fmaf(o[d][r], mine, n ? sum : 0.f);
         }
     }
     __syncthreads();
   }
-  for (int row = w; row < 32 && first + row < len; row += NW) {
+  for (int row = w; row < 16 && first + row < len; row += NW) {
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NW; ++n) top = fmaxf(top, sm[n][row]);
@@ -447,7 +450,7 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   auto run = [&](auto w) {
     constexpr int HD = decltype(w)::value;
     if (dtype == FSTU_F32) {
-      const dim3 grid((unsigned)(rows / 32 + seqs) * heads);
+      const dim3 grid((unsigned)(rows / 16 + seqs) * heads);
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, hq, hk, hv, (float*)out, cu, slopes, rows, seqs, heads, kvh, window, softcap);
       };

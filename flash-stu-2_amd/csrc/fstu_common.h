@@ -179,6 +179,27 @@ __device__ __forceinline__ int fstu_last_where(int n, F below) {
   return lo;
 }
 
+// tanh of N values a lane to some 2^-22 of themselves: below 0.55 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))), which
+// is off by 3e-10 of itself there, beyond it 1 - 2 / (exp(2x) + 1), which a wave forms only where one of its values is as large.
+template <int N>
+__device__ __forceinline__ void fstu_tanh(float (&x)[N]) {
+  float most = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) most = fmaxf(most, fabsf(x[i]));
+  float far[N];
+  const bool some = __any(!(most < 0.55f));
+  if (some) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      far[i] = fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[i] * 2.8853900817779268f) + 1.0f), 1.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = x[i] * x[i], near = x[i] * fmaf(y, y + 105.0f, 945.0f) * __builtin_amdgcn_rcpf(fmaf(y, fmaf(y, 15.0f, 420.0f), 945.0f));
+    x[i] = some && !(fabsf(x[i]) < 0.55f) ? far[i] : near;
+  }
+}
+
 // tanh-approximated GELU as torch evaluates it in fp32
 __device__ __forceinline__ float gelu_tanh_f32(float x) {
   const float kBeta = 0.7978845608028654f;  // sqrt(2/pi)

@@ -323,9 +323,17 @@ typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ float cap_scale(float softcap) { return (sizeof(T) == 2 ? 2.0f * 1.4426950408889634f : 1.0f) / softcap; }
 template <typename T>
-__device__ __forceinline__ float capped(float s, float scale, float capA) {
-  if (sizeof(T) == 2) return fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * scale) + 1.0f), capA);
-  return capA * tanhf(s * scale);
+__device__ __forceinline__ void cap_scores(float (&s)[8], float scale, float capA) {
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[j] * scale) + 1.0f), capA);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] *= scale;
+    fstu_tanh(s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] *= capA;
+  }
 }
 
 #define KV4_MOST_PARTS 64  // more: workgroups that all keys are dealt to
@@ -572,10 +580,7 @@ kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, 
       float vs[8] = {scale_of<0>(now.vs), scale_of<1>(now.vs), scale_of<2>(now.vs), scale_of<3>(now.vs),
                      scale_of<4>(now.vs), scale_of<5>(now.vs), scale_of<6>(now.vs), scale_of<7>(now.vs)};
       float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (CAP) s[j] = capped<T>(s[j], scale, capA);
-      }
+      if (CAP) cap_scores<T>(s, scale, capA);
       if (whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j] = fmaf(s[j], CAP ? 1.f : scale, slope * (float)j);
