@@ -100,6 +100,8 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
 #pragma unroll
     for (int s = 0; s < PART / 4; ++s) qf[s] = *(const floatx4_t*)(qr + 4 * s);
   }
+#pragma unroll
+  for (int s = 0; s < PART / 4; ++s) asm volatile("" : "+v"(qf[s]));         // waited for here, not among the loop's requests
   floatx4_t o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
@@ -204,7 +206,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   constexpr int TILE = KB * CH;                              // 16-byte pieces
   extern __shared__ u32x4_t lds[];                               // two tiles of keys, two of values
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
-  const int h = blockIdx.x % heads, hk = h / (heads / kvh);
+  // neighbouring workgroups go to the eight XCDs in turn: the query heads of a key head to one of them, whose L2 then holds its keys and values
+  const int hx = blockIdx.x % heads, h = heads % 8 ? hx : hx % 8 * (heads / 8) + hx / 8, hk = h / (heads / kvh);
   int at, len, first;
   packed_tile(cu, seqs, rows, NW * 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
   if (first < 0 || first >= len) return;
@@ -358,6 +361,9 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     }
   };
   fetch(k_first);
+  // the queries are waited for here: left to their first use in the loop, that wait would be one for the loop's own requests too
+#pragma unroll
+  for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
   store(0);
   if (k_first + KB <= k_last) fetch(k_first + KB);
   auto tile = [&](int b, auto bufs) {
@@ -368,6 +374,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     if (!on || b > qs + 31 || b + KB - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
     const float base = slope * (float)(b - qi), base1 = base + slope * 32.f;
     const Keys k0 = get_keys(buf, 0);
+    __builtin_amdgcn_sched_barrier(0);                           // all of them asked for before the first product waits for one
     if constexpr (KB == 32) {
       floatx16_t s0 = scores(k0);
       shape(s0, b);
