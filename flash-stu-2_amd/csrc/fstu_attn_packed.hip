@@ -198,7 +198,8 @@ struct Frag8 { u32x2_t lo, hi; };
 // Keys and values go straight to LDS, one barrier a tile; values are read back transposed.  The second half's first product runs beside the
 // first half's softmax, the first half's second product beside the second half's: the maximum that a probability is taken from is the one
 // before these keys, and where a score exceeds it by more than 2^16 (the first keys, and hardly any after) that half is formed once more.
-template <int HD, int NW, bool CAP, bool BIAS>
+// CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
+template <int HD, int NW, int CAP, bool BIAS>
 __global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : HD <= 64 && NW == 4 ? 3 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
                        float softcap) {
@@ -308,10 +309,14 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     return s;
   };
   auto shape = [&](floatx16_t& s, int b0) {                      // soft-cap, and what the lane's query does not see
-    if (CAP) {
+    if (CAP == 1) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         s[r] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * scale) + 1.0f), BIAS ? capA + bias[r] : capA);
+    }
+    if (CAP == 2) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fstu_wide_cap(s[r], scale, capA) + (BIAS ? bias[r] : 0.f);
     }
     if (b0 + 31 > qs || b0 < qs + 31 - window) {                 // wave-uniform: some key is not visible to some query
       asm volatile("");
@@ -442,12 +447,14 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   FSTU_REQUIRE(rows >= 0 && rows <= (1 << 30) && seqs >= 0 && seqs <= (1 << 30) && kvh >= 1 && heads >= 1 && heads % kvh == 0 && heads <= 65535, FSTU_ESHAPE,
                "fstu_swa_packed: bad shape rows=%d sequences=%d heads=%d key heads=%d", rows, seqs, heads, kvh);
   FSTU_REQUIRE(window >= 0, FSTU_EARG, "fstu_swa_packed: window<0");
-  FSTU_REQUIRE(softcap >= 0.f && softcap < INFINITY, FSTU_EARG, "fstu_swa_packed: softcap must be zero (none) or a positive number");
+  FSTU_REQUIRE(fstu_softcap_ok(softcap), FSTU_EARG, "fstu_swa_packed: softcap must be zero (none) or a number from 2^-40 to 2^40");
   const int size = dtype == FSTU_BF16 ? 2 : 4;
   FSTU_REQUIRE(fstu_heads_aligned(q, q_row, q_head, size) && fstu_heads_aligned(k, k_row, k_head, size) && fstu_heads_aligned(v, v_row, v_head, size) &&
                    fstu_aligned(out, 16),
                FSTU_EALIGN, "fstu_swa_packed: rows and heads of q, k and v and out must begin at multiples of 16 bytes");
   FSTU_REQUIRE(rows == 0 || (k_row < (1 << 23) && v_row < (1 << 23)), FSTU_ESHAPE, "fstu_swa_packed: rows of k and v 2^23 elements apart and more");
+  // fp32: 16 threads a row; bf16: 2; up to 512 more a sequence
+  FSTU_REQUIRE(((int64_t)rows * (dtype == FSTU_F32 ? 16 : 2) + (int64_t)seqs * 512) * heads < 1ll << 32, FSTU_ESHAPE, "fstu_swa_packed: %d rows of %d sequences and %d heads are more than a launch takes", rows, seqs, heads);
   const int64_t n = (int64_t)rows * heads * hd * size;
   FSTU_REQUIRE(!fstu_heads_touch(q, q_row, q_head, rows, heads, hd, size, out, n) && !fstu_heads_touch(k, k_row, k_head, rows, kvh, hd, size, out, n) &&
                    !fstu_heads_touch(v, v_row, v_head, rows, kvh, hd, size, out, n),
@@ -471,13 +478,16 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
         hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * 32) + seqs) * heads), dim3(NW * 64), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes,
                            rows, seqs, heads, kvh, window, softcap);
       };
-      if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, true, true>) : go(swa_packed_mfma_kernel<HD, NW, true, false>);
-      else slopes ? go(swa_packed_mfma_kernel<HD, NW, false, true>) : go(swa_packed_mfma_kernel<HD, NW, false, false>);
+      if (softcap > FSTU_FAST_CAP) slopes ? go(swa_packed_mfma_kernel<HD, 4, 2, true>) : go(swa_packed_mfma_kernel<HD, 4, 2, false>);
+      else if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, 1, true>) : go(swa_packed_mfma_kernel<HD, NW, 1, false>);
+      else slopes ? go(swa_packed_mfma_kernel<HD, NW, 0, true>) : go(swa_packed_mfma_kernel<HD, NW, 0, false>);
     };
     // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 720 us,
     // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238), two where there are few (4096 rows of 12 heads of 64, window 512, 25 and 30; heads of
     // 128 do not fit their tiles' share into registers then).
-    if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(std::integral_constant<int, HD == 128 ? 8 : 4>{});
+    // Soft-caps of no ordinary size have the kernel of four waves alone.
+    if (softcap > FSTU_FAST_CAP) bf16(std::integral_constant<int, 4>{});
+    else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(std::integral_constant<int, HD == 128 ? 8 : 4>{});
     else if (HD <= 64 && (int64_t)(rows / 128) * heads < 768) bf16(std::integral_constant<int, HD <= 64 ? 2 : 4>{});
     else bf16(std::integral_constant<int, 4>{});
   };

@@ -101,6 +101,8 @@ static inline bool fstu_heads_touch(const void* p, int64_t row, int64_t head, in
   const uintptr_t a = reinterpret_cast<uintptr_t>(p), o = reinterpret_cast<uintptr_t>(out);
   return rows > 0 && n > 0 && o < a + ((rows - 1) * row + (heads - 1) * head + hd) * size && a < o + n;
 }
+// a soft-cap that scores over it, and it over scores, stay in fp32's range with
+static inline bool fstu_softcap_ok(float c) { return c == 0.f || (c >= 0x1p-40f && c <= 0x1p40f); }
 // the optional exact head of the distilled filter: ring, taps and their count go together; count a power of two in 8..1024
 static inline bool fstu_fir_ok(const void* ring, const float* fir, int taps) {
   if (!ring && !fir && taps == 0) return true;
@@ -177,6 +179,16 @@ __device__ __forceinline__ int fstu_last_where(int n, F below) {
     n = min(step, n - last * step);
   }
   return lo;
+}
+
+// capA * tanh(x) of 2 log2(e) x = s * scale for soft-caps beyond FSTU_FAST_CAP, where 1 - 2 / (exp(2x) + 1), off by 2^-21 of capA, leaves too little of a small
+// score: below x = 0.25 the Taylor series to x^7 (off by 4e-7 of itself there).
+#define FSTU_FAST_CAP 512.0f
+__device__ __forceinline__ float fstu_wide_cap(float s, float scale, float capA) {
+  const float t = s * scale, x = t * 0.34657359027997264f, y = x * x;
+  const float near = capA * x * fmaf(y, fmaf(y, fmaf(y, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  const float far = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t) + 1.0f), capA);
+  return fabsf(x) < 0.25f ? near : far;
 }
 
 // tanh of N values a lane to some 2^-22 of themselves: below 0.55 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))), which

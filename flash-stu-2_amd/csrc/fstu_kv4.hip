@@ -319,14 +319,20 @@ typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 // capA * tanh(x / softcap) of scale * s = x (fp32) or 2 log2(e) x (bf16: 1 - 2 / (exp(2x) + 1) on the hardware's exp and reciprocal, which is off by
-// up to 2^-21 of capA, where the bf16 queries' own rounding moves a score by 2^-9 of itself)
+// up to 2^-21 of capA, where the bf16 queries' own rounding moves a score by 2^-9 of itself; fstu_wide_cap where capA is so large that this would show)
 template <typename T>
 __device__ __forceinline__ float cap_scale(float softcap) { return (sizeof(T) == 2 ? 2.0f * 1.4426950408889634f : 1.0f) / softcap; }
 template <typename T>
 __device__ __forceinline__ void cap_scores(float (&s)[8], float scale, float capA) {
   if (sizeof(T) == 2) {
+    if (capA <= FSTU_FAST_CAP * 1.4426950408889634f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[j] * scale) + 1.0f), capA);
+      for (int j = 0; j < 8; ++j) s[j] = fmaf(-2.0f * capA, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[j] * scale) + 1.0f), capA);
+    } else {
+      asm volatile("");
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = fstu_wide_cap(s[j], scale, capA);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] *= scale;
@@ -863,7 +869,7 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
   FSTU_REQUIRE(heads >= 1 && heads % kvh == 0 && heads <= 65535 && seqs <= 65535 && (int64_t)seqs * heads <= 0x7fffffff, FSTU_ESHAPE, "fstu_kv4_attend: %d heads over %d key heads, %d sequences", heads,
                kvh, seqs);
   FSTU_REQUIRE(window >= 0 && window < cap, FSTU_EARG, "fstu_kv4_attend: window %d with a capacity of %d", window, cap);
-  FSTU_REQUIRE(softcap >= 0.f && softcap < INFINITY, FSTU_EARG, "fstu_kv4_attend: softcap must be zero (none) or a positive number");
+  FSTU_REQUIRE(fstu_softcap_ok(softcap), FSTU_EARG, "fstu_kv4_attend: softcap must be zero (none) or a number from 2^-40 to 2^40");
   FSTU_REQUIRE(splits >= 1 && splits <= 65535 && (splits == 1 || ws), FSTU_EARG, "fstu_kv4_attend: %d splits need their workspace", splits);
   const int size = dtype == FSTU_BF16 ? 2 : 4;
   FSTU_REQUIRE(fstu_heads_aligned(q, q_row, q_head, size) && fstu_aligned(out, 16) && fstu_aligned(ws, 4), FSTU_EALIGN,
@@ -873,6 +879,8 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
                    !fstu_heads_touch(cache, fstu_kv4_bytes(seqs, kvh, hd, cap), 0, 2, 1, 0, 1, out, n),
                FSTU_EARG, "fstu_kv4_attend: out overlaps q or the cache");
   const int group = heads / kvh, chunks = (group + KV4_COLS - 1) / KV4_COLS;
+  FSTU_REQUIRE((int64_t)seqs * heads < 1 << 23 && (splits > KV4_MOST_PARTS || (int64_t)seqs * kvh * chunks * splits < 1 << 23), FSTU_ESHAPE,
+               "fstu_kv4_attend: %d sequences of %d heads in %d parts are more than a launch takes", seqs, heads, splits);
   KV4_DISPATCH(dtype, hd, "fstu_kv4_attend", {
     auto run = [&](auto kernel, dim3 grid, int waves) {
       const unsigned lds = waves * (2 * KV4_COLS + (group < KV4_COLS ? group : KV4_COLS) * HD) * sizeof(float);

@@ -1542,7 +1542,7 @@ def swa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     """Causal attention over whole prompts packed behind one another: q (rows, heads, head_dim), k and v (rows, key_heads, head_dim) float32 or
     bfloat16, key_heads a divisor of heads (query head h reads key head h // (heads / key_heads)), head_dim 32, 64, 128 or 256.  Row i of a sequence
     sees its rows max(0, i - window) .. i (window None: all of them); scores are softcap * tanh(q . k * head_dim^-1/2 / softcap) - slopes[h] *
-    distance (softcap 0 or None: uncapped; slopes (heads,) float32, None: zero).  Returns out (rows, heads, head_dim); rows in front of the first
+    distance (softcap 0 or None: uncapped, else 2^-40 to 2^40; slopes (heads,) float32, None: zero).  Returns out (rows, heads, head_dim); rows in front of the first
     sequence and behind the last are left as they were (without out: they are not set)."""
     if (q.requires_grad or k.requires_grad or v.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
         raise _fp8_forward_only("swa_packed")
@@ -1642,15 +1642,15 @@ def _kv4_splits(seqs: int, heads: int, kvh: int, hd: int, cap: int, window: int)
     return splits, load().fstu_kv4_attend_ws(seqs, heads, kvh, hd, splits)
 
 
-def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, softcap: float = 0.0,
-               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None,
+               slopes: Optional[torch.Tensor] = None, window: Optional[int] = None, softcap: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     if (q.requires_grad or slopes is not None and slopes.requires_grad or out is not None and out.requires_grad) and _grad_on():
         raise _fp8_forward_only("KV4Cache.attend")
     data = cache.data
     dev = data.get_device()
     if dev != _device_now():
         with torch.cuda.device(dev):
-            return kv4_attend(cache, q, pos, slopes, window, softcap, out)
+            return kv4_attend(cache, q, pos, k, v, slopes, window, softcap, out)
     seqs, kvh, hd, cap = cache.batch, cache.kv_heads, cache.head_dim, cache.capacity
     shape, dtype = q.shape, q.dtype
     dt, heads = _kv4_types.get(dtype), shape[1] if len(shape) == 3 else 0
@@ -1664,10 +1664,16 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch
         window = cap - 1
     elif not 0 <= window < cap:
         raise FlashSTUHipError(f"KV4Cache.attend: window {window} does not fit a ring of {cap} (0 to {cap - 1})")
+    if softcap and not 2.0 ** -40 <= softcap <= 2.0 ** 40:
+        raise FlashSTUHipError(f"KV4Cache.attend: softcap must be zero (none) or a number from 2^-40 to 2^40, got {softcap}")
     if out is None:
         out = _empty(shape, dtype=dtype, device=data.device)
     else:
         _written(out)
+    if k is not None or v is not None:
+        if k is None or v is None:
+            raise FlashSTUHipError("KV4Cache.attend: k and v go together")
+        kv4_write(cache, k, v, pos)
     splits, floats = _kv4_splits(seqs, heads, kvh, hd, cap, window)
     ws = _empty(floats, dtype=_f32, device=data.device).data_ptr() if floats else None      # its memory is this stream's until what runs on it next
     qr, qh, _ = q.stride()

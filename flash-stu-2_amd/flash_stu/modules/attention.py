@@ -95,10 +95,10 @@ class KV4Cache:
     one.  32 values with an infinity or a NaN among them stand for NaN.  A key and its value take 17/16 of a byte for each dim, bf16 ones 4.
 
     `pos` is (batch,) int32 on the GPU and counted by the caller, so that a captured step runs for every position; a sequence at a negative position
-    is not in use.  capacity beyond the window leaves room for nothing but is allowed; head_dim is 32, 64, 128 or 256.  Forward only."""
+    is not in use.  The capacity may exceed a window by any number; head_dim is 32, 64, 128 or 256.  Forward only."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, capacity: int, device=None):
-        if batch < 1 or kv_heads < 1 or not 1 <= capacity <= 1 << 30 or head_dim not in (32, 64, 128, 256):
+        if batch < 1 or kv_heads < 1 or not 1 <= capacity <= 1 << 30 or head_dim not in (32, 64, 128, 256) or batch * kv_heads * capacity > 1 << 40:
             raise _hip.FlashSTUHipError(f"KV4Cache: batch {batch}, {kv_heads} key heads, capacity {capacity} (up to 2^30) and head_dim {head_dim} "
                                         "(32, 64, 128 or 256) are no cache")
         device = torch.device("cuda" if device is None else device)
@@ -121,9 +121,5 @@ class KV4Cache:
                softcap: float = 0.0, out: torch.Tensor = None) -> torch.Tensor:
         """One query a sequence, q (batch, heads, head_dim), at position pos[s], over the positions max(0, pos[s] - window) .. pos[s] as the cache holds
         them (window None: capacity - 1); heads a multiple of kv_heads, scores as swa_packed's.  k, v (batch, kv_heads, head_dim): those of position
-        pos[s], written first.  Returns out (batch, heads, head_dim), zero for a sequence not in use."""
-        if (k is None) != (v is None):
-            raise _hip.FlashSTUHipError("KV4Cache.attend: k and v go together")
-        if k is not None:
-            _hip.kv4_write(self, k, v, pos)
-        return _hip.kv4_attend(self, q, pos, slopes, window, softcap, out)
+        pos[s], written first.  Returns out (batch, heads, head_dim), zero for a sequence not in use; out must not overlap q or the cache."""
+        return _hip.kv4_attend(self, q, pos, k, v, slopes, window, softcap, out)

@@ -28,16 +28,16 @@ def attention(q, k, v, far, slope, softcap, p_step):
 
     In fp32 a score is off by (hd + 16) * 2^-23 of the sum of its products' sizes (each product and addition 2^-24 at most of a partial sum, twice
     that where a value goes in three bf16 parts), 2^-22 of itself (the scale, the soft-cap's argument, ALiBi's product and its difference), and, capped, by
-    2^-20 * softcap (1 - 2 / (exp(2x) + 1) on the hardware's exp and reciprocal); a probability by that, by 2^-22 * (1 + |s - max|) for its
+    2^-20 * softcap (1 - 2 / (exp(2x) + 1) on the hardware's exp and reciprocal: the reciprocal's, the exp's and the difference's last bit, 2^-22 each), from soft-caps
+    of 512 on by 2^-18 of itself instead (a series where x < 0.25, and 2^-20 of softcap is 2^-18 of what is larger); a probability by that, by 2^-22 * (1 + |s - max|) for its
     exp, and by p_step where it is cut to bf16 parts.  A probability's error e_j changes the output by p_j e_j (|v_j| + |o|) at most.  Sums over m keys and
     their rescaling: (2 m + 16) * 2^-24 of the sum of sizes, for numerator and denominator."""
     hd = q.shape[1]
     raw = q @ k.t() * hd ** -0.5
     size = q.abs() @ k.abs().t() * hd ** -0.5
     s = softcap * torch.tanh(raw / softcap) if softcap else raw
-    s = s - slope * far
-    off = (hd + 16) * 2.0 ** -23 * size + 2.0 ** -22 * (raw.abs() + slope * far.abs()) + (2.0 ** -20 * softcap if softcap else 0.0)
-    s = s.masked_fill(far < 0, -math.inf)
+    off = (hd + 16) * 2.0 ** -23 * size + 2.0 ** -22 * (raw.abs() + slope * far.abs()) + (2.0 ** -20 * softcap if 0 < softcap <= 512 else 2.0 ** -18 * s.abs() if softcap else 0.0)
+    s = (s - slope * far).masked_fill(far < 0, -math.inf)
     top = s.amax(-1, keepdim=True)
     p = torch.exp(s - top)
     p = p / p.sum(-1, keepdim=True)

@@ -187,6 +187,27 @@ def test_attend(fs, heads, kvh, hd, cap, window, pos, softcap, alibi, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [2.0 ** -40, 0.01, 1.0, 511.0, 513.0, 1e5, 2.0 ** 40])
+def test_attend_under_any_soft_cap(fs, softcap, dtype):
+    cache, ring = filled(fs, 2, 2, 64, 100, 60)
+    for size in (1.0, 40.0):
+        q = (rand(8, 2, 4, 64) * size).to(dtype)
+        y = cache.attend(q.cuda(), ints([99, 130]), softcap=softcap)
+        check(y, *ring.attend(q, [99, 130], None, None, softcap, P_STEP), dtype)
+
+
+def test_a_refused_call_writes_nothing(fs):
+    from flash_stu._hip import FlashSTUHipError
+    cache = fs.KV4Cache(2, 2, 64, 40)
+    k, q, pos = torch.ones(2, 2, 64, device="cuda"), torch.ones(2, 4, 64, device="cuda"), ints([0, 0])
+    for call in (lambda: cache.attend(q[:, :3], pos, k, k), lambda: cache.attend(q, pos, k, k, window=40), lambda: cache.attend(q, pos, k, k, softcap=-1.0),
+                 lambda: cache.attend(q, pos, k), lambda: cache.attend(q, pos, k, k, slopes=torch.ones(3, device="cuda")), lambda: cache.attend(q, pos, k, k, out=q[:1])):
+        with pytest.raises(FlashSTUHipError):
+            call()
+    assert not cache.data.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("splits", [1, 2, 7, 64, 65, 100, 300])
 @pytest.mark.parametrize("heads,kvh,hd,cap,window,pos", [(4, 2, 64, 700, None, [699, 20, -1, 1500]), (9, 1, 128, 300, 250, [299, 0, 310]), (2, 2, 256, 90, 63, [-1, 500]),
                                                         (3, 3, 32, 64, None, [-1, -1])])

@@ -96,6 +96,16 @@ def test_what_a_row_does_not_see_may_be_anything(fs, hd, window, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("softcap", [2.0 ** -40, 0.01, 1.0, 511.0, 513.0, 1e5, 2.0 ** 40])
+def test_under_any_soft_cap(fs, softcap, dtype):
+    for size in (1.0, 40.0):
+        (q, k, v), dev = fused(4, 150, 2, 1, 64, dtype)
+        q = (q.float() * size).to(dtype)
+        y = fs.swa_packed(q.cuda(), dev[1], dev[2], bounds([70, 80]), softcap=softcap, slopes=slopes_of(2).cuda())
+        check(y, *packed(q, k, v, [70, 80], slopes_of(2), None, softcap, P_STEP[dtype]), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_of_no_sequence_are_left(fs, dtype):
     (q, k, v), dev = fused(5, 200, 3, 3, 64, dtype)
     out = torch.full((200, 3, 64), 7.0, dtype=dtype, device="cuda")

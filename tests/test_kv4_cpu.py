@@ -53,7 +53,8 @@ def test_cache_entry_points_refuse(lib, mem):
     assert attend(q=None) == -1 and attend(c=None) == -1 and attend(out=None) == -1 and attend(pos=None) == -1
     assert attend(hd=96) == -3 and attend(heads=3) == -3 and attend(heads=0) == -3 and attend(seqs=65536) == -3 and attend(cap=0) == -3
     assert attend(window=8) == -5 and attend(window=-1) == -5 and "window" in why(lib)
-    assert attend(softcap=-1.0) == -5 and attend(softcap=math.nan) == -5 and attend(softcap=math.inf) == -5
+    assert attend(softcap=-1.0) == -5 and attend(softcap=math.nan) == -5 and attend(softcap=math.inf) == -5 and attend(softcap=1e-13) == -5 and attend(softcap=2e12) == -5
+    assert attend(seqs=60000, heads=256, out=p + (1 << 40), splits=1) == -3 and attend(seqs=4096, splits=64, ws=p, kvh=32, heads=32, out=p + (1 << 40)) == -3 and "launch" in why(lib)
     assert attend(q=p + 8) == -4 and attend(qr=100) == -4 and attend(qh=-64) == -4 and attend(out=p + 4096 + 4) == -4 and attend(c=p + 8200) == -4
     assert attend(out=p) == -5 and "overlaps" in why(lib)
     assert attend(out=p + 8192) == -5 and attend(out=p + 8192 + 2 * 2 * 32 * 68 - 16) == -5
@@ -71,7 +72,7 @@ def test_packed_entry_point_refuses(lib, mem):
 
     assert f(q=None) == -1 and f(k=None) == -1 and f(v=None) == -1 and f(out=None) == -1 and f(cu=None) == -1
     assert f(hd=80) == -3 and f(heads=5) == -3 and f(kvh=0) == -3 and f(rows=-1) == -3 and f(seqs=-1) == -3 and f(heads=0) == -3
-    assert f(rows=(1 << 30) + 1) == -3
+    assert f(rows=(1 << 30) + 1) == -3 and f(rows=1 << 28, heads=8) == -3 and "launch" in why(lib) and f(kr=1 << 23) == -3
     assert f(window=-1) == -5 and f(softcap=-0.5) == -5 and f(softcap=math.nan) == -5 and f(softcap=math.inf) == -5
     assert f(q=p + 4) == -4 and f(k=p + 2) == -4 and f(v=p + 8) == -4 and f(out=p + 8196) == -4 and f(qr=257) == -4 and f(kh=60) == -4 and f(kr=-8) == -4
     assert f(out=p) == -5 and f(out=p + 256 * 7 * 2) == -5 and "overlaps" in why(lib)
