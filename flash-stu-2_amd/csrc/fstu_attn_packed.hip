@@ -14,15 +14,47 @@ struct Heads {                 // rows of heads: strides in elements
   int64_t row, head;
 };
 
-// The sequence that row tile t (of `per` rows) belongs to, and its number there: sequence i has the tiles from cu[i] / per + i on, which are as many as it
-// needs or one more (a sequence's rows begin anywhere), so that no count has to be added up on the way.
-__device__ __forceinline__ int packed_tile(const int* cu, int seqs, int rows, int per, int t, int* at, int* len, int* first) {
+// The tile of `per` rows that workgroup t of a head takes: its sequence's first row and length and the tile's first row there (behind the sequence: none).
+// Where a call fills the card more than once (many), the tiles of the highest number within their sequences come first: they have the most keys to walk, and the short
+// ones fill the gaps of the last round.  A sequence's tiles behind another's: two documents of 4096 and 8 heads of 256 318 us, so 284; 16000 rows of 8
+// prompts and 12 heads of 64 under a window of 512 68 and 63; two of 8192 and 16 heads of 128 711 and 715.  A wave looks for that number with a lane to each of 63 candidates, a sequence to a lane;
+// more than 64 sequences, whose tiles are short or many, come one behind the other, and so do few tiles (58 rows of three sequences 5.3 us, 5.5 by that search).
+#define PACKED_WAVES 2048                                        // that the card holds at once, two to a SIMD
+__device__ __forceinline__ void packed_tile(const int* cu, int seqs, int rows, int per, int t, int tiles, bool many, int* at, int* len, int* first) {
+  const int lane = (int)threadIdx.x & 63;
+  if (many && seqs <= 64) {
+    const int a = min(max(cu[min(lane, seqs - 1)], 0), rows), b = min(max(cu[min(lane, seqs - 1) + 1], a), rows);
+    const int mine = lane < seqs ? (b - a + per - 1) / per : 0;  // tiles of the lane's sequence
+    int stride = 1, level = 0, above;
+    while (__any(mine > 63 * stride)) stride *= 63;
+    for (;; stride /= 63) {                                      // above: the tiles of number level + lane * stride and more, which are all that come before
+      above = 0;
+      for (int i = 0; i < seqs; ++i) above += max(0, __builtin_amdgcn_readlane(mine, i) - (level + lane * stride));
+      const int last = __builtin_popcountll(__ballot(above > t)) - 1;
+      if (last < 0) {                                            // no such tile: the grid has one to spare for each sequence
+        *at = *len = *first = 0;
+        return;
+      }
+      level += last * stride;
+      if (stride == 1) {
+        const int rank = t - __builtin_amdgcn_readlane(above, last + 1);
+        const unsigned long long with = __ballot(mine > level);
+        const int seq = __builtin_ctzll(__ballot(mine > level && (int)__builtin_popcountll(with & ((1ull << lane) - 1)) == rank));
+        *at = __builtin_amdgcn_readlane(a, seq);
+        *len = __builtin_amdgcn_readlane(b, seq) - *at;
+        *first = level * per;
+        return;
+      }
+    }
+  }
+  // sequence i has the tiles from cu[i] / per + i on, which are as many as it needs or one more (a sequence's rows begin anywhere), so that no count has to be
+  // added up on the way
+  t = tiles - 1 - t;
   const int lo = fstu_last_where(seqs, [&](int i) { return max(cu[i], 0) / per + i <= t; });
   const int a = min(max(cu[lo], 0), rows), b = min(max(cu[lo + 1], a), rows);
   *at = a;
   *len = b - a;
   *first = (t - (a / per + lo)) * per;
-  return lo;
 }
 
 // One query of one head by a wave, key by key: 8 lanes to a key, 8 keys side by side, each group with a softmax of its own.  i: the query's row in its sequence, which
@@ -86,7 +118,7 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % heads, hk = h / (heads / kvh);
   int at, len, first;
-  packed_tile(cu, seqs, rows, 16, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  packed_tile(cu, seqs, rows, 16, blockIdx.x / heads, gridDim.x / heads, gridDim.x * NW > PACKED_WAVES, &at, &len, &first);
   if (first < 0 || first >= len) return;
   const int qi = first + c, last = min(len - 1, first + 15);
   const int64_t k_row = k.row, v_row = v.row;
@@ -210,7 +242,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   // neighbouring workgroups go to the eight XCDs in turn: the query heads of a key head to one of them, whose L2 then holds its keys and values
   const int hx = blockIdx.x % heads, h = heads % 8 ? hx : hx % 8 * (heads / 8) + hx / 8, hk = h / (heads / kvh);
   int at, len, first;
-  packed_tile(cu, seqs, rows, NW * 32, gridDim.x / heads - 1 - blockIdx.x / heads, &at, &len, &first);
+  const bool many = gridDim.x * NW > PACKED_WAVES;
+  packed_tile(cu, seqs, rows, NW * 32, blockIdx.x / heads, gridDim.x / heads, many, &at, &len, &first);
   if (first < 0 || first >= len) return;
   const int qs = first + w * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
@@ -365,19 +398,25 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v.f[t][d]), __builtin_bit_cast(bf16x8_t, pf), o[d], 0, 0, 0);
     }
   };
-  fetch(k_first);
+  // With ALiBi the largest scores are a query's latest keys': from those backwards the maximum settles at once (two documents of 8192, 16 heads of 128, 719 us, 785
+  // forwards; 16383 rows of 16 heads of 128 under a window of 1024 218 and 229).  Without it forwards, where the workgroups of a document read the same keys at the
+  // same time (two of 4096, 8 heads of 256, 287 us, 297 backwards), and where all the call's workgroups run at once (8 prompts, 4096 rows of 12 heads of 64, 23.5 and 24.5).
+  const bool back = BIAS && many;
+  const int b_first = back ? k_last / KB * KB : k_first, b_step = back ? -KB : KB;
+  int left = (k_last - k_first) / KB;                            // tiles after this one: k_first is a multiple of KB
+  fetch(b_first);
   // the queries are waited for here: left to their first use in the loop, that wait would be one for the loop's own requests too
 #pragma unroll
   for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
   store(0);
-  if (k_first + KB <= k_last) fetch(k_first + KB);
+  if (left > 0) fetch(b_first + b_step);
   auto tile = [&](int b, auto bufs) {
     constexpr int buf = decltype(bufs)::value;
     __syncthreads();                                             // this tile is there, and the one before it has been read
-    if (b + KB <= k_last) store(buf ^ 1);
-    if (b + 2 * KB <= k_last) fetch(b + 2 * KB);
+    if (left > 0) store(buf ^ 1);
+    if (left > 1) fetch(b + 2 * b_step);
     if (!on || b > qs + 31 || b + KB - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
-    const float base = slope * (float)(b - qi), base1 = base + slope * 32.f;
+    const float base = slope * (float)(b - qi);
     const Keys k0 = get_keys(buf, 0);
     __builtin_amdgcn_sched_barrier(0);                           // all of them asked for before the first product waits for one
     if constexpr (KB == 32) {
@@ -388,6 +427,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
       add_values(get_values(buf, 0));
       return;
     }
+    const float base1 = base + slope * 32.f;
     const Keys k1 = get_keys(buf, KB / 32 - 1);
     floatx16_t s0 = scores(k0);
     shape(s0, b);
@@ -402,9 +442,11 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     settle(s1, base1);
     add_values(v1);
   };
-  for (int b = k_first; b <= k_last; b += 2 * KB) {
+  for (int b = b_first;; b += 2 * b_step) {
     tile(b, std::integral_constant<int, 0>{});
-    if (b + KB <= k_last) tile(b + KB, std::integral_constant<int, 1>{});
+    if (--left < 0) break;
+    tile(b + b_step, std::integral_constant<int, 1>{});
+    if (--left < 0) break;
   }
   if (!on) return;
   l += __shfl_xor(l, 32, FSTU_WAVE);

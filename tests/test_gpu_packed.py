@@ -67,6 +67,25 @@ def test_packed(fs, heads, kvh, hd, lengths, window, softcap, alibi, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kvh,hd,lengths,window,softcap,alibi", [
+    (32, 1, 64, [1, 4200, 0, 130, 64, 17], 70, 0.0, True),
+    (32, 4, 32, [33, 2] * 35 + [80], 50, 50.0, True),
+    (32, 2, 128, [700, 1500, 90], None, 50.0, True),
+    (32, 32, 128, [0, 900, 1100, 0], None, 0.0, False),
+    (64, 8, 256, [520, 300, 1], 200, 0.0, True),
+    (64, 64, 64, [65] * 64, None, 0.0, True),
+])
+def test_more_workgroups_than_the_card_holds(fs, heads, kvh, hd, lengths, window, softcap, alibi, dtype):
+    (q, k, v), dev = fused(17, sum(lengths), heads, kvh, hd, dtype)
+    slopes = slopes_of(heads) * 4
+    y = fs.swa_packed(*dev, bounds(lengths), slopes=slopes.cuda() if alibi else None, window=window, softcap=softcap)
+    h = torch.tensor([0, 1, heads // 2 + 3, heads - 1])
+    kv = h // (heads // kvh)
+    check(y.cpu()[:, h], *packed(q[:, h], k[:, kv], v[:, kv], lengths, slopes[h] if alibi else None, window, softcap, P_STEP[dtype]), dtype)
+    assert bool(torch.isfinite(y).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128])
 def test_one_long_document(fs, hd, dtype):
     (q, k, v), dev = fused(3, 2100, 2, 1, hd, dtype)
