@@ -234,21 +234,21 @@ struct Frag8 { u32x2_t lo, hi; };
 // busy 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %, three
 // exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 % slower.
 // CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
-template <int HD, int NW, int CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : HD <= 64 && NW == 4 ? 3 : 2)
+// PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
+template <int HD, int NQ, int PARTS, int CAP, bool BIAS>
+__global__ void __launch_bounds__(NQ * PARTS * 64, HD == 256 ? 1 : HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
                        float softcap) {
-  constexpr int KB = HD == 256 ? 32 : 64, CH = HD / 8, KS = HD / 16, ND = HD / 32;
+  constexpr int NW = NQ * PARTS, KB = HD == 256 ? 32 : 64, CH = HD / 8, KS = HD / 16, ND = HD / 32;
   constexpr int TILE = KB * CH;                              // 16-byte pieces
   extern __shared__ u32x4_t lds[];                               // two tiles of keys, two of values
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
   // neighbouring workgroups go to the eight XCDs in turn: the query heads of a key head to one of them, whose L2 then holds its keys and values
   const int hx = blockIdx.x % heads, h = heads % 8 ? hx : hx % 8 * (heads / 8) + hx / 8, hk = h / (heads / kvh);
   int at, len, first;
-  const bool many = gridDim.x * NW > PACKED_WAVES;
-  packed_tile(cu, seqs, rows, NW * 32, blockIdx.x / heads, gridDim.x / heads, many, &at, &len, &first);
+  packed_tile(cu, seqs, rows, NQ * 32, blockIdx.x / heads, gridDim.x / heads, gridDim.x * NW > PACKED_WAVES, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int qs = first + w * 32, qi = qs + c;                    // the wave's first query, this lane's
+  const int part = PARTS == 1 ? 0 : w / NQ, wq = PARTS == 1 ? w : w % NQ, qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
   const int64_t k_row = k.row, v_row = v.row;
   const bf16_t* kb = (const bf16_t*)k.p + at * k_row + hk * k.head;
@@ -273,7 +273,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   for (int r = 0; r < 16; ++r) bias[r] = BIAS ? slope * (float)((r & 3) + 8 * (r >> 2) + 4 * hi) / (CAP ? 1.f : scale) : 0.f;
   float m = -INFINITY, l = 0.f;
 
-  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NW * 32 - 1);
+  const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NQ * 32 - 1);
   // A tile's rows through a buffer descriptor: what lies behind the sequence's last row reads as zeros
   constexpr int NT = NW * 64, PR = (TILE + NT - 1) / NT, STEP = NT / CH;      // 16-byte pieces of a tile to a thread, rows between them
   u32x4_t kr[PR], vr[PR];
@@ -402,10 +402,9 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     }
   };
   // With ALiBi the largest scores are a query's latest keys': from those backwards the maximum settles at once (two documents of 8192, 16 heads of 128, 719 us, 785
-  // forwards; 16383 rows of 16 heads of 128 under a window of 1024 218 and 229).  Without it forwards, where the workgroups of a document read the same keys at the
-  // same time (two of 4096, 8 heads of 256, 287 us, 297 backwards), and where all the call's workgroups run at once (8 prompts, 4096 rows of 12 heads of 64, 23.5 and 24.5).
-  const bool back = BIAS && many;
-  const int b_first = back ? k_last / KB * KB : k_first, b_step = back ? -KB : KB;
+  // forwards; 16383 rows of 16 heads of 128 under a window of 1024 218 and 229; 512 rows of 12 heads of 64 10.6 and 11.0).  Without it forwards, where the workgroups of a
+  // document read the same keys at the same time (two of 4096, 8 heads of 256, 287 us, 297 backwards).
+  const int b_first = BIAS ? k_last / KB * KB : k_first, b_step = BIAS ? -KB : KB;
   int left = (k_last - k_first) / KB;                            // tiles after this one: k_first is a multiple of KB
   fetch(b_first);
   // the queries are waited for here: left to their first use in the loop, that wait would be one for the loop's own requests too
@@ -418,16 +417,17 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     __syncthreads();                                             // this tile is there, and the one before it has been read
     if (left > 0) store(buf ^ 1);
     if (left > 1) fetch(b + 2 * b_step);
-    if (!on || b > qs + 31 || b + KB - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
+    if (PARTS == 2) b += 32 * part;
+    if (!on || b > qs + 31 || b + KB / PARTS - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
     const float base = slope * (float)(b - qi);
-    const Keys k0 = get_keys(buf, 0);
+    const Keys k0 = get_keys(buf, part);
     __builtin_amdgcn_sched_barrier(0);                           // all of them asked for before the first product waits for one
-    if constexpr (KB == 32) {
+    if constexpr (KB / PARTS == 32) {
       floatx16_t s0 = scores(k0);
       shape(s0, b);
       weigh(s0, base);
       settle(s0, base);
-      add_values(get_values(buf, 0));
+      add_values(get_values(buf, part));
       return;
     }
     const float base1 = base + slope * 32.f;
@@ -451,8 +451,30 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     tile(b + b_step, std::integral_constant<int, 1>{});
     if (--left < 0) break;
   }
-  if (!on) return;
   l += __shfl_xor(l, 32, FSTU_WAVE);
+  if constexpr (PARTS == 2) {
+    constexpr int EACH = ND * 16 + 2;
+    float* const theirs = (float*)lds + wq * EACH * 64 + lane;
+    __syncthreads();
+    if (part) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) theirs[(d * 16 + r) * 64] = o[d][r];
+      theirs[(EACH - 2) * 64] = m;
+      theirs[(EACH - 1) * 64] = l;
+    }
+    __syncthreads();
+    if (part) return;
+    const float other = theirs[(EACH - 2) * 64], mn = fmaxf(m, other), off = mn == -INFINITY ? 0.f : mn;
+    const float mf = __builtin_amdgcn_exp2f(m - off), of = __builtin_amdgcn_exp2f(other - off);
+    l = fmaf(l, mf, theirs[(EACH - 1) * 64] * of);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], mf, theirs[(d * 16 + r) * 64] * of);
+  }
+  if (!on) return;
   const float inv = 1.0f / l;
   bool fine = true;
 #pragma unroll
@@ -516,25 +538,32 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
       softcap > 0.f ? go(swa_packed_f32_kernel<HD, 4, true>) : go(swa_packed_f32_kernel<HD, 4, false>);
       return;
     }
-    auto bf16 = [&](auto nw) {
-      constexpr int NW = decltype(nw)::value;
+    auto bf16 = [&](auto nq, auto parts) {
+      constexpr int NQ = decltype(nq)::value, PARTS = decltype(parts)::value;
       auto go = [&](auto kernel) {
         constexpr unsigned lds = 4 * (HD == 256 ? 32 : 64) * HD * 2;       // two tiles of keys, two of values
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NW * 32) + seqs) * heads), dim3(NW * 64), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes,
-                           rows, seqs, heads, kvh, window, softcap);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NQ * 32) + seqs) * heads), dim3(NQ * PARTS * 64), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu,
+                           slopes, rows, seqs, heads, kvh, window, softcap);
       };
-      if (softcap > FSTU_FAST_CAP) slopes ? go(swa_packed_mfma_kernel<HD, 4, 2, true>) : go(swa_packed_mfma_kernel<HD, 4, 2, false>);
-      else if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NW, 1, true>) : go(swa_packed_mfma_kernel<HD, NW, 1, false>);
-      else slopes ? go(swa_packed_mfma_kernel<HD, NW, 0, true>) : go(swa_packed_mfma_kernel<HD, NW, 0, false>);
+      if (softcap > FSTU_FAST_CAP) slopes ? go(swa_packed_mfma_kernel<HD, 4, 1, 2, true>) : go(swa_packed_mfma_kernel<HD, 4, 1, 2, false>);
+      else if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NQ, PARTS, 1, true>) : go(swa_packed_mfma_kernel<HD, NQ, PARTS, 1, false>);
+      else slopes ? go(swa_packed_mfma_kernel<HD, NQ, PARTS, 0, true>) : go(swa_packed_mfma_kernel<HD, NQ, PARTS, 0, false>);
     };
-    // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 720 us,
-    // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238), two where there are few (4096 rows of 12 heads of 64, window 512, 25 and 30; heads of
-    // 128 do not fit their tiles' share into registers then).
-    // Soft-caps of no ordinary size have the kernel of four waves alone.
-    if (softcap > FSTU_FAST_CAP) bf16(std::integral_constant<int, 4>{});
-    else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(std::integral_constant<int, HD == 128 ? 8 : 4>{});
-    else if (HD <= 64 && (int64_t)(rows / 128) * heads < 768) bf16(std::integral_constant<int, HD <= 64 ? 2 : 4>{});
-    else bf16(std::integral_constant<int, 4>{});
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 4> Four;
+    typedef std::integral_constant<int, HD == 128 ? 8 : 4> Eight;
+    typedef std::integral_constant<int, HD == 256 ? 4 : 2> Pair;
+    typedef std::integral_constant<int, HD == 256 ? 1 : 2> Halves;
+    // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 710 us,
+    // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them: two waves of queries, each
+    // with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7, 4096 27.5 / 19.1, 12288 50.5 / 48.2, one
+    // document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71.
+    // Partners for quarters of the keys: 512 rows of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the
+    // kernel of four waves alone.
+    if (softcap > FSTU_FAST_CAP) bf16(Four{}, One{});
+    else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(Eight{}, One{});
+    else if (HD <= 128 && (int64_t)(rows / 128) * heads < (HD == 128 ? 576 : 768)) bf16(Pair{}, Halves{});
+    else bf16(Four{}, One{});
   };
   if (hd == 32) run(std::integral_constant<int, 32>{});
   else if (hd == 64) run(std::integral_constant<int, 64>{});

@@ -74,6 +74,12 @@ def test_packed(fs, heads, kvh, hd, lengths, window, softcap, alibi, dtype):
     (32, 32, 128, [0, 900, 1100, 0], None, 0.0, False),
     (64, 8, 256, [520, 300, 1], 200, 0.0, True),
     (64, 64, 64, [65] * 64, None, 0.0, True),
+    (128, 16, 32, [33, 2] * 35 + [80], 50, 50.0, True),
+    (128, 16, 32, [700, 130], None, 0.0, False),
+    (48, 3, 128, [700, 1500, 90], None, 50.0, True),
+    (64, 64, 128, [0, 900, 1100, 0], 333, 0.0, True),
+    (64, 8, 128, [1300, 33], None, 0.0, False),
+    (64, 8, 64, [1700, 33], 1000, 30.0, False),
 ])
 def test_more_workgroups_than_the_card_holds(fs, heads, kvh, hd, lengths, window, softcap, alibi, dtype):
     (q, k, v), dev = fused(17, sum(lengths), heads, kvh, hd, dtype)
@@ -83,6 +89,19 @@ def test_more_workgroups_than_the_card_holds(fs, heads, kvh, hd, lengths, window
     kv = h // (heads // kvh)
     check(y.cpu()[:, h], *packed(q[:, h], k[:, kv], v[:, kv], lengths, slopes[h] if alibi else None, window, softcap, P_STEP[dtype]), dtype)
     assert bool(torch.isfinite(y).all())
+
+
+@pytest.mark.parametrize("lengths,window,softcap,alibi", [
+    ([4500], None, 0.0, False),
+    ([4500], None, 50.0, False),
+    ([4131], 4100, 0.0, True),
+    ([8190, 33], 4096, 50.0, True),
+])
+def test_documents_of_many_thousands(fs, lengths, window, softcap, alibi):
+    (q, k, v), dev = fused(23, sum(lengths), 2, 1, 128, torch.bfloat16)
+    y = fs.swa_packed(*dev, bounds(lengths), slopes=slopes_of(2).cuda() if alibi else None, window=window, softcap=softcap)
+    one = slice(1, 2)
+    check(y[:, one], *packed(q[:, one], k, v, lengths, slopes_of(2)[one] if alibi else None, window, softcap, P_STEP[torch.bfloat16]), torch.bfloat16)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
