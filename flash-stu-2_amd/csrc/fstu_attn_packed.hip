@@ -109,11 +109,13 @@ typedef float floatx4_t __attribute__((ext_vector_type(4)));
 // fp32: v_mfma_f32_16x16x4_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
 // A workgroup takes 16 queries of one head; its waves take 32 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
 // first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 16 t + 4 g + r.
-// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / so: 777 rows of 4 x 64 under a window of 129 12.7 / 13.1 / 9.8, 4096 of 8 x 64 under 512 267 / 76 / 74.
+// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / these / with values asked for before the products and a lane's dims beside each other: 777 rows of
+// 4 x 64 under a window of 129 12.7 / 13.1 / 9.8 / 9.2, 4096 of 8 x 64 under 512 267 / 76 / 74 / 65 (the L2's reads of keys and values, once for each 16 queries).
 template <int HD, int NW, bool CAP>
 __global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : 2)
 swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
   constexpr int ND = HD / 16, PART = HD / 4;
+  typedef float Dims __attribute__((ext_vector_type(ND)));         // a lane's dims of a value: ND c ..
   __shared__ float sm[NW][16], sl[NW][16], so[16][HD + 1];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % heads, hk = h / (heads / kvh);
@@ -139,18 +141,24 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
   for (int d = 0; d < ND; ++d) o[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   for (int b = max(0, first - window) / 32 * 32 + 32 * w; b <= last; b += 32 * NW) {
-    floatx4_t s[2];
+    // all of the step's keys and values before the first product; rows behind the sequence: its last one, which no query of these sees
+    floatx4_t s[2], kf[2][PART / 4];
+    Dims vf[8];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-      const float* kr = kb + min(b + 16 * t + c, len - 1) * k_row + g * PART;            // rows behind the sequence: its last one, which no query of these sees
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int x = 0; x < PART / 4; ++x) {
-        const floatx4_t f = *(const floatx4_t*)(kr + 4 * x);
+      for (int x = 0; x < PART / 4; ++x) kf[t][x] = *(const floatx4_t*)(kb + min(b + 16 * t + c, len - 1) * k_row + g * PART + 4 * x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[e], qf[x][e], s[t], 0, 0, 0);
-      }
-    }
+    for (int e = 0; e < 8; ++e) vf[e] = *(const Dims*)(vb + min(b + 16 * (e >> 2) + 4 * g + (e & 3), len - 1) * v_row + c * ND);
+    if (HD == 128) __builtin_amdgcn_sched_barrier(0);          // 4096 rows of 8 heads 129 us, 138 without; heads of 64 and 256 66 and 159, 65 and 140 without
+#pragma unroll
+    for (int t = 0; t < 2; ++t) s[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < PART / 4; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[t][x][e], qf[x][e], s[t], 0, 0, 0);
     float top = -INFINITY, y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3] * scale;
@@ -176,9 +184,8 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
     for (int e = 0; e < 8; ++e) {
       const float p = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - off);
       l += p;
-      const float* vr = vb + min(b + 16 * (e >> 2) + 4 * g + (e & 3), len - 1) * v_row + c;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[16 * d], p, o[d], 0, 0, 0);
+      for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d], p, o[d], 0, 0, 0);
     }
   }
   l += fstu_swz16(l);
@@ -196,7 +203,7 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float& sum = so[c][d * 16 + 4 * g + r];
+          float& sum = so[c][(4 * g + r) * ND + d];
           sum = fmaf(o[d][r], mine, n ? sum : 0.f);
         }
     }
