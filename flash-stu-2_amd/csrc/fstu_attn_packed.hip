@@ -227,6 +227,8 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
   }
 }
 
+constexpr int packed_dims(int hd) { return hd == 256 ? 2 : 1; }             // waves that share a query's dims
+
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 struct Frag8 { u32x2_t lo, hi; };
@@ -241,12 +243,14 @@ struct Frag8 { u32x2_t lo, hi; };
 // busy 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %, three
 // exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 % slower.
 // CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
-// PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
+// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128 (two documents
+// of 4096 and 8 heads 292 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 33 and 37; the next tile's first product beside this one's softmax 281 and 34,
+// but with ALiBi, which spills then, 310 instead of 280).  PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
 template <int HD, int NQ, int PARTS, int CAP, bool BIAS>
-__global__ void __launch_bounds__(NQ * PARTS * 64, HD == 256 ? 1 : HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
+__global__ void __launch_bounds__(NQ * PARTS * packed_dims(HD) * 64, HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
                        float softcap) {
-  constexpr int NW = NQ * PARTS, KB = HD == 256 ? 32 : 64, CH = HD / 8, KS = HD / 16, ND = HD / 32;
+  constexpr int DIMS = packed_dims(HD), NW = NQ * PARTS * DIMS, KB = HD == 256 ? 32 : 64, CH = HD / 8, KS = HD / 16 / DIMS, ND = HD / 32 / DIMS;
   constexpr int TILE = KB * CH;                              // 16-byte pieces
   extern __shared__ u32x4_t lds[];                               // two tiles of keys, two of values
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 31, hi = lane >> 5;
@@ -255,7 +259,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   int at, len, first;
   packed_tile(cu, seqs, rows, NQ * 32, blockIdx.x / heads, gridDim.x / heads, gridDim.x * NW > PACKED_WAVES, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int part = PARTS == 1 ? 0 : w / NQ, wq = PARTS == 1 ? w : w % NQ, qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
+  const int part = PARTS == 1 ? 0 : w / NQ, share = DIMS == 1 ? 0 : w / NQ, wq = w - (part + share) * NQ, qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
   const int64_t k_row = k.row, v_row = v.row;
   const bf16_t* kb = (const bf16_t*)k.p + at * k_row + hk * k.head;
@@ -265,7 +269,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
 
   u32x4_t qf[KS];
   {
-    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + hi * 8;
+    const bf16_t* qr = (const bf16_t*)q.p + (at + min(qi, len - 1)) * q.row + h * q.head + share * (HD / 2) + hi * 8;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *(const u32x4_t*)(qr + s * 16);
   }
@@ -277,7 +281,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   // ALiBi of a half's key: without a soft-cap what the scores' sums begin with, in units of theirs
   floatx16_t bias;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) bias[r] = BIAS ? slope * (float)((r & 3) + 8 * (r >> 2) + 4 * hi) / (CAP ? 1.f : scale) : 0.f;
+  for (int r = 0; r < 16; ++r) bias[r] = BIAS ? slope * (float)((r & 3) + 8 * (r >> 2) + 4 * hi) / (CAP ? 1.f : scale * DIMS) : 0.f;
   float m = -INFINITY, l = 0.f;
 
   const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NQ * 32 - 1);
@@ -314,9 +318,9 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     const int ksw = HD >= 128 ? c & 15 : HD == 64 ? (c >> 1) & 7 : (c >> 2) & 3;
     const int li = lane & 15, vx = HD >= 128 ? (li >> 2) & 3 : HD == 64 ? (li >> 3) & 1 : 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_at[s] = c * CH + ((2 * s + hi) ^ ksw);
+    for (int s = 0; s < KS; ++s) k_at[s] = c * CH + ((2 * (s + share * KS) + hi) ^ ksw);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) v_at[d] = (4 * hi + (li >> 2)) * HD + 16 * (lane >> 4 & 1) + 4 * (li & 3) + (d ^ vx) * 32;
+    for (int d = 0; d < ND; ++d) v_at[d] = (4 * hi + (li >> 2)) * HD + 16 * (lane >> 4 & 1) + 4 * (li & 3) + ((d + share * ND) ^ vx) * 32;
   }
   const float kk = CAP ? 1.f : scale;
   unsigned pk[8];
@@ -425,8 +429,32 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     if (left > 0) store(buf ^ 1);
     if (left > 1) fetch(b + 2 * b_step);
     if (PARTS == 2) b += 32 * part;
-    if (!on || b > qs + 31 || b + KB / PARTS - 1 < qs - window) return;  // wave-uniform: the wave sees none of it
+    const bool seen = on && b <= qs + 31 && b + KB / PARTS - 1 >= qs - window;      // wave-uniform: the wave sees some of it
     const float base = slope * (float)(b - qi);
+    if constexpr (DIMS == 2) {
+      floatx4_t* const across = (floatx4_t*)(lds + 4 * TILE) + lane;               // 16 values a lane, of each wave
+      floatx16_t s0;
+      if (seen) {
+        s0 = scores(get_keys(buf, 0));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) across[(w * 4 + r) * 64] = floatx4_t{s0[4 * r], s0[4 * r + 1], s0[4 * r + 2], s0[4 * r + 3]};
+      }
+      __syncthreads();
+      if (!seen) return;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const floatx4_t x = across[((w ^ NQ) * 4 + r) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s0[4 * r + e] += x[e];
+      }
+      shape(s0, b);
+      const Values v0 = get_values(buf, 0);
+      weigh(s0, base);
+      settle(s0, base);
+      add_values(v0);
+      return;
+    }
+    if (!seen) return;
     const Keys k0 = get_keys(buf, part);
     __builtin_amdgcn_sched_barrier(0);                           // all of them asked for before the first product waits for one
     if constexpr (KB / PARTS == 32) {
@@ -481,7 +509,6 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = fmaf(o[d][r], mf, theirs[(d * 16 + r) * 64] * of);
   }
-  if (!on) return;
   const float inv = 1.0f / l;
   bool fine = true;
 #pragma unroll
@@ -491,19 +518,28 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
       o[d][r] *= inv;
       fine = fine && o[d][r] == o[d][r];
     }
-  if (qi < len) {
-    bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + 4 * hi;
+  // A NaN comes from a row's own scores and values, or from a value that it does not see (0 * infinity): a wave forms such rows once more, key by key.
+  unsigned long long both = __ballot(!fine && qi < len);
+  unsigned bad = (unsigned)both | (unsigned)(both >> 32);
+  if constexpr (DIMS == 2) {
+    unsigned* const rows_of = (unsigned*)(lds + 4 * TILE);
+    __syncthreads();
+    if (lane == 0) rows_of[w] = bad;
+    __syncthreads();
+    bad |= rows_of[w ^ NQ];
+  }
+  if (!on) return;
+  if (qi < len && !(bad >> c & 1)) {
+    bf16_t* orow = out + ((int64_t)(at + qi) * heads + h) * HD + share * (HD / 2) + 4 * hi;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         *(uint2*)(orow + d * 32 + e * 8) = make_uint2(pack2_bf16(o[d][4 * e], o[d][4 * e + 1]), pack2_bf16(o[d][4 * e + 2], o[d][4 * e + 3]));
   }
-  // A NaN comes from a row's own scores and values, or from a value that it does not see (0 * infinity): the wave forms such rows once more, key by key.
-  unsigned long long bad = __ballot(!fine && qi < len);
-  bad = (bad | bad >> 32) & 0xffffffffull;
+  if (share) return;
   while (bad) {
-    const int i = qs + __builtin_ctzll(bad);
+    const int i = qs + __builtin_ctz(bad);
     bad &= bad - 1;
     packed_one<bf16_t, HD>((const bf16_t*)q.p + (at + i) * q.row + h * q.head, kb, vb, out + ((int64_t)(at + i) * heads + h) * HD, k_row, v_row, i, window,
                            raw_slope, softcap);
@@ -527,13 +563,14 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
                    fstu_aligned(out, 16),
                FSTU_EALIGN, "fstu_swa_packed: rows and heads of q, k and v and out must begin at multiples of 16 bytes");
   FSTU_REQUIRE(rows == 0 || (k_row < (1 << 23) && v_row < (1 << 23)), FSTU_ESHAPE, "fstu_swa_packed: rows of k and v 2^23 elements apart and more");
-  // fp32: 16 threads a row; bf16: 2; up to 512 more a sequence
-  FSTU_REQUIRE(((int64_t)rows * (dtype == FSTU_F32 ? 16 : 2) + (int64_t)seqs * 512) * heads < 1ll << 32, FSTU_ESHAPE, "fstu_swa_packed: %d rows of %d sequences and %d heads are more than a launch takes", rows, seqs, heads);
+  // fp32: 16 threads a row; bf16: 2 or 4; up to 512 more a sequence
+  FSTU_REQUIRE(((int64_t)rows * (dtype == FSTU_F32 ? 16 : hd == 256 ? 4 : 2) + (int64_t)seqs * 512) * heads < 1ll << 32, FSTU_ESHAPE, "fstu_swa_packed: %d rows of %d sequences and %d heads are more than a launch takes", rows, seqs, heads);
   const int64_t n = (int64_t)rows * heads * hd * size;
   FSTU_REQUIRE(!fstu_heads_touch(q, q_row, q_head, rows, heads, hd, size, out, n) && !fstu_heads_touch(k, k_row, k_head, rows, kvh, hd, size, out, n) &&
                    !fstu_heads_touch(v, v_row, v_head, rows, kvh, hd, size, out, n),
                FSTU_EARG, "fstu_swa_packed: out overlaps q, k or v");
   if (rows == 0 || seqs == 0) return FSTU_OK;
+  int rc = FSTU_OK;
   const Heads hq{q, q_row, q_head}, hk{k, k_row, k_head}, hv{v, v_row, v_head};
   auto run = [&](auto w) {
     constexpr int HD = decltype(w)::value;
@@ -547,14 +584,22 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
     }
     auto bf16 = [&](auto nq, auto parts) {
       constexpr int NQ = decltype(nq)::value, PARTS = decltype(parts)::value;
-      auto go = [&](auto kernel) {
-        constexpr unsigned lds = 4 * (HD == 256 ? 32 : 64) * HD * 2;       // two tiles of keys, two of values
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NQ * 32) + seqs) * heads), dim3(NQ * PARTS * 64), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu,
-                           slopes, rows, seqs, heads, kvh, window, softcap);
+      auto go = [&](auto cap, auto bias) {
+        constexpr unsigned threads = NQ * PARTS * packed_dims(HD) * 64, lds = 4 * (HD == 256 ? 32 : 64) * HD * 2 + (HD == 256 ? threads * 64 : 0);
+        const auto kernel = swa_packed_mfma_kernel<HD, NQ, PARTS, decltype(cap)::value, decltype(bias)::value>;
+        if constexpr (lds > 65536) {
+          static fstu_lds_limit most;
+          rc = fstu_need_lds((const void*)kernel, most, lds, "fstu_swa_packed");
+          if (rc != FSTU_OK) return;
+        }
+        // two tiles of keys and two of values; with heads of 256 the scores' sums besides, 16 a thread
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NQ * 32) + seqs) * heads), dim3(threads), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes, rows,
+                           seqs, heads, kvh, window, softcap);
       };
-      if (softcap > FSTU_FAST_CAP) slopes ? go(swa_packed_mfma_kernel<HD, 4, 1, 2, true>) : go(swa_packed_mfma_kernel<HD, 4, 1, 2, false>);
-      else if (softcap > 0.f) slopes ? go(swa_packed_mfma_kernel<HD, NQ, PARTS, 1, true>) : go(swa_packed_mfma_kernel<HD, NQ, PARTS, 1, false>);
-      else slopes ? go(swa_packed_mfma_kernel<HD, NQ, PARTS, 0, true>) : go(swa_packed_mfma_kernel<HD, NQ, PARTS, 0, false>);
+      auto capped = [&](auto cap) { slopes ? go(cap, std::true_type{}) : go(cap, std::false_type{}); };
+      if constexpr (NQ == 4 && PARTS == 1)
+        if (softcap > FSTU_FAST_CAP) return capped(std::integral_constant<int, 2>{});
+      softcap > 0.f ? capped(std::integral_constant<int, 1>{}) : capped(std::integral_constant<int, 0>{});
     };
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 4> Four;
@@ -576,6 +621,7 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   else if (hd == 64) run(std::integral_constant<int, 64>{});
   else if (hd == 128) run(std::integral_constant<int, 128>{});
   else run(std::integral_constant<int, 256>{});
+  if (rc != FSTU_OK) return rc;
   FSTU_CHECK_LAUNCH("fstu_swa_packed");
   return FSTU_OK;
 }

@@ -359,7 +359,7 @@ int fstu_swa_prefill_mfma(const void* qkv, void* vt_ws, void* out, const float* 
  * sees its rows max(0,i-window) .. i.  q (rows,heads,hd), k and v (rows,kvh,hd) by row and head strides in elements (multiples of 16 bytes),
  * query head h reads key head h / (heads/kvh); out (rows,heads,hd) dense, not overlapping the others.  Scores as above, slopes (heads) or NULL,
  * softcap 0: none, else 2^-40..2^40.  Rows of no sequence are left as they were.  Refused: k and v rows 2^23 elements apart and more, and
- * (rows * (fp32 ? 16 : 2) + 512 seqs) * heads from 2^32 on. */
+ * (16 rows + 512 seqs) * heads (bf16: 2 rows, 4 at hd 256) from 2^32 on. */
 int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                     int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
                     float softcap, int dtype, void* stream);
