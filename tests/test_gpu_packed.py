@@ -133,6 +133,33 @@ def test_what_a_row_does_not_see_may_be_anything(fs, hd, window, dtype):
         assert bool(torch.isnan(y[r, n % 2]).any()) and not bool(torch.isfinite(y[r, 1 - n % 2, n::7]).any())
 
 
+@pytest.mark.parametrize("hd,heads,lengths,window,softcap,alibi", [
+    (32, 128, [400, 500, 130], None, 0.0, True),
+    (64, 128, [400, 500, 130], 90, 50.0, True),
+    (64, 128, [400, 500, 130], None, 0.0, False),
+    (128, 128, [400, 500, 130], 90, 0.0, True),
+    (128, 128, [400, 500, 130], None, 50.0, False),
+    (256, 32, [400, 500, 130], 90, 50.0, True),
+    (128, 2, [4200], None, 0.0, True),
+])
+def test_what_a_row_does_not_see_may_be_anything_in_large_calls(fs, hd, heads, lengths, window, softcap, alibi):
+    rows, dtype, slopes = sum(lengths), torch.bfloat16, slopes_of(heads)
+    q, k, v = rand(0, rows, heads, hd, dtype=dtype), rand(1, rows, 2, hd, dtype=dtype), rand(2, rows, 2, hd, dtype=dtype)
+    start = [sum(lengths[:i]) for i, n in enumerate(lengths) for _ in range(n)]
+    bad = [r for r in (rows - 7, 300, 399, 520, 521, 899) if window or r > rows - 10 or start[r] + 350 < r]
+    k[bad[0], 0], v[bad[0], 1, 3::5] = math.nan, math.inf
+    for n, r in enumerate(bad):
+        k[r, n % 2], v[r, 1 - n % 2, n::7] = math.nan, (math.inf, -math.inf, math.nan)[n % 3]
+    h = torch.tensor([0, heads - 1])
+    y = fs.swa_packed(q.cuda(), k.cuda(), v.cuda(), bounds(lengths), slopes=slopes.cuda() if alibi else None, window=window, softcap=softcap).cpu()[:, h]
+    o, bound = packed(q[:, h], k.nan_to_num(0.0, 0.0, 0.0), v.nan_to_num(0.0, 0.0, 0.0), lengths, slopes[h] if alibi else None, window, softcap, P_STEP[dtype])
+    clean = torch.tensor([not any(start[r] <= b <= r and (window is None or r - b <= window) for b in bad) for r in range(rows)])
+    assert int(clean.sum()) >= 300
+    check(y[clean], o[clean], bound[clean], dtype)
+    for n, r in enumerate(bad):
+        assert bool(torch.isnan(y[r, n % 2]).all()) and not bool(torch.isfinite(y[r, 1 - n % 2, n::7]).any())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("softcap", [2.0 ** -40, 0.01, 1.0, 511.0, 513.0, 1e5, 2.0 ** 40])
 def test_under_any_soft_cap(fs, softcap, dtype):
