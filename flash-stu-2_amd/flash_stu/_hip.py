@@ -82,6 +82,7 @@ SIGNATURES = {
     "fstu_kv4_write": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "fstu_kv4_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "fstu_kv4_step": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "fstu_kv4_attend_splits": [_i, _i, _i, _i, _i, _i],
     "fstu_kv4_attend_ws": [_i, _i, _i, _i, _i],
     "fstu_sample": [_vp, _vp, _i64, _i, _i, _f, _i, _f, _i, _u64, _i, _i, _vp],
@@ -1570,7 +1571,7 @@ def swa_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: to
     else:
         _written(out)
     if rows:
-        rc = load().fstu_swa_packed(q.data_ptr(), qr if rows > 1 else 0, qh, k.data_ptr(), kr if rows > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(),
+        rc = load().fstu_swa_packed(q.data_ptr(), qr if rows > 1 else 0, qh if heads > 1 else 0, k.data_ptr(), kr if rows > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(),
                                     vr if rows > 1 else 0, vh if kvh > 1 else 0, out.data_ptr(), cu_seqlens.data_ptr(), None if slopes is None else slopes.data_ptr(),
                                     rows, seqs, heads, kvh, hd, 0x7fffffff if window is None or window > 0x7fffffff else window, softcap or 0.0, dt, raw_stream(dev))
         if rc:
@@ -1670,15 +1671,30 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tens
         out = _empty(shape, dtype=dtype, device=data.device)
     else:
         _written(out)
+    one_call = False
     if k is not None or v is not None:
         if k is None or v is None:
             raise FlashSTUHipError("KV4Cache.attend: k and v go together")
-        kv4_write(cache, k, v, pos)
+        if (k.requires_grad or v.requires_grad) and _grad_on():
+            raise _fp8_forward_only("KV4Cache.attend")
+        one_call = (k.dtype is dtype and v.dtype is dtype and k.shape == v.shape == (seqs, kvh, hd) and k.get_device() == v.get_device() == dev
+                    and k.stride(2) == v.stride(2) == 1)
+        if not one_call:                                         # of another type than q, or nothing that can be written
+            kv4_write(cache, k, v, pos)
     splits, floats = _kv4_splits(seqs, heads, kvh, hd, cap, window)
     ws = _empty(floats, dtype=_f32, device=data.device).data_ptr() if floats else None      # its memory is this stream's until what runs on it next
     qr, qh, _ = q.stride()
-    rc = load().fstu_kv4_attend(q.data_ptr(), qr if seqs > 1 else 0, qh if heads > 1 else 0, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(),
-                                None if slopes is None else slopes.data_ptr(), seqs, heads, kvh, hd, cap, window, softcap or 0.0, dt, raw_stream(dev))
+    lib, stream = load(), raw_stream(dev)
+    qr, qh = qr if seqs > 1 else 0, qh if heads > 1 else 0
+    slopes_at = None if slopes is None else slopes.data_ptr()
+    if one_call:
+        (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
+        rc = lib.fstu_kv4_step(q.data_ptr(), qr, qh, k.data_ptr(), kr if seqs > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(), vr if seqs > 1 else 0,
+                               vh if kvh > 1 else 0, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
+                               softcap or 0.0, dt, stream)
+    else:
+        rc = lib.fstu_kv4_attend(q.data_ptr(), qr, qh, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
+                                 softcap or 0.0, dt, stream)
     if rc:
         _check(rc, "fstu_kv4_attend")
     return out

@@ -121,5 +121,6 @@ class KV4Cache:
                softcap: float = 0.0, out: torch.Tensor = None) -> torch.Tensor:
         """One query a sequence, q (batch, heads, head_dim), at position pos[s], over the positions max(0, pos[s] - window) .. pos[s] as the cache holds
         them (window None: capacity - 1); heads a multiple of kv_heads, scores as swa_packed's.  k, v (batch, kv_heads, head_dim): those of position
-        pos[s], written first.  Returns out (batch, heads, head_dim), zero for a sequence not in use; out must not overlap q or the cache."""
+        pos[s], written first (in the same launch but for very long calls, where they are of q's type).  Returns out (batch, heads, head_dim), zero for a
+        sequence not in use; out must not overlap q, k, v or the cache."""
         return _hip.kv4_attend(self, q, pos, k, v, slopes, window, softcap, out)

@@ -196,12 +196,50 @@ def test_attend_under_any_soft_cap(fs, softcap, dtype):
         check(y, *ring.attend(q, [99, 130], None, None, softcap, P_STEP), dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,heads,kvh,hd,cap,window,softcap", [
+    (3, 4, 4, 32, 20, None, 0.0),
+    (2, 22, 2, 64, 513, 512, 50.0),              # 11 query heads to a key head: two workgroups to a head
+    (1, 12, 12, 64, 2500, None, 0.0),            # in parts
+    (1, 34, 2, 128, 1700, None, 50.0),           # both
+    (5, 16, 8, 128, 100, 70, 0.0),
+    (2, 3, 1, 256, 33, 32, 0.0),
+    (2, 8, 8, 256, 1400, 1200, 0.0),
+    (64, 32, 32, 32, 6200, None, 0.0),           # dealt evenly
+    (40, 20, 10, 64, 64, None, 0.0),             # more workgroups than compute units
+])
+def test_a_step_is_its_write_and_its_attend(fs, batch, heads, kvh, hd, cap, window, softcap, dtype):
+    one, two = fs.KV4Cache(batch, kvh, hd, cap), fs.KV4Cache(batch, kvh, hd, cap)
+    n = min(cap, 300)
+    prompt = rand(1, n * batch, 2 * kvh, hd).to(dtype).cuda()
+    cu = ints(range(0, n * batch + 1, n))
+    at = ints([(0, cap - n // 2, 3 * cap + 7)[b % 3] for b in range(batch)])
+    for c in (one, two):
+        c.write(prompt[:, :kvh], prompt[:, kvh:], at, cu)
+    pos = at + n
+    pos[batch // 2 if batch > 1 else 1:][:1] = -1
+    slopes = slopes_of(heads).cuda()
+    for step in range(3):
+        qkv = rand(2 + step, batch, heads + 2 * kvh, hd).to(dtype).cuda()
+        q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
+        y = one.attend(q, pos, k, v, slopes=slopes, window=window, softcap=softcap)
+        two.write(k, v, pos)
+        assert torch.equal(y, two.attend(q, pos, slopes=slopes, window=window, softcap=softcap)) and torch.equal(one.data, two.data)
+        pos = torch.where(pos < 0, pos, pos + (1 if step == 0 else cap // 2 + 1))
+    k = rand(9, batch, kvh, hd).to(torch.bfloat16 if dtype is torch.float32 else torch.float32).cuda()       # of another type than q
+    y = one.attend(q, pos, k, k, slopes=slopes, window=window, softcap=softcap)
+    two.write(k, k, pos)
+    assert torch.equal(y, two.attend(q, pos, slopes=slopes, window=window, softcap=softcap)) and torch.equal(one.data, two.data)
+
+
 def test_a_refused_call_writes_nothing(fs):
     from flash_stu._hip import FlashSTUHipError
     cache = fs.KV4Cache(2, 2, 64, 40)
     k, q, pos = torch.ones(2, 2, 64, device="cuda"), torch.ones(2, 4, 64, device="cuda"), ints([0, 0])
     for call in (lambda: cache.attend(q[:, :3], pos, k, k), lambda: cache.attend(q, pos, k, k, window=40), lambda: cache.attend(q, pos, k, k, softcap=-1.0),
-                 lambda: cache.attend(q, pos, k), lambda: cache.attend(q, pos, k, k, slopes=torch.ones(3, device="cuda")), lambda: cache.attend(q, pos, k, k, out=q[:1])):
+                 lambda: cache.attend(q, pos, k), lambda: cache.attend(q, pos, k, k, slopes=torch.ones(3, device="cuda")), lambda: cache.attend(q, pos, k, k, out=q[:1]),
+                 lambda: cache.attend(q, pos, k, k, out=q), lambda: cache.attend(q, pos, k[:1], k[:1]), lambda: cache.attend(q, pos, k, k[..., :32]),
+                 lambda: cache.attend(q[:, :2], pos, k, k, out=k)):
         with pytest.raises(FlashSTUHipError):
             call()
     assert not cache.data.any()

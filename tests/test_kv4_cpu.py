@@ -64,6 +64,20 @@ def test_cache_entry_points_refuse(lib, mem):
     assert lib.fstu_kv4_attend_splits(1, 8, 8, 64, 1 << 20, (1 << 20) - 1) > 64 and lib.fstu_kv4_attend_ws(1, 9, 1, 64, 256) == (2 + 256) * 8 * 66
 
 
+def test_step_entry_point_refuses(lib, mem):
+    p = mem[0]
+
+    def step(q=p, k=p + 2048, kr=128, kh=64, v=p + 2048, c=p + 8192, out=p + 4096, splits=1, ws=None, window=7, cap=40, dt=1):
+        return lib.fstu_kv4_step(q, 256, 64, k, kr, kh, v, 128, 64, c, out, ws, splits, p, None, 2, 4, 2, 64, cap, window, 0.0, dt, None)
+
+    assert step(k=None) == -1 and step(v=None) == -1 and step(q=None) == -1 and step(c=None) == -1
+    assert step(window=40) == -5 and step(splits=2) == -5 and "fstu_kv4_step" in why(lib)
+    assert step(k=p + 2056) == -4 and step(v=p + 2050) == -4 and step(kr=100) == -4 and step(kh=-64) == -4 and "of k and v" in why(lib)
+    assert step(k=p + 4096) == -5 and step(v=p + 4096 + 512) == -5 and step(k=p + 8192) == -5 and "overlaps k or v" in why(lib)
+    assert step(out=p) == -5 and "overlaps q" in why(lib)
+    assert step(dt=2) == -2
+
+
 def test_packed_entry_point_refuses(lib, mem):
     p = mem[0]
 
