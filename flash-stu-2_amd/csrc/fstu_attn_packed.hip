@@ -107,12 +107,14 @@ __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb,
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 
 // fp32: v_mfma_f32_16x16x4_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
-// A workgroup takes 16 queries of one head; its waves take 32 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
-// first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 16 t + 4 g + r.
-// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / these / with values asked for before the products and a lane's dims beside each other: 777 rows of
-// 4 x 64 under a window of 129 12.7 / 13.1 / 9.8 / 9.2, 4096 of 8 x 64 under 512 267 / 76 / 74 / 65 (the L2's reads of keys and values, once for each 16 queries).
+// A workgroup takes 16 queries of one head; its waves take 16 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
+// first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 4 g + r.
+// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / 16 queries, 32 keys a step / with values asked for before the products and a lane's dims beside each
+// other / 16 keys a step: 777 rows of 4 x 64 under a window of 129 12.7 / 13.1 / 9.8 / 9.3 / 8.7, 4096 of 8 x 64 under 512 267 / 76 / 74 / 65 / 61 (the L2's reads of keys and
+// values, once for each 16 queries), of 8 x 128 - / - / 161 / 129 / 108.  Two workgroups to a compute unit at heads of 256 (251 rows of 50 sequences and 64 heads 74 us, 127 with the
+// registers of one; 2000 rows of 8 heads 145 and 129).
 template <int HD, int NW, bool CAP>
-__global__ void __launch_bounds__(NW * 64, HD == 256 ? 1 : 2)
+__global__ void __launch_bounds__(NW * 64, 2)
 swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
   constexpr int ND = HD / 16, PART = HD / 4;
   typedef float Dims __attribute__((ext_vector_type(ND)));         // a lane's dims of a value: ND c ..
@@ -140,35 +142,29 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  for (int b = max(0, first - window) / 32 * 32 + 32 * w; b <= last; b += 32 * NW) {
+  for (int b = max(0, first - window) / 16 * 16 + 16 * w; b <= last; b += 16 * NW) {
     // all of the step's keys and values before the first product; rows behind the sequence: its last one, which no query of these sees
-    floatx4_t s[2], kf[2][PART / 4];
-    Dims vf[8];
+    floatx4_t s = {0.f, 0.f, 0.f, 0.f}, kf[PART / 4];
+    Dims vf[4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int x = 0; x < PART / 4; ++x) kf[x] = *(const floatx4_t*)(kb + min(b + c, len - 1) * k_row + g * PART + 4 * x);
 #pragma unroll
-      for (int x = 0; x < PART / 4; ++x) kf[t][x] = *(const floatx4_t*)(kb + min(b + 16 * t + c, len - 1) * k_row + g * PART + 4 * x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) vf[e] = *(const Dims*)(vb + min(b + 16 * (e >> 2) + 4 * g + (e & 3), len - 1) * v_row + c * ND);
-    if (HD == 128) __builtin_amdgcn_sched_barrier(0);          // 4096 rows of 8 heads 129 us, 138 without; heads of 64 and 256 66 and 159, 65 and 140 without
-#pragma unroll
-    for (int t = 0; t < 2; ++t) s[t] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 4; ++e) vf[e] = *(const Dims*)(vb + min(b + 4 * g + e, len - 1) * v_row + c * ND);
+    if (HD < 256) __builtin_amdgcn_sched_barrier(0);           // 4096 rows of 8 heads of 128 108 us, 142 without; 2000 rows of 8 of 256 158 and 146
 #pragma unroll
     for (int x = 0; x < PART / 4; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x][e], qf[x][e], s, 0, 0, 0);
+    float top = -INFINITY, y[4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[t][x][e], qf[x][e], s[t], 0, 0, 0);
-    float top = -INFINITY, y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = s[e >> 2][e & 3] * scale;
+    for (int e = 0; e < 4; ++e) y[e] = s[e] * scale;
     if (CAP) fstu_tanh(y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int far = qi - b - (16 * (e >> 2) + 4 * g + (e & 3));
+    for (int e = 0; e < 4; ++e) {
+      const int far = qi - b - (4 * g + e);
       const float x = (CAP ? capA * y[e] : y[e]) - slope * (float)far;
-      s[e >> 2][e & 3] = far >= 0 && far <= window ? x : -INFINITY;
-      top = fmaxf(top, s[e >> 2][e & 3]);
+      s[e] = far >= 0 && far <= window ? x : -INFINITY;
+      top = fmaxf(top, s[e]);
     }
     top = fmaxf(top, fstu_swz16(top));
     top = fmaxf(top, __shfl_xor(top, 32, FSTU_WAVE));
@@ -181,8 +177,8 @@ swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, cons
     }
     const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - off);
+    for (int e = 0; e < 4; ++e) {
+      const float p = __builtin_amdgcn_exp2f(s[e] - off);
       l += p;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[e][d], p, o[d], 0, 0, 0);
@@ -243,9 +239,10 @@ struct Frag8 { u32x2_t lo, hi; };
 // busy 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %, three
 // exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 % slower.
 // CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
-// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128 (two documents
-// of 4096 and 8 heads 292 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 33 and 37; the next tile's first product beside this one's softmax 281 and 34,
-// but with ALiBi, which spills then, 310 instead of 280).  PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
+// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128.  Two documents
+// of 4096 and 8 heads 253 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 8 heads with ALiBi 39 and 47 with 128 queries a workgroup instead of 64,
+// which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi (a tenth slower).
+// PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
 template <int HD, int NQ, int PARTS, int CAP, bool BIAS>
 __global__ void __launch_bounds__(NQ * PARTS * packed_dims(HD) * 64, HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
@@ -597,20 +594,20 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
                            seqs, heads, kvh, window, softcap);
       };
       auto capped = [&](auto cap) { slopes ? go(cap, std::true_type{}) : go(cap, std::false_type{}); };
-      if constexpr (NQ == 4 && PARTS == 1)
+      if constexpr (NQ == (HD == 256 ? 2 : 4) && PARTS == 1)
         if (softcap > FSTU_FAST_CAP) return capped(std::integral_constant<int, 2>{});
       softcap > 0.f ? capped(std::integral_constant<int, 1>{}) : capped(std::integral_constant<int, 0>{});
     };
     typedef std::integral_constant<int, 1> One;
-    typedef std::integral_constant<int, 4> Four;
-    typedef std::integral_constant<int, HD == 128 ? 8 : 4> Eight;
-    typedef std::integral_constant<int, HD == 256 ? 4 : 2> Pair;
+    typedef std::integral_constant<int, HD == 256 ? 2 : 4> Four;
+    typedef std::integral_constant<int, HD == 128 ? 8 : 2> Eight;
+    typedef std::integral_constant<int, 2> Pair;
     typedef std::integral_constant<int, HD == 256 ? 1 : 2> Halves;
     // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 710 us,
     // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them: two waves of queries, each
     // with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7, 4096 27.5 / 19.1, 12288 50.5 / 48.2, one
     // document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71.
-    // Partners for quarters of the keys: 512 rows of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the
+    // Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the
     // kernel of four waves alone.
     if (softcap > FSTU_FAST_CAP) bf16(Four{}, One{});
     else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(Eight{}, One{});
