@@ -15,10 +15,11 @@ struct Heads {                 // rows of heads: strides in elements
 };
 
 // The tile of `per` rows that workgroup t of a head takes: its sequence's first row and length and the tile's first row there (behind the sequence: none).
-// Where a call fills the card more than once (many), the tiles of the highest number within their sequences come first: they have the most keys to walk, and the short
-// ones fill the gaps of the last round.  A sequence's tiles behind another's: two documents of 4096 and 8 heads of 256 318 us, so 284; 16000 rows of 8
-// prompts and 12 heads of 64 under a window of 512 68 and 63; two of 8192 and 16 heads of 128 711 and 715.  A wave looks for that number with a lane to each of 63 candidates, a sequence to a lane;
-// more than 64 sequences, whose tiles are short or many, come one behind the other, and so do few tiles (58 rows of three sequences 5.3 us, 5.5 by that search).
+// Where a call fills the card more than once (many), the tiles of the highest number within their sequences come first: they have the most keys to walk, and
+// the short ones fill the gaps of the last round.  A sequence's tiles behind another's: two documents of 4096 and 8 heads of 256 318 us, so 284; 16000 rows of
+// 8 prompts and 12 heads of 64 under a window of 512 68 and 63; two of 8192 and 16 heads of 128 711 and 715.  A wave looks for that number with a lane to each
+// of 63 candidates, a sequence to a lane; more than 64 sequences, whose tiles are short or many, come one behind the other, and so do few tiles (58 rows of
+// three sequences 5.3 us, 5.5 by that search).
 #define PACKED_WAVES 2048                                        // that the card holds at once, two to a SIMD
 __device__ __forceinline__ void packed_tile(const int* cu, int seqs, int rows, int per, int t, int tiles, bool many, int* at, int* len, int* first) {
   const int lane = (int)threadIdx.x & 63;
@@ -57,8 +58,8 @@ __device__ __forceinline__ void packed_tile(const int* cu, int seqs, int rows, i
   *first = (t - (a / per + lo)) * per;
 }
 
-// One query of one head by a wave, key by key: 8 lanes to a key, 8 keys side by side, each group with a softmax of its own.  i: the query's row in its sequence, which
-// begins at row `at`.
+// One query of one head by a wave, key by key: 8 lanes to a key, 8 keys side by side, each group with a softmax of its own.  i: the query's row in its
+// sequence, which begins at row `at`.
 template <typename T, int HD>
 __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb, T* out, int64_t k_row, int64_t v_row, int i, int window, float slope,
                                            float softcap) {
@@ -107,12 +108,12 @@ __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb,
 typedef float floatx4_t __attribute__((ext_vector_type(4)));
 
 // fp32: v_mfma_f32_16x16x4_f32, whose operands are one value a lane, so that rows come straight from memory and probabilities straight from their registers.
-// A workgroup takes 16 queries of one head; its waves take 16 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims in the
-// first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 4 g + r.
-// us, a wave to a query / tiles of 32 queries on the 32x32x2 form / 16 queries, 32 keys a step / with values asked for before the products and a lane's dims beside each
-// other / 16 keys a step: 777 rows of 4 x 64 under a window of 129 12.7 / 13.1 / 9.8 / 9.3 / 8.7, 4096 of 8 x 64 under 512 267 / 76 / 74 / 65 / 61 (the L2's reads of keys and
-// values, once for each 16 queries), of 8 x 128 - / - / 161 / 129 / 108.  Two workgroups to a compute unit at heads of 256 (251 rows of 50 sequences and 64 heads 74 us, 127 with the
-// registers of one; 2000 rows of 8 heads 145 and 129).
+// A workgroup takes 16 queries of one head; its waves take 16 keys in turn, each with a softmax of its own, and add up through LDS in order.  The order of dims
+// in the first product and of keys in the second is what lanes hold: lane (g, c) the dims g hd/4 .. of key c, scores of keys 4 g + r. us, a wave to a query /
+// tiles of 32 queries on the 32x32x2 form / 16 queries, 32 keys a step / with values asked for before the products and a lane's dims beside each other / 16
+// keys a step: 777 rows of 4 x 64 under a window of 129 12.7 / 13.1 / 9.8 / 9.3 / 8.7, 4096 of 8 x 64 under 512 267 / 76 / 74 / 65 / 61 (the L2's reads of keys
+// and values, once for each 16 queries), of 8 x 128 - / - / 161 / 129 / 108.  Two workgroups to a compute unit at heads of 256 (251 rows of 50 sequences and 64
+// heads 74 us, 127 with the registers of one; 2000 rows of 8 heads 145 and 129).
 template <int HD, int NW, bool CAP>
 __global__ void __launch_bounds__(NW * 64, 2)
 swa_packed_f32_kernel(Heads q, Heads k, Heads v, float* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window, float softcap) {
@@ -232,16 +233,18 @@ struct Frag8 { u32x2_t lo, hi; };
 // bf16 on the matrix cores: a wave owns 32 queries of one head and walks their keys 64 at a time in two halves,
 //   S^T (keys x queries) = K Q^T      lane (c, hi) ends up with query c's scores of keys (r & 3) + 8 (r >> 2) + 4 hi of 32, which is
 //   O^T (dims x queries) = V^T P^T    what it holds of the second product: no score crosses a lane, only the maxima do, between two lanes.
-// Keys and values go to LDS by way of registers, which hold the next tile, one barrier a tile; values are read back transposed.  The second half's first product runs beside the
-// first half's softmax, the first half's second product beside the second half's: the maximum that a probability is taken from is the one
-// before these keys, and where a score exceeds it by more than 2^16 (the first keys, and hardly any after) that half is formed once more.
-// Two documents of 8192 rows, 16 heads of 128 on 4 key heads: 0.70 ms, 1.0 PFLOP/s, which the power of both units bounds: at the 1.84 GHz that it leaves, matrix cores are
-// busy 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %, three
-// exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 % slower.
+// Keys and values go to LDS by way of registers, which hold the next tile, one barrier a tile; values are read back transposed.  The second half's first
+// product runs beside the first half's softmax, the first half's second product beside the second half's: the maximum that a probability is taken from is the
+// one before these keys, and where a score exceeds it by more than 2^16 (the first keys, and hardly any after) that half is formed once more. Two documents of
+// 8192 rows, 16 heads of 128 on 4 key heads: 0.70 ms, 1.0 PFLOP/s, which the power of both units bounds: at the 1.84 GHz that it leaves, matrix cores are busy
+// 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %,
+// three exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 %
+// slower.
 // CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
-// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128.  Two documents
-// of 4096 and 8 heads 253 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 8 heads with ALiBi 39 and 47 with 128 queries a workgroup instead of 64,
-// which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi (a tenth slower).
+// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128. 
+// Two documents of 4096 and 8 heads 253 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 8 heads with ALiBi 39 and 47 with 128
+// queries a workgroup instead of 64, which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi
+// (a tenth slower).
 // PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
 template <int HD, int NQ, int PARTS, int CAP, bool BIAS>
 __global__ void __launch_bounds__(NQ * PARTS * packed_dims(HD) * 64, HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
@@ -256,7 +259,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   int at, len, first;
   packed_tile(cu, seqs, rows, NQ * 32, blockIdx.x / heads, gridDim.x / heads, gridDim.x * NW > PACKED_WAVES, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int part = PARTS == 1 ? 0 : w / NQ, share = DIMS == 1 ? 0 : w / NQ, wq = w - (part + share) * NQ, qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
+  const int part = PARTS == 1 ? 0 : w / NQ, share = DIMS == 1 ? 0 : w / NQ, wq = w - (part + share) * NQ, 
+            qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
   const int64_t k_row = k.row, v_row = v.row;
   const bf16_t* kb = (const bf16_t*)k.p + at * k_row + hk * k.head;
@@ -414,8 +418,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     }
   };
   // With ALiBi the largest scores are a query's latest keys': from those backwards the maximum settles at once (two documents of 8192, 16 heads of 128, 719 us, 785
-  // forwards; 16383 rows of 16 heads of 128 under a window of 1024 218 and 229; 512 rows of 12 heads of 64 10.6 and 11.0).  Without it forwards, where the workgroups of a
-  // document read the same keys at the same time (two of 4096, 8 heads of 256, 287 us, 297 backwards).
+  // forwards; 16383 rows of 16 heads of 128 under a window of 1024 218 and 229; 512 rows of 12 heads of 64 10.6 and 11.0).  Without it forwards, where the
+  // workgroups of a document read the same keys at the same time (two of 4096, 8 heads of 256, 287 us, 297 backwards).
   const int b_first = BIAS ? k_last / KB * KB : k_first, b_step = BIAS ? -KB : KB;
   int left = (k_last - k_first) / KB;                            // tiles after this one: k_first is a multiple of KB
   fetch(b_first);
@@ -607,12 +611,12 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
     typedef std::integral_constant<int, HD == 128 ? 8 : 2> Eight;
     typedef std::integral_constant<int, 2> Pair;
     typedef std::integral_constant<int, HD == 256 ? 1 : 2> Halves;
-    // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of 128 710 us,
-    // 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them: two waves of queries, each
-    // with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7, 4096 27.5 / 19.1, 12288 50.5 / 48.2, one
-    // document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71.
-    // Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the
-    // kernel of four waves alone.
+    // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of
+    // 128 710 us, 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them:
+    // two waves of queries, each with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7,
+    // 4096 27.5 / 19.1, 12288 50.5 / 48.2, one document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096
+    // 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71. Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows
+    // of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the kernel of four waves alone.
     if (softcap > FSTU_FAST_CAP) bf16(Four{}, One{});
     else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(Eight{}, One{});
     else if (HD <= 128 && (int64_t)(rows / 128) * heads < (HD == 128 ? 576 : 768)) bf16(Pair{}, Halves{});

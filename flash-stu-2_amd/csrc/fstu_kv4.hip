@@ -167,7 +167,8 @@ __device__ __forceinline__ Eight eight_of(const int* cu, const int* pos, int seq
 
 // A workgroup takes a group of eight slots (ONE: one row of a sequence), keys where y = 0 and values where y = 1; a thread eight dims of a head.  Each thread's
 // eight rows are asked for together, and what it leaves is 32 bytes beside each other (keys: 4 in each of eight rows).  16384 rows of 16 x 128 in bf16, written and
-// read back: 132 us with a row's eight dims to a thread, 76 so, 4.5 TB/s: bytes bound it, the bf16 rows 79 % of them; a token a row the launch and one trip to memory.
+// read back: 132 us with a row's eight dims to a thread, 76 so, 4.5 TB/s: bytes bound it, the bf16 rows 79 % of them; a token a row the launch and one trip to
+// memory.
 template <typename T, int HD, bool ONE>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(const T* k, const T* v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, void* cache, const int* pos, const int* cu, int rows,
@@ -488,8 +489,9 @@ __device__ __forceinline__ int sequence_of(const int* pos, int seqs, int cap, in
 // PLAN: the tiles of all sequences are dealt evenly to the workgroups; without, a workgroup takes a key head of a sequence or one of gridDim.z parts of its tiles.
 // kv4_join_kernel adds up what is in parts.
 // Bytes bound it where there are many: 16 sequences of up to 32768 positions, 8 key heads of 128, 84 us, 5.5 TB/s (an instruction undoes two codes and applies
-// their scale, a fourth of the vector ALUs' time; a look-up and a product for each would be more than memory takes), 32 of 1025 positions and 16 heads of 128 17 us, of which 4 are the launch and the first trip.  12 heads of 64 over 513
-// positions 6 us: the launch, the trip for the position, the trip for the codes, the join through LDS.
+// their scale, a fourth of the vector ALUs' time; a look-up and a product for each would be more than memory takes), 32 of 1025 positions and 16 heads of 128
+// 17 us, of which 4 are the launch and the first trip.  12 heads of 64 over 513 positions 6 us: the launch, the trip for the position, the trip for the codes,
+// the join through LDS.
 template <typename T, int HD, int NW, bool CAP, bool PLAN>
 __global__ void __launch_bounds__(NW * 64, HD == 256 || NW == 8 ? 1 : HD == 128 ? 2 : 3)
 kv4_attend_kernel(const T* q, int64_t q_row, int64_t q_head, const void* cache, T* out, float* ws, const int* pos, const float* slopes, int seqs, int heads,
@@ -866,9 +868,9 @@ extern "C" int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos
 // How a call's keys are cut: 1: a workgroup to each key head of a sequence; up to 64: that many parts of each; more: that many workgroups, to which all keys are
 // dealt evenly.  Parts cost a second launch and its boundary, some 3 us, and pay where few heads leave compute units idle through more than a thousand positions;
 // dealing evenly costs two looks at all positions besides, and pays where there is so much to do that an uneven end is more.  us, a workgroup to a head / parts (how
-// many) / dealt to 256: 16 heads of 128 over 1025 positions 9.1 / 7.5 (16) / -, 700 7.9 / 7.4 (16), 2048 12.5 / 7.8 (16) / 9.9; 12 heads of 64 over 2048 9.9 / 7.6 (16) /
-// 11.0; 4 of 128 over 32768 138 / 12.9 (64) / 14.9; 32 of 128 over 4200 23.8 / 11.8 (8) / 17.8; 8 of 256 over 700 12.7 / 8.8 (16); sequences of uneven length, 128
-// heads of 128: 8192 39 / 27 (2) / 31, 32768 155 / 106 (2) / 88; 512 of 128 over 4096 49 / - / 52.
+// many) / dealt to 256: 16 heads of 128 over 1025 positions 9.1 / 7.5 (16) / -, 700 7.9 / 7.4 (16), 2048 12.5 / 7.8 (16) / 9.9; 12 heads of 64 over 2048 9.9 /
+// 7.6 (16) / 11.0; 4 of 128 over 32768 138 / 12.9 (64) / 14.9; 32 of 128 over 4200 23.8 / 11.8 (8) / 17.8; 8 of 256 over 700 12.7 / 8.8 (16); sequences of
+// uneven length, 128 heads of 128: 8192 39 / 27 (2) / 31, 32768 155 / 106 (2) / 88; 512 of 128 over 4096 49 / - / 52.
 extern "C" int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window) {
   if (seqs < 1 || kvh < 1 || heads < kvh || cap < 1 || window < 0) return 1;
   const int chunks = (heads / kvh + KV4_COLS - 1) / KV4_COLS;
