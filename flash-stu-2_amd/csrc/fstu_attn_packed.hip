@@ -241,7 +241,7 @@ struct Frag8 { u32x2_t lo, hi; };
 // three exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 %
 // slower.
 // CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
-// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128. 
+// Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128.
 // Two documents of 4096 and 8 heads 253 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 8 heads with ALiBi 39 and 47 with 128
 // queries a workgroup instead of 64, which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi
 // (a tenth slower).
@@ -259,7 +259,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   int at, len, first;
   packed_tile(cu, seqs, rows, NQ * 32, blockIdx.x / heads, gridDim.x / heads, gridDim.x * NW > PACKED_WAVES, &at, &len, &first);
   if (first < 0 || first >= len) return;
-  const int part = PARTS == 1 ? 0 : w / NQ, share = DIMS == 1 ? 0 : w / NQ, wq = w - (part + share) * NQ, 
+  const int part = PARTS == 1 ? 0 : w / NQ, share = DIMS == 1 ? 0 : w / NQ, wq = w - (part + share) * NQ,
             qs = first + wq * 32, qi = qs + c;                    // the wave's first query, this lane's
   const bool on = qs < len;
   const int64_t k_row = k.row, v_row = v.row;

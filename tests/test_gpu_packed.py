@@ -197,6 +197,22 @@ def test_bounds_beyond_the_rows_touch_nothing_else(fs):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,hd", [(96, 64), (80, 256)])
+def test_rows_and_bounds_of_large_calls(fs, heads, hd, dtype):
+    """As the two tests before, where long tiles come first: rows of no sequence, then bounds beyond the rows."""
+    (q, k, v), dev = fused(31, 1300, heads, 2, hd, dtype)
+    h = torch.tensor([1, heads - 1])
+    out = torch.full((1310, heads, hd), 7.0, dtype=dtype, device="cuda")
+    fs.swa_packed(*dev, bounds([500, 0, 3, 700], begin=10), window=200, out=out[:1300])
+    assert bool((out[:10] == 7).all()) and bool((out[1213:] == 7).all())
+    o, bound = packed(q[10:, h], k[10:], v[10:], [500, 0, 3, 700], None, 200, 0.0, P_STEP[dtype])
+    check(out[10:1213].cpu()[:, h], o[:1203], bound[:1203], dtype)
+    fs.swa_packed(*dev, torch.tensor([-4, 700, 9000, 9000], dtype=torch.int32, device="cuda"), window=200, out=out[:1300])
+    check(out[:1300].cpu()[:, h], *packed(q[:, h], k, v, [700, 600], None, 200, 0.0, P_STEP[dtype]), dtype)
+    assert bool((out[1300:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_and_heads_far_apart_and_in_other_orders(fs, dtype):
     lengths, heads, kvh, hd = [65, 30], 4, 2, 64
     q, k, v = rand(1, 95, heads, hd, dtype=dtype), rand(2, 95, kvh, hd, dtype=dtype), rand(3, 95, kvh, hd, dtype=dtype)
