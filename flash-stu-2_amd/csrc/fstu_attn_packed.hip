@@ -286,7 +286,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   float m = -INFINITY, l = 0.f;
 
   const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NQ * 32 - 1);
-  // A tile's rows through a buffer descriptor: what lies behind the sequence's last row reads as zeros
+  // A tile's rows through a buffer descriptor: what lies behind the sequence's last row reads as zeros.  The range is checked against the lane's offset, which
+  // therefore holds the row; the scalar one takes no part in it (sums made in the loop and not kept in registers: 16383 rows of 16 heads of 128 221 us, 231).
   constexpr int NT = NW * 64, PR = (TILE + NT - 1) / NT, STEP = NT / CH;      // 16-byte pieces of a tile to a thread, rows between them
   u32x4_t kr[PR], vr[PR];
   const int row0 = tid / CH, ch0 = tid % CH;
@@ -295,10 +296,12 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
     const int last = min(KB, len - b) - 1;
     const rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + b * k_row), 0, (unsigned)(last * (int)k_row + HD) * 2, 0x00020000);
     const rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + b * v_row), 0, (unsigned)(last * (int)v_row + HD) * 2, 0x00020000);
+    int ks = STEP * (int)k_row * 2, vs = STEP * (int)v_row * 2;
+    asm volatile("" : "+s"(ks), "+s"(vs));
 #pragma unroll
     for (int i = 0; i < PR; ++i) {
-      kr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, i * STEP * (int)k_row * 2, 0));
-      vr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, i * STEP * (int)v_row * 2, 0));
+      kr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + i * ks, 0, 0));
+      vr[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off + i * vs, 0, 0));
     }
   };
   // The 16-byte pieces of a row are XOR-ed with bits of it, so that what 16 lanes read together lies in different banks

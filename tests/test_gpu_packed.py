@@ -314,3 +314,30 @@ def test_refusals(fs):
         fs.swa_packed(q.requires_grad_(), k, k, cu)
     with torch.no_grad():
         fs.swa_packed(q, k, k, cu)
+
+
+@pytest.mark.parametrize("hd,heads,rows,window,softcap,alibi", [
+    (32, 2, 320, 100, 50.0, True),
+    (64, 2, 320, None, 0.0, False),
+    (64, 2, 320, None, 600.0, False),
+    (64, 96, 1024, 300, 50.0, True),
+    (128, 2, 320, 100, 0.0, True),
+    (128, 96, 1024, None, 0.0, False),
+    (128, 2, 8192, 5000, 0.0, True),
+    (256, 2, 320, None, 50.0, False),
+])
+@pytest.mark.parametrize("tail", [1, 2, 40])
+def test_a_tile_ends_with_its_sequence(fs, tail, hd, heads, rows, window, softcap, alibi):
+    """A tile holds zeros behind its sequence's last row: a NaN from there would send rows to the form that goes key by key, whose roundings differ."""
+    n, after = rows + tail, 90
+    (q, k, v), dev = fused(37, n + after, heads, 2, hd, torch.bfloat16)
+    args = dict(slopes=slopes_of(heads).cuda() if alibi else None, window=window, softcap=softcap)
+    want = fs.swa_packed(*dev, bounds([n, after]), **args)[:n]
+    assert bool(torch.isfinite(want).all())
+    dirty = [t.clone() for t in dev]
+    dirty[1][n:], dirty[2][n:] = math.nan, math.nan
+    assert torch.equal(fs.swa_packed(*dirty, bounds([n, after]), **args)[:n], want)
+    assert torch.equal(fs.swa_packed(*dirty, bounds([n]), **args)[:n], want)
+    if tail > 2:                                                         # that it would show: a NaN inside of the tile does
+        dirty[2][n - 1] = math.nan
+        assert not torch.equal(fs.swa_packed(*dirty, bounds([n, after]), **args)[:n - 1], want[:n - 1])
