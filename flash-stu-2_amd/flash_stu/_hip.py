@@ -1682,7 +1682,10 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tens
         if not one_call:                                         # of another type than q, or nothing that can be written
             kv4_write(cache, k, v, pos)
     splits, floats = _kv4_splits(seqs, heads, kvh, hd, cap, window)
-    ws = _empty(floats, dtype=_f32, device=data.device).data_ptr() if floats else None      # its memory is this stream's until what runs on it next
+    # held until the library has queued both of its launches: it runs without the interpreter's lock, and memory given back before could go to another thread's
+    # call between them (afterwards what takes it comes behind them on the stream)
+    ws = _empty(floats, dtype=_f32, device=data.device) if floats else None
+    ws_at = None if ws is None else ws.data_ptr()
     qr, qh, _ = q.stride()
     lib, stream = load(), raw_stream(dev)
     qr, qh = qr if seqs > 1 else 0, qh if heads > 1 else 0
@@ -1690,10 +1693,10 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tens
     if one_call:
         (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
         rc = lib.fstu_kv4_step(q.data_ptr(), qr, qh, k.data_ptr(), kr if seqs > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(), vr if seqs > 1 else 0,
-                               vh if kvh > 1 else 0, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
+                               vh if kvh > 1 else 0, data.data_ptr(), out.data_ptr(), ws_at, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
                                softcap or 0.0, dt, stream)
     else:
-        rc = lib.fstu_kv4_attend(q.data_ptr(), qr, qh, data.data_ptr(), out.data_ptr(), ws, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
+        rc = lib.fstu_kv4_attend(q.data_ptr(), qr, qh, data.data_ptr(), out.data_ptr(), ws_at, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
                                  softcap or 0.0, dt, stream)
     if rc:
         _check(rc, "fstu_kv4_attend")

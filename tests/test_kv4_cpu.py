@@ -123,3 +123,60 @@ def test_the_reference_of_the_tests():
     o, bound = attention(q, k, v, far, 0.0, 0.0, 0.0)
     want = torch.nn.functional.scaled_dot_product_attention(q[None], k[None], v[None], is_causal=True)[0]
     assert torch.allclose(o, want) and bool((bound < 1e-4).all())
+
+
+class OnGpu(torch.Tensor):
+    """A tensor of the CPU that says it is on device 0."""
+
+    def get_device(self):
+        return 0
+
+
+class Recorded:
+    """A library whose attention entry points note the calls and answer what is asked of them; all else is the real one's."""
+
+    def __init__(self, lib, seen, rc=0):
+        self.lib, self.seen, self.rc = lib, seen, rc
+
+    def __getattr__(self, name):
+        if name.startswith(("fstu_kv4_attend", "fstu_kv4_step", "fstu_kv4_write")) and name not in ("fstu_kv4_attend_ws", "fstu_kv4_attend_splits"):
+            return lambda *args: self.seen(name, args) or self.rc
+        return getattr(self.lib, name)
+
+
+def stand_in(monkeypatch, lib, seen, rc=0):
+    """Calls of a cache without a GPU: (cache of 2 sequences, 1 key head of 64 and long rings, a maker of tensors)."""
+    from flash_stu import KV4Cache, _hip
+    monkeypatch.setattr(_hip, "load", lambda: Recorded(lib, seen, rc))
+    monkeypatch.setattr(_hip, "_device_now", lambda: 0)
+    monkeypatch.setattr(_hip, "raw_stream", lambda dev: 0)
+
+    def on_gpu(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+
+    cache = object.__new__(KV4Cache)
+    cache.batch, cache.kv_heads, cache.head_dim, cache.capacity = 2, 1, 64, 20000
+    cache.data = on_gpu(lib.fstu_kv4_bytes(2, 1, 64, 20000), dtype=torch.uint8)
+    return cache, on_gpu
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_the_parts_stay_this_calls_until_it_has_returned(lib, monkeypatch, step):
+    """The library is called without the interpreter's lock: memory of the parts that the allocator had back by then could become another thread's."""
+    import weakref
+
+    from flash_stu import _hip
+    given, held = [], []
+    empty = _hip._empty
+
+    def recorded(*args, **kw):
+        x = empty(*args, **kw)
+        if kw.get("dtype") is torch.float32:
+            given.append((weakref.ref(x), x.data_ptr()))
+        return x
+
+    monkeypatch.setattr(_hip, "_empty", recorded)
+    cache, on_gpu = stand_in(monkeypatch, lib, lambda name, args: held.append([name, [ref() is not None and at in args for ref, at in given]]))
+    k = on_gpu(2, 1, 64)
+    cache.attend(on_gpu(2, 4, 64), on_gpu(2, dtype=torch.int32), *((k, k) if step else ()))
+    assert len(held) == 1 and held[0][0].startswith("fstu_kv4_step" if step else "fstu_kv4_attend") and held[0][1] == [True]
