@@ -871,11 +871,16 @@ extern "C" int fstu_kv4_read(const void* cache, void* k, void* v, const int* pos
 // many) / dealt to 256: 16 heads of 128 over 1025 positions 9.1 / 7.5 (16) / -, 700 7.9 / 7.4 (16), 2048 12.5 / 7.8 (16) / 9.9; 12 heads of 64 over 2048 9.9 /
 // 7.6 (16) / 11.0; 4 of 128 over 32768 138 / 12.9 (64) / 14.9; 32 of 128 over 4200 23.8 / 11.8 (8) / 17.8; 8 of 256 over 700 12.7 / 8.8 (16); sequences of
 // uneven length, 128 heads of 128: 8192 39 / 27 (2) / 31, 32768 155 / 106 (2) / 88; 512 of 128 over 4096 49 / - / 52.
+// The even deal counts a call's tiles in an int: each sequence's window's, and one more where the ring's end cuts it.
+static bool kv4_can_deal(int seqs, int heads, int kvh, int cap, int window) {
+  const int64_t tiles = ((int64_t)(window < cap ? window : cap - 1) + 3 * KV4_TILE - 1) / KV4_TILE;
+  return tiles * seqs * kvh * ((heads / kvh + KV4_COLS - 1) / KV4_COLS) <= 0x7fffffff;
+}
 extern "C" int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window) {
   if (seqs < 1 || kvh < 1 || heads < kvh || cap < 1 || window < 0) return 1;
   const int chunks = (heads / kvh + KV4_COLS - 1) / KV4_COLS;
   const int64_t tiles = ((int64_t)(window < cap ? window : cap - 1) + 2 * KV4_TILE - 1) / KV4_TILE, groups = (int64_t)seqs * kvh * chunks;
-  if (groups * tiles >= 98304 && tiles >= 192) return 256;
+  if (groups * tiles >= 98304 && tiles >= 192 && kv4_can_deal(seqs, heads, kvh, cap, window)) return 256;
   int64_t parts = 256 / groups;
   if (parts > tiles / 3) parts = tiles / 3;
   return tiles < (hd == 256 ? 20 : 40) || parts < 2 ? 1 : (int)(parts < KV4_MOST_PARTS ? parts : KV4_MOST_PARTS);
@@ -904,7 +909,8 @@ static int kv4_attend_call(const char* name, const void* q, int64_t q_row, int64
                    !fstu_heads_touch(cache, fstu_kv4_bytes(seqs, kvh, hd, cap), 0, 2, 1, 0, 1, out, n),
                FSTU_EARG, "%s: out overlaps q or the cache", name);
   const int group = heads / kvh, chunks = (group + KV4_COLS - 1) / KV4_COLS;
-  FSTU_REQUIRE((int64_t)seqs * heads < 1 << 23 && (splits > KV4_MOST_PARTS || (int64_t)seqs * kvh * chunks * splits < 1 << 23), FSTU_ESHAPE,
+  FSTU_REQUIRE((int64_t)seqs * heads < 1 << 23 &&
+                   (splits > KV4_MOST_PARTS ? kv4_can_deal(seqs, heads, kvh, cap, window) : (int64_t)seqs * kvh * chunks * splits < 1 << 23), FSTU_ESHAPE,
                "%s: %d sequences of %d heads in %d parts are more than a launch takes", name, seqs, heads, splits);
   if (fresh.k) {
     FSTU_REQUIRE(fstu_heads_aligned(fresh.k, fresh.k_row, fresh.k_head, size) && fstu_heads_aligned(fresh.v, fresh.v_row, fresh.v_head, size), FSTU_EALIGN,

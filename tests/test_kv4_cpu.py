@@ -180,3 +180,17 @@ def test_the_parts_stay_this_calls_until_it_has_returned(lib, monkeypatch, step)
     k = on_gpu(2, 1, 64)
     cache.attend(on_gpu(2, 4, 64), on_gpu(2, dtype=torch.int32), *((k, k) if step else ()))
     assert len(held) == 1 and held[0][0].startswith("fstu_kv4_step" if step else "fstu_kv4_attend") and held[0][1] == [True]
+
+
+def test_tiles_past_31_bits_are_not_dealt(lib, mem):
+    """The even deal counts all tiles of 32 slots of a call's key heads (and chunks of 8 query heads) in an int."""
+    p, ring = mem[0], 1 << 30
+    assert 1 <= lib.fstu_kv4_attend_splits(1, 512, 1, 32, ring, ring - 1) <= 64          # 64 chunks of 2^25 tiles
+    assert lib.fstu_kv4_attend_splits(1, 504, 1, 32, ring, ring - 1) == 256              # 63
+    assert 1 <= lib.fstu_kv4_attend_splits(64, 8, 1, 32, ring, ring - 1) <= 64
+
+    def attend(heads, splits, window=ring - 1):
+        return lib.fstu_kv4_attend(p, 32 * heads, 32, p + 8192, p + (1 << 40), p, splits, p, None, 1, heads, 1, 32, ring, window, 0.0, 1, None)
+
+    assert attend(512, 256) == -3 and "launch" in why(lib)
+    assert attend(512, 65535) == -3 and attend(8192, 65, window=(1 << 26) - 1) == -3
