@@ -83,7 +83,7 @@ __device__ __forceinline__ void packed_one(const T* q, const T* kb, const T* vb,
     s *= scale;
     if (softcap > 0.f) s = softcap * tanhf(s / softcap);
     s -= slope * (float)(i - j);
-    const float mn = fmaxf(m, s), corr = __expf(m - mn), p = __expf(s - mn);
+    const float mn = fmaxf(m, s), off = mn == -INFINITY ? 0.f : mn, corr = __expf(m - off), p = __expf(s - off);      // no weight for scores of -infinity
     l = l * corr + p;
     m = mn;
 #pragma unroll

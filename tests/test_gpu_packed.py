@@ -341,3 +341,28 @@ def test_a_tile_ends_with_its_sequence(fs, tail, hd, heads, rows, window, softca
     if tail > 2:                                                         # that it would show: a NaN inside of the tile does
         dirty[2][n - 1] = math.nan
         assert not torch.equal(fs.swa_packed(*dirty, bounds([n, after]), **args)[:n - 1], want[:n - 1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("window", [None, 20])
+@pytest.mark.parametrize("size", [-math.inf, -3.3e38])
+def test_a_score_of_minus_infinity_beside_an_infinity_that_is_not_seen(fs, size, window, hd, dtype):
+    """A key whose score is -infinity (an infinite key, or a product past fp32's range) has no weight, whether or not its row is formed key by key."""
+    from attention_reference import attention
+    n, heads = 75, 2
+    q, k, v = (rand(50 + i, n, heads, hd, dtype=dtype) for i in range(3))
+    q[:, :, 0] = q[:, :, 0].abs() + 2
+    gone = [0, 30, 31]
+    k[gone], v[70, :, ::9] = 0, 0
+    far = torch.arange(n)[:, None] - torch.arange(n)
+    far = torch.where((far >= 0) & (far <= (n if window is None else window)), far, -1)
+    far[:, gone] = -1
+    dk, dv = k.clone(), v.clone()
+    dk[gone, :, 0], dv[70, :, ::9] = size, math.inf
+    y = fs.swa_packed(q.cuda(), dk.cuda(), dv.cuda(), bounds([n]), window=window).cpu()
+    clean = torch.arange(1, 70)                                          # row 0 sees nothing else, row 70 and those behind it the infinity
+    for h in range(heads):
+        o, bound = attention(q[:, h].double(), k[:, h].double(), v[:, h].double(), far.double(), 0.0, 0.0, P_STEP[dtype])
+        check(y[clean, h], o[clean], bound[clean], dtype)
+    assert bool(torch.isnan(y[0]).all()) and not bool(torch.isfinite(y[70, :, ::9]).any())
