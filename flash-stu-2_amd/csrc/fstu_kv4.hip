@@ -435,6 +435,7 @@ __device__ __forceinline__ Tiles tiles_of(int p, int cap, int window, int tiles)
 struct NewRows {               // the keys and values of the queries' own positions, or nothing: strides in elements
   const void *k, *v;
   int64_t k_row, k_head, v_row, v_head;
+  int dtype;
 };
 
 // All sequences' tiles behind one another, `per_seq` groups (key heads, chunks of query heads) each: workgroup w of W takes per or per + 1 of them.
@@ -904,6 +905,7 @@ static int kv4_attend_call(const char* name, const void* q, int64_t q_row, int64
   const int size = dtype == FSTU_BF16 ? 2 : 4;
   FSTU_REQUIRE(fstu_heads_aligned(q, q_row, q_head, size) && fstu_aligned(out, 16) && fstu_aligned(ws, 4), FSTU_EALIGN,
                "%s: rows and heads of q and out must begin at multiples of 16 bytes", name);
+  FSTU_REQUIRE(dtype == FSTU_F32 || dtype == FSTU_BF16, FSTU_EDTYPE, "%s: unknown dtype %d", name, dtype);
   const int64_t n = (int64_t)seqs * heads * hd * size;
   FSTU_REQUIRE(!fstu_heads_touch(q, q_row, q_head, seqs, heads, hd, size, out, n) &&
                    !fstu_heads_touch(cache, fstu_kv4_bytes(seqs, kvh, hd, cap), 0, 2, 1, 0, 1, out, n),
@@ -913,16 +915,20 @@ static int kv4_attend_call(const char* name, const void* q, int64_t q_row, int64
                    (splits > KV4_MOST_PARTS ? kv4_can_deal(seqs, heads, kvh, cap, window) : (int64_t)seqs * kvh * chunks * splits < 1 << 23), FSTU_ESHAPE,
                "%s: %d sequences of %d heads in %d parts are more than a launch takes", name, seqs, heads, splits);
   if (fresh.k) {
-    FSTU_REQUIRE(fstu_heads_aligned(fresh.k, fresh.k_row, fresh.k_head, size) && fstu_heads_aligned(fresh.v, fresh.v_row, fresh.v_head, size), FSTU_EALIGN,
+    FSTU_REQUIRE(fresh.dtype == FSTU_F32 || fresh.dtype == FSTU_BF16, FSTU_EDTYPE, "%s: unknown dtype %d of k and v", name, fresh.dtype);
+    const int wide = fresh.dtype == FSTU_BF16 ? 2 : 4;
+    FSTU_REQUIRE(fstu_heads_aligned(fresh.k, fresh.k_row, fresh.k_head, wide) && fstu_heads_aligned(fresh.v, fresh.v_row, fresh.v_head, wide), FSTU_EALIGN,
                  "%s: rows and heads of k and v must begin at multiples of 16 bytes", name);
     const int64_t held = fstu_kv4_bytes(seqs, kvh, hd, cap);
-    FSTU_REQUIRE(!fstu_heads_touch(fresh.k, fresh.k_row, fresh.k_head, seqs, kvh, hd, size, out, n) &&
-                     !fstu_heads_touch(fresh.v, fresh.v_row, fresh.v_head, seqs, kvh, hd, size, out, n) &&
-                     !fstu_heads_touch(fresh.k, fresh.k_row, fresh.k_head, seqs, kvh, hd, size, cache, held) &&
-                     !fstu_heads_touch(fresh.v, fresh.v_row, fresh.v_head, seqs, kvh, hd, size, cache, held),
+    FSTU_REQUIRE(!fstu_heads_touch(fresh.k, fresh.k_row, fresh.k_head, seqs, kvh, hd, wide, out, n) &&
+                     !fstu_heads_touch(fresh.v, fresh.v_row, fresh.v_head, seqs, kvh, hd, wide, out, n) &&
+                     !fstu_heads_touch(fresh.k, fresh.k_row, fresh.k_head, seqs, kvh, hd, wide, cache, held) &&
+                     !fstu_heads_touch(fresh.v, fresh.v_row, fresh.v_head, seqs, kvh, hd, wide, cache, held),
                  FSTU_EARG, "%s: out or the cache overlaps k or v", name);
-    if (splits > KV4_MOST_PARTS) {                               // dealt evenly: a call that long does not feel a launch
-      const int wrote = fstu_kv4_write(fresh.k, fresh.k_row, fresh.k_head, fresh.v, fresh.v_row, fresh.v_head, cache, pos, nullptr, seqs, seqs, kvh, hd, cap, dtype, stream);
+    // written by a launch of its own, once nothing is left to refuse: where keys are dealt evenly (a call that long does not feel a launch), or of another type
+    if (splits > KV4_MOST_PARTS || fresh.dtype != dtype) {
+      const int wrote = fstu_kv4_write(fresh.k, fresh.k_row, fresh.k_head, fresh.v, fresh.v_row, fresh.v_head, cache, pos, nullptr, seqs, seqs, kvh, hd, cap, fresh.dtype,
+                                       stream);
       if (wrote) return wrote;
       fresh.k = nullptr;
     }
@@ -955,12 +961,19 @@ extern "C" int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, con
                          stream);
 }
 
+extern "C" int fstu_kv4_step_of(const void* q, int64_t q_row, int64_t q_head, int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                                int64_t v_head, int kv_dtype, void* cache, void* out, float* ws, int splits, const int* pos, const float* slopes, int seqs, int heads,
+                                int kvh, int hd, int cap, int window, float softcap, void* stream) {
+  FSTU_REQUIRE(k && v, FSTU_ENULL, "fstu_kv4_step: null pointer");
+  return kv4_attend_call("fstu_kv4_step", q, q_row, q_head, NewRows{k, v, k_row, k_head, v_row, v_head, kv_dtype}, cache, out, ws, splits, pos, slopes, seqs, heads,
+                         kvh, hd, cap, window, softcap, dtype, stream);
+}
+
 // One launch with the write where a workgroup has its head to itself or shares it in parts: a step of one sequence, 12 heads of 64 over 513 positions 5.75 us,
 // 7.6 in two and 5.15 without its write; 32 sequences of 16 heads of 128 over 1025 16.4, 18.6 and 15.8; called from Python 9.4, 14.7 and 8.3.
 extern "C" int fstu_kv4_step(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                              int64_t v_head, void* cache, void* out, float* ws, int splits, const int* pos, const float* slopes, int seqs, int heads, int kvh,
                              int hd, int cap, int window, float softcap, int dtype, void* stream) {
-  FSTU_REQUIRE(k && v, FSTU_ENULL, "fstu_kv4_step: null pointer");
-  return kv4_attend_call("fstu_kv4_step", q, q_row, q_head, NewRows{k, v, k_row, k_head, v_row, v_head}, cache, out, ws, splits, pos, slopes, seqs, heads, kvh, hd,
-                         cap, window, softcap, dtype, stream);
+  return fstu_kv4_step_of(q, q_row, q_head, dtype, k, k_row, k_head, v, v_row, v_head, dtype, cache, out, ws, splits, pos, slopes, seqs, heads, kvh, hd, cap, window,
+                          softcap, stream);
 }

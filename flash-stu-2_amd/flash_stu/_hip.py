@@ -83,6 +83,7 @@ SIGNATURES = {
     "fstu_kv4_read": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
     "fstu_kv4_attend": [_vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "fstu_kv4_step": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "fstu_kv4_step_of": [_vp, _i64, _i64, _i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp],
     "fstu_kv4_attend_splits": [_i, _i, _i, _i, _i, _i],
     "fstu_kv4_attend_ws": [_i, _i, _i, _i, _i],
     "fstu_sample": [_vp, _vp, _i64, _i, _i, _f, _i, _f, _i, _u64, _i, _i, _vp],
@@ -1667,20 +1668,19 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tens
         raise FlashSTUHipError(f"KV4Cache.attend: window {window} does not fit a ring of {cap} (0 to {cap - 1})")
     if softcap and not 2.0 ** -40 <= softcap <= 2.0 ** 40:
         raise FlashSTUHipError(f"KV4Cache.attend: softcap must be zero (none) or a number from 2^-40 to 2^40, got {softcap}")
-    if out is None:
-        out = _empty(shape, dtype=dtype, device=data.device)
-    else:
-        _written(out)
-    one_call = False
     if k is not None or v is not None:
         if k is None or v is None:
             raise FlashSTUHipError("KV4Cache.attend: k and v go together")
         if (k.requires_grad or v.requires_grad) and _grad_on():
             raise _fp8_forward_only("KV4Cache.attend")
-        one_call = (k.dtype is dtype and v.dtype is dtype and k.shape == v.shape == (seqs, kvh, hd) and k.get_device() == v.get_device() == dev
-                    and k.stride(2) == v.stride(2) == 1)
-        if not one_call:                                         # of another type than q, or nothing that can be written
-            kv4_write(cache, k, v, pos)
+        kv_dt = _kv4_types.get(k.dtype)
+        if not (kv_dt is not None and v.dtype is k.dtype and k.shape == v.shape == (seqs, kvh, hd) and k.get_device() == v.get_device() == dev
+                and k.stride(2) == v.stride(2) == 1):
+            _refuse_heads("KV4Cache.attend", dev, [("k", k, (seqs, kvh, hd), k.dtype), ("v", v, (seqs, kvh, hd), k.dtype)])
+    if out is None:
+        out = _empty(shape, dtype=dtype, device=data.device)
+    else:
+        _written(out)
     splits, floats = _kv4_splits(seqs, heads, kvh, hd, cap, window)
     # held until the library has queued both of its launches: it runs without the interpreter's lock, and memory given back before could go to another thread's
     # call between them (afterwards what takes it comes behind them on the stream)
@@ -1690,11 +1690,11 @@ def kv4_attend(cache, q: torch.Tensor, pos: torch.Tensor, k: Optional[torch.Tens
     lib, stream = load(), raw_stream(dev)
     qr, qh = qr if seqs > 1 else 0, qh if heads > 1 else 0
     slopes_at = None if slopes is None else slopes.data_ptr()
-    if one_call:
+    if k is not None:
         (kr, kh, _), (vr, vh, _) = k.stride(), v.stride()
-        rc = lib.fstu_kv4_step(q.data_ptr(), qr, qh, k.data_ptr(), kr if seqs > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(), vr if seqs > 1 else 0,
-                               vh if kvh > 1 else 0, data.data_ptr(), out.data_ptr(), ws_at, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
-                               softcap or 0.0, dt, stream)
+        rc = lib.fstu_kv4_step_of(q.data_ptr(), qr, qh, dt, k.data_ptr(), kr if seqs > 1 else 0, kh if kvh > 1 else 0, v.data_ptr(), vr if seqs > 1 else 0,
+                                  vh if kvh > 1 else 0, kv_dt, data.data_ptr(), out.data_ptr(), ws_at, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap,
+                                  window, softcap or 0.0, stream)
     else:
         rc = lib.fstu_kv4_attend(q.data_ptr(), qr, qh, data.data_ptr(), out.data_ptr(), ws_at, splits, pos.data_ptr(), slopes_at, seqs, heads, kvh, hd, cap, window,
                                  softcap or 0.0, dt, stream)

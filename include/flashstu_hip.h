@@ -377,7 +377,8 @@ int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k,
  *   splits: 1: a workgroup to each key head of a sequence; up to 64: that many parts of its keys each; more: that many workgroups, to which the keys of all
  *   sequences are dealt evenly.  Parts are joined by a second launch (ws: fstu_kv4_attend_ws floats, not shared with a call that may run at the same
  *   time; NULL with 1); fstu_kv4_attend_splits says what pays.
- * fstu_kv4_step: fstu_kv4_write of a row to each sequence, then fstu_kv4_attend, with the same results; one launch up to 64 parts.  k and v of q's dtype. */
+ * fstu_kv4_step: fstu_kv4_write of a row to each sequence, then fstu_kv4_attend, with the same results; one launch up to 64 parts.  k and v of q's dtype.
+ * fstu_kv4_step_of: the same with k and v of a dtype of their own (two launches and more where it is another).  A refused call writes nothing. */
 int64_t fstu_kv4_bytes(int seqs, int kvh, int hd, int cap);
 int fstu_kv4_write(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* cache, const int* pos,
                    const int* cu, int rows, int seqs, int kvh, int hd, int cap, int dtype, void* stream);
@@ -388,6 +389,9 @@ int fstu_kv4_attend(const void* q, int64_t q_row, int64_t q_head, const void* ca
 int fstu_kv4_step(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                   int64_t v_head, void* cache, void* out, float* ws, int splits, const int* pos, const float* slopes, int seqs, int heads, int kvh,
                   int hd, int cap, int window, float softcap, int dtype, void* stream);
+int fstu_kv4_step_of(const void* q, int64_t q_row, int64_t q_head, int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                     int64_t v_head, int kv_dtype, void* cache, void* out, float* ws, int splits, const int* pos, const float* slopes, int seqs, int heads,
+                     int kvh, int hd, int cap, int window, float softcap, void* stream);
 int fstu_kv4_attend_splits(int seqs, int heads, int kvh, int hd, int cap, int window);
 int64_t fstu_kv4_attend_ws(int seqs, int heads, int kvh, int hd, int splits);
 

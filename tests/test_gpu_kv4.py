@@ -423,3 +423,20 @@ def test_refusals(fs):
     with torch.no_grad():
         cache.write(k, k, pos)
     assert not cache.data[:64].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_refused_call_of_another_type_writes_nothing(fs, dtype):
+    from flash_stu._hip import FlashSTUHipError
+    cache = fs.KV4Cache(2, 2, 64, 40)
+    other = torch.bfloat16 if dtype is torch.float32 else torch.float32
+    k, q, pos = torch.ones(2, 2, 64, dtype=other, device="cuda"), torch.ones(2, 4, 64, dtype=dtype, device="cuda"), ints([0, 0])
+    wide, ends = torch.ones(2 * 4 * 64 + 1, dtype=dtype, device="cuda"), torch.ones(2, 2, 72, dtype=other, device="cuda")
+    for call in (lambda: cache.attend(q, pos, k, k, out=q), lambda: cache.attend(wide[1:].view(2, 4, 64), pos, k, k), lambda: cache.attend(q, pos, k, k[:1]),
+                 lambda: cache.attend(q, pos, k, k.to(dtype)), lambda: cache.attend(q, pos, k.half(), k.half()), lambda: cache.attend(q, pos, k, k.transpose(0, 1)[..., :32]),
+                 lambda: cache.attend(q, pos, ends[..., 1:65], k), lambda: cache.attend(q, pos, k.cpu(), k), lambda: cache.attend(q, pos, None, k),
+                 lambda: cache.attend(q, pos, k, k, out=q.to(other))):
+        with pytest.raises(FlashSTUHipError):
+            call()
+    assert not cache.data.any()
+    assert bool(torch.isfinite(cache.attend(q, pos, k, k)).all()) and bool(cache.data.any())

@@ -194,3 +194,27 @@ def test_tiles_past_31_bits_are_not_dealt(lib, mem):
 
     assert attend(512, 256) == -3 and "launch" in why(lib)
     assert attend(512, 65535) == -3 and attend(8192, 65, window=(1 << 26) - 1) == -3
+
+
+def test_a_refused_step_of_another_type_writes_nothing(lib, mem, monkeypatch):
+    """k and v of another type than q go to the cache in a launch of their own: after everything that the attention refuses."""
+    from flash_stu import _hip
+    names = []
+    cache, on_gpu = stand_in(monkeypatch, lib, lambda name, args: names.append(name), rc=-5)
+    k = on_gpu(2, 1, 64, dtype=torch.float32)
+    with pytest.raises(_hip.FlashSTUHipError):
+        cache.attend(on_gpu(2, 4, 64), on_gpu(2, dtype=torch.int32), k, k)
+    assert names == ["fstu_kv4_step_of"]
+
+    p = mem[0]
+
+    def step(q=p, dt=1, k=p + 2048, kr=128, kh=64, v=p + 2048, kv_dt=0, c=p + 16384, out=p + 4096, splits=1, ws=None, window=7, heads=4):
+        return lib.fstu_kv4_step_of(q, 64 * heads, 64, dt, k, kr, kh, v, 128, 64, kv_dt, c, out, ws, splits, p, None, 2, heads, 2, 64, 40, window, 0.0, None)
+
+    for other in (dict(dt=1, kv_dt=0), dict(dt=0, kv_dt=1)):
+        assert step(k=None, **other) == -1 and step(window=40, **other) == -5 and step(splits=2, **other) == -5 and step(heads=3, **other) == -3
+        assert step(out=p, **other) == -5 and "overlaps q" in why(lib)
+        assert step(out=p + 16384, **other) == -5 and step(k=p + 4096, **other) == -5 and step(v=p + 16384, **other) == -5
+        assert step(out=p + 4100, **other) == -4 and step(q=p + 2, **other) == -4 and step(k=p + 2056, **other) == -4
+    assert step(dt=1, kv_dt=1, kr=68) == -4 and step(kv_dt=7) == -2 and step(dt=7) == -2 and step(kv_dt=7, splits=65, ws=p) == -2
+    assert step(k=p + 4096 - 1008) == -5                                 # its end, by its own type's size: 1024 bytes
