@@ -95,11 +95,13 @@ class KV4Cache:
     one.  32 values with an infinity or a NaN among them stand for NaN.  A key and its value take 17/16 of a byte for each dim, bf16 ones 4.
 
     `pos` is (batch,) int32 on the GPU and counted by the caller, so that a captured step runs for every position; a sequence at a negative position
-    is not in use.  The capacity may exceed a window by any number; head_dim is 32, 64, 128 or 256.  Forward only."""
+    is not in use.  The capacity may exceed a window by any number and is 2^30 at most; head_dim is 32, 64, 128 or 256.  One launch attends over all of it:
+    batch and heads are 65535 at most, batch * heads less than 2^23.  Forward only."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, capacity: int, device=None):
-        if batch < 1 or kv_heads < 1 or not 1 <= capacity <= 1 << 30 or head_dim not in (32, 64, 128, 256) or batch * kv_heads * capacity > 1 << 40:
-            raise _hip.FlashSTUHipError(f"KV4Cache: batch {batch}, {kv_heads} key heads, capacity {capacity} (up to 2^30) and head_dim {head_dim} "
+        if (not 1 <= batch <= 65535 or not 1 <= kv_heads <= 65535 or batch * kv_heads >= 1 << 23 or not 1 <= capacity <= 1 << 30
+                or head_dim not in (32, 64, 128, 256) or batch * kv_heads * capacity > 1 << 40):
+            raise _hip.FlashSTUHipError(f"KV4Cache: batch {batch}, {kv_heads} key heads (each up to 65535, less than 2^23 together), capacity {capacity} (up to 2^30) and head_dim {head_dim} "
                                         "(32, 64, 128 or 256) are no cache")
         device = torch.device("cuda" if device is None else device)
         if device.type != "cuda":

@@ -358,8 +358,8 @@ int fstu_swa_prefill_mfma(const void* qkv, void* vt_ws, void* out, const float* 
 /* Attention over whole prompts packed behind one another: sequence s is rows cu[s] .. cu[s+1]-1 (cu: seqs+1 device ints, rising), row i of it
  * sees its rows max(0,i-window) .. i.  q (rows,heads,hd), k and v (rows,kvh,hd) by row and head strides in elements (multiples of 16 bytes),
  * query head h reads key head h / (heads/kvh); out (rows,heads,hd) dense, not overlapping the others.  Scores as above, slopes (heads) or NULL,
- * softcap 0: none, else 2^-40..2^40.  Rows of no sequence are left as they were.  Refused: k and v rows 2^23 elements apart and more, and
- * (16 rows + 512 seqs) * heads (bf16: 2 rows, 4 at hd 256) from 2^32 on. */
+ * softcap 0: none, else 2^-40..2^40.  Rows of no sequence are left as they were.  Refused: k and v rows 2^23 elements apart and more, more than
+ * 65535 heads, and (16 rows + 512 seqs) * heads (bf16: 2 rows, 4 at hd 256) from 2^32 on. */
 int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                     int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
                     float softcap, int dtype, void* stream);
@@ -368,7 +368,8 @@ int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k,
  * fstu_kv4_bytes(...) bytes, cleared once by the caller, for seqs sequences of kvh key heads of hd (32, 64, 128, 256) dims; position j of a sequence
  * lives in slot j % cap.  Values are e2m1 codes; 32 values of a head's row share a scale 2^e, e the smallest of -120..125 with amax <= 7 * 2^e;
  * code: the nearest, ties to the even one.  A block with a value that is not finite stands for NaN.  csrc/fstu_kv4.h says where what lies.
- * Refused: sizes beyond a launch (rows / 8 + 2 seqs from 2^23 on; seqs * heads, and times splits, from 2^23 on).
+ * Refused: sizes beyond a launch (write and read: rows / 8 + 2 seqs from 2^23 on; attend and step: more than 65535 sequences or heads, seqs * heads and,
+ * in up to 64 splits, the key heads' chunks of 8 query heads times splits from 2^23 on, in more those chunks' tiles of 32 slots beyond 31 bits).
  * pos: seqs device ints; a sequence at a negative position is not in use (nothing written, zeros read, out zero).
  * cu as above, or NULL: row s is sequence s's only one.
  * fstu_kv4_write: rows cu[s].. become positions pos[s].. (of more than cap rows the last cap).

@@ -218,3 +218,14 @@ def test_a_refused_step_of_another_type_writes_nothing(lib, mem, monkeypatch):
         assert step(out=p + 4100, **other) == -4 and step(q=p + 2, **other) == -4 and step(k=p + 2056, **other) == -4
     assert step(dt=1, kv_dt=1, kr=68) == -4 and step(kv_dt=7) == -2 and step(dt=7) == -2 and step(kv_dt=7, splits=65, ws=p) == -2
     assert step(k=p + 4096 - 1008) == -5                                 # its end, by its own type's size: 1024 bytes
+
+
+def test_a_batch_that_no_launch_attends_over_is_no_cache(lib, mem):
+    from flash_stu import KV4Cache, _hip
+    p = mem[0]
+    for batch, kv_heads in ((65536, 1), (1 << 40, 1), (1, 65536), (65535, 129), (1 << 12, 1 << 11)):
+        with pytest.raises(_hip.FlashSTUHipError, match="up to 65535"):
+            KV4Cache(batch, kv_heads, 32, 4)
+    for splits in (1, 64, 65):
+        assert lib.fstu_kv4_attend(p, 64, 32, p + 8192, p + 4096, p, splits, p, None, 65536, 2, 1, 32, 4, 3, 0.0, 1, None) == -3
+    assert lib.fstu_kv4_attend(p, 0, 32, p + 8192, p + 4096, p, 1, p, None, 1, 65536, 1, 32, 4, 3, 0.0, 1, None) == -3
