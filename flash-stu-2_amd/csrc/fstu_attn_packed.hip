@@ -611,19 +611,20 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
     };
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, HD == 256 ? 2 : 4> Four;
-    typedef std::integral_constant<int, HD == 128 ? 8 : 2> Eight;
+    typedef std::integral_constant<int, 8> Eight;
     typedef std::integral_constant<int, 2> Pair;
-    typedef std::integral_constant<int, HD == 256 ? 1 : 2> Halves;
     // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of
     // 128 710 us, 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them:
     // two waves of queries, each with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7,
     // 4096 27.5 / 19.1, 12288 50.5 / 48.2, one document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096
     // 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71. Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows
     // of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the kernel of four waves alone.
-    if (softcap > FSTU_FAST_CAP) bf16(Four{}, One{});
-    else if (HD == 128 && window >= 4096 && rows / seqs >= 4096) bf16(Eight{}, One{});
-    else if (HD <= 128 && (int64_t)(rows / 128) * heads < (HD == 128 ? 576 : 768)) bf16(Pair{}, Halves{});
-    else bf16(Four{}, One{});
+    const bool usual = softcap <= FSTU_FAST_CAP;
+    if constexpr (HD == 128)
+      if (usual && window >= 4096 && rows / seqs >= 4096) return bf16(Eight{}, One{});
+    if constexpr (HD <= 128)
+      if (usual && (int64_t)(rows / 128) * heads < (HD == 128 ? 576 : 768)) return bf16(Pair{}, Pair{});
+    bf16(Four{}, One{});
   };
   if (hd == 32) run(std::integral_constant<int, 32>{});
   else if (hd == 64) run(std::integral_constant<int, 64>{});
