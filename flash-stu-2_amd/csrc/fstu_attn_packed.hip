@@ -246,7 +246,10 @@ struct Frag8 { u32x2_t lo, hi; };
 // queries a workgroup instead of 64, which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi
 // (a tenth slower).
 // PARTS: 2 gives each half of 32 keys to a wave of its own, and adds the two up in the end.
-template <int HD, int NQ, int PARTS, int CAP, bool BIAS>
+// A probability goes into the second product as one bf16 value, which adds as much to the result's error as its own rounding does (in 2-norm 0.0017 to 0.0022 of it
+// where fp32 probabilities leave 0.0016).  FINE: as a bf16 value and what its rounding left, two products, as the layers' attention has it (0.0016): that takes
+// 4096 rows of 12 heads of 64 from 20.6 us to 22.2, 16383 of 16 heads of 128 under a window from 218 to 295, two documents of 8192 from 704 to 954.
+template <int HD, int NQ, int PARTS, int CAP, bool BIAS, bool FINE>
 __global__ void __launch_bounds__(NQ * PARTS * packed_dims(HD) * 64, HD <= 64 && NQ * PARTS == 4 ? 3 : 2)
 swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int window,
                        float softcap) {
@@ -287,7 +290,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
 
   const int k_first = max(0, first - window) / KB * KB, k_last = min(len - 1, first + NQ * 32 - 1);
   // A tile's rows through a buffer descriptor: what lies behind the sequence's last row reads as zeros.  The range is checked against the lane's offset, which
-  // therefore holds the row; the scalar one takes no part in it (sums made in the loop and not kept in registers: 16383 rows of 16 heads of 128 221 us, 231).
+  // therefore holds the row; the scalar one takes no part in it (sums made in the loop and not kept in registers: 16383 rows of 16 heads of 128 221 us, 231 with them kept).
   constexpr int NT = NW * 64, PR = (TILE + NT - 1) / NT, STEP = NT / CH;      // 16-byte pieces of a tile to a thread, rows between them
   u32x4_t kr[PR], vr[PR];
   const int row0 = tid / CH, ch0 = tid % CH;
@@ -330,7 +333,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   // (two documents of 8192, 16 heads of 128, 883 us, so 870; of 64 581 and 560)
   constexpr bool FOLD = CAP == 1 && !BIAS;
   const float unit = FOLD ? 2.0f * capA : CAP ? 1.f : scale, lift = FOLD ? capA : 0.f;
-  unsigned pk[8];
+  unsigned pk[8], rest[8];
   float add, top;
   struct Keys { u32x4_t f[KS]; };
   struct Values { Frag8 f[2][ND]; };
@@ -393,6 +396,7 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
       add += a;
       add += z;
       pk[e] = pack2_bf16(a, z);
+      if (FINE) rest[e] = pack2_bf16(a - __uint_as_float(pk[e] << 16), z - __uint_as_float(pk[e] & 0xffff0000u));
       if (e) t = fmaxf(fmaxf(t, s[2 * e]), s[2 * e + 1]);
     }
     top = fmaf(t, unit, base + lift);
@@ -418,6 +422,12 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
 #pragma unroll
       for (int d = 0; d < ND; ++d)
         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v.f[t][d]), __builtin_bit_cast(bf16x8_t, pf), o[d], 0, 0, 0);
+      if constexpr (FINE) {
+        const u32x4_t rf = u32x4_t{rest[4 * t], rest[4 * t + 1], rest[4 * t + 2], rest[4 * t + 3]};
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v.f[t][d]), __builtin_bit_cast(bf16x8_t, rf), o[d], 0, 0, 0);
+      }
     }
   };
   // With ALiBi the largest scores are a query's latest keys': from those backwards the maximum settles at once (two documents of 8192, 16 heads of 128, 719 us, 785
@@ -554,11 +564,8 @@ swa_packed_mfma_kernel(Heads q, Heads k, Heads v, bf16_t* out, const int* cu, co
   }
 }
 
-}  // namespace
-
-extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
-                               int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
-                               float softcap, int dtype, void* stream) {
+int packed_call(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out,
+                const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window, float softcap, bool two_parts, int dtype, void* stream) {
   FSTU_REQUIRE(q && k && v && out && cu, FSTU_ENULL, "fstu_swa_packed: null pointer");
   FSTU_REQUIRE(dtype == FSTU_F32 || dtype == FSTU_BF16, FSTU_EDTYPE, "fstu_swa_packed: unknown dtype %d", dtype);
   FSTU_REQUIRE(hd == 32 || hd == 64 || hd == 128 || hd == 256, FSTU_ESHAPE, "fstu_swa_packed: head dim %d not in {32,64,128,256}", hd);
@@ -592,9 +599,9 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
     }
     auto bf16 = [&](auto nq, auto parts) {
       constexpr int NQ = decltype(nq)::value, PARTS = decltype(parts)::value;
-      auto go = [&](auto cap, auto bias) {
+      auto form = [&](auto cap, auto bias, auto fine) {
         constexpr unsigned threads = NQ * PARTS * packed_dims(HD) * 64, lds = 4 * (HD == 256 ? 32 : 64) * HD * 2 + (HD == 256 ? threads * 64 : 0);
-        const auto kernel = swa_packed_mfma_kernel<HD, NQ, PARTS, decltype(cap)::value, decltype(bias)::value>;
+        const auto kernel = swa_packed_mfma_kernel<HD, NQ, PARTS, decltype(cap)::value, decltype(bias)::value, decltype(fine)::value>;
         if constexpr (lds > 65536) {
           static fstu_lds_limit most;
           rc = fstu_need_lds((const void*)kernel, most, lds, "fstu_swa_packed");
@@ -604,6 +611,7 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
         hipLaunchKernelGGL(kernel, dim3((unsigned)(rows / (NQ * 32) + seqs) * heads), dim3(threads), lds, (hipStream_t)stream, hq, hk, hv, (bf16_t*)out, cu, slopes, rows,
                            seqs, heads, kvh, window, softcap);
       };
+      auto go = [&](auto cap, auto bias) { two_parts ? form(cap, bias, std::true_type{}) : form(cap, bias, std::false_type{}); };
       auto capped = [&](auto cap) { slopes ? go(cap, std::true_type{}) : go(cap, std::false_type{}); };
       if constexpr (NQ == (HD == 256 ? 2 : 4) && PARTS == 1)
         if (softcap > FSTU_FAST_CAP) return capped(std::integral_constant<int, 2>{});
@@ -633,4 +641,18 @@ extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, con
   if (rc != FSTU_OK) return rc;
   FSTU_CHECK_LAUNCH("fstu_swa_packed");
   return FSTU_OK;
+}
+
+}  // namespace
+
+extern "C" int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                               int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
+                               float softcap, int dtype, void* stream) {
+  return packed_call(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, out, cu, slopes, rows, seqs, heads, kvh, hd, window, softcap, false, dtype, stream);
+}
+
+extern "C" int fstu_swa_packed_fine(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                                    int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
+                                    float softcap, int dtype, void* stream) {
+  return packed_call(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, out, cu, slopes, rows, seqs, heads, kvh, hd, window, softcap, true, dtype, stream);
 }

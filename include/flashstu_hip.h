@@ -359,10 +359,16 @@ int fstu_swa_prefill_mfma(const void* qkv, void* vt_ws, void* out, const float* 
  * sees its rows max(0,i-window) .. i.  q (rows,heads,hd), k and v (rows,kvh,hd) by row and head strides in elements (multiples of 16 bytes),
  * query head h reads key head h / (heads/kvh); out (rows,heads,hd) dense, not overlapping the others.  Scores as above, slopes (heads) or NULL,
  * softcap 0: none, else 2^-40..2^40.  Rows of no sequence are left as they were.  Refused: k and v rows 2^23 elements apart and more, more than
- * 65535 heads, and (16 rows + 512 seqs) * heads (bf16: 2 rows, 4 at hd 256) from 2^32 on. */
+ * 65535 heads, and (16 rows + 512 seqs) * heads (bf16: 2 rows, 4 at hd 256) from 2^32 on.
+ * bf16: a probability goes into the product with v as one bf16 value, which adds an error as large as the output's own rounding (2-norm 0.0017 to 0.0022 of
+ * it, 0.0016 with fp32 ones).  fstu_swa_packed_fine: as a bf16 value and what its rounding left, as fstu_swa_prefill_mfma has it (0.0016; up to 1.4 times
+ * as long).  fp32: the same in both, nothing is cut. */
 int fstu_swa_packed(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                     int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
                     float softcap, int dtype, void* stream);
+int fstu_swa_packed_fine(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                         int64_t v_head, void* out, const int* cu, const float* slopes, int rows, int seqs, int heads, int kvh, int hd, int window,
+                         float softcap, int dtype, void* stream);
 
 /* ---- 4-bit ring cache ----------------------------------------------------------
  * fstu_kv4_bytes(...) bytes, cleared once by the caller, for seqs sequences of kvh key heads of hd (32, 64, 128, 256) dims; position j of a sequence

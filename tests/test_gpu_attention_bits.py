@@ -107,19 +107,21 @@ FORMS = [
 ]
 
 
+@pytest.mark.parametrize("fine", [False, True])
 @pytest.mark.parametrize("heads,kvh,hd,lengths,window,softcap,alibi", FORMS)
-def test_packed_prompts_round_each_probability_once(fs, heads, kvh, hd, lengths, window, softcap, alibi):
+def test_packed_prompts_round_each_probability_once_or_not_at_all(fs, heads, kvh, hd, lengths, window, softcap, alibi, fine):
     x = rand(1, sum(lengths), heads + 2 * kvh, hd, dtype=torch.bfloat16)
     q, k, v = x[:, :heads], x[:, heads:heads + kvh], x[:, heads + kvh:]
     slopes, d, some = slopes_of(heads) if alibi else None, x.cuda(), [0, heads - 1]
     cu = ints([0] + list(torch.tensor(lengths).cumsum(0)))
-    y = fs.swa_packed(d[:, :heads], d[:, heads:heads + kvh], d[:, heads + kvh:], cu, slopes=None if slopes is None else slopes.cuda(), window=window, softcap=softcap)
+    y = fs.swa_packed(d[:, :heads], d[:, heads:heads + kvh], d[:, heads + kvh:], cu, slopes=None if slopes is None else slopes.cuda(), window=window, softcap=softcap,
+                      fine=fine)
     o, squares, _, _ = packed(q, k, v, lengths, slopes, window, softcap, some)
-    assert off_in_norm(y[:, some], o, squares) <= MARGIN
+    assert off_in_norm(y[:, some], o, 0 * squares if fine else squares) <= MARGIN
 
 
 def test_prompts_of_one_length_keep_more_in_the_layers_own_attention(fs):
-    """swa_prefill holds a probability in two bf16 parts: of its error only the output's own rounding is left."""
+    """swa_prefill holds a probability in two bf16 parts: of its error only the output's own rounding is left.  swa_packed does that where it is asked to."""
     from flash_stu import _hip
     heads, hd, T, window = 4, 64, 512, 300
     x, slopes = rand(2, 2 * T, 3 * heads, hd, dtype=torch.bfloat16), slopes_of(heads)
@@ -127,9 +129,13 @@ def test_prompts_of_one_length_keep_more_in_the_layers_own_attention(fs):
     o, squares, _, _ = packed(q, k, v, [T, T], slopes, window, 50.0, range(heads))
     d = x.cuda()
     layer = _hip.swa_prefill(d.reshape(2, T, 3 * heads * hd), slopes.cuda(), heads, window, 50.0).view(2 * T, heads, hd)
-    mine = fs.swa_packed(d[:, :heads], d[:, heads:2 * heads], d[:, 2 * heads:], ints([0, T, 2 * T]), slopes=slopes.cuda(), window=window, softcap=50.0)
-    assert off_in_norm(layer, o, torch.zeros(1)) <= MARGIN
-    assert off_in_norm(mine, o, squares) <= MARGIN
+    once, fine = (fs.swa_packed(d[:, :heads], d[:, heads:2 * heads], d[:, 2 * heads:], ints([0, T, 2 * T]), slopes=slopes.cuda(), window=window, softcap=50.0, fine=f)
+                  for f in (False, True))
+    none = torch.zeros(1)
+    assert off_in_norm(layer, o, none) <= MARGIN and off_in_norm(fine, o, none) <= MARGIN
+    assert off_in_norm(once, o, squares) <= MARGIN and off_in_norm(fine, o, none) < off_in_norm(once, o, none)
+    # what is left between the two is outputs next to the middle of two bf16 values
+    assert float((layer.double() - fine.double()).norm()) < 0.5 * float((layer.double() - once.double()).norm())
 
 
 ATTENDS = [

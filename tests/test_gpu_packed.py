@@ -366,3 +366,65 @@ def test_a_score_of_minus_infinity_beside_an_infinity_that_is_not_seen(fs, size,
         o, bound = attention(q[:, h].double(), k[:, h].double(), v[:, h].double(), far.double(), 0.0, 0.0, P_STEP[dtype])
         check(y[clean, h], o[clean], bound[clean], dtype)
     assert bool(torch.isnan(y[0]).all()) and not bool(torch.isfinite(y[70, :, ::9]).any())
+
+
+@pytest.mark.parametrize("heads,kvh,hd,lengths,window,softcap,alibi", [
+    (12, 12, 64, [17, 1, 40], 512, 50.0, True),
+    (1, 1, 128, [0, 2, 0, 0, 3, 0], None, 0.0, True),
+    (4, 2, 64, [129, 63, 64, 65, 128], 31, 600.0, True),
+    (4, 1, 128, [300, 33, 127], None, 0.0, False),
+    (6, 2, 32, [100, 257, 5], 0, 0.0, True),
+    (2, 1, 256, [150, 70, 1], 100, 0.0, True),
+    (5, 5, 256, [33, 64], None, 50.0, False),
+    (64, 1, 64, [1, 1700, 0, 130, 64, 17], 70, 50.0, True),
+    (128, 16, 32, [700, 130], None, 50.0, False),
+    (64, 32, 128, [0, 900, 500, 0], 333, 50.0, True),
+    (2, 1, 128, [4500], None, 0.0, True),
+])
+def test_probabilities_in_two_parts(fs, heads, kvh, hd, lengths, window, softcap, alibi):
+    """fine: as a bf16 value and what its rounding left, 2^-16 of them; in fp32 the same bits as without."""
+    rows = sum(lengths)
+    (q, k, v), dev = fused(7, rows, heads, kvh, hd, torch.bfloat16)
+    slopes, h = slopes_of(heads), torch.tensor([0, heads - 1])
+    args = dict(slopes=slopes.cuda() if alibi else None, window=window, softcap=softcap)
+    y = fs.swa_packed(*dev, bounds(lengths), fine=True, **args)
+    kv = h // (heads // kvh)
+    check(y.cpu()[:, h], *packed(q[:, h], k[:, kv], v[:, kv], lengths, slopes[h] if alibi else None, window, softcap, 2.0 ** -16), torch.bfloat16)
+    assert bool(torch.isfinite(y).all())
+    wide = [t.float() for t in dev]
+    assert torch.equal(fs.swa_packed(*wide, bounds(lengths), fine=True, **args), fs.swa_packed(*wide, bounds(lengths), **args))
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("heads,window,softcap,alibi", [(2, 20, 50.0, True), (96, None, 0.0, False)])
+def test_what_a_row_does_not_see_leaves_its_two_parts_alone(fs, heads, window, softcap, alibi, hd):
+    lengths, bad = [300, 330], [250, 299, 620]
+    (q, k, v), dev = fused(41, sum(lengths), heads, 2, hd, torch.bfloat16)
+    args = dict(slopes=slopes_of(heads).cuda() if alibi else None, window=window, softcap=softcap, fine=True)
+    dirty = [t.clone() for t in dev]
+    dirty[1][bad, 0], dirty[2][bad, 1, ::5] = math.nan, math.inf
+    y = fs.swa_packed(*dirty, bounds(lengths), **args)
+    start = [0] * 300 + [300] * 330
+    clean = [r for r in range(630) if not any(start[r] <= b <= r and (window is None or r - b <= window) for b in bad)]
+    h = torch.tensor([0, heads - 1])
+    kv = h // (heads // 2)
+    o, bound = packed(q[:, h], k[:, kv], v[:, kv], lengths, slopes_of(heads)[h] if alibi else None, window, softcap, 2.0 ** -16)
+    check(y.cpu()[clean][:, h], o[clean], bound[clean], torch.bfloat16)
+    assert bool(torch.isnan(y[bad, 0]).all()) and not bool(torch.isfinite(y[bad, heads - 1, ::5]).any())
+
+
+def test_two_parts_in_a_captured_graph(fs):
+    (_, _, _), dev = fused(8, 300, 4, 2, 64, torch.bfloat16)
+    x, cu = [t.clone() for t in dev], bounds([100, 150, 20])
+    fs.swa_packed(*x, cu, window=64, fine=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fs.swa_packed(*x, cu, window=64, fine=True)
+    for n in range(3):
+        for a, b in zip(x, dev):
+            a.copy_(b.roll(n, 0))
+        graph.replay()
+        want = fs.swa_packed(*x, cu, window=64, fine=True)
+        torch.cuda.synchronize()
+        assert torch.equal(y[:270], want[:270])

@@ -232,12 +232,12 @@ def test_a_batch_that_no_launch_attends_over_is_no_cache(lib, mem):
 
 
 def test_only_kernels_that_a_call_reaches_are_built(lib):
-    """Of the packed prompts' bf16 kernels <head dim, waves of queries, waves to their keys, soft-cap, ALiBi>: four waves of queries (heads of 256: two) for all
+    """Of the packed prompts' bf16 kernels <head dim, waves of queries, waves to their keys, soft-cap, ALiBi, two parts of a probability>: four waves of queries (heads of 256: two) for all
     calls, eight for long documents of heads of 128, two with partners for few workgroups of heads up to 128, these two under ordinary soft-caps."""
     import re
     from flash_stu import _hip
     with open(_hip.LIB_PATH, "rb") as f:
-        built = set(re.findall(rb"swa_packed_mfma_kernelILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb([01])E", f.read()))
+        built = set(re.findall(rb"swa_packed_mfma_kernelILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb([01])ELb([01])E", f.read()))
     forms = [(hd, 2 if hd == 256 else 4, 1, cap) for hd in (32, 64, 128, 256) for cap in (0, 1, 2)]
     forms += [(128, 8, 1, cap) for cap in (0, 1)] + [(hd, 2, 2, cap) for hd in (32, 64, 128) for cap in (0, 1)]
-    assert built == {tuple(b"%d" % x for x in f + (bias,)) for f in forms for bias in (0, 1)}
+    assert built == {tuple(b"%d" % x for x in f + (bias, fine)) for f in forms for bias in (0, 1) for fine in (0, 1)}
