@@ -236,11 +236,15 @@ struct Frag8 { u32x2_t lo, hi; };
 // Keys and values go to LDS by way of registers, which hold the next tile, one barrier a tile; values are read back transposed.  The second half's first
 // product runs beside the first half's softmax, the first half's second product beside the second half's: the maximum that a probability is taken from is the
 // one before these keys, and where a score exceeds it by more than 2^16 (the first keys, and hardly any after) that half is formed once more. Two documents of
-// 8192 rows, 16 heads of 128 on 4 key heads: 0.70 ms, 1.0 PFLOP/s, which the power of both units bounds: at the 1.84 GHz that it leaves, matrix cores are busy
-// 47 % of the time and vector ALUs 36 %.  Soft-cap and ALiBi (16384 rows of 16 heads of 128, window 1024: 215 us, 0.56 PFLOP/s) take the vector ALUs to 52 %,
+// 8192 rows, 16 heads of 128 on 4 key heads: 0.70 ms, 1.0 PFLOP/s, which the power of both units bounds: at the 1.80 GHz that it leaves, matrix cores are busy
+// 48 % of the time and vector ALUs 42 %.  Soft-cap and ALiBi (16383 rows of 16 heads of 128, window 1024: 202-221 us) take the vector ALUs to 52 %,
 // three exp or rcp to a score, matrix cores 27 %.  Instructions of 16x16x32, memory straight to LDS, halves of a workgroup in opposite phases were 7 to 15 %
 // slower.
-// CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).
+// CAP: 0 no soft-cap, 1 up to FSTU_FAST_CAP, 2 a larger one (a branch on that inside costs the windowed prompts 50 % by the registers it spills).  1 is
+// 1 - 2 / (exp(2x) + 1) on the hardware's exp and reciprocal, off by up to 2^-21 of the soft-cap (2e-5 at 50), where a bf16 query's own rounding moves a score by
+// 2^-9 of itself; 2 keeps small scores exact (fstu_wide_cap).
+// Registers: four waves to heads of 64 are held to three a SIMD and spill 1 to 6 of 168 with ALiBi, to heads of 128 1 or 2 of 256 with ALiBi and soft-cap (FINE: up
+// to 16 and 9).
 // Heads of 256 are shared by two waves, a half of the dims to each: 16 registers of scores' sums cross over LDS, and a wave has what it has with heads of 128.
 // Two documents of 4096 and 8 heads 253 us, 301 with all dims in a wave, which fits only one to a SIMD; 1000 rows of two 8 heads with ALiBi 39 and 47 with 128
 // queries a workgroup instead of 64, which leaves room for a second one beside it.  The next tile's first product beside this one's softmax spilled with ALiBi
@@ -622,10 +626,10 @@ int packed_call(const void* q, int64_t q_row, int64_t q_head, const void* k, int
     typedef std::integral_constant<int, 8> Eight;
     typedef std::integral_constant<int, 2> Pair;
     // Waves of 32 queries to a workgroup: eight share a tile of keys where documents are long and nothing but the products counts (two of 8192 and 16 heads of
-    // 128 710 us, 780 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them:
-    // two waves of queries, each with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.8 / 16.7,
-    // 4096 27.5 / 19.1, 12288 50.5 / 48.2, one document of 16 heads 4096 61 / 55, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 21.7, 4096
-    // 58.7 / 56, 5120 68 / 71; heads of 32 22.5 / 16.4, 75 / 71. Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows
+    // 128 699 us, 722 with four; heads of 64 469 and 444; a window of 1024 253 and 238).  Where there are few workgroups a wave's chain of steps bounds them:
+    // two waves of queries, each with a partner for half of its keys.  us, four waves / two and partners: heads of 64, window 512, 2048 rows of 12 20.0 / 16.1,
+    // 4096 27.3 / 19.4, 6144 29.5 / 26.7, one document of 16 heads 4096 61 / 55.6, 6144 109 / 112; heads of 128, window 1024, 2048 rows of 16 26.4 / 22.2, 4096
+    // 61.8 / 58, 5120 68 / 71; heads of 32 21.8 / 15.9, 77 / 75. Heads of 256: two waves of queries, two of dims.  Partners for quarters of the keys: 512 rows
     // of 12 heads of 64 10.9, 11.4 with halves, 58 rows 6.2 and 5.2, 2000 rows 21 and 17.  Soft-caps of no ordinary size have the kernel of four waves alone.
     const bool usual = softcap <= FSTU_FAST_CAP;
     if constexpr (HD == 128)

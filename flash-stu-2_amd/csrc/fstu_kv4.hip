@@ -7,7 +7,8 @@ namespace {
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // The scale's byte for a block whose largest size has these bits: the smallest power of two with amax <= 7 * 2^e.  Its codes end at 6
-// and steps beside that are 2 wide, so nothing is off by more than 2^e.  -120 <= e <= 125: every code's value is a normal bf16.
+// and steps beside that are 2 wide, so nothing is off by more than 2^e.  -120 <= e <= 125: every code's value is a normal bf16 (sizes beyond 7 * 2^125, 1.75 * 2^127,
+// become 6 * 2^125 all the same, off by up to 2 * 2^125).
 __device__ __forceinline__ unsigned kv4_scale(unsigned amax) {
   const unsigned ex = amax >> 23;
   if (ex == 255) return 255;
@@ -486,7 +487,8 @@ __device__ __forceinline__ int sequence_of(const int* pos, int seqs, int cap, in
 
 // One query a sequence.  S^T = K Q^T over 32 slots at a time as two tiles of 16 keys, rows dealt so that lane (g, col) ends up with query col's scores of slots
 // 8 g .. 8 g + 7, which is what it holds of the second product O^T = V^T P^T: no score crosses a lane, only the maxima do.  Codes become bf16 in registers (exact),
-// probabilities go in as a bf16 head and, in the columns 8 further on, what its rounding left (fp32: two such parts).
+// probabilities go in as a bf16 head and, in the columns 8 further on, what its rounding left.  fp32: queries and probabilities in three such parts, 24 bits of them,
+// since codes widen to bf16 at once and the fp32 instruction would take them at a sixteenth of the rate; in 2-norm 2.4e-7 to 2.8e-7 off (plain fp32 1.8e-7 to 2.6e-7).
 // PLAN: the tiles of all sequences are dealt evenly to the workgroups; without, a workgroup takes a key head of a sequence or one of gridDim.z parts of its tiles.
 // kv4_join_kernel adds up what is in parts.
 // Bytes bound it where there are many: 16 sequences of up to 32768 positions, 8 key heads of 128, 84 us, 5.5 TB/s (an instruction undoes two codes and applies

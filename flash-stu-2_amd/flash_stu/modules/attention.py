@@ -91,8 +91,8 @@ class KV4Cache:
     """A ring cache of keys and values in 4 bits for a batch of sequences, each at a position of its own.
 
     Position j of a sequence lives in slot j % capacity.  Values are e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives); 32 values of a head's
-    row share a power of two 2^e, e the smallest whole number from -120 to 125 with amax <= 7 * 2^e; a value's code is the nearest, ties to the even
-    one.  32 values with an infinity or a NaN among them stand for NaN.  A key and its value take 17/16 of a byte for each dim, bf16 ones 4.
+    row share a power of two 2^e, e the smallest whole number from -120 to 125 with amax <= 7 * 2^e (125 where none is; values beyond 7 * 2^125 become
+    6 * 2^125); a value's code is the nearest, ties to the even one.  32 values with an infinity or a NaN among them stand for NaN.  A key and its value take 17/16 of a byte for each dim, bf16 ones 4.
 
     `pos` is (batch,) int32 on the GPU and counted by the caller, so that a captured step runs for every position; a sequence at a negative position
     is not in use.  The capacity may exceed a window by any number and is 2^30 at most; head_dim is 32, 64, 128 or 256.  One launch attends over all of it:

@@ -372,8 +372,8 @@ int fstu_swa_packed_fine(const void* q, int64_t q_row, int64_t q_head, const voi
 
 /* ---- 4-bit ring cache ----------------------------------------------------------
  * fstu_kv4_bytes(...) bytes, cleared once by the caller, for seqs sequences of kvh key heads of hd (32, 64, 128, 256) dims; position j of a sequence
- * lives in slot j % cap.  Values are e2m1 codes; 32 values of a head's row share a scale 2^e, e the smallest of -120..125 with amax <= 7 * 2^e;
- * code: the nearest, ties to the even one.  A block with a value that is not finite stands for NaN.  csrc/fstu_kv4.h says where what lies.
+ * lives in slot j % cap.  Values are e2m1 codes; 32 values of a head's row share a scale 2^e, e the smallest of -120..125 with amax <= 7 * 2^e
+ * (125 beyond 7 * 2^125 too: such values become 6 * 2^125); code: the nearest, ties to the even one.  A block with a value that is not finite stands for NaN.  csrc/fstu_kv4.h says where what lies.
  * Refused: sizes beyond a launch (write and read: rows / 8 + 2 seqs from 2^23 on; attend and step: more than 65535 sequences or heads, seqs * heads and,
  * in up to 64 splits, the key heads' chunks of 8 query heads times splits from 2^23 on, in more those chunks' tiles of 32 slots beyond 31 bits).
  * pos: seqs device ints; a sequence at a negative position is not in use (nothing written, zeros read, out zero).
