@@ -488,7 +488,8 @@ __device__ __forceinline__ int sequence_of(const int* pos, int seqs, int cap, in
 // One query a sequence.  S^T = K Q^T over 32 slots at a time as two tiles of 16 keys, rows dealt so that lane (g, col) ends up with query col's scores of slots
 // 8 g .. 8 g + 7, which is what it holds of the second product O^T = V^T P^T: no score crosses a lane, only the maxima do.  Codes become bf16 in registers (exact),
 // probabilities go in as a bf16 head and, in the columns 8 further on, what its rounding left.  fp32: queries and probabilities in three such parts, 24 bits of them,
-// since codes widen to bf16 at once and the fp32 instruction would take them at a sixteenth of the rate; in 2-norm 2.4e-7 to 2.8e-7 off (plain fp32 1.8e-7 to 2.6e-7).
+// since codes widen to bf16 at once and the fp32 instruction would take them at a sixteenth of the rate; in 2-norm 2.4e-7 to 8e-7 off (plain fp32 1.8e-7 to 1.7e-6,
+// the more the longer the ring).
 // PLAN: the tiles of all sequences are dealt evenly to the workgroups; without, a workgroup takes a key head of a sequence or one of gridDim.z parts of its tiles.
 // kv4_join_kernel adds up what is in parts.
 // Bytes bound it where there are many: 16 sequences of up to 32768 positions, 8 key heads of 128, 84 us, 5.5 TB/s (an instruction undoes two codes and applies

@@ -440,3 +440,30 @@ def test_a_refused_call_of_another_type_writes_nothing(fs, dtype):
             call()
     assert not cache.data.any()
     assert bool(torch.isfinite(cache.attend(q, pos, k, k)).all()) and bool(cache.data.any())
+
+
+def test_two_threads_on_one_stream(fs):
+    """Calls in parts from two threads, whose workspaces come from the same stream's memory."""
+    import threading
+    caches = [filled(fs, 1, 2, 64, 6000, 30 + i)[0] for i in range(2)]
+    qs = [rand(i, 1, 4, 64, dtype=torch.bfloat16).cuda() for i in range(2)]
+    pos = [ints([5999]), ints([3000])]
+    want = [caches[i].attend(qs[i], pos[i]) for i in range(2)]
+    got, errors = [[], []], []
+
+    def calls(i):
+        try:
+            for _ in range(300):
+                got[i].append(caches[i].attend(qs[i], pos[i]))
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not errors and all(len(g) == 300 for g in got)
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
